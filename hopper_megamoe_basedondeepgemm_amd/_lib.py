@@ -31,6 +31,8 @@ EXPORTS = [
     "dgm_router_logits_topk_launch", "dgm_router_topk_launch_stamped", "dgm_frontend_workgroups",
     "dgm_quantize_mxfp4_typed", "dgm_quantize_nvfp4_typed", "dgm_quantize_qoq_typed", "dgm_quantize_qoq_int4_typed",
     "dgm_transform_qoq_weights_checked", "dgm_transform_qoq_int4_weights_checked",
+    "dgm_rms_norm_residual", "dgm_rms_norm_residual_groups", "dgm_rms_norm_residual_backward",
+    "dgm_norm_struct_sizes",
 ]
 # source element types of the weight packers (DGM_SRC_*)
 SRC_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -76,6 +78,23 @@ class MoeArgs(ctypes.Structure):
                 ("hidden_states", ctypes.c_void_p), ("router_weight", ctypes.c_void_p),
                 ("fe_keys", ctypes.c_void_p), ("host_error", ctypes.c_void_p), ("debug_flags", ctypes.c_int32),
                 ("launch_flags", ctypes.c_int32)]
+
+
+class NormArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "residual", "post_weight", "pre_weight", "gate", "residual_out", "h",
+                                                "q", "q_sf", "rstd_post", "rstd_pre")] +
+                [(n, ctypes.c_int64) for n in ("rows", "x_stride", "residual_stride", "gate_stride",
+                                               "residual_out_stride", "h_stride")] +
+                [(n, ctypes.c_int32) for n in ("hidden", "dtype", "weights_f32", "gate_mode", "gate_sigmoid")] +
+                [("residual_scale", ctypes.c_float), ("eps", ctypes.c_float)])
+
+
+class NormGradArgs(ctypes.Structure):
+    _fields_ = ([("forward", NormArgs)] +
+                [(n, ctypes.c_void_p) for n in ("d_residual_out", "d_h", "d_x", "d_residual", "d_gate", "d_post_weight",
+                                                "d_pre_weight", "workspace")] +
+                [(n, ctypes.c_int64) for n in ("workspace_bytes", "d_residual_out_stride", "d_h_stride", "d_x_stride",
+                                               "d_residual_stride", "d_gate_stride")])
 
 
 _lib = None
@@ -129,6 +148,10 @@ def load():
         "dgm_untransform_fp4_weights": ([vp, vp, i32, i32, i32, i32, i32, vp, vp, vp], i32),
         "dgm_untransform_nvfp4_weights": ([vp, vp, i32, i32, i32, i32, i32, vp, vp, vp], i32),
     }
+    sig["dgm_rms_norm_residual"] = ([ctypes.POINTER(NormArgs), vp], i32)
+    sig["dgm_norm_struct_sizes"] = ([ctypes.POINTER(ctypes.c_size_t)] * 2, i32)
+    sig["dgm_rms_norm_residual_groups"] = ([i64, i32], i32)
+    sig["dgm_rms_norm_residual_backward"] = ([ctypes.POINTER(NormGradArgs), vp], i32)
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
         fn.argtypes = args
@@ -194,6 +217,26 @@ def require_gpu(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("MI355X path: tensors must live on the GPU (no CPU fallback)")
+
+
+def require_one_device(first, *tensors):
+    """All tensors on the GPU that is current (work is enqueued on its current stream)."""
+    dev = first.device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"MI355X path: tensors on {dev} and {t.device}")
+    require_gpu(first)
+    if dev.index != torch.cuda.current_device():
+        raise RuntimeError(f"MI355X path: tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()}")
+
+
+def no_graph_under_capture():
+    """Refuses to record an autograd graph while the current stream is captured: its leaves may belong to
+    an eager graph too, and the engine then joins the capture with that graph's stream, which ends the
+    process. The explicit backward calls can be captured."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("no autograd under graph capture: call with torch.no_grad() and capture the explicit "
+                           "*_backward call")
 
 
 def host_device_pointer(t):

@@ -1,0 +1,517 @@
+// Norms around a block (gfx950): the root-mean-square norm behind it, its gate, the scaled residual
+// add and the norm before the next block in one pass over the rows, and the gradients of all of them.
+//
+// Row of H elements, n = x rstd1 w1 (rstd1 = rsqrt(mean x^2 + eps); n = x without w1), a = gate or
+// sigmoid(gate), t = r + s a n, u = t rstd2, h = u w2. Everything between the loads and the stores is
+// fp32 and t enters the second norm unrounded. A workgroup owns a row, a thread 8 NV of its elements in
+// registers, so each input is read once whatever the number of norms; the bound is HBM.
+// Gradients, with R = dL/dt (of the stored t) and D = dL/dh:
+//   du = D w2, R' = R + rstd2 (du - u mean(du u)), dr = R', dw2 = sum D u,
+//   da = s R' n, dn = s R' a, dw1 = sum dn z, dz = dn w1, dx = rstd1 (dz - z mean(dz z)), z = x rstd1.
+#include "dgm_common.hpp"
+#include "dgm_abi_internal.hpp"
+
+using namespace dgm;
+
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+enum { T_BF16 = DGM_SRC_BF16, T_F16 = DGM_SRC_F16, T_F32 = DGM_SRC_F32 };
+
+template <int T>
+DGM_DEV float load1(const void* p, int64_t i) {
+  if constexpr (T == T_F32) return reinterpret_cast<const float*>(p)[i];
+  else if constexpr (T == T_F16) return (float)reinterpret_cast<const _Float16*>(p)[i];
+  else return bf16_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
+}
+template <int T>
+DGM_DEV void store1(void* p, int64_t i, float v) {
+  if constexpr (T == T_F32) reinterpret_cast<float*>(p)[i] = v;
+  else if constexpr (T == T_F16) reinterpret_cast<_Float16*>(p)[i] = (_Float16)v;
+  else reinterpret_cast<uint16_t*>(p)[i] = f32_to_bf16(v);
+}
+// eight consecutive elements from element i (16-byte aligned) as fp32, and back (round to nearest even)
+template <int T>
+DGM_DEV void load8(const void* p, int64_t i, float* v) {
+  if constexpr (T == T_F32) {
+    const f4* q = reinterpret_cast<const f4*>(reinterpret_cast<const float*>(p) + i);
+    const f4 a = q[0], b = q[1];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { v[k] = a[k]; v[4 + k] = b[k]; }
+  } else {
+    const u4 w = *reinterpret_cast<const u4*>(reinterpret_cast<const uint16_t*>(p) + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t d = w[k];      // (a scalar: the cast of a vector's element reads its first one)
+      if constexpr (T == T_F16) {
+        const h2 f = __builtin_bit_cast(h2, d);
+        v[2 * k] = (float)f[0];
+        v[2 * k + 1] = (float)f[1];
+      } else {
+        v[2 * k] = __uint_as_float(d << 16);
+        v[2 * k + 1] = __uint_as_float(d & 0xffff0000u);
+      }
+    }
+  }
+}
+template <int T>
+DGM_DEV void store8(void* p, int64_t i, const float* v) {
+  if constexpr (T == T_F32) {
+    f4* q = reinterpret_cast<f4*>(reinterpret_cast<float*>(p) + i);
+    q[0] = f4{v[0], v[1], v[2], v[3]};
+    q[1] = f4{v[4], v[5], v[6], v[7]};
+  } else {
+    u4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const f2 f = {v[2 * k], v[2 * k + 1]};
+      if constexpr (T == T_F16) w[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f, h2));
+      else w[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf2));
+    }
+    *reinterpret_cast<u4*>(reinterpret_cast<uint16_t*>(p) + i) = w;
+  }
+}
+
+// The elements of a row that a thread holds. VEC: eight consecutive ones per 16-byte aligned chunk
+// (H a multiple of 8), else single ones, a wave's loads contiguous in both.
+template <int NV, int THREADS, bool VEC>
+struct Row {
+  static constexpr int N = 8 * NV;
+  static DGM_DEV int index(int k) {
+    if constexpr (VEC) return ((k >> 3) * THREADS + (int)threadIdx.x) * 8 + (k & 7);
+    else return k * THREADS + (int)threadIdx.x;
+  }
+  template <int T>
+  static DGM_DEV void load(const void* p, int64_t off, int H, float* v) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int i = (j * THREADS + (int)threadIdx.x) * 8;
+        if (i < H) load8<T>(p, off + i, v + 8 * j);
+        else
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[8 * j + k] = 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] = index(k) < H ? load1<T>(p, off + index(k)) : 0.f;
+    }
+  }
+  template <int T>
+  static DGM_DEV void store(void* p, int64_t off, int H, const float* v) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int i = (j * THREADS + (int)threadIdx.x) * 8;
+        if (i < H) store8<T>(p, off + i, v + 8 * j);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (index(k) < H) store1<T>(p, off + index(k), v[k]);
+    }
+  }
+  // norm weights: the rows' type or fp32
+  template <int T>
+  static DGM_DEV void weight(const void* p, bool f32, int H, float* v) {
+    if (f32) load<T_F32>(p, 0, H, v);
+    else load<T>(p, 0, H, v);
+  }
+};
+
+DGM_DEV float wave_sum(float v) {
+  v += dpp_f32<0xB1>(v);        // quad_perm [1,0,3,2]
+  v += dpp_f32<0x4E>(v);        // quad_perm [2,3,0,1]
+  v += dpp_f32<0x141>(v);       // row_half_mirror
+  v += dpp_f32<0x140>(v);       // row_mirror: every lane of a 16-lane row holds its sum
+  const int u = __float_as_int(v);
+  return (__int_as_float(__builtin_amdgcn_readlane(u, 0)) + __int_as_float(__builtin_amdgcn_readlane(u, 16))) +
+         (__int_as_float(__builtin_amdgcn_readlane(u, 32)) + __int_as_float(__builtin_amdgcn_readlane(u, 48)));
+}
+DGM_DEV float wave_max(float v) {
+  v = max_lanes16(v);
+  const int u = __float_as_int(v);
+  return fmaxf(fmaxf(__int_as_float(__builtin_amdgcn_readlane(u, 0)), __int_as_float(__builtin_amdgcn_readlane(u, 16))),
+               fmaxf(__int_as_float(__builtin_amdgcn_readlane(u, 32)), __int_as_float(__builtin_amdgcn_readlane(u, 48))));
+}
+
+// Workgroup reductions of up to two values, in a fixed order, one barrier each. Two LDS sets taken in
+// turn: a set is written again only after the barrier of the other one, which a wave reaches after it
+// has read the first.
+template <int THREADS>
+struct Reduce {
+  static constexpr int W = THREADS / 64;
+  float (*lds)[W][2];
+  int turn = 0;
+  template <bool MAX = false>
+  DGM_DEV void run(float& a, float& b) {
+    a = MAX ? wave_max(a) : wave_sum(a);
+    b = MAX ? wave_max(b) : wave_sum(b);
+    if constexpr (W > 1) {
+      const int w = threadIdx.x >> 6;
+      if ((threadIdx.x & 63) == 0) {
+        lds[turn][w][0] = a;
+        lds[turn][w][1] = b;
+      }
+      __syncthreads();
+      a = lds[turn][0][0];
+      b = lds[turn][0][1];
+#pragma unroll
+      for (int i = 1; i < W; ++i) {
+        a = MAX ? fmaxf(a, lds[turn][i][0]) : a + lds[turn][i][0];
+        b = MAX ? fmaxf(b, lds[turn][i][1]) : b + lds[turn][i][1];
+      }
+      turn ^= 1;
+    }
+  }
+};
+
+DGM_DEV float sigmoid_exact(float g) { return 1.0f / (1.0f + expf(-g)); }
+
+enum { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_TOKEN = 2, GATE_FULL = 3 };
+
+template <int T, int NV, int THREADS, bool VEC>
+__global__ void __launch_bounds__(THREADS) k_norm_fwd(const DgmNormArgs P) {
+  using R = Row<NV, THREADS, VEC>;
+  constexpr int N = R::N;
+  __shared__ float lds[2][THREADS / 64][2];
+  Reduce<THREADS> red{lds};
+  const int H = P.hidden;
+  const int64_t row = blockIdx.x;
+  const bool wf = P.weights_f32;
+  const float inv_h = 1.0f / (float)H;
+  float t[N], w[N], none = 0.f;
+  R::template load<T>(P.x, row * P.x_stride, H, t);
+  if (P.post_weight) {
+    R::template weight<T>(P.post_weight, wf, H, w);
+    float ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) ss += t[k] * t[k];
+    red.run(ss, none);
+    const float rstd = 1.0f / sqrtf(ss * inv_h + P.eps);
+    if (P.rstd_post && threadIdx.x == 0) P.rstd_post[row] = rstd;
+#pragma unroll
+    for (int k = 0; k < N; ++k) t[k] = t[k] * rstd * w[k];
+  }
+  if (P.gate_mode != GATE_NONE) {
+    if (P.gate_mode == GATE_TOKEN) {
+      float a = load1<T>(P.gate, row * P.gate_stride);
+      if (P.gate_sigmoid) a = sigmoid_exact(a);
+#pragma unroll
+      for (int k = 0; k < N; ++k) t[k] *= a;
+    } else {
+      R::template load<T>(P.gate, P.gate_mode == GATE_FULL ? row * P.gate_stride : 0, H, w);
+#pragma unroll
+      for (int k = 0; k < N; ++k) t[k] *= P.gate_sigmoid ? sigmoid_exact(w[k]) : w[k];
+    }
+  }
+  if (P.residual) {
+    R::template load<T>(P.residual, row * P.residual_stride, H, w);
+#pragma unroll
+    for (int k = 0; k < N; ++k) t[k] = w[k] + P.residual_scale * t[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) t[k] *= P.residual_scale;
+  }
+  if (P.residual_out) R::template store<T>(P.residual_out, row * P.residual_out_stride, H, t);
+  if (!P.pre_weight) return;
+  R::template weight<T>(P.pre_weight, wf, H, w);
+  float ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (R::index(k) < H) ss += t[k] * t[k];
+  red.run(ss, none);
+  const float rstd = 1.0f / sqrtf(ss * inv_h + P.eps);
+  if (P.rstd_pre && threadIdx.x == 0) P.rstd_pre[row] = rstd;
+#pragma unroll
+  for (int k = 0; k < N; ++k) t[k] = t[k] * rstd * w[k];
+  if (P.h) R::template store<T>(P.h, row * P.h_stride, H, t);
+  if constexpr (T == T_BF16) {
+    if (!P.q) return;
+    // int8 rows of the rounded h (the rule of dgm_cast_int8_rows): sf = max(amax, 1e-30) / 127,
+    // q = clamp(rne(h / sf), +-127)
+    float amax = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      t[k] = round_bf16(t[k]);
+      amax = fmaxf(amax, R::index(k) < H ? fabsf(t[k]) : 0.f);
+    }
+    red.template run<true>(amax, none);
+    const float s = fmaxf(amax, 1e-30f) / 127.0f;
+    if (threadIdx.x == 0) P.q_sf[row] = s;
+#pragma unroll
+    for (int k = 0; k < N; ++k) t[k] = fminf(fmaxf(rintf(t[k] / s), -127.f), 127.f);
+    int8_t* q = P.q + row * (int64_t)H;
+    if constexpr (VEC) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int i = (j * THREADS + (int)threadIdx.x) * 8;
+        uint32_t d[2] = {0u, 0u};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) d[k >> 2] |= ((uint32_t)(int)t[8 * j + k] & 0xffu) << (8 * (k & 3));
+        if (i < H) *reinterpret_cast<uint2*>(q + i) = uint2{d[0], d[1]};
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (R::index(k) < H) q[R::index(k)] = (int8_t)t[k];
+    }
+  }
+}
+
+// Gradients: workgroup g takes rows g, g + G, ...; the columns' sums over its rows stay in registers and
+// go to partial[set][g][H] (set 0 pre weight, 1 post weight, 2 channel gate), which k_norm_columns adds up
+// in a fixed order.
+template <int T, int NV, int THREADS, bool VEC>
+__global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
+  using R = Row<NV, THREADS, VEC>;
+  constexpr int N = R::N;
+  __shared__ float lds[2][THREADS / 64][2];
+  Reduce<THREADS> red{lds};
+  const DgmNormArgs& F = P.forward;
+  const int H = F.hidden;
+  const float inv_h = 1.0f / (float)H;
+  float dw2[N], dw1[N], dg[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) dw2[k] = dw1[k] = dg[k] = 0.f;
+  for (int64_t row = blockIdx.x; row < F.rows; row += gridDim.x) {
+    float x[N], t[N], a[N], w[N], g[N];
+    R::template load<T>(F.x, row * F.x_stride, H, x);
+    const float rstd1 = F.post_weight ? F.rstd_post[row] : 1.f;
+    // z (kept in x), a, t
+#pragma unroll
+    for (int k = 0; k < N; ++k) { x[k] *= rstd1; t[k] = x[k]; a[k] = 1.f; }
+    if (F.post_weight) {
+      R::template weight<T>(F.post_weight, F.weights_f32, H, w);
+#pragma unroll
+      for (int k = 0; k < N; ++k) t[k] *= w[k];
+    }
+    if (F.gate_mode == GATE_TOKEN) {
+      float v = load1<T>(F.gate, row * F.gate_stride);
+      if (F.gate_sigmoid) v = sigmoid_exact(v);
+#pragma unroll
+      for (int k = 0; k < N; ++k) a[k] = v;
+    } else if (F.gate_mode != GATE_NONE) {
+      R::template load<T>(F.gate, F.gate_mode == GATE_FULL ? row * F.gate_stride : 0, H, a);
+      if (F.gate_sigmoid)
+#pragma unroll
+        for (int k = 0; k < N; ++k) a[k] = sigmoid_exact(a[k]);
+    }
+    // g = R' = the gradient of t
+    if (P.d_residual_out) R::template load<T>(P.d_residual_out, row * P.d_residual_out_stride, H, g);
+    else
+#pragma unroll
+      for (int k = 0; k < N; ++k) g[k] = 0.f;
+    if (P.d_h) {
+      float d[N], u[N];
+      R::template load<T>(P.d_h, row * P.d_h_stride, H, d);
+      if (F.residual) R::template load<T>(F.residual, row * F.residual_stride, H, u);
+      else
+#pragma unroll
+        for (int k = 0; k < N; ++k) u[k] = 0.f;
+      const float rstd2 = F.rstd_pre[row];
+      R::template weight<T>(F.pre_weight, F.weights_f32, H, w);
+      float dot = 0.f, none = 0.f;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        u[k] = (u[k] + F.residual_scale * a[k] * t[k]) * rstd2;
+        dw2[k] += d[k] * u[k];
+        d[k] *= w[k];
+        dot += d[k] * u[k];
+      }
+      red.run(dot, none);
+      dot *= inv_h;
+#pragma unroll
+      for (int k = 0; k < N; ++k) g[k] += rstd2 * (d[k] - u[k] * dot);
+    }
+    if (P.d_residual) R::template store<T>(P.d_residual, row * P.d_residual_stride, H, g);
+    // g = s R'; da = g n, dn = g a
+    float dot = 0.f, tok = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) g[k] *= F.residual_scale;
+    if (F.gate_mode != GATE_NONE) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float da = g[k] * t[k] * (F.gate_sigmoid ? a[k] * (1.f - a[k]) : 1.f);
+        g[k] *= a[k];
+        a[k] = da;
+      }
+      if (F.gate_mode == GATE_TOKEN) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) tok += a[k];
+      } else if (F.gate_mode == GATE_CHANNEL) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) dg[k] += a[k];
+      } else if (P.d_gate) {
+        R::template store<T>(P.d_gate, row * P.d_gate_stride, H, a);
+      }
+    }
+    if (F.post_weight) {
+      R::template weight<T>(F.post_weight, F.weights_f32, H, w);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        dw1[k] += g[k] * x[k];
+        g[k] *= w[k];
+        dot += g[k] * x[k];
+      }
+    }
+    if (F.post_weight || F.gate_mode == GATE_TOKEN) {
+      red.run(dot, tok);
+      dot *= inv_h;
+      if (F.gate_mode == GATE_TOKEN && P.d_gate && threadIdx.x == 0) store1<T>(P.d_gate, row * P.d_gate_stride, tok);
+      if (F.post_weight)
+#pragma unroll
+        for (int k = 0; k < N; ++k) g[k] = rstd1 * (g[k] - x[k] * dot);
+    }
+    if (P.d_x) R::template store<T>(P.d_x, row * P.d_x_stride, H, g);
+  }
+  const int64_t set = (int64_t)gridDim.x * H, off = (int64_t)blockIdx.x * H;
+  if (P.d_pre_weight) R::template store<T_F32>(P.workspace, off, H, dw2);
+  if (P.d_post_weight) R::template store<T_F32>(P.workspace, set + off, H, dw1);
+  if (P.d_gate && F.gate_mode == GATE_CHANNEL) R::template store<T_F32>(P.workspace, 2 * set + off, H, dg);
+}
+
+// Column sums of partial[G][H]: a workgroup takes 64 columns, its wave i rows i, i + W, ...
+template <int T>
+__global__ void __launch_bounds__(1024) k_norm_columns(const DgmNormGradArgs P, int groups) {
+  const DgmNormArgs& F = P.forward;
+  __shared__ float lds[16][64];
+  const int H = F.hidden, col = blockIdx.x * 64 + (threadIdx.x & 63), wv = threadIdx.x >> 6, set = blockIdx.y;
+  void* out = set == 0 ? P.d_pre_weight : set == 1 ? P.d_post_weight : F.gate_mode == GATE_CHANNEL ? P.d_gate : nullptr;
+  if (!out) return;                               // (the whole workgroup)
+  const float* src = (const float*)P.workspace + (int64_t)set * groups * H;
+  float s = 0.f;
+  if (col < H)
+    for (int i = wv; i < groups; i += 16) s += src[(int64_t)i * H + col];
+  lds[wv][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (wv == 0 && col < H) {
+    for (int i = 1; i < 16; ++i) s += lds[i][threadIdx.x];
+    if (set < 2 && F.weights_f32) store1<T_F32>(out, col, s);
+    else store1<T>(out, col, s);
+  }
+}
+
+bool aligned(const void* p, int64_t stride, int size) {
+  return !p || (((uintptr_t)p & 15) == 0 && (stride * size) % 16 == 0);
+}
+
+int check_forward(const DgmNormArgs* A) {
+  DGM_CHECK_ARG(A->dtype >= DGM_SRC_BF16 && A->dtype <= DGM_SRC_F32, "dtype 0 bf16, 1 fp16, 2 fp32");
+  DGM_CHECK_ARG(A->rows >= 0 && A->rows <= 0x7fffffff, "rows below 2^31");
+  DGM_CHECK_ARG(A->hidden > 0 && A->hidden <= DGM_NORM_MAX_HIDDEN, "hidden 1 to 16384");
+  DGM_CHECK_ARG(A->gate_mode >= 0 && A->gate_mode <= GATE_FULL, "gate_mode 0 none, 1 channel, 2 token, 3 full");
+  DGM_CHECK_ARG(A->eps >= 0.f, "eps >= 0");
+  if (A->rows == 0) return 0;
+  DGM_CHECK_ARG(A->x, "null x");
+  DGM_CHECK_ARG((A->gate != nullptr) == (A->gate_mode != GATE_NONE), "gate and gate_mode");
+  return 0;
+}
+
+// Threads of a row's workgroup: eight elements each up to 8192, then sixteen (unaligned rows alike).
+template <class F>
+void dispatch_hidden(int H, F&& f) {
+  using std::integral_constant;
+  if (H <= 512) f(integral_constant<int, 1>{}, integral_constant<int, 64>{});
+  else if (H <= 1024) f(integral_constant<int, 1>{}, integral_constant<int, 128>{});
+  else if (H <= 2048) f(integral_constant<int, 1>{}, integral_constant<int, 256>{});
+  else if (H <= 4096) f(integral_constant<int, 1>{}, integral_constant<int, 512>{});
+  else if (H <= 8192) f(integral_constant<int, 1>{}, integral_constant<int, 1024>{});
+  else f(integral_constant<int, 2>{}, integral_constant<int, 1024>{});
+}
+template <class F>
+void dispatch_type(int dtype, bool vec, F&& f) {
+  using std::integral_constant;
+  auto v = [&](auto t) {
+    if (vec) f(t, std::true_type{});
+    else f(t, std::false_type{});
+  };
+  if (dtype == DGM_SRC_BF16) v(integral_constant<int, T_BF16>{});
+  else if (dtype == DGM_SRC_F16) v(integral_constant<int, T_F16>{});
+  else v(integral_constant<int, T_F32>{});
+}
+
+int element_size(int dtype) { return dtype == DGM_SRC_F32 ? 4 : 2; }
+
+bool forward_aligned(const DgmNormArgs* A) {
+  const int e = element_size(A->dtype);
+  return A->hidden % 8 == 0 && aligned(A->x, A->x_stride, e) && aligned(A->residual, A->residual_stride, e) &&
+         aligned(A->post_weight, 0, e) && aligned(A->pre_weight, 0, e) &&
+         (A->gate_mode == GATE_TOKEN || aligned(A->gate, A->gate_mode == GATE_FULL ? A->gate_stride : 0, e)) &&
+         aligned(A->residual_out, A->residual_out_stride, e) && aligned(A->h, A->h_stride, e) &&
+         ((uintptr_t)A->q & 7) == 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dgm_norm_struct_sizes(size_t* norm_args, size_t* norm_grad_args) {
+  DGM_CHECK_ARG(norm_args && norm_grad_args, "null pointer");
+  *norm_args = sizeof(DgmNormArgs);
+  *norm_grad_args = sizeof(DgmNormGradArgs);
+  return 0;
+}
+
+int dgm_rms_norm_residual(const DgmNormArgs* args, hipStream_t stream) {
+  DGM_CHECK_ARG(args, "null arguments");
+  if (int st = check_forward(args)) return st;
+  const DgmNormArgs A = *args;
+  DGM_CHECK_ARG(!A.q || (A.dtype == DGM_SRC_BF16 && A.q_sf && A.pre_weight), "int8 rows: of bf16 rows with a pre weight");
+  if (A.rows == 0) return 0;
+  dispatch_type(A.dtype, forward_aligned(&A), [&](auto t, auto vec) {
+    dispatch_hidden(A.hidden, [&](auto nv, auto threads) {
+      hipLaunchKernelGGL((k_norm_fwd<t.value, nv.value, threads.value, vec.value>), dim3((unsigned)A.rows),
+                         dim3(threads.value), 0, stream, A);
+    });
+  });
+  return dgm_last_launch_status();
+}
+
+int dgm_rms_norm_residual_groups(int64_t rows, int hidden) {
+  (void)hidden;
+  const int64_t most = 512;
+  return (int)(rows < 1 ? 1 : rows < most ? rows : most);
+}
+
+int dgm_rms_norm_residual_backward(const DgmNormGradArgs* args, hipStream_t stream) {
+  DGM_CHECK_ARG(args, "null arguments");
+  const DgmNormGradArgs A = *args;
+  const DgmNormArgs& F = A.forward;
+  if (int st = check_forward(&F)) return st;
+  const bool columns = A.d_pre_weight || A.d_post_weight || (A.d_gate && F.gate_mode == GATE_CHANNEL);
+  const int groups = dgm_rms_norm_residual_groups(F.rows, F.hidden);
+  if (F.rows > 0) {
+    DGM_CHECK_ARG(!F.post_weight || F.rstd_post, "rstd_post of the forward pass");
+    DGM_CHECK_ARG(!A.d_h || (F.pre_weight && F.rstd_pre), "pre weight and rstd_pre of the forward pass");
+    DGM_CHECK_ARG(!A.d_residual || F.residual, "d_residual without a residual");
+  }
+  DGM_CHECK_ARG(!A.d_pre_weight || F.pre_weight, "d_pre_weight without its weight");
+  DGM_CHECK_ARG(!A.d_post_weight || F.post_weight, "d_post_weight without its weight");
+  DGM_CHECK_ARG(!A.d_gate || F.gate_mode != GATE_NONE, "d_gate without a gate");
+  DGM_CHECK_ARG(!columns || (A.workspace && A.workspace_bytes >= (int64_t)groups * F.hidden * 12 &&
+                             ((uintptr_t)A.workspace & 15) == 0),
+                "workspace of 3 x groups x hidden floats, 16-byte aligned");
+  const int e = element_size(F.dtype);
+  const bool vec = forward_aligned(&F) && aligned(A.d_residual_out, A.d_residual_out_stride, e) &&
+                   aligned(A.d_h, A.d_h_stride, e) && aligned(A.d_x, A.d_x_stride, e) &&
+                   aligned(A.d_residual, A.d_residual_stride, e) &&
+                   (F.gate_mode != GATE_FULL || aligned(A.d_gate, A.d_gate_stride, e));
+  // (no rows: the partial sums of the one group are written as zeros)
+  dispatch_type(F.dtype, vec, [&](auto t, auto v) {
+    dispatch_hidden(F.hidden, [&](auto nv, auto threads) {
+      hipLaunchKernelGGL((k_norm_bwd<t.value, nv.value, threads.value, v.value>), dim3(groups), dim3(threads.value), 0,
+                         stream, A);
+    });
+    if (columns)
+      hipLaunchKernelGGL((k_norm_columns<t.value>), dim3((F.hidden + 63) / 64, 3), dim3(1024), 0, stream, A, groups);
+  });
+  return dgm_last_launch_status();
+}
+
+}  // extern "C"

@@ -1,0 +1,247 @@
+"""Norms around a block with its gate and scaled residual add, on the GPU, and their gradients.
+
+No counterpart in the reference, whose layer starts at the router: these are the row passes that a
+decoder block needs before ``fable_router_quant_topk_frontend`` and behind the layer's combine."""
+import ctypes
+
+import torch
+
+from . import _lib
+
+MAX_HIDDEN = 16384
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
+
+
+def _rows(t):
+    """t as the kernels read it: rows of contiguous elements (any row stride)."""
+    return t if t.stride(1) == 1 or t.size(1) == 1 else t.contiguous()
+
+
+def _gate_mode(gate, T, H):
+    shape = tuple(gate.shape)
+    if shape == (H,):
+        return GATE_CHANNEL
+    if shape == (T, 1):
+        return GATE_TOKEN
+    if shape == (T, H):
+        return GATE_FULL
+    raise ValueError(f"gate of shape {shape}: [hidden], [tokens, 1] or [tokens, hidden]")
+
+
+def _check(x, residual, post_weight, pre_weight, gate, quant=None, residual_out=None, out=None):
+    if x.dim() != 2 or x.dtype not in _lib.SRC_DTYPES:
+        raise TypeError(f"x must be bf16, fp16 or fp32 [tokens, hidden], got {x.dtype} {tuple(x.shape)}")
+    T, H = x.shape
+    if not 1 <= H <= MAX_HIDDEN:
+        raise ValueError(f"hidden {H}: 1 to {MAX_HIDDEN}")
+    for t in (residual, residual_out, out):
+        if t is not None and (t.dtype != x.dtype or t.shape != x.shape):
+            raise TypeError(f"rows of {x.dtype} {tuple(x.shape)} expected, got {t.dtype} {tuple(t.shape)}")
+    wdt = None
+    for w in (post_weight, pre_weight):
+        if w is not None:
+            if w.dim() != 1 or w.size(0) != H or w.dtype not in (x.dtype, torch.float32) or wdt not in (None, w.dtype):
+                raise TypeError(f"norm weights must be [hidden] of {x.dtype} or fp32, both of one type; got "
+                                f"{w.dtype} {tuple(w.shape)}")
+            wdt = w.dtype
+    if gate is not None and gate.dtype != x.dtype:
+        raise TypeError(f"gate of {x.dtype} expected, got {gate.dtype}")
+    if quant not in (None, "int8"):
+        raise ValueError(f"quant {quant!r}: None or 'int8'")
+    if quant and (x.dtype != torch.bfloat16 or pre_weight is None):
+        raise ValueError("int8 rows are cast from bf16 rows and need a pre_weight")
+    for t in (residual_out, out):
+        if t is not None and t.numel() and t.stride(1) != 1 and H > 1:
+            raise ValueError("output rows must be contiguous")
+        if t is not None and T > 1 and t.stride(0) < H:
+            raise ValueError("output rows overlap")
+    if out is not None and pre_weight is None:
+        raise ValueError("out is written with a pre_weight only")
+    if gate is not None:
+        _gate_mode(gate, T, H)
+
+
+def _same_rows(a, b):
+    return a.data_ptr() == b.data_ptr() and a.stride(0) == b.stride(0)
+
+
+def _span(t):
+    return t.data_ptr(), t.data_ptr() + ((t.size(0) - 1) * t.stride(0) + t.size(1)) * t.element_size()
+
+
+def _check_outputs(outs, ins):
+    """An output may be an input's own rows (each row is read before it is written), nothing else that overlaps."""
+    for i, o in enumerate(outs):
+        lo, hi = _span(o)
+        for t in outs[:i]:
+            a, z = _span(t)
+            if lo < z and a < hi:
+                raise ValueError("the outputs overlap")
+        for t in ins:
+            a, z = _span(t if t.dim() == 2 else t[None])
+            if lo < z and a < hi and not (t.dim() == 2 and t.shape == o.shape and _same_rows(o, t)):
+                raise ValueError("an output overlaps an input other than as the same rows")
+
+
+def _forward_args(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, mode, r_out, h, q, sf,
+                  rstd_post, rstd_pre):
+    p = lambda t: 0 if t is None else t.data_ptr()
+    s = lambda t: 0 if t is None else t.stride(0)
+    w = post_weight if post_weight is not None else pre_weight
+    return _lib.NormArgs(p(x), p(residual), p(post_weight), p(pre_weight), p(gate), p(r_out), p(h), p(q), p(sf),
+                         p(rstd_post), p(rstd_pre), x.size(0), x.stride(0), s(residual),
+                         s(gate) if mode in (GATE_TOKEN, GATE_FULL) else 0, s(r_out), s(h), x.size(1),
+                         _lib.SRC_DTYPES[x.dtype], int(w is not None and w.dtype == torch.float32), mode,
+                         int(bool(gate_sigmoid)), float(residual_scale), float(eps))
+
+
+def _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, quant, residual_out, out, keep):
+    """The launch, after the checks: (residual rows, h, q, sf, rstd_post, rstd_pre)."""
+    T, H = x.shape
+    x = _rows(x)
+    residual = None if residual is None else _rows(residual)
+    post_weight = None if post_weight is None else post_weight.contiguous()
+    pre_weight = None if pre_weight is None else pre_weight.contiguous()
+    mode = GATE_NONE
+    if gate is not None:
+        mode = _gate_mode(gate, T, H)
+        gate = _rows(gate) if mode == GATE_FULL else gate.contiguous() if mode == GATE_CHANNEL else gate
+    same = residual is None and post_weight is None and gate is None and residual_scale == 1.0 and residual_out is None
+    new = lambda: torch.empty((T, H), dtype=x.dtype, device=x.device)
+    r_out = None if same else residual_out if residual_out is not None else new()
+    h = None if pre_weight is None else out if out is not None else new()
+    q = sf = rstd_post = rstd_pre = None
+    if quant:
+        q = torch.empty((T, H), dtype=torch.int8, device=x.device)
+        sf = torch.empty((T,), dtype=torch.float32, device=x.device)
+    if keep and post_weight is not None:
+        rstd_post = torch.empty((T,), dtype=torch.float32, device=x.device)
+    if keep and pre_weight is not None:
+        rstd_pre = torch.empty((T,), dtype=torch.float32, device=x.device)
+    if (residual_out is not None or out is not None) and T > 0:
+        _check_outputs([t for t in (residual_out, out) if t is not None],
+                       [t for t in (x, residual, post_weight, pre_weight, gate) if t is not None])
+    if T > 0 and not (same and h is None):
+        args = _forward_args(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, mode, r_out, h,
+                             q, sf, rstd_post, rstd_pre)
+        _lib.check(_lib.load().dgm_rms_norm_residual(ctypes.byref(args), _lib.stream()))
+    return x if same else r_out, h, q, sf, rstd_post, rstd_pre
+
+
+class _RmsNormResidual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps):
+        r, h, _, _, rstd_post, rstd_pre = _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale,
+                                                   eps, None, None, None, True)
+        ctx.save_for_backward(x, residual, post_weight, pre_weight, gate, rstd_post, rstd_pre)
+        ctx.options = gate_sigmoid, residual_scale, eps
+        ctx.set_materialize_grads(False)
+        return (None if r is x else r), h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_r, d_h):
+        x, residual, post_weight, pre_weight, gate, rstd_post, rstd_pre = ctx.saved_tensors
+        gate_sigmoid, residual_scale, eps = ctx.options
+        grads = rms_norm_residual_backward(d_r, d_h, x, residual, rstd_post, rstd_pre, post_weight=post_weight,
+                                           pre_weight=pre_weight, gate=gate, gate_sigmoid=gate_sigmoid,
+                                           residual_scale=residual_scale, eps=eps, needs=ctx.needs_input_grad[:5])
+        return (*grads, None, None, None)
+
+
+def rms_norm_residual(x, residual=None, post_weight=None, pre_weight=None, gate=None, gate_sigmoid=False,
+                      residual_scale=1.0, eps=1e-6, quant=None, residual_out=None, out=None):
+    """The norm behind a block, its gate, the scaled residual add and the norm before the next block, in
+    one pass over the rows:
+
+        n = x / sqrt(mean(x^2) + eps) * post_weight       (n = x without post_weight)
+        r = residual + residual_scale * a * n             (a = gate, or sigmoid(gate) with gate_sigmoid)
+        h = r / sqrt(mean(r^2) + eps) * pre_weight
+
+    x, residual: bf16, fp16 or fp32 [tokens, hidden <= 16384], any row stride; norm weights [hidden] of
+    that type or fp32; gate [hidden], [tokens, 1] or [tokens, hidden]. Every part but x may be absent.
+    Arithmetic in fp32 (the squares of a row have to add up below 3.4e38); r enters the second norm
+    unrounded. Returns ``(r, h)``, h None without pre_weight, r x itself where nothing changes it; with
+    ``quant="int8"`` (bf16) ``(r, h, (q, sf))``: the int8 rows and scales [tokens] of the rounded h
+    (bit for bit ``per_token_cast_to_int8(h)``), as ``int8_gemm_nt`` takes them. ``residual_out`` /
+    ``out``: where r and h go; either may be x's or residual's own rows.
+
+    Differentiable in x, residual, gate and the weights (not with quant, residual_out or out; under graph
+    capture use ``rms_norm_residual_forward`` and ``rms_norm_residual_backward``). Work runs on the
+    current stream of the tensors' device, which has to be the current one."""
+    _check(x, residual, post_weight, pre_weight, gate, quant, residual_out, out)
+    _lib.require_one_device(x, residual, post_weight, pre_weight, gate, residual_out, out)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, residual, post_weight, pre_weight, gate)):
+        _lib.no_graph_under_capture()
+        if quant or residual_out is not None or out is not None:
+            raise ValueError("quant, residual_out and out have no gradient: call under torch.no_grad()")
+        r, h = _RmsNormResidual.apply(x, residual, post_weight, pre_weight, gate, bool(gate_sigmoid),
+                                      float(residual_scale), float(eps))
+        return (x if r is None else r), h
+    r, h, q, sf, _, _ = _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, quant,
+                                 residual_out, out, False)
+    return (r, h, (q, sf)) if quant else (r, h)
+
+
+def rms_norm_residual_forward(x, residual=None, post_weight=None, pre_weight=None, gate=None, gate_sigmoid=False,
+                              residual_scale=1.0, eps=1e-6):
+    """``rms_norm_residual`` with what its explicit backward call needs: ``(r, h, rstd_post, rstd_pre)``
+    (fp32 [tokens] each, None without that norm). Records no autograd graph."""
+    _check(x, residual, post_weight, pre_weight, gate)
+    _lib.require_one_device(x, residual, post_weight, pre_weight, gate)
+    with torch.no_grad():
+        r, h, _, _, rstd_post, rstd_pre = _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid,
+                                                   residual_scale, eps, None, None, None, True)
+    return r, h, rstd_post, rstd_pre
+
+
+def rms_norm_residual_backward(d_r, d_h, x, residual, rstd_post, rstd_pre, post_weight=None, pre_weight=None, gate=None,
+                               gate_sigmoid=False, residual_scale=1.0, eps=1e-6, needs=(True,) * 5):
+    """Gradients of ``rms_norm_residual``: ``(d_x, d_residual, d_post_weight, d_pre_weight, d_gate)`` from
+    d_r = dL/dr and d_h = dL/dh (either may be None: zero), the forward call's inputs and the rstd rows of
+    ``rms_norm_residual_forward``; None for an absent input or one that ``needs`` leaves out. r is
+    recomputed in fp32 from x and residual. Sums over tokens (the weights, a channel gate) are taken in
+    fp32 in a fixed order."""
+    _check(x, residual, post_weight, pre_weight, gate)
+    T, H = x.shape
+    for d in (d_r, d_h):
+        if d is not None and (d.dtype != x.dtype or d.shape != x.shape):
+            raise TypeError(f"gradient rows of {x.dtype} {tuple(x.shape)} expected, got {d.dtype} {tuple(d.shape)}")
+    if d_h is not None and pre_weight is None:
+        raise ValueError("d_h without a pre_weight")
+    for w, rstd in ((post_weight, rstd_post), (pre_weight, rstd_pre)):
+        if w is not None and (rstd is None or rstd.dtype != torch.float32 or tuple(rstd.shape) != (T,)
+                              or not rstd.is_contiguous()):
+            raise ValueError("rstd rows of rms_norm_residual_forward (fp32 [tokens]) expected")
+    _lib.require_one_device(x, d_r, d_h, residual, post_weight, pre_weight, gate, rstd_post, rstd_pre)
+    with torch.no_grad():
+        x = _rows(x)
+        residual = None if residual is None else _rows(residual)
+        d_r = None if d_r is None else _rows(d_r)
+        d_h = None if d_h is None else _rows(d_h)
+        post_weight = None if post_weight is None else post_weight.contiguous()
+        pre_weight = None if pre_weight is None else pre_weight.contiguous()
+        mode = GATE_NONE
+        if gate is not None:
+            mode = _gate_mode(gate, T, H)
+            gate = _rows(gate) if mode == GATE_FULL else gate.contiguous() if mode == GATE_CHANNEL else gate
+        new = lambda t, need: torch.empty(t.shape, dtype=t.dtype, device=t.device) if need and t is not None else None
+        d_x, d_residual, d_post, d_pre, d_gate = (new(t, n) for t, n in zip((x, residual, post_weight, pre_weight, gate),
+                                                                            needs))
+        lib = _lib.load()
+        ws = None
+        if d_post is not None or d_pre is not None or (d_gate is not None and mode == GATE_CHANNEL):
+            ws = torch.empty((3, lib.dgm_rms_norm_residual_groups(T, H), H), dtype=torch.float32, device=x.device)
+        fwd = _forward_args(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, mode, None, None,
+                            None, None, rstd_post, rstd_pre)
+        p = lambda t: 0 if t is None else t.data_ptr()
+        s = lambda t: 0 if t is None else t.stride(0)
+        args = _lib.NormGradArgs(fwd, p(d_r), p(d_h), p(d_x), p(d_residual), p(d_gate), p(d_post), p(d_pre), p(ws),
+                                 0 if ws is None else ws.nbytes, s(d_r), s(d_h), s(d_x), s(d_residual),
+                                 s(d_gate) if mode in (GATE_TOKEN, GATE_FULL) else 0)
+        _lib.check(lib.dgm_rms_norm_residual_backward(ctypes.byref(args), _lib.stream()))
+    return d_x, d_residual, d_post, d_pre, d_gate
+
+
+__all__ = ["rms_norm_residual", "rms_norm_residual_forward", "rms_norm_residual_backward"]

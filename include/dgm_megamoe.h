@@ -372,6 +372,68 @@ int dgm_fused_workgroups(int hidden, int intermediate, int act_format);
 int dgm_abi_struct_sizes(size_t* moe_args, size_t* buffer_layout);
 int dgm_fused_last_form(int hidden, int intermediate, int act_format);
 
+/* ---------------------------------------------------------------- operators around the layer
+ * (no counterpart in the reference, whose layer starts at the router and ends at the combine)
+ *
+ * dgm_rms_norm_residual: the norm behind a block, its gate, the scaled residual add and the norm
+ * before the next block, one pass:
+ *   n = x rsqrt(mean x^2 + eps) post_weight (n = x without post_weight), a = gate or sigmoid(gate),
+ *   t = residual + residual_scale a n, h = t rsqrt(mean t^2 + eps) pre_weight.
+ * All arithmetic in fp32 (a row's squares have to add up below 3.4e38), t unrounded into the second
+ * norm. Rows of `hidden` (1 to 16384) contiguous elements of type dtype (DGM_SRC_*) at row strides in
+ * elements; norm weights of that type or fp32. NULL: no such part (residual, post_weight, pre_weight,
+ * gate) or output (residual_out, h, rstd_*, q). gate_mode 1: gate [hidden], 2: [rows] at gate_stride,
+ * 3: [rows, hidden]. residual_out may be residual, or x, at the same stride; h may be x. q / q_sf (bf16 rows): int8
+ * rows [rows, hidden] of the rounded h and their scales, by the rule of dgm_cast_int8_rows.
+ * rstd_post / rstd_pre [rows] fp32 are what the backward pass needs of the forward one. */
+#define DGM_NORM_MAX_HIDDEN 16384
+typedef struct DgmNormArgs {
+  const void* x;
+  const void* residual;
+  const void* post_weight;
+  const void* pre_weight;
+  const void* gate;
+  void* residual_out;
+  void* h;
+  int8_t* q;
+  float* q_sf;
+  float* rstd_post;
+  float* rstd_pre;
+  int64_t rows;
+  int64_t x_stride, residual_stride, gate_stride, residual_out_stride, h_stride;
+  int32_t hidden;
+  int32_t dtype;
+  int32_t weights_f32;
+  int32_t gate_mode;
+  int32_t gate_sigmoid;
+  float residual_scale;
+  float eps;
+} DgmNormArgs;
+int dgm_rms_norm_residual(const DgmNormArgs* args, hipStream_t stream);
+
+/* Its gradients, from d_residual_out = dL/dt and d_h = dL/dh (each may be NULL: zero). `forward`: the
+ * forward call's arguments (its outputs but rstd_* are not read). Outputs that are NULL are not
+ * computed; weight gradients have their weights' type, d_gate the rows' type, in the gate's shape.
+ * workspace: 3 x dgm_rms_norm_residual_groups(rows, hidden) x hidden floats where a gradient is a sum
+ * over rows (weights, channel gate); the sums are taken in a fixed order. No rows: zero sums. */
+typedef struct DgmNormGradArgs {
+  DgmNormArgs forward;
+  const void* d_residual_out;
+  const void* d_h;
+  void* d_x;
+  void* d_residual;
+  void* d_gate;
+  void* d_post_weight;
+  void* d_pre_weight;
+  float* workspace;
+  int64_t workspace_bytes;
+  int64_t d_residual_out_stride, d_h_stride, d_x_stride, d_residual_stride, d_gate_stride;
+} DgmNormGradArgs;
+int dgm_rms_norm_residual_groups(int64_t rows, int hidden);
+int dgm_rms_norm_residual_backward(const DgmNormGradArgs* args, hipStream_t stream);
+/* sizeof of the two structs as built, as dgm_abi_struct_sizes */
+int dgm_norm_struct_sizes(size_t* norm_args, size_t* norm_grad_args);
+
 #ifdef __cplusplus
 }
 #endif
