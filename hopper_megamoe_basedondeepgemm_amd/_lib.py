@@ -32,7 +32,7 @@ EXPORTS = [
     "dgm_quantize_mxfp4_typed", "dgm_quantize_nvfp4_typed", "dgm_quantize_qoq_typed", "dgm_quantize_qoq_int4_typed",
     "dgm_transform_qoq_weights_checked", "dgm_transform_qoq_int4_weights_checked",
     "dgm_rms_norm_residual", "dgm_rms_norm_residual_groups", "dgm_rms_norm_residual_backward",
-    "dgm_norm_struct_sizes",
+    "dgm_norm_struct_sizes", "dgm_int8_gemm_nt", "dgm_int8_gemm_struct_size",
 ]
 # source element types of the weight packers (DGM_SRC_*)
 SRC_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -97,6 +97,14 @@ class NormGradArgs(ctypes.Structure):
                                                "d_residual_stride", "d_gate_stride")])
 
 
+class Int8GemmArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("a", "sfa", "b", "sfb", "c", "d")] +
+                [(n, ctypes.c_int64) for n in ("m", "n", "k", "a_stride", "sfa_stride", "b_stride", "sfb_stride",
+                                               "c_stride", "d_stride")] +
+                [("dtype", ctypes.c_int32), ("swiglu", ctypes.c_int32), ("clamp", ctypes.c_float),
+                 ("fast_math", ctypes.c_int32)])
+
+
 _lib = None
 
 
@@ -149,6 +157,8 @@ def load():
         "dgm_untransform_nvfp4_weights": ([vp, vp, i32, i32, i32, i32, i32, vp, vp, vp], i32),
     }
     sig["dgm_rms_norm_residual"] = ([ctypes.POINTER(NormArgs), vp], i32)
+    sig["dgm_int8_gemm_nt"] = ([ctypes.POINTER(Int8GemmArgs), vp], i32)
+    sig["dgm_int8_gemm_struct_size"] = ([ctypes.POINTER(ctypes.c_size_t)], i32)
     sig["dgm_norm_struct_sizes"] = ([ctypes.POINTER(ctypes.c_size_t)] * 2, i32)
     sig["dgm_rms_norm_residual_groups"] = ([i64, i32], i32)
     sig["dgm_rms_norm_residual_backward"] = ([ctypes.POINTER(NormGradArgs), vp], i32)

@@ -1,0 +1,85 @@
+"""int8 products with a scale for each token and channel, on the GPU: the dense (shared) expert beside
+the routed ones, on the int8 rows that ``per_token_cast_to_int8`` and ``rms_norm_residual`` write."""
+import ctypes
+
+import torch
+
+from . import _lib
+
+MAX_K = 131071          # sums of K products of up to 128 * 128 stay below 2^31
+
+
+def _operand(name, pair):
+    """(int8 rows, fp32 scales, scale stride): scales [rows], or one scale per row repeated [rows, groups]
+    as ``per_token_cast_to_int8`` returns them (the first column is read)."""
+    q, sf = pair
+    if q.dtype != torch.int8 or q.dim() != 2:
+        raise TypeError(f"{name}: int8 [rows, k] expected, got {q.dtype} {tuple(q.shape)}")
+    if sf.dtype != torch.float32 or sf.dim() not in (1, 2) or sf.size(0) != q.size(0) or (sf.dim() == 2 and sf.size(1) < 1):
+        raise TypeError(f"{name}: fp32 scales [{q.size(0)}] (or repeated [{q.size(0)}, groups]) expected, got {sf.dtype} "
+                        f"{tuple(sf.shape)}")
+    return q, sf
+
+
+def _rows(t):
+    return t if t.stride(1) == 1 or t.size(1) == 1 else t.contiguous()
+
+
+def int8_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_math=True):
+    """d = (a @ b.T) with a scale for each row of both, into d (bf16, fp16 or fp32 [m, n], any row stride):
+
+        d[m, n] = sfa[m] * sfb[n] * sum_k a[m, k] * b[n, k] (+ c[m, n], or c[n] for a 1-D c)
+
+    a = (int8 [m, k], fp32 scales), b = (int8 [n, k], fp32 scales); scales [rows], or repeated per row as
+    ``per_token_cast_to_int8`` returns them (it also packs the weights: one scale per channel). c has d's
+    type and may be d itself. ``activation="swiglu"``: b holds gate rows, then up rows, and d [m, n / 2] =
+    silu(min(gate, clamp)) * clamp(up, -clamp, clamp), the layer's SwiGLU (``activation_clamp`` None: no
+    clamp; ``fast_math`` as in ``mxfp4_mega_moe_fused``). Sums are exact in int32 (k <= 131071), the rest is
+    fp32, rounded once. 16-byte aligned rows (k a multiple of 16) take the fast kernels. No gradient. Work
+    runs on the current stream of the tensors' device, which has to be the current one. Returns d."""
+    aq, asf = _operand("a", a)
+    bq, bsf = _operand("b", b)
+    m, k = aq.shape
+    n = bq.size(0)
+    if bq.size(1) != k or not 1 <= k <= MAX_K:
+        raise ValueError(f"k of a {k} and of b {bq.size(1)}: equal, 1 to {MAX_K}")
+    if activation not in (None, "swiglu"):
+        raise ValueError(f"activation {activation!r}: None or 'swiglu'")
+    swiglu = activation is not None
+    if swiglu and (n % 2 or c is not None):
+        raise ValueError("swiglu takes a gate and an up half of b's rows, and no c")
+    if m >= 1 << 20 or n >= 1 << 24:
+        raise ValueError(f"m {m} and n {n}: below 2^20 and 2^24")
+    n_out = n // 2 if swiglu else n
+    if d.dtype not in _lib.SRC_DTYPES or tuple(d.shape) != (m, n_out):
+        raise TypeError(f"d: bf16, fp16 or fp32 [{m}, {n_out}] expected, got {d.dtype} {tuple(d.shape)}")
+    if d.numel() and ((n_out > 1 and d.stride(1) != 1) or (m > 1 and d.stride(0) < n_out)):
+        raise ValueError("d: rows must be contiguous and must not overlap")
+    if c is not None and (c.dtype != d.dtype or tuple(c.shape) not in ((m, n_out), (n_out,))):
+        raise TypeError(f"c: {d.dtype} [{m}, {n_out}] or [{n_out}] expected, got {c.dtype} {tuple(c.shape)}")
+    _lib.require_one_device(d, aq, asf, bq, bsf, c)
+    if torch.is_grad_enabled() and (d.requires_grad or (c is not None and c.requires_grad)):
+        raise RuntimeError("int8_gemm_nt has no gradient: call it under torch.no_grad()")
+    if m == 0 or n_out == 0:
+        return d
+    aq, bq = _rows(aq), _rows(bq)
+    c_stride = 0
+    if c is not None:
+        if c.dim() == 1:
+            c = c.contiguous()
+        else:
+            c = _rows(c)
+            c_stride = c.stride(0)
+        lo, hi = d.data_ptr(), d.data_ptr() + ((m - 1) * d.stride(0) + n_out) * d.element_size()
+        end = c.data_ptr() + (n_out if c.dim() == 1 else (m - 1) * c_stride + n_out) * c.element_size()
+        if c.data_ptr() < hi and lo < end and not (c.dim() == 2 and c.data_ptr() == lo and (m == 1 or c_stride == d.stride(0))):
+            raise ValueError("c overlaps d other than as the same rows")
+    args = _lib.Int8GemmArgs(aq.data_ptr(), asf.data_ptr(), bq.data_ptr(), bsf.data_ptr(), 0 if c is None else c.data_ptr(),
+                             d.data_ptr(), m, n, k, aq.stride(0), asf.stride(0), bq.stride(0), bsf.stride(0), c_stride,
+                             d.stride(0), _lib.SRC_DTYPES[d.dtype], int(swiglu),
+                             float(activation_clamp if activation_clamp is not None else 3.0e38), int(bool(fast_math)))
+    _lib.check(_lib.load().dgm_int8_gemm_nt(ctypes.byref(args), _lib.stream()))
+    return d
+
+
+__all__ = ["int8_gemm_nt"]

@@ -434,6 +434,31 @@ int dgm_rms_norm_residual_backward(const DgmNormGradArgs* args, hipStream_t stre
 /* sizeof of the two structs as built, as dgm_abi_struct_sizes */
 int dgm_norm_struct_sizes(size_t* norm_args, size_t* norm_grad_args);
 
+/* int8 x int8 product of rows (a token each) with weight rows (a channel each), with their scales:
+ *   d[m][n] = sfa[m] sfb[n] sum_k a[m][k] b[n][k] (+ c[m][n]; c_stride 0: one row c[n] for every token)
+ * or with `swiglu` over b's gate rows [0, n/2) and up rows [n/2, n), as the layer's:
+ *   d[m][i] = silu(min(gate, clamp)) * clamp(up, -clamp, clamp)
+ * Sums exact in int32 (k 1 to 131071), the rest fp32, one rounding to dtype (DGM_SRC_*), which c shares.
+ * Rows of k (a, b) and n (c, d) contiguous elements at strides in elements; scales at their strides.
+ * c may be d at the same stride. m below 2^20, n below 2^24. No counterpart in the reference. */
+#define DGM_INT8_GEMM_MAX_K 131071
+typedef struct DgmInt8GemmArgs {
+  const int8_t* a;
+  const float* sfa;
+  const int8_t* b;
+  const float* sfb;
+  const void* c;
+  void* d;
+  int64_t m, n, k;
+  int64_t a_stride, sfa_stride, b_stride, sfb_stride, c_stride, d_stride;
+  int32_t dtype;
+  int32_t swiglu;
+  float clamp;
+  int32_t fast_math; /* SwiGLU's sigmoid: 1 hardware exp2 and reciprocal, 0 IEEE */
+} DgmInt8GemmArgs;
+int dgm_int8_gemm_nt(const DgmInt8GemmArgs* args, hipStream_t stream);
+int dgm_int8_gemm_struct_size(size_t* args);
+
 #ifdef __cplusplus
 }
 #endif
