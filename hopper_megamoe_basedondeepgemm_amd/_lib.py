@@ -33,6 +33,7 @@ EXPORTS = [
     "dgm_transform_qoq_weights_checked", "dgm_transform_qoq_int4_weights_checked",
     "dgm_rms_norm_residual", "dgm_rms_norm_residual_groups", "dgm_rms_norm_residual_backward",
     "dgm_norm_struct_sizes", "dgm_int8_gemm_nt", "dgm_int8_gemm_struct_size",
+    "dgm_int8_gemm_workspace_bytes",
 ]
 # source element types of the weight packers (DGM_SRC_*)
 SRC_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -102,7 +103,7 @@ class Int8GemmArgs(ctypes.Structure):
                 [(n, ctypes.c_int64) for n in ("m", "n", "k", "a_stride", "sfa_stride", "b_stride", "sfb_stride",
                                                "c_stride", "d_stride")] +
                 [("dtype", ctypes.c_int32), ("swiglu", ctypes.c_int32), ("clamp", ctypes.c_float),
-                 ("fast_math", ctypes.c_int32)])
+                 ("fast_math", ctypes.c_int32), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)])
 
 
 _lib = None
@@ -158,6 +159,7 @@ def load():
     }
     sig["dgm_rms_norm_residual"] = ([ctypes.POINTER(NormArgs), vp], i32)
     sig["dgm_int8_gemm_nt"] = ([ctypes.POINTER(Int8GemmArgs), vp], i32)
+    sig["dgm_int8_gemm_workspace_bytes"] = ([i64, i64, i64, i32], i64)
     sig["dgm_int8_gemm_struct_size"] = ([ctypes.POINTER(ctypes.c_size_t)], i32)
     sig["dgm_norm_struct_sizes"] = ([ctypes.POINTER(ctypes.c_size_t)] * 2, i32)
     sig["dgm_rms_norm_residual_groups"] = ([i64, i32], i32)

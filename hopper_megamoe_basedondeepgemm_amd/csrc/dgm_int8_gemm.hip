@@ -9,7 +9,6 @@
 // registers hold consecutive channels of one token.
 #include "dgm_common.hpp"
 #include "dgm_abi_internal.hpp"
-#include <stdlib.h>
 
 using namespace dgm;
 
@@ -174,10 +173,11 @@ DGM_DEV v4i load16(const int8_t* row, int k, int K) {
   }
 }
 
-// Few tokens (16 MT at most per workgroup): the weights are read once, straight into registers. A
-// workgroup takes 16 channels (SwiGLU: their gate and up rows), its eight waves the K blocks of 128 in
-// turn (lane l: 32 bytes of row l % 16, so a block's rows are read in whole 128-byte lines); the waves'
-// int32 sums meet in LDS.
+// Few tokens, or rows off 16-byte alignment (16 MT tokens per workgroup): the weights are read once per
+// workgroup row, straight into registers. A workgroup takes 16 channels (SwiGLU: their gate and up rows),
+// its eight waves the K blocks of 128 in turn (lane l: 32 bytes of row l % 16, so a block's rows are read in
+// whole 128-byte lines); the waves' int32 sums meet in LDS. One token, 4096 x 2048: 4.2 us, 2.0 TB/s. (Two or
+// four K blocks requested at once: no faster, or slower.)
 template <int MT, bool SWIGLU, bool ALIGNED>
 __global__ void __launch_bounds__(512) k_int8_gemm_rows(const DgmInt8GemmArgs P, int vec) {
   constexpr int W = 8, H = SWIGLU ? 2 : 1;
@@ -238,23 +238,26 @@ __global__ void __launch_bounds__(512) k_int8_gemm_rows(const DgmInt8GemmArgs P,
   });
 }
 
-#ifndef SWZ
-#define SWZ(r) (((r) >> 1) & 7)
-#endif
 __device__ const uint4 k_zeros = {0u, 0u, 0u, 0u};
 
-// Many tokens: a workgroup computes BM tokens x BN channels over K steps of 128 bytes. Both operands' rows
-// go from HBM / L2 straight into LDS, the next step's while the current one is multiplied (two buffers,
-// one barrier a step). A row's eight 16-byte pieces lie permuted by the row's number, so that eight lanes
-// reading one piece of eight rows meet eight different bank groups.
+// More tokens: a workgroup computes BM tokens x BN channels over K steps of 128 bytes (whole 128-byte lines:
+// half lines, 64-byte steps, cost as many cycles of a CU's 64 B / clock). Both operands' rows go from HBM /
+// L2 straight into LDS, STAGES - 1 steps ahead of the one that is multiplied, with one barrier a step. A
+// row's eight 16-byte pieces lie permuted by the row's number, so that the lanes reading one piece of 16
+// rows meet 16 different bank groups (no conflicts counted).
 // SwiGLU: blocks of 32 channel rows alternate between gate and up rows, so that a wave holds both of a
 // channel.
-template <int BM, int BN, int WM, int WN, bool SWIGLU>
-__global__ void __launch_bounds__(64 * WM * WN) k_int8_gemm_tiles(const DgmInt8GemmArgs P, int vec, int tiles_m, int tiles_n) {
+// Few tiles: gridDim.y workgroups share a tile, each a range of K, and leave their int32 sums in the
+// workspace [split][token][channel] for k_int8_gemm_join.
+template <int BM, int BN, int WM, int WN, int STAGES, bool SWIGLU>
+__global__ void __launch_bounds__(64 * WM * WN) k_int8_gemm_tiles(const DgmInt8GemmArgs P, int vec, int tiles_m, int tiles_n,
+                                                                  int steps_per_split) {
   constexpr int W = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, ROWS = BM + BN, LOADS = ROWS / (8 * W);
-  static_assert(ROWS % (8 * W) == 0 && BM % (8 * W) == 0 && (!SWIGLU || TN % 2 == 0), "whole loads per wave");
-  __shared__ __attribute__((aligned(1024))) int8_t lds[2][ROWS * 128];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), K = (int)P.k;
+  static_assert(ROWS % (8 * W) == 0 && BM % (8 * W) == 0 && W % 2 == 0 && (!SWIGLU || TN % 2 == 0), "whole loads per wave");
+  __shared__ __attribute__((aligned(1024))) int8_t lds[STAGES][ROWS * 128];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int split = blockIdx.y, k_begin = split * steps_per_split * 128;
+  const int K = min((int)P.k, k_begin + steps_per_split * 128);          // end of this workgroup's range
   // Workgroups go to the 8 XCDs in turn: each XCD gets a contiguous run of tiles, ordered in bands of 8
   // token tiles, so that the tiles an XCD works on at a time share rows in its L2.
   const int tiles = tiles_m * tiles_n, per = (tiles + 7) / 8;
@@ -264,7 +267,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_int8_gemm_tiles(const DgmInt8G
   const int64_t m0 = (int64_t)(8 * band + in_band % bm) * BM, n0 = (int64_t)(in_band / bm) * (SWIGLU ? BN / 2 : BN);
   const int64_t n_out = SWIGLU ? P.n / 2 : P.n;
   // each wave's loads: LOADS times eight rows of the token tile, then of the channel tile
-  const int piece = (lane & 7) ^ SWZ((wave & 1) * 8 + (lane >> 3));
+  const int piece = (lane & 7) ^ ((wave & 1) * 4 + (lane >> 4));
   const int8_t* src[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
@@ -280,19 +283,22 @@ __global__ void __launch_bounds__(64 * WM * WN) k_int8_gemm_tiles(const DgmInt8G
       src[i] = P.b + n * P.b_stride + 16 * piece;
     }
   }
+  auto load = [&](const int8_t* from, int8_t* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+  };
+  // Pieces behind K are zeros. (Their address is kept from the compiler's view: it would branch on a lane's
+  // piece and issue two loads, and the waits below count them.)
+  uint64_t zeros = (uint64_t)&k_zeros;
+  asm("" : "+v"(zeros));
   auto fetch = [&](int k0, int8_t* to) {
     if (k0 + 128 <= K) {
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[i] + k0),
-                                         (__attribute__((address_space(3))) void*)(to + (i * W + wave) * 1024), 16, 0, 0);
+      for (int i = 0; i < LOADS; ++i) load(src[i] + k0, to + (i * W + wave) * 1024);
     } else {
-      // (the pieces behind K: zeros)
 #pragma unroll
       for (int i = 0; i < LOADS; ++i)
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)(k0 + 16 * piece < K ? src[i] + k0 : (const int8_t*)&k_zeros),
-            (__attribute__((address_space(3))) void*)(to + (i * W + wave) * 1024), 16, 0, 0);
+        load((const int8_t*)(k0 + 16 * piece < K ? (uint64_t)src[i] + (uint64_t)k0 : zeros), to + (i * W + wave) * 1024);
     }
   };
   v16i acc[TN][TM];
@@ -305,7 +311,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_int8_gemm_tiles(const DgmInt8G
   auto multiply = [&](const int8_t* from) {
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      const int at = ((2 * kk + half) ^ SWZ(r)) * 16;
+      const int at = ((2 * kk + half) ^ ((r >> 1) & 7)) * 16;
       v4i av[TM], bv[TN];
 #pragma unroll
       for (int m = 0; m < TM; ++m) av[m] = *reinterpret_cast<const v4i*>(from + (row_a + 32 * m) * 128 + at);
@@ -317,20 +323,58 @@ __global__ void __launch_bounds__(64 * WM * WN) k_int8_gemm_tiles(const DgmInt8G
         for (int m = 0; m < TM; ++m) acc[n][m] = mfma_i8_32x32x32(bv[n], av[m], acc[n][m]);
     }
   };
-  fetch(0, lds[0]);
-  for (int k0 = 0, turn = 0; k0 < K; k0 += 128, turn ^= 1) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);      // this wave's loads of the step have landed,
-    __syncthreads();                         // everyone's, and the other buffer is read
-    if (k0 + 128 < K) fetch(k0 + 128, lds[turn ^ 1]);
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) fetch(k_begin + 128 * i, lds[i]);
+  // A step: this wave's loads of it have landed (those of the STAGES - 2 steps behind it may be under way)
+  // and its LDS reads of the step before have returned; behind the barrier that holds for every wave, so
+  // the step can be read and the buffer of the step before filled again.
+  for (int k0 = k_begin, turn = 0; k0 < K; k0 += 128) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * LOADS) : "memory");
+    fetch(k0 + 128 * (STAGES - 1), lds[turn == 0 ? STAGES - 1 : turn - 1]);
     multiply(lds[turn]);
+    turn = turn + 1 == STAGES ? 0 : turn + 1;
   }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");      // (the zeros behind the last step)
   // Results through LDS, 32 tokens of a wave at a time: from the lanes' four channels of 32 tokens to 16-byte
-  // pieces of whole token rows (rows padded by 16 bytes, so that neither side meets bank conflicts).
+  // pieces of whole token rows (stored from the lanes, a 8192 x 8192 output took 80 us longer). Rows are
+  // padded by 16 bytes, so that neither side meets bank conflicts.
   constexpr int H = SWIGLU ? 2 : 1, CW = 32 * TN / H, PITCH = CW + 4;
   static_assert(W * 32 * PITCH * 4 <= (int)sizeof(lds), "the waves' parts fit");
   __syncthreads();
   float* part = reinterpret_cast<float*>(&lds[0][0]) + wave * 32 * PITCH;
   const int64_t c0 = n0 + wn * CW, t0 = m0 + wm * (BM / WM);
+  if (gridDim.y > 1) {
+    int* ws = P.workspace + (int64_t)split * P.m * P.n;
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+#pragma unroll
+        for (int n = h; n < TN; n += H)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const v16i& x = acc[n][m];
+            *reinterpret_cast<v4i*>(part + r * PITCH + 32 * (n / H) + 8 * q + 4 * half) = v4i{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+          }
+        wave_sync();
+        constexpr int L = CW / 4;
+#pragma unroll
+        for (int j = 0; j < 32 * L / 64; ++j) {
+          const int row = (64 * j + lane) / L, col = (64 * j + lane) % L * 4;
+          const int64_t token = t0 + 32 * m + row, c = c0 + col;
+          if (token >= P.m || c >= n_out) continue;
+          const v4i v = *reinterpret_cast<const v4i*>(part + row * PITCH + col);
+          int* to = ws + token * P.n + (h ? n_out : 0) + c;
+          if (P.n % 4 == 0 && n_out % 4 == 0) *reinterpret_cast<v4i*>(to) = v;
+          else
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (c + i < n_out) to[i] = v[i];
+        }
+        wave_sync();
+      }
+    return;
+  }
   v4f sb[TN][4];
 #pragma unroll
   for (int n = 0; n < TN; n += H)
@@ -370,6 +414,34 @@ __global__ void __launch_bounds__(64 * WM * WN) k_int8_gemm_tiles(const DgmInt8G
   }
 }
 
+// The splits' sums added, then as the tiles' epilogue: a thread takes four channels of a token.
+template <bool SWIGLU>
+__global__ void __launch_bounds__(256) k_int8_gemm_join(const DgmInt8GemmArgs P, int vec, int splits) {
+  const int64_t n_out = SWIGLU ? P.n / 2 : P.n, quads = (n_out + 3) / 4;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= quads * P.m) return;
+  const int64_t m = id / quads, n = (id - m * quads) * 4;
+  v4i s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  const bool four = P.n % 4 == 0 && n_out % 4 == 0;
+#pragma unroll 4
+  for (int k = 0; k < splits; ++k)
+#pragma unroll
+    for (int h = 0; h < (SWIGLU ? 2 : 1); ++h) {
+      const int* from = P.workspace + ((int64_t)k * P.m + m) * P.n + (h ? n_out : 0) + n;
+      if (four) s[h] += *reinterpret_cast<const v4i*>(from);
+      else
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < n_out) s[h][i] += from[i];
+    }
+  const float sa = P.sfa[m * P.sfa_stride];
+  const v4f sb = load_scales(P, n, n_out), su = SWIGLU ? load_scales(P, n_out + n, 2 * n_out) : sb;
+  with_epilogue(P, [&](auto t, auto add) {
+    if (vec && n + 3 < n_out) put4<t.value, add.value, SWIGLU, true>(P, m, n, n_out, sa, sb, su, s[0], s[1]);
+    else put4<t.value, add.value, SWIGLU, false>(P, m, n, n_out, sa, sb, su, s[0], s[1]);
+  });
+}
+
 template <int MT>
 void launch_rows(const DgmInt8GemmArgs& A, bool aligned, int vec, hipStream_t stream) {
   const int64_t n_out = A.swiglu ? A.n / 2 : A.n;
@@ -380,13 +452,58 @@ void launch_rows(const DgmInt8GemmArgs& A, bool aligned, int vec, hipStream_t st
   else hipLaunchKernelGGL((k_int8_gemm_rows<MT, false, false>), grid, dim3(512), 0, stream, A, vec);
 }
 
-template <int BM, int BN, int WM, int WN>
-void launch_tiles(const DgmInt8GemmArgs& A, int vec, hipStream_t stream) {
-  const int tiles_m = (int)((A.m + BM - 1) / BM), tiles_n = (int)((A.n + BN - 1) / BN);
-  const dim3 grid((unsigned)((tiles_m * tiles_n + 7) / 8 * 8));
-  if (A.swiglu) hipLaunchKernelGGL((k_int8_gemm_tiles<BM, BN, WM, WN, true>), grid, dim3(64 * WM * WN), 0, stream, A, vec, tiles_m, tiles_n);
-  else hipLaunchKernelGGL((k_int8_gemm_tiles<BM, BN, WM, WN, false>), grid, dim3(64 * WM * WN), 0, stream, A, vec, tiles_m, tiles_n);
+template <int BM, int BN, int WM, int WN, int STAGES>
+void launch_tiles(const DgmInt8GemmArgs& A, int vec, int splits, hipStream_t stream) {
+  const int tiles_m = (int)((A.m + BM - 1) / BM), tiles_n = (int)((A.n + BN - 1) / BN), steps = (int)((A.k + 127) / 128);
+  const int per = (steps + splits - 1) / splits;
+  splits = (steps + per - 1) / per;                // (every split has a step)
+  const dim3 grid((unsigned)((tiles_m * tiles_n + 7) / 8 * 8), (unsigned)splits), block(64 * WM * WN);
+  if (A.swiglu) hipLaunchKernelGGL((k_int8_gemm_tiles<BM, BN, WM, WN, STAGES, true>), grid, block, 0, stream, A, vec, tiles_m, tiles_n, per);
+  else hipLaunchKernelGGL((k_int8_gemm_tiles<BM, BN, WM, WN, STAGES, false>), grid, block, 0, stream, A, vec, tiles_m, tiles_n, per);
+  if (splits == 1) return;
+  const int64_t quads = ((A.swiglu ? A.n / 2 : A.n) + 3) / 4 * A.m;
+  const dim3 join((unsigned)((quads + 255) / 256));
+  if (A.swiglu) hipLaunchKernelGGL(k_int8_gemm_join<true>, join, dim3(256), 0, stream, A, vec, splits);
+  else hipLaunchKernelGGL(k_int8_gemm_join<false>, join, dim3(256), 0, stream, A, vec, splits);
 }
+
+// Which kernel takes an aligned product, from estimates of its time in us (256 CUs). A tile form takes
+// `alone` us per K step while every workgroup has a CU to itself, `full` us when the CUs hold as many as
+// fit (2 or 1), and 4 us around it; splitting K costs a second launch and the sums' way through memory
+// (3.5 TB/s). The step times were measured with K = 4096:
+//   64 x 128 tokens x channels, 3 stages:  0.60 / 0.97 us  (256 x 4096: 20 us; the 128 x 128 forms 24 and 32)
+//   128 x 128, 4 stages (one a CU):        0.77 us         (1024 x 4096: 27 us; 2 stages 35, 256 x 256 58)
+//   128 x 128, 2 stages:                   1.0 / 1.33 us   (2048 x 4096: 43 us; 4 stages 50, 256 x 256 59)
+//   256 x 256, 2 stages (one a CU):        2.0 us          (4096 x 4096: 70 us; 128 x 128 84 and 98)
+// The rows form takes 2 us and, per 1024 of K and 256 workgroups, 0.8 us up to 4 tokens, 1.0 up to 16, 1.4
+// up to 32 and 2.4 up to 64 (SwiGLU: 2.5 times the first two, 1.5 times the others): 16 x 4096, K 4096: 7 us
+// (tiles, 4 splits 11); 64 x 4096, K 7168: 22 us (tiles, 8 splits 16).
+struct Form { int kind, splits; };
+enum { ROWS = 0, T64, T128_DEEP, T128, T256 };
+Form choose(int64_t m, int64_t n, int64_t k, bool swiglu, int64_t workspace_bytes) {
+  static const struct { int bm, bn, per_cu; double alone, full; } tiles[] = {
+      {0, 0, 0, 0, 0}, {64, 128, 2, 0.60, 0.97}, {128, 128, 1, 0.77, 0.77}, {128, 128, 2, 1.0, 1.33}, {256, 256, 1, 2.0, 2.0}};
+  const int64_t steps = (k + 127) / 128;
+  Form best = {ROWS, 1};
+  double least = 1e30;
+  if (m <= 64) {
+    const double c = (m <= 4 ? 0.8 : m <= 16 ? 1.0 : m <= 32 ? 1.4 : 2.4) * (!swiglu ? 1.0 : m <= 16 ? 2.5 : 1.5);
+    const double wgs = (double)((n / (swiglu ? 2 : 1) + 15) / 16) / 256;
+    least = 2 + (double)((k + 1023) / 1024) * c * (wgs < 1 ? 1 : wgs);
+  }
+  for (int t = T64; t <= T256; ++t)
+    for (int s = 1; s <= 8; s *= 2) {
+      if (s > 1 && (steps < 2 * s || (int64_t)s * m * n * 4 > workspace_bytes)) break;
+      const int64_t wgs = ((m + tiles[t].bm - 1) / tiles[t].bm) * ((n + tiles[t].bn - 1) / tiles[t].bn) * s;
+      const int64_t rounds = (wgs + 256 * tiles[t].per_cu - 1) / (256 * tiles[t].per_cu);
+      double us = 4 + (double)((steps + s - 1) / s) * (wgs <= 256 ? tiles[t].alone : tiles[t].full * (double)rounds);
+      if (s > 1) us += 3 + 8e-6 / 3.5 * (double)s * (double)m * (double)n;
+      if (us < least) least = us, best = {t, s};
+    }
+  return best;
+}
+// Sums of a split call above this are not worth their way through memory.
+constexpr int64_t MOST_WORKSPACE = 64 << 20;
 
 }  // namespace
 
@@ -396,6 +513,12 @@ int dgm_int8_gemm_struct_size(size_t* args) {
   DGM_CHECK_ARG(args, "null pointer");
   *args = sizeof(DgmInt8GemmArgs);
   return 0;
+}
+
+int64_t dgm_int8_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int swiglu) {
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  const Form f = choose(m, n, k, swiglu != 0, MOST_WORKSPACE);
+  return f.splits == 1 ? 0 : (int64_t)f.splits * m * n * 4;
 }
 
 int dgm_int8_gemm_nt(const DgmInt8GemmArgs* args, hipStream_t stream) {
@@ -413,10 +536,12 @@ int dgm_int8_gemm_nt(const DgmInt8GemmArgs* args, hipStream_t stream) {
   const int e = A.dtype == DGM_SRC_F32 ? 4 : 2;
   const bool aligned = (A.k % 16 | A.a_stride % 16 | A.b_stride % 16) == 0 && (((uintptr_t)A.a | (uintptr_t)A.b) & 15) == 0;
   const int vec = (((uintptr_t)A.d | (uintptr_t)A.c | (uint64_t)(A.d_stride * e) | (uint64_t)(A.c_stride * e)) & 15) == 0;
-  const char* force = getenv("DGM_GEMM");
-  const int f = force ? atoi(force) : 0;
-  if (f == 1 || (f == 0 && A.m >= 512 && aligned)) launch_tiles<256, 256, 2, 4>(A, vec, stream);
-  else if (f == 2 || (f == 0 && A.m > 64 && aligned)) launch_tiles<128, 128, 2, 2>(A, vec, stream);
+  const int64_t held = A.workspace && ((uintptr_t)A.workspace & 15) == 0 ? A.workspace_bytes : 0;
+  const Form f = aligned ? choose(A.m, A.n, A.k, A.swiglu != 0, held < MOST_WORKSPACE ? held : MOST_WORKSPACE) : Form{ROWS, 1};
+  if (f.kind == T256) launch_tiles<256, 256, 2, 4, 2>(A, vec, f.splits, stream);
+  else if (f.kind == T128) launch_tiles<128, 128, 2, 2, 2>(A, vec, f.splits, stream);
+  else if (f.kind == T128_DEEP) launch_tiles<128, 128, 2, 2, 4>(A, vec, f.splits, stream);
+  else if (f.kind == T64) launch_tiles<64, 128, 2, 2, 3>(A, vec, f.splits, stream);
   else if (A.m <= 16) launch_rows<1>(A, aligned, vec, stream);
   else if (A.m <= 32) launch_rows<2>(A, aligned, vec, stream);
   else launch_rows<4>(A, aligned, vec, stream);

@@ -1,6 +1,7 @@
 """int8 products with a scale for each token and channel, on the GPU: the dense (shared) expert beside
 the routed ones, on the int8 rows that ``per_token_cast_to_int8`` and ``rms_norm_residual`` write."""
 import ctypes
+import functools
 
 import torch
 
@@ -19,6 +20,11 @@ def _operand(name, pair):
         raise TypeError(f"{name}: fp32 scales [{q.size(0)}] (or repeated [{q.size(0)}, groups]) expected, got {sf.dtype} "
                         f"{tuple(sf.shape)}")
     return q, sf
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(m, n, k, swiglu):
+    return _lib.load().dgm_int8_gemm_workspace_bytes(m, n, k, int(swiglu))
 
 
 def _rows(t):
@@ -74,10 +80,13 @@ def int8_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_m
         end = c.data_ptr() + (n_out if c.dim() == 1 else (m - 1) * c_stride + n_out) * c.element_size()
         if c.data_ptr() < hi and lo < end and not (c.dim() == 2 and c.data_ptr() == lo and (m == 1 or c_stride == d.stride(0))):
             raise ValueError("c overlaps d other than as the same rows")
+    need = _workspace_bytes(m, n, k, swiglu)
+    ws = torch.empty(need, dtype=torch.uint8, device=d.device) if need else None
     args = _lib.Int8GemmArgs(aq.data_ptr(), asf.data_ptr(), bq.data_ptr(), bsf.data_ptr(), 0 if c is None else c.data_ptr(),
                              d.data_ptr(), m, n, k, aq.stride(0), asf.stride(0), bq.stride(0), bsf.stride(0), c_stride,
                              d.stride(0), _lib.SRC_DTYPES[d.dtype], int(swiglu),
-                             float(activation_clamp if activation_clamp is not None else 3.0e38), int(bool(fast_math)))
+                             float(activation_clamp if activation_clamp is not None else 3.0e38), int(bool(fast_math)),
+                             0 if ws is None else ws.data_ptr(), need)
     _lib.check(_lib.load().dgm_int8_gemm_nt(ctypes.byref(args), _lib.stream()))
     return d
 

@@ -455,7 +455,11 @@ typedef struct DgmInt8GemmArgs {
   int32_t swiglu;
   float clamp;
   int32_t fast_math; /* SwiGLU's sigmoid: 1 hardware exp2 and reciprocal, 0 IEEE */
+  int32_t* workspace; /* of this call until it has run; without it (NULL) K is not split */
+  int64_t workspace_bytes;
 } DgmInt8GemmArgs;
+/* bytes of workspace a call of this size uses (0: none), 16-byte aligned */
+int64_t dgm_int8_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int swiglu);
 int dgm_int8_gemm_nt(const DgmInt8GemmArgs* args, hipStream_t stream);
 int dgm_int8_gemm_struct_size(size_t* args);
 
