@@ -17,6 +17,7 @@ from .mega import (FusedSymmBuffer, get_fused_symm_buffer_for_mega_moe,
                    get_nvfp4_mega_moe_sm90_weight_layout)
 from . import quantization_mxfp4, quantization_mxfp4_fused, quantization_nvfp4, quantization_qoq_fused
 from .utils import per_token_cast_to_fp4, per_token_cast_to_fp8, ceil_div, align
+from .balance import router_balance_loss, router_balance_loss_backward, router_balance_loss_forward
 from .int8_gemm import int8_gemm_nt
 from .norm import rms_norm_residual, rms_norm_residual_backward, rms_norm_residual_forward
 from . import checkpoint
@@ -42,5 +43,6 @@ __all__ = [
     "mega_moe_to_nvfp4_checkpoint", "untransform_mxfp4_weights_for_mega_moe_fused",
     "untransform_nvfp4_weights_for_mega_moe_fused", "fable_frontend_stamps", "get_nvfp4_mega_moe_sm90_block_n",
     "get_nvfp4_mega_moe_sm90_weight_layout",
+    "router_balance_loss", "router_balance_loss_forward", "router_balance_loss_backward",
     "int8_gemm_nt", "rms_norm_residual", "rms_norm_residual_forward", "rms_norm_residual_backward",
 ]

@@ -33,7 +33,8 @@ EXPORTS = [
     "dgm_transform_qoq_weights_checked", "dgm_transform_qoq_int4_weights_checked",
     "dgm_rms_norm_residual", "dgm_rms_norm_residual_groups", "dgm_rms_norm_residual_backward",
     "dgm_norm_struct_sizes", "dgm_int8_gemm_nt", "dgm_int8_gemm_struct_size",
-    "dgm_int8_gemm_workspace_bytes",
+    "dgm_int8_gemm_workspace_bytes", "dgm_router_balance_loss", "dgm_router_balance_loss_backward",
+    "dgm_router_balance_workspace_bytes", "dgm_balance_struct_size",
 ]
 # source element types of the weight packers (DGM_SRC_*)
 SRC_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -106,6 +107,15 @@ class Int8GemmArgs(ctypes.Structure):
                  ("fast_math", ctypes.c_int32), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)])
 
 
+class BalanceArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "topk_idx", "cu_seqlens", "loss", "counts", "seq_stats", "totals",
+                                                "d_loss", "d_logits", "workspace")] +
+                [(n, ctypes.c_int64) for n in ("workspace_bytes", "tokens", "logits_stride", "idx_stride",
+                                               "d_logits_stride")] +
+                [(n, ctypes.c_int32) for n in ("experts", "topk", "seqs", "dtype", "idx_i64", "score")] +
+                [("balance_coef", ctypes.c_float), ("z_coef", ctypes.c_float)])
+
+
 _lib = None
 
 
@@ -158,6 +168,10 @@ def load():
         "dgm_untransform_nvfp4_weights": ([vp, vp, i32, i32, i32, i32, i32, vp, vp, vp], i32),
     }
     sig["dgm_rms_norm_residual"] = ([ctypes.POINTER(NormArgs), vp], i32)
+    sig["dgm_router_balance_loss"] = ([ctypes.POINTER(BalanceArgs), vp], i32)
+    sig["dgm_router_balance_loss_backward"] = ([ctypes.POINTER(BalanceArgs), vp], i32)
+    sig["dgm_router_balance_workspace_bytes"] = ([i64, i32, i32], i64)
+    sig["dgm_balance_struct_size"] = ([ctypes.POINTER(ctypes.c_size_t)], i32)
     sig["dgm_int8_gemm_nt"] = ([ctypes.POINTER(Int8GemmArgs), vp], i32)
     sig["dgm_int8_gemm_workspace_bytes"] = ([i64, i64, i64, i32], i64)
     sig["dgm_int8_gemm_struct_size"] = ([ctypes.POINTER(ctypes.c_size_t)], i32)

@@ -1,0 +1,139 @@
+"""The router's balance loss, per-expert counts and the gradient of its logits, on the GPU.
+
+No counterpart in the reference, whose frontend stops at the top-k: this is what training the router, or
+watching its balance in service, needs of the same logits and indices (``FusedSymmBuffer.logits`` and
+``topk_idx`` as the frontend leaves them)."""
+import ctypes
+
+import torch
+
+from . import _lib
+
+MAX_EXPERTS = 1024
+SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def _rows(t):
+    return t if t.stride(1) == 1 or t.size(1) == 1 else t.contiguous()
+
+
+def _check(logits, topk_idx, cu_seqlens, score, z_coef):
+    if logits.dim() != 2 or logits.dtype not in _lib.SRC_DTYPES:
+        raise TypeError(f"logits must be bf16, fp16 or fp32 [tokens, experts], got {logits.dtype} {tuple(logits.shape)}")
+    T, E = logits.shape
+    if not 1 <= E <= MAX_EXPERTS:
+        raise ValueError(f"experts {E}: 1 to {MAX_EXPERTS}")
+    if topk_idx.dim() != 2 or topk_idx.dtype not in (torch.int64, torch.int32) or topk_idx.size(0) != T:
+        raise TypeError(f"topk_idx must be int64 or int32 [{T}, topk], got {topk_idx.dtype} {tuple(topk_idx.shape)}")
+    if not 1 <= topk_idx.size(1) <= E or T * topk_idx.size(1) >= 1 << 31:
+        raise ValueError(f"topk {topk_idx.size(1)}: 1 to {E}, tokens x topk below 2^31")
+    if cu_seqlens is not None and (cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1
+                                   or not 2 <= cu_seqlens.size(0) <= 1 << 24):
+        raise TypeError(f"cu_seqlens must be int32 [sequences + 1], got {cu_seqlens.dtype} {tuple(cu_seqlens.shape)}")
+    if score not in SCORES:
+        raise ValueError(f"score {score!r}: one of {sorted(SCORES)}")
+    if score == "sigmoid" and z_coef:
+        raise ValueError("z_coef belongs to score='softmax'")
+    _lib.require_one_device(logits, topk_idx, cu_seqlens)
+
+
+def _args(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score, counts, seq_stats, totals, loss=None, ws=None,
+          d_loss=None, d_logits=None):
+    p = lambda t: 0 if t is None else t.data_ptr()
+    return _lib.BalanceArgs(p(logits), p(topk_idx), p(cu_seqlens), p(loss), p(counts), p(seq_stats), p(totals), p(d_loss),
+                            p(d_logits), p(ws), 0 if ws is None else ws.nbytes, logits.size(0), logits.stride(0),
+                            topk_idx.stride(0), 0 if d_logits is None else d_logits.stride(0), logits.size(1),
+                            topk_idx.size(1), 1 if cu_seqlens is None else cu_seqlens.size(0) - 1,
+                            _lib.SRC_DTYPES[logits.dtype], int(topk_idx.dtype == torch.int64), SCORES[score],
+                            float(balance_coef), float(z_coef))
+
+
+def _forward(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score):
+    dev = logits.device
+    logits, topk_idx = _rows(logits), _rows(topk_idx)
+    cu_seqlens = None if cu_seqlens is None else cu_seqlens.contiguous()
+    seqs = 1 if cu_seqlens is None else cu_seqlens.size(0) - 1
+    E = logits.size(1)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    counts = torch.empty((E,) if cu_seqlens is None else (seqs, E), dtype=torch.int32, device=dev)
+    stats = torch.empty(4 * seqs + 4, dtype=torch.int32, device=dev)       # per sequence, then the totals
+    lib = _lib.load()
+    need = lib.dgm_router_balance_workspace_bytes(logits.size(0), seqs, E)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    args = _args(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score, counts, stats, stats[4 * seqs:], loss, ws)
+    _lib.check(lib.dgm_router_balance_loss(ctypes.byref(args), _lib.stream()))
+    return loss, counts, stats
+
+
+class _RouterBalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, topk_idx, cu_seqlens, balance_coef, z_coef, score):
+        loss, counts, stats = _forward(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score)
+        ctx.save_for_backward(logits, topk_idx, cu_seqlens, counts, stats)
+        ctx.options = balance_coef, z_coef, score
+        ctx.mark_non_differentiable(counts)
+        return loss, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_loss, _):
+        logits, topk_idx, cu_seqlens, counts, stats = ctx.saved_tensors
+        balance_coef, z_coef, score = ctx.options
+        return (router_balance_loss_backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, balance_coef, z_coef, score),
+                None, None, None, None, None)
+
+
+def router_balance_loss(logits, topk_idx, cu_seqlens=None, balance_coef=1.0, z_coef=0.0, score="softmax"):
+    """The auxiliary loss that keeps experts evenly used, and their counts:
+
+        loss = balance_coef * mean over sequences( sum_e f_e P_e ) + z_coef * mean over tokens( logsumexp^2 )
+
+    f_e = experts * (slots of expert e) / (slots) and P_e = the mean of p_e over the sequence's routed
+    tokens, p = softmax(logits) or, with ``score="sigmoid"``, sigmoid(logits) / their sum (then no z_coef).
+    logits: bf16, fp16 or fp32 [tokens, experts <= 1024]; topk_idx: int64 or int32 [tokens, topk], ids
+    outside [0, experts) are no slot (-1: unrouted), and a token without a slot adds nothing; cu_seqlens
+    (int32 [sequences + 1], ascending): packed sequences, each with its own f and P, those without a routed
+    token left out of the mean, tokens behind the last one ignored. An expert masked with -inf has p = 0.
+
+    Returns ``(loss, counts)``: fp32 scalar and int32 [experts] (with cu_seqlens [sequences, experts]).
+    Differentiable in logits through P and logsumexp (counts are constants); under graph capture use
+    ``router_balance_loss_forward`` and ``router_balance_loss_backward``. Sums over tokens are taken in a
+    fixed order. Work runs on the current stream of the tensors' device, which has to be the current one."""
+    _check(logits, topk_idx, cu_seqlens, score, z_coef)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        _lib.no_graph_under_capture()
+        return _RouterBalanceLoss.apply(logits, topk_idx, cu_seqlens, float(balance_coef), float(z_coef), score)
+    return _forward(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score)[:2]
+
+
+def router_balance_loss_forward(logits, topk_idx, cu_seqlens=None, balance_coef=1.0, z_coef=0.0, score="softmax"):
+    """``router_balance_loss`` with what its explicit backward call needs: ``(loss, counts, stats)``. Records
+    no autograd graph."""
+    _check(logits, topk_idx, cu_seqlens, score, z_coef)
+    with torch.no_grad():
+        return _forward(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score)
+
+
+def router_balance_loss_backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens=None, balance_coef=1.0, z_coef=0.0,
+                                 score="softmax"):
+    """The logits' gradient (logits' type) from d_loss (fp32 scalar tensor), the forward call's inputs and the
+    counts and stats of ``router_balance_loss_forward``; zeros for tokens that add nothing."""
+    _check(logits, topk_idx, cu_seqlens, score, z_coef)
+    seqs = 1 if cu_seqlens is None else cu_seqlens.size(0) - 1
+    E = logits.size(1)
+    if (d_loss.dtype != torch.float32 or d_loss.numel() != 1 or counts.dtype != torch.int32 or counts.numel() != seqs * E
+            or stats.dtype != torch.int32 or stats.numel() != 4 * seqs + 4 or not counts.is_contiguous()
+            or not stats.is_contiguous()):
+        raise TypeError("d_loss fp32 scalar, counts and stats of router_balance_loss_forward expected")
+    _lib.require_one_device(logits, d_loss, counts, stats)
+    with torch.no_grad():
+        logits, topk_idx = _rows(logits), _rows(topk_idx)
+        cu_seqlens = None if cu_seqlens is None else cu_seqlens.contiguous()
+        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        args = _args(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score, counts, stats, stats[4 * seqs:], d_loss=d_loss,
+                     d_logits=d_logits)
+        _lib.check(_lib.load().dgm_router_balance_loss_backward(ctypes.byref(args), _lib.stream()))
+    return d_logits
+
+
+__all__ = ["router_balance_loss", "router_balance_loss_forward", "router_balance_loss_backward"]

@@ -14,7 +14,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdgm_megamoe.so")
 PROBE_LIB = os.path.join(HERE, "libdgm_probe.so")
 SOURCES = ["dgm_megamoe.hip", "dgm_fused.hip", "dgm_packers.hip", "dgm_noalloc.hip", "dgm_norm.hip",
-           "dgm_int8_gemm.hip"]
+           "dgm_int8_gemm.hip", "dgm_balance.hip"]
 PROBE_SOURCES = ["dgm_probe.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

@@ -463,6 +463,43 @@ int64_t dgm_int8_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int swigl
 int dgm_int8_gemm_nt(const DgmInt8GemmArgs* args, hipStream_t stream);
 int dgm_int8_gemm_struct_size(size_t* args);
 
+/* The router's balance loss over logits [tokens, experts] (rows at logits_stride, type DGM_SRC_*) and the
+ * chosen experts topk_idx [tokens, topk] (rows at idx_stride; int64 or int32; ids outside [0, experts) are
+ * no slot, a token without a slot is unrouted and adds nothing). Sequences: tokens [cu_seqlens[b],
+ * cu_seqlens[b + 1]), ascending (int32 [seqs + 1]); NULL: one of all tokens; tokens of none add nothing.
+ * Per sequence with n routed tokens, count_e slots of expert e and p = softmax(logits) or (score 1)
+ * sigmoid / sum of sigmoids:
+ *   loss = balance_coef mean_sequences( experts sum_e count_e / sum(count) mean_tokens p_e )
+ *        + z_coef mean_tokens( logsumexp(logits)^2 )          (softmax; means over routed ones)
+ * Writes loss (fp32), counts int32 [seqs, experts], and seq_stats int32 [seqs, 4] and totals int32 [2] for
+ * the backward call, which takes the same arguments with those, d_loss (fp32, on the device) and writes
+ * d_logits [tokens, experts] (rows at d_logits_stride; zeros for tokens that add nothing). Sums over tokens
+ * are taken in a fixed order. No counterpart in the reference. */
+#define DGM_BALANCE_MAX_EXPERTS 1024
+typedef struct DgmBalanceArgs {
+  const void* logits;
+  const void* topk_idx;
+  const int32_t* cu_seqlens;
+  float* loss;
+  int32_t* counts;
+  int32_t* seq_stats;
+  int32_t* totals;
+  const float* d_loss;
+  void* d_logits;
+  void* workspace; /* forward, of this call until it has run */
+  int64_t workspace_bytes;
+  int64_t tokens, logits_stride, idx_stride, d_logits_stride;
+  int32_t experts, topk, seqs;
+  int32_t dtype;
+  int32_t idx_i64;
+  int32_t score;
+  float balance_coef, z_coef;
+} DgmBalanceArgs;
+int64_t dgm_router_balance_workspace_bytes(int64_t tokens, int seqs, int experts);
+int dgm_router_balance_loss(const DgmBalanceArgs* args, hipStream_t stream);
+int dgm_router_balance_loss_backward(const DgmBalanceArgs* args, hipStream_t stream);
+int dgm_balance_struct_size(size_t* args);
+
 #ifdef __cplusplus
 }
 #endif
