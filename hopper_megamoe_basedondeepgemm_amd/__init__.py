@@ -20,6 +20,7 @@ from .utils import per_token_cast_to_fp4, per_token_cast_to_fp8, ceil_div, align
 from .balance import router_balance_loss, router_balance_loss_backward, router_balance_loss_forward
 from .int8_gemm import int8_gemm_nt
 from .norm import rms_norm_residual, rms_norm_residual_backward, rms_norm_residual_forward
+from .block import mega_moe_block
 from . import checkpoint
 from .checkpoint import (mxfp4_checkpoint_to_mega_moe, nvfp4_checkpoint_to_mega_moe, mega_moe_to_mxfp4_checkpoint,
                          mega_moe_to_nvfp4_checkpoint, untransform_mxfp4_weights_for_mega_moe_fused,
@@ -44,5 +45,5 @@ __all__ = [
     "untransform_nvfp4_weights_for_mega_moe_fused", "fable_frontend_stamps", "get_nvfp4_mega_moe_sm90_block_n",
     "get_nvfp4_mega_moe_sm90_weight_layout",
     "router_balance_loss", "router_balance_loss_forward", "router_balance_loss_backward",
-    "int8_gemm_nt", "rms_norm_residual", "rms_norm_residual_forward", "rms_norm_residual_backward",
+    "mega_moe_block", "int8_gemm_nt", "rms_norm_residual", "rms_norm_residual_forward", "rms_norm_residual_backward",
 ]

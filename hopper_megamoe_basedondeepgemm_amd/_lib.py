@@ -265,6 +265,12 @@ def no_graph_under_capture():
                            "*_backward call")
 
 
+def no_second_derivative():
+    """In a backward pass: refuses create_graph=True (the gradients are not differentiable themselves)."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("this operator has no second derivative (create_graph=True)")
+
+
 def host_device_pointer(t):
     """Device address of a pinned host tensor (for words the kernels write and the host reads)."""
     assert t.is_pinned()

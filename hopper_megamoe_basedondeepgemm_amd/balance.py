@@ -60,9 +60,20 @@ def _forward(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score):
     lib = _lib.load()
     need = lib.dgm_router_balance_workspace_bytes(logits.size(0), seqs, E)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    args = _args(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score, counts, stats, stats[4 * seqs:], loss, ws)
+    args = _args(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score, counts, stats, stats[-4:], loss, ws)
     _lib.check(lib.dgm_router_balance_loss(ctypes.byref(args), _lib.stream()))
     return loss, counts, stats
+
+
+def _backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, balance_coef, z_coef, score):
+    """The launch of the backward pass, after the checks."""
+    logits, topk_idx = _rows(logits), _rows(topk_idx)
+    cu_seqlens = None if cu_seqlens is None else cu_seqlens.contiguous()
+    d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    args = _args(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score, counts, stats, stats[-4:], d_loss=d_loss,
+                 d_logits=d_logits)
+    _lib.check(_lib.load().dgm_router_balance_loss_backward(ctypes.byref(args), _lib.stream()))
+    return d_logits
 
 
 class _RouterBalanceLoss(torch.autograd.Function):
@@ -75,12 +86,10 @@ class _RouterBalanceLoss(torch.autograd.Function):
         return loss, counts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_loss, _):
+        _lib.no_second_derivative()
         logits, topk_idx, cu_seqlens, counts, stats = ctx.saved_tensors
-        balance_coef, z_coef, score = ctx.options
-        return (router_balance_loss_backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, balance_coef, z_coef, score),
-                None, None, None, None, None)
+        return _backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, *ctx.options), None, None, None, None, None
 
 
 def router_balance_loss(logits, topk_idx, cu_seqlens=None, balance_coef=1.0, z_coef=0.0, score="softmax"):
@@ -110,8 +119,7 @@ def router_balance_loss_forward(logits, topk_idx, cu_seqlens=None, balance_coef=
     """``router_balance_loss`` with what its explicit backward call needs: ``(loss, counts, stats)``. Records
     no autograd graph."""
     _check(logits, topk_idx, cu_seqlens, score, z_coef)
-    with torch.no_grad():
-        return _forward(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score)
+    return _forward(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score)
 
 
 def router_balance_loss_backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens=None, balance_coef=1.0, z_coef=0.0,
@@ -126,14 +134,7 @@ def router_balance_loss_backward(d_loss, logits, topk_idx, counts, stats, cu_seq
             or not stats.is_contiguous()):
         raise TypeError("d_loss fp32 scalar, counts and stats of router_balance_loss_forward expected")
     _lib.require_one_device(logits, d_loss, counts, stats)
-    with torch.no_grad():
-        logits, topk_idx = _rows(logits), _rows(topk_idx)
-        cu_seqlens = None if cu_seqlens is None else cu_seqlens.contiguous()
-        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        args = _args(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score, counts, stats, stats[4 * seqs:], d_loss=d_loss,
-                     d_logits=d_logits)
-        _lib.check(_lib.load().dgm_router_balance_loss_backward(ctypes.byref(args), _lib.stream()))
-    return d_logits
+    return _backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, balance_coef, z_coef, score)
 
 
 __all__ = ["router_balance_loss", "router_balance_loss_forward", "router_balance_loss_backward"]

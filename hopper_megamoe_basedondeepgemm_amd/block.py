@@ -1,0 +1,54 @@
+"""A decoder block's feed-forward half around the MoE layer, on the GPU (no counterpart in the reference,
+whose calls start at the router and end at the combine)."""
+import torch
+
+from .int8_gemm import int8_gemm_nt
+from .mega import mxfp4_mega_moe_from_bf16
+from .norm import rms_norm_residual
+from .quantization_qoq_fused import per_token_cast_to_int8
+
+
+def mega_moe_block(x, norm_weight, router_weight, l1, l2, sym_buffer, residual=None, shared_expert=None, post_weight=None,
+                   gate=None, gate_sigmoid=False, residual_scale=1.0, next_weight=None, eps=1e-6,
+                   cumulative_local_expert_recv_stats=None, activation_clamp=10.0, **layer):
+    """Norm, MoE layer with an optional dense expert beside it, and the way back into the residual stream:
+
+        s, h  = rms_norm_residual(x, residual, pre_weight=norm_weight)       (s = residual + x, or x)
+        y     = mxfp4_mega_moe_from_bf16(h, ...) on ``sym_buffer`` (its other options through ``layer``)
+        y    += down(swiglu(gate_up(h)))                                      (shared_expert)
+        return rms_norm_residual(y, s, post_weight, next_weight, gate, gate_sigmoid, residual_scale)
+
+    x, residual: bf16 [tokens, hidden] (the block before's output and the residual stream it is added to).
+    ``shared_expert = ((int8 [2 I, hidden], scales), (int8 [hidden, I], scales))``: gate rows then up rows, and
+    down, each as ``per_token_cast_to_int8`` packs bf16 weights (one scale per channel, I a multiple of
+    128); its products are int8 (``int8_gemm_nt``) on the rows that the first norm writes beside h and on
+    the cast of the SwiGLU output, and the down product adds to the experts' output in fp32, rounded once.
+    Returns ``(r, h)``: the new residual stream and, with ``next_weight``, the next norm's output (else
+    None). Inference only: under autograd it raises."""
+    weights = () if shared_expert is None else tuple(t for pair in shared_expert for t in pair)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, residual, norm_weight, router_weight, post_weight, gate, next_weight)):
+        raise RuntimeError("mega_moe_block has no gradient: call it under torch.no_grad()")
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.size(1) != sym_buffer.hidden:
+        raise TypeError(f"x must be bf16 [tokens, {sym_buffer.hidden}], got {x.dtype} {tuple(x.shape)}")
+    if weights:
+        inner = weights[2].size(1)
+        if weights[0].size(0) != 2 * inner or inner % 128:
+            raise ValueError(f"shared_expert: gate and up rows [2 I, hidden] for down [hidden, I], I a multiple of 128; got "
+                             f"{tuple(weights[0].shape)} and {tuple(weights[2].shape)}")
+    with torch.no_grad():
+        if weights:
+            s, h, rows = rms_norm_residual(x, residual, pre_weight=norm_weight, eps=eps, quant="int8")
+        else:
+            s, h = rms_norm_residual(x, residual, pre_weight=norm_weight, eps=eps)
+        y = torch.empty_like(h)
+        mxfp4_mega_moe_from_bf16(y, h, router_weight, l1, l2, sym_buffer, cumulative_local_expert_recv_stats,
+                                 activation_clamp, **layer)
+        if weights and x.size(0):
+            act = torch.empty((x.size(0), inner), dtype=torch.bfloat16, device=x.device)
+            int8_gemm_nt(rows, shared_expert[0], act, activation="swiglu", activation_clamp=activation_clamp)
+            int8_gemm_nt(per_token_cast_to_int8(act), shared_expert[1], y, c=y)
+        return rms_norm_residual(y, s, post_weight, next_weight, gate, gate_sigmoid, residual_scale, eps)
+
+
+__all__ = ["mega_moe_block"]

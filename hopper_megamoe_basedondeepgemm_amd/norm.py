@@ -128,6 +128,38 @@ def _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_
     return x if same else r_out, h, q, sf, rstd_post, rstd_pre
 
 
+def _backward(d_r, d_h, x, residual, rstd_post, rstd_pre, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps,
+              needs):
+    """The launches of the backward pass, after the checks."""
+    T, H = x.shape
+    x = _rows(x)
+    residual = None if residual is None else _rows(residual)
+    d_r = None if d_r is None else _rows(d_r)
+    d_h = None if d_h is None else _rows(d_h)
+    post_weight = None if post_weight is None else post_weight.contiguous()
+    pre_weight = None if pre_weight is None else pre_weight.contiguous()
+    mode = GATE_NONE
+    if gate is not None:
+        mode = _gate_mode(gate, T, H)
+        gate = _rows(gate) if mode == GATE_FULL else gate.contiguous() if mode == GATE_CHANNEL else gate
+    new = lambda t, need: torch.empty(t.shape, dtype=t.dtype, device=t.device) if need and t is not None else None
+    d_x, d_residual, d_post, d_pre, d_gate = (new(t, n) for t, n in zip((x, residual, post_weight, pre_weight, gate),
+                                                                        needs))
+    lib = _lib.load()
+    ws = None
+    if d_post is not None or d_pre is not None or (d_gate is not None and mode == GATE_CHANNEL):
+        ws = torch.empty((3, lib.dgm_rms_norm_residual_groups(T, H), H), dtype=torch.float32, device=x.device)
+    fwd = _forward_args(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, mode, None, None,
+                        None, None, rstd_post, rstd_pre)
+    p = lambda t: 0 if t is None else t.data_ptr()
+    s = lambda t: 0 if t is None else t.stride(0)
+    args = _lib.NormGradArgs(fwd, p(d_r), p(d_h), p(d_x), p(d_residual), p(d_gate), p(d_post), p(d_pre), p(ws),
+                             0 if ws is None else ws.nbytes, s(d_r), s(d_h), s(d_x), s(d_residual),
+                             s(d_gate) if mode in (GATE_TOKEN, GATE_FULL) else 0)
+    _lib.check(lib.dgm_rms_norm_residual_backward(ctypes.byref(args), _lib.stream()))
+    return d_x, d_residual, d_post, d_pre, d_gate
+
+
 class _RmsNormResidual(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps):
@@ -139,14 +171,11 @@ class _RmsNormResidual(torch.autograd.Function):
         return (None if r is x else r), h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_r, d_h):
+        _lib.no_second_derivative()
         x, residual, post_weight, pre_weight, gate, rstd_post, rstd_pre = ctx.saved_tensors
-        gate_sigmoid, residual_scale, eps = ctx.options
-        grads = rms_norm_residual_backward(d_r, d_h, x, residual, rstd_post, rstd_pre, post_weight=post_weight,
-                                           pre_weight=pre_weight, gate=gate, gate_sigmoid=gate_sigmoid,
-                                           residual_scale=residual_scale, eps=eps, needs=ctx.needs_input_grad[:5])
-        return (*grads, None, None, None)
+        return (*_backward(d_r, d_h, x, residual, rstd_post, rstd_pre, post_weight, pre_weight, gate, *ctx.options,
+                           ctx.needs_input_grad), None, None, None)
 
 
 def rms_norm_residual(x, residual=None, post_weight=None, pre_weight=None, gate=None, gate_sigmoid=False,
@@ -190,9 +219,8 @@ def rms_norm_residual_forward(x, residual=None, post_weight=None, pre_weight=Non
     (fp32 [tokens] each, None without that norm). Records no autograd graph."""
     _check(x, residual, post_weight, pre_weight, gate)
     _lib.require_one_device(x, residual, post_weight, pre_weight, gate)
-    with torch.no_grad():
-        r, h, _, _, rstd_post, rstd_pre = _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid,
-                                                   residual_scale, eps, None, None, None, True)
+    r, h, _, _, rstd_post, rstd_pre = _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps,
+                                               None, None, None, True)
     return r, h, rstd_post, rstd_pre
 
 
@@ -215,33 +243,8 @@ def rms_norm_residual_backward(d_r, d_h, x, residual, rstd_post, rstd_pre, post_
                               or not rstd.is_contiguous()):
             raise ValueError("rstd rows of rms_norm_residual_forward (fp32 [tokens]) expected")
     _lib.require_one_device(x, d_r, d_h, residual, post_weight, pre_weight, gate, rstd_post, rstd_pre)
-    with torch.no_grad():
-        x = _rows(x)
-        residual = None if residual is None else _rows(residual)
-        d_r = None if d_r is None else _rows(d_r)
-        d_h = None if d_h is None else _rows(d_h)
-        post_weight = None if post_weight is None else post_weight.contiguous()
-        pre_weight = None if pre_weight is None else pre_weight.contiguous()
-        mode = GATE_NONE
-        if gate is not None:
-            mode = _gate_mode(gate, T, H)
-            gate = _rows(gate) if mode == GATE_FULL else gate.contiguous() if mode == GATE_CHANNEL else gate
-        new = lambda t, need: torch.empty(t.shape, dtype=t.dtype, device=t.device) if need and t is not None else None
-        d_x, d_residual, d_post, d_pre, d_gate = (new(t, n) for t, n in zip((x, residual, post_weight, pre_weight, gate),
-                                                                            needs))
-        lib = _lib.load()
-        ws = None
-        if d_post is not None or d_pre is not None or (d_gate is not None and mode == GATE_CHANNEL):
-            ws = torch.empty((3, lib.dgm_rms_norm_residual_groups(T, H), H), dtype=torch.float32, device=x.device)
-        fwd = _forward_args(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, mode, None, None,
-                            None, None, rstd_post, rstd_pre)
-        p = lambda t: 0 if t is None else t.data_ptr()
-        s = lambda t: 0 if t is None else t.stride(0)
-        args = _lib.NormGradArgs(fwd, p(d_r), p(d_h), p(d_x), p(d_residual), p(d_gate), p(d_post), p(d_pre), p(ws),
-                                 0 if ws is None else ws.nbytes, s(d_r), s(d_h), s(d_x), s(d_residual),
-                                 s(d_gate) if mode in (GATE_TOKEN, GATE_FULL) else 0)
-        _lib.check(lib.dgm_rms_norm_residual_backward(ctypes.byref(args), _lib.stream()))
-    return d_x, d_residual, d_post, d_pre, d_gate
+    return _backward(d_r, d_h, x, residual, rstd_post, rstd_pre, post_weight, pre_weight, gate, gate_sigmoid, residual_scale,
+                     eps, needs)
 
 
 __all__ = ["rms_norm_residual", "rms_norm_residual_forward", "rms_norm_residual_backward"]
