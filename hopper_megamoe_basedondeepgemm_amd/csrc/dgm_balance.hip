@@ -19,7 +19,7 @@ using namespace dgm;
 
 namespace {
 
-constexpr int WAVES = 4;                 // of a workgroup over tokens
+constexpr int WAVES = 16;                // of a workgroup over tokens
 
 // Row of the workspace: per slot E floats of p sums, E counts; then per slot lse^2 sum and n.
 struct Slots {
@@ -64,13 +64,17 @@ DGM_DEV int64_t seq_begin(const DgmBalanceArgs& P, int b) {
   const int64_t v = P.cu_seqlens[b];
   return v < 0 ? 0 : v > P.tokens ? P.tokens : v;
 }
-// the first sequence that ends behind token t (seqs if none)
+// The first sequence that ends behind token t (seqs if none), by a whole wave: 64 ends are looked at a step.
 DGM_DEV int seq_of(const DgmBalanceArgs& P, int64_t t) {
+  if (!P.cu_seqlens) return t < P.tokens ? 0 : P.seqs;
+  const int lane = threadIdx.x & 63;
   int lo = 0, hi = P.seqs;
   while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (seq_begin(P, mid + 1) > t) hi = mid;
-    else lo = mid + 1;
+    const int step = (hi - lo + 63) / 64, at = lo + lane * step;
+    const uint64_t behind = __ballot(at < hi && seq_begin(P, at + 1) > t);
+    const int probes = (hi - lo + step - 1) / step, first = behind ? __builtin_ctzll(behind) : probes;
+    if (behind) hi = lo + first * step;
+    if (first > 0) lo += (first - 1) * step + 1;
   }
   return lo;
 }
@@ -82,22 +86,35 @@ DGM_DEV int slot_expert(const DgmBalanceArgs& P, int64_t t, int k) {
                               : (int64_t)reinterpret_cast<const int32_t*>(P.topk_idx)[at];
   return e >= 0 && e < P.experts ? (int)e : -1;
 }
-DGM_DEV bool token_routed(const DgmBalanceArgs& P, int64_t t, int lane) {
-  bool any = false;
-  for (int k = lane; k < P.topk; k += 64) any |= slot_expert(P, t, k) >= 0;
-  return __ballot(any) != 0;
-}
-
-// A token's probabilities (lane holds experts lane + 64 i) and its log-sum-exp (softmax; 0 where nothing is
-// left). A sum of zero (all masked) gives zeros. sig: sigmoid(l), of the sigmoid form.
-template <int T, int NE, bool SOFTMAX>
-DGM_DEV void probabilities(const DgmBalanceArgs& P, int64_t t, int lane, float* p, float* sig, float& lse) {
+// What a wave reads of a token: its logits (lane: experts lane + 64 i, -inf behind the last) and whether it
+// is routed; `hit` its lane's slot (of the first 64).
+template <int T, int NE>
+struct Token {
   float l[NE];
+  int hit;
+  DGM_DEV void load(const DgmBalanceArgs& P, int64_t t, int lane) {
+    hit = lane < P.topk ? slot_expert(P, t, lane) : -1;
 #pragma unroll
-  for (int i = 0; i < NE; ++i) {
-    const int e = lane + 64 * i;
-    l[i] = e < P.experts ? load1<T>(P.logits, t * P.logits_stride + e) : -INFINITY;
+    for (int i = 0; i < NE; ++i) {
+      const int e = lane + 64 * i;
+      l[i] = e < P.experts ? load1<T>(P.logits, t * P.logits_stride + e) : -INFINITY;
+    }
   }
+  DGM_DEV bool routed(const DgmBalanceArgs& P, int64_t t, int lane) const {
+    bool any = hit >= 0;
+    for (int k = lane + 64; k < P.topk; k += 64) any |= slot_expert(P, t, k) >= 0;
+    return __ballot(any) != 0;
+  }
+};
+
+// e^x by the hardware's exp2: within (2 + |x|) 2^-24 of the value, so a probability's error stays that of its
+// rounded fp32 exponent (a third of the instructions of expf, and these passes were bound by them).
+DGM_DEV float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+
+// A token's probabilities and its log-sum-exp (softmax; 0 where nothing is left). A sum of zero (all masked)
+// gives zeros. sig: sigmoid(l), of the sigmoid form.
+template <int NE, bool SOFTMAX>
+DGM_DEV void probabilities(const float* l, float* p, float* sig, float& lse) {
   float s = 0.f;
   lse = 0.f;
   if constexpr (SOFTMAX) {
@@ -108,7 +125,7 @@ DGM_DEV void probabilities(const DgmBalanceArgs& P, int64_t t, int lane, float* 
     const float shift = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      p[i] = expf(l[i] - shift);
+      p[i] = exp_fast(l[i] - shift);
       s += p[i];
     }
     s = wave_sum(s);
@@ -116,7 +133,7 @@ DGM_DEV void probabilities(const DgmBalanceArgs& P, int64_t t, int lane, float* 
   } else {
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      sig[i] = p[i] = 1.0f / (1.0f + expf(-l[i]));
+      sig[i] = p[i] = __builtin_amdgcn_rcpf(1.0f + exp_fast(-l[i]));
       s += p[i];
     }
     s = wave_sum(s);
@@ -135,16 +152,19 @@ DGM_DEV void sum_tokens(const DgmBalanceArgs& P, int64_t lo, int64_t hi, float (
   int n = 0;
 #pragma unroll
   for (int i = 0; i < NE; ++i) acc[i] = 0.f;
-  for (int64_t t = lo + wave; t < hi; t += W) {
-    bool any = false;
-    for (int k = lane; k < P.topk; k += 64) {
+  // (the next token is requested before the current one is worked on)
+  Token<T, NE> cur, next;
+  if (lo + wave < hi) cur.load(P, lo + wave, lane);
+  for (int64_t t = lo + wave; t < hi; t += W, cur = next) {
+    next.load(P, t + W < hi ? t + W : t, lane);
+    if (cur.hit >= 0) atomicAdd(&hist[cur.hit], 1);
+    for (int k = lane + 64; k < P.topk; k += 64) {
       const int e = slot_expert(P, t, k);
       if (e >= 0) atomicAdd(&hist[e], 1);
-      any |= e >= 0;
     }
-    if (__ballot(any) == 0) continue;
+    if (!cur.routed(P, t, lane)) continue;
     float p[NE], sig[NE], lse;
-    probabilities<T, NE, SOFTMAX>(P, t, lane, p, sig, lse);
+    probabilities<NE, SOFTMAX>(cur.l, p, sig, lse);
 #pragma unroll
     for (int i = 0; i < NE; ++i) acc[i] += p[i];
     z += lse * lse;
@@ -218,6 +238,7 @@ __global__ void __launch_bounds__(1024) k_balance_columns(const DgmBalanceArgs P
   if (hi > lo) {
     const int64_t first = lo / chunk + b, last = (hi - 1) / chunk + b;
     if (e < P.experts)
+#pragma unroll 8
       for (int64_t s = first + wave; s <= last; s += 16) {
         p += (double)S.p[s * P.experts + e];
         c += S.c[s * P.experts + e];
@@ -340,7 +361,10 @@ __global__ void __launch_bounds__(256) k_balance_grad(const DgmBalanceArgs P, in
   float f[NE], coef = 0.f;
 #pragma unroll
   for (int i = 0; i < NE; ++i) f[i] = 0.f;
-  for (int64_t t = first; t < last; ++t) {
+  Token<T, NE> cur, next;
+  cur.load(P, first, lane);
+  for (int64_t t = first; t < last; ++t, cur = next) {
+    next.load(P, t + 1 < last ? t + 1 : t, lane);
     if (t >= end) {
       do {
         ++b;
@@ -359,9 +383,9 @@ __global__ void __launch_bounds__(256) k_balance_grad(const DgmBalanceArgs P, in
       }
     }
     float d[NE];
-    if (n > 0 && t >= begin && token_routed(P, t, lane)) {
+    if (n > 0 && t >= begin && cur.routed(P, t, lane)) {
       float p[NE], sig[NE], lse, dot = 0.f;
-      probabilities<T, NE, SOFTMAX>(P, t, lane, p, sig, lse);
+      probabilities<NE, SOFTMAX>(cur.l, p, sig, lse);
 #pragma unroll
       for (int i = 0; i < NE; ++i) dot += f[i] * p[i];
       dot = wave_sum(dot);
@@ -464,8 +488,8 @@ int dgm_router_balance_loss_backward(const DgmBalanceArgs* args, hipStream_t str
   if (int st = check(A)) return st;
   if (A.tokens == 0) return 0;
   DGM_CHECK_ARG(A.d_loss && A.d_logits, "null pointer");
-  // (consecutive tokens of a wave share their sequence's f: 4096 waves, a token each at least)
-  const int64_t per = (A.tokens + 4095) / 4096;
+  // (consecutive tokens of a wave share their sequence's f: 8192 waves, a token each at least)
+  const int64_t per = (A.tokens + 8191) / 8192;
   const int64_t waves = (A.tokens + per - 1) / per;
   dispatch(A, [&](auto t, auto ne, auto softmax) {
     hipLaunchKernelGGL((k_balance_grad<t.value, ne.value, softmax.value>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0,

@@ -25,6 +25,23 @@ DGM_DEV void store1(void* p, int64_t i, float v) {
   else if constexpr (T == T_F16) reinterpret_cast<_Float16*>(p)[i] = (_Float16)v;
   else reinterpret_cast<uint16_t*>(p)[i] = f32_to_bf16(v);
 }
+// eight 16-bit elements as fp32
+template <int T>
+DGM_DEV void unpack8(u4 w, float* v) {
+  static_assert(T != T_F32, "16-bit elements");
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t d = w[k];        // (a scalar: the cast of a vector's element reads its first one)
+    if constexpr (T == T_F16) {
+      const h2 f = __builtin_bit_cast(h2, d);
+      v[2 * k] = (float)f[0];
+      v[2 * k + 1] = (float)f[1];
+    } else {
+      v[2 * k] = __uint_as_float(d << 16);
+      v[2 * k + 1] = __uint_as_float(d & 0xffff0000u);
+    }
+  }
+}
 // eight consecutive elements from element i (16-byte aligned) as fp32, and back (round to nearest even)
 template <int T>
 DGM_DEV void load8(const void* p, int64_t i, float* v) {
@@ -34,19 +51,7 @@ DGM_DEV void load8(const void* p, int64_t i, float* v) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) { v[k] = a[k]; v[4 + k] = b[k]; }
   } else {
-    const u4 w = *reinterpret_cast<const u4*>(reinterpret_cast<const uint16_t*>(p) + i);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t d = w[k];      // (a scalar: the cast of a vector's element reads its first one)
-      if constexpr (T == T_F16) {
-        const h2 f = __builtin_bit_cast(h2, d);
-        v[2 * k] = (float)f[0];
-        v[2 * k + 1] = (float)f[1];
-      } else {
-        v[2 * k] = __uint_as_float(d << 16);
-        v[2 * k + 1] = __uint_as_float(d & 0xffff0000u);
-      }
-    }
+    unpack8<T>(*reinterpret_cast<const u4*>(reinterpret_cast<const uint16_t*>(p) + i), v);
   }
 }
 template <int T>
