@@ -219,7 +219,7 @@ def load_probe():
 
 
 def check(status):
-    if status != 0:
+    if status:
         msg = load().dgm_last_error().decode(errors="replace")
         raise RuntimeError(f"dgm error {status}: {msg}")
 
@@ -247,12 +247,13 @@ def require_gpu(*tensors):
 
 def require_one_device(first, *tensors):
     """All tensors on the GPU that is current (work is enqueued on its current stream)."""
-    dev = first.device
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"MI355X path: tensors on {dev} and {t.device}")
     require_gpu(first)
-    if dev.index != torch.cuda.current_device():
+    index = first.get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f"MI355X path: tensors on {first.device} and {t.device}")
+    if index != torch.cuda.current_device():
+        dev = first.device
         raise RuntimeError(f"MI355X path: tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()}")
 
 

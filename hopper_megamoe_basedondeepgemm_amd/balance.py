@@ -28,8 +28,8 @@ def _check(logits, topk_idx, cu_seqlens, score, z_coef):
     if not 1 <= topk_idx.size(1) <= E or T * topk_idx.size(1) >= 1 << 31:
         raise ValueError(f"topk {topk_idx.size(1)}: 1 to {E}, tokens x topk below 2^31")
     if cu_seqlens is not None and (cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1
-                                   or not 2 <= cu_seqlens.size(0) <= 1 << 24):
-        raise TypeError(f"cu_seqlens must be int32 [sequences + 1], got {cu_seqlens.dtype} {tuple(cu_seqlens.shape)}")
+                                   or not 2 <= cu_seqlens.size(0) <= 1 << 21):
+        raise TypeError(f"cu_seqlens must be int32 [sequences + 1], got {cu_seqlens.dtype} {tuple(cu_seqlens.shape)} (below 2^21 sequences)")
     if score not in SCORES:
         raise ValueError(f"score {score!r}: one of {sorted(SCORES)}")
     if score == "sigmoid" and z_coef:

@@ -411,7 +411,8 @@ int check(const DgmBalanceArgs& A) {
   DGM_CHECK_ARG(A.experts >= 1 && A.experts <= DGM_BALANCE_MAX_EXPERTS, "experts 1 to 1024");
   DGM_CHECK_ARG(A.topk >= 1 && A.topk <= A.experts, "topk 1 to experts");
   DGM_CHECK_ARG(A.tokens >= 0 && A.tokens * A.topk < (int64_t)1 << 31, "tokens x topk below 2^31");
-  DGM_CHECK_ARG(A.seqs >= 1 && A.seqs < (1 << 24) && (A.cu_seqlens || A.seqs == 1), "seqs 1 to 2^24, more than one with cu_seqlens");
+  // (a launch has fewer than 2^32 threads, a sequence 1024 of them)
+  DGM_CHECK_ARG(A.seqs >= 1 && A.seqs < (1 << 21) && (A.cu_seqlens || A.seqs == 1), "seqs 1 to 2^21, more than one with cu_seqlens");
   DGM_CHECK_ARG(A.score == 0 || (A.score == 1 && A.z_coef == 0.f), "score 0 softmax, 1 sigmoid (without z_coef)");
   DGM_CHECK_ARG(A.counts && A.seq_stats && A.totals, "null pointer");
   DGM_CHECK_ARG(A.tokens == 0 || (A.logits && A.topk_idx), "null pointer");

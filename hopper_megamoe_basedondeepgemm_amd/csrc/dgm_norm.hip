@@ -362,7 +362,8 @@ bool aligned(const void* p, int64_t stride, int size) {
 
 int check_forward(const DgmNormArgs* A) {
   DGM_CHECK_ARG(A->dtype >= DGM_SRC_BF16 && A->dtype <= DGM_SRC_F32, "dtype 0 bf16, 1 fp16, 2 fp32");
-  DGM_CHECK_ARG(A->rows >= 0 && A->rows <= 0x7fffffff, "rows below 2^31");
+  // (a launch has fewer than 2^32 threads, a row up to 1024 of them)
+  DGM_CHECK_ARG(A->rows >= 0 && A->rows < (1 << 22), "rows below 2^22");
   DGM_CHECK_ARG(A->hidden > 0 && A->hidden <= DGM_NORM_MAX_HIDDEN, "hidden 1 to 16384");
   DGM_CHECK_ARG(A->gate_mode >= 0 && A->gate_mode <= GATE_FULL, "gate_mode 0 none, 1 channel, 2 token, 3 full");
   DGM_CHECK_ARG(A->eps >= 0.f, "eps >= 0");

@@ -54,6 +54,8 @@ def int8_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_m
     swiglu = activation is not None
     if swiglu and (n % 2 or c is not None):
         raise ValueError("swiglu takes a gate and an up half of b's rows, and no c")
+    if activation_clamp is not None and not activation_clamp >= 0:
+        raise ValueError(f"activation_clamp {activation_clamp}: at least 0, or None")
     if m >= 1 << 20 or n >= 1 << 24:
         raise ValueError(f"m {m} and n {n}: below 2^20 and 2^24")
     n_out = n // 2 if swiglu else n
@@ -69,6 +71,10 @@ def int8_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_m
     if m == 0 or n_out == 0:
         return d
     aq, bq = _rows(aq), _rows(bq)
+    lo, hi = d.data_ptr(), d.data_ptr() + ((m - 1) * d.stride(0) + n_out) * d.element_size()
+    pa, pb = aq.data_ptr(), bq.data_ptr()
+    if (pa < hi and lo < pa + (m - 1) * aq.stride(0) + k) or (pb < hi and lo < pb + (n - 1) * bq.stride(0) + k):
+        raise ValueError("d overlaps an operand")
     c_stride = 0
     if c is not None:
         if c.dim() == 1:
@@ -76,14 +82,13 @@ def int8_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_m
         else:
             c = _rows(c)
             c_stride = c.stride(0)
-        lo, hi = d.data_ptr(), d.data_ptr() + ((m - 1) * d.stride(0) + n_out) * d.element_size()
         end = c.data_ptr() + (n_out if c.dim() == 1 else (m - 1) * c_stride + n_out) * c.element_size()
         if c.data_ptr() < hi and lo < end and not (c.dim() == 2 and c.data_ptr() == lo and (m == 1 or c_stride == d.stride(0))):
             raise ValueError("c overlaps d other than as the same rows")
     need = _workspace_bytes(m, n, k, swiglu)
     ws = torch.empty(need, dtype=torch.uint8, device=d.device) if need else None
-    args = _lib.Int8GemmArgs(aq.data_ptr(), asf.data_ptr(), bq.data_ptr(), bsf.data_ptr(), 0 if c is None else c.data_ptr(),
-                             d.data_ptr(), m, n, k, aq.stride(0), asf.stride(0), bq.stride(0), bsf.stride(0), c_stride,
+    args = _lib.Int8GemmArgs(pa, asf.data_ptr(), pb, bsf.data_ptr(), 0 if c is None else c.data_ptr(),
+                             lo, m, n, k, aq.stride(0), asf.stride(0), bq.stride(0), bsf.stride(0), c_stride,
                              d.stride(0), _lib.SRC_DTYPES[d.dtype], int(swiglu),
                              float(activation_clamp if activation_clamp is not None else 3.0e38), int(bool(fast_math)),
                              0 if ws is None else ws.data_ptr(), need)

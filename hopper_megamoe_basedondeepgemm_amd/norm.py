@@ -8,13 +8,17 @@ import torch
 
 from . import _lib
 
-MAX_HIDDEN = 16384
+MAX_HIDDEN, MAX_TOKENS = 16384, 1 << 22
 GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
 
 
 def _rows(t):
     """t as the kernels read it: rows of contiguous elements (any row stride)."""
     return t if t.stride(1) == 1 or t.size(1) == 1 else t.contiguous()
+
+
+def _new_rows(x):
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def _gate_mode(gate, T, H):
@@ -34,6 +38,8 @@ def _check(x, residual, post_weight, pre_weight, gate, quant=None, residual_out=
     T, H = x.shape
     if not 1 <= H <= MAX_HIDDEN:
         raise ValueError(f"hidden {H}: 1 to {MAX_HIDDEN}")
+    if T >= MAX_TOKENS:
+        raise ValueError(f"tokens {T}: below {MAX_TOKENS}")
     for t in (residual, residual_out, out):
         if t is not None and (t.dtype != x.dtype or t.shape != x.shape):
             raise TypeError(f"rows of {x.dtype} {tuple(x.shape)} expected, got {t.dtype} {tuple(t.shape)}")
@@ -85,14 +91,34 @@ def _check_outputs(outs, ins):
 
 def _forward_args(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, mode, r_out, h, q, sf,
                   rstd_post, rstd_pre):
-    p = lambda t: 0 if t is None else t.data_ptr()
-    s = lambda t: 0 if t is None else t.stride(0)
+    T, H = x.shape
     w = post_weight if post_weight is not None else pre_weight
-    return _lib.NormArgs(p(x), p(residual), p(post_weight), p(pre_weight), p(gate), p(r_out), p(h), p(q), p(sf),
-                         p(rstd_post), p(rstd_pre), x.size(0), x.stride(0), s(residual),
-                         s(gate) if mode in (GATE_TOKEN, GATE_FULL) else 0, s(r_out), s(h), x.size(1),
-                         _lib.SRC_DTYPES[x.dtype], int(w is not None and w.dtype == torch.float32), mode,
-                         int(bool(gate_sigmoid)), float(residual_scale), float(eps))
+    args = _lib.NormArgs(x=x.data_ptr(), rows=T, x_stride=x.stride(0), hidden=H, dtype=_lib.SRC_DTYPES[x.dtype],
+                         residual_scale=residual_scale, eps=eps)
+    # (the fields of absent parts stay at their zero: each one set costs time on a call that the GPU finishes in 3 us)
+    if residual is not None:
+        args.residual, args.residual_stride = residual.data_ptr(), residual.stride(0)
+    if post_weight is not None:
+        args.post_weight = post_weight.data_ptr()
+    if pre_weight is not None:
+        args.pre_weight = pre_weight.data_ptr()
+    if w is not None and w.dtype == torch.float32:
+        args.weights_f32 = 1
+    if gate is not None:
+        args.gate, args.gate_mode, args.gate_sigmoid = gate.data_ptr(), mode, int(bool(gate_sigmoid))
+        if mode != GATE_CHANNEL:
+            args.gate_stride = gate.stride(0)
+    if r_out is not None:
+        args.residual_out, args.residual_out_stride = r_out.data_ptr(), r_out.stride(0)
+    if h is not None:
+        args.h, args.h_stride = h.data_ptr(), h.stride(0)
+    if q is not None:
+        args.q, args.q_sf = q.data_ptr(), sf.data_ptr()
+    if rstd_post is not None:
+        args.rstd_post = rstd_post.data_ptr()
+    if rstd_pre is not None:
+        args.rstd_pre = rstd_pre.data_ptr()
+    return args
 
 
 def _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, quant, residual_out, out, keep):
@@ -100,16 +126,17 @@ def _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_
     T, H = x.shape
     x = _rows(x)
     residual = None if residual is None else _rows(residual)
-    post_weight = None if post_weight is None else post_weight.contiguous()
-    pre_weight = None if pre_weight is None else pre_weight.contiguous()
+    if post_weight is not None and post_weight.stride(0) != 1:
+        post_weight = post_weight.contiguous()
+    if pre_weight is not None and pre_weight.stride(0) != 1:
+        pre_weight = pre_weight.contiguous()
     mode = GATE_NONE
     if gate is not None:
         mode = _gate_mode(gate, T, H)
         gate = _rows(gate) if mode == GATE_FULL else gate.contiguous() if mode == GATE_CHANNEL else gate
     same = residual is None and post_weight is None and gate is None and residual_scale == 1.0 and residual_out is None
-    new = lambda: torch.empty((T, H), dtype=x.dtype, device=x.device)
-    r_out = None if same else residual_out if residual_out is not None else new()
-    h = None if pre_weight is None else out if out is not None else new()
+    r_out = None if same else residual_out if residual_out is not None else _new_rows(x)
+    h = None if pre_weight is None else out if out is not None else _new_rows(x)
     q = sf = rstd_post = rstd_pre = None
     if quant:
         q = torch.empty((T, H), dtype=torch.int8, device=x.device)
@@ -187,7 +214,7 @@ def rms_norm_residual(x, residual=None, post_weight=None, pre_weight=None, gate=
         r = residual + residual_scale * a * n             (a = gate, or sigmoid(gate) with gate_sigmoid)
         h = r / sqrt(mean(r^2) + eps) * pre_weight
 
-    x, residual: bf16, fp16 or fp32 [tokens, hidden <= 16384], any row stride; norm weights [hidden] of
+    x, residual: bf16, fp16 or fp32 [tokens < 2^22, hidden <= 16384], any row stride; norm weights [hidden] of
     that type or fp32; gate [hidden], [tokens, 1] or [tokens, hidden]. Every part but x may be absent.
     Arithmetic in fp32 (the squares of a row have to add up below 3.4e38); r enters the second norm
     unrounded. Returns ``(r, h)``, h None without pre_weight, r x itself where nothing changes it; with
@@ -200,8 +227,10 @@ def rms_norm_residual(x, residual=None, post_weight=None, pre_weight=None, gate=
     current stream of the tensors' device, which has to be the current one."""
     _check(x, residual, post_weight, pre_weight, gate, quant, residual_out, out)
     _lib.require_one_device(x, residual, post_weight, pre_weight, gate, residual_out, out)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, residual, post_weight, pre_weight, gate)):
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)
+                                    or (post_weight is not None and post_weight.requires_grad)
+                                    or (pre_weight is not None and pre_weight.requires_grad)
+                                    or (gate is not None and gate.requires_grad)):
         _lib.no_graph_under_capture()
         if quant or residual_out is not None or out is not None:
             raise ValueError("quant, residual_out and out have no gradient: call under torch.no_grad()")

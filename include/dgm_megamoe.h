@@ -380,7 +380,7 @@ int dgm_fused_last_form(int hidden, int intermediate, int act_format);
  *   n = x rsqrt(mean x^2 + eps) post_weight (n = x without post_weight), a = gate or sigmoid(gate),
  *   t = residual + residual_scale a n, h = t rsqrt(mean t^2 + eps) pre_weight.
  * All arithmetic in fp32 (a row's squares have to add up below 3.4e38), t unrounded into the second
- * norm. Rows of `hidden` (1 to 16384) contiguous elements of type dtype (DGM_SRC_*) at row strides in
+ * norm. Fewer than 2^22 rows of `hidden` (1 to 16384) contiguous elements of type dtype (DGM_SRC_*) at row strides in
  * elements; norm weights of that type or fp32. NULL: no such part (residual, post_weight, pre_weight,
  * gate) or output (residual_out, h, rstd_*, q). gate_mode 1: gate [hidden], 2: [rows] at gate_stride,
  * 3: [rows, hidden]. residual_out may be residual, or x, at the same stride; h may be x. q / q_sf (bf16 rows): int8
@@ -466,7 +466,7 @@ int dgm_int8_gemm_struct_size(size_t* args);
 /* The router's balance loss over logits [tokens, experts] (rows at logits_stride, type DGM_SRC_*) and the
  * chosen experts topk_idx [tokens, topk] (rows at idx_stride; int64 or int32; ids outside [0, experts) are
  * no slot, a token without a slot is unrouted and adds nothing). Sequences: tokens [cu_seqlens[b],
- * cu_seqlens[b + 1]), ascending (int32 [seqs + 1]); NULL: one of all tokens; tokens of none add nothing.
+ * cu_seqlens[b + 1]), ascending (int32 [seqs + 1], seqs below 2^21); NULL: one of all tokens; tokens of none add nothing.
  * Per sequence with n routed tokens, count_e slots of expert e and p = softmax(logits) or (score 1)
  * sigmoid / sum of sigmoids:
  *   loss = balance_coef mean_sequences( experts sum_e count_e / sum(count) mean_tokens p_e )

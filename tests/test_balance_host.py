@@ -28,6 +28,7 @@ def test_struct_size():
     ((torch.zeros(4, 8), idx(4, 0)), {}, ValueError, "topk 0"),
     ((torch.zeros(4, 8), idx(4, 2), torch.tensor([0, 4])), {}, TypeError, "cu_seqlens must be"),
     ((torch.zeros(4, 8), idx(4, 2), torch.tensor([0], dtype=torch.int32)), {}, TypeError, "cu_seqlens must be"),
+    ((torch.zeros(4, 8), idx(4, 2), torch.zeros((1 << 21) + 1, dtype=torch.int32)), {}, TypeError, "cu_seqlens must be"),
     ((torch.zeros(4, 8), idx(4, 2)), dict(score="tanh"), ValueError, "score"),
     ((torch.zeros(4, 8), idx(4, 2)), dict(score="sigmoid", z_coef=0.1), ValueError, "z_coef"),
     ((torch.zeros(4, 8), idx(4, 2)), {}, RuntimeError, "GPU"),
@@ -43,7 +44,7 @@ def test_c_entry_refusals():
                 experts=8, topk=2, seqs=1, dtype=2, idx_i64=1)
     for kw, what in ((dict(dtype=3), b"dtype"), (dict(experts=0), b"experts"), (dict(experts=1025), b"experts"),
                      (dict(topk=9), b"topk"), (dict(topk=0), b"topk"), (dict(tokens=-1), b"tokens"),
-                     (dict(tokens=1 << 30), b"tokens"), (dict(seqs=0), b"seqs"), (dict(seqs=2), b"seqs"),
+                     (dict(tokens=1 << 30), b"tokens"), (dict(seqs=0), b"seqs"), (dict(seqs=2), b"seqs"), (dict(seqs=1 << 21, cu_seqlens=p), b"seqs"),
                      (dict(score=2), b"score"), (dict(score=1, z_coef=0.5), b"score"), (dict(counts=None), b"null"),
                      (dict(logits=None), b"null"), (dict(loss=None), b"null loss"), ({}, b"workspace"),
                      (dict(workspace=p, workspace_bytes=lib.dgm_router_balance_workspace_bytes(1000, 1, 8) - 1), b"workspace"),

@@ -143,6 +143,9 @@ def test_strides_and_alignment(m):
     bigd = torch.empty((m + 1, n), device="cuda")
     with pytest.raises(ValueError, match="c overlaps d"):
         dgm.int8_gemm_nt(a, b, bigd[:m], c=bigd[1:])
+    raw = torch.zeros(m * k + m * n * 4, dtype=torch.int8, device="cuda")
+    with pytest.raises(ValueError, match="d overlaps an operand"):
+        dgm.int8_gemm_nt((raw[:m * k].view(m, k), a[1]), b, raw[m * k - 16:m * k - 16 + m * n * 2].view(torch.bfloat16).view(m, n))
     dgm.int8_gemm_nt((a[0][:0], a[1][:0]), b, d[:0])
     dgm.int8_gemm_nt(a, (b[0][:0], b[1][:0]), d[:, :0])
 

@@ -38,6 +38,8 @@ def test_struct_size():
     (rows(4, 32), rows(8, 32), bf(4, 8), dict(activation="gelu"), ValueError, "activation"),
     (rows(4, 32), rows(7, 32), bf(4, 3), dict(activation="swiglu"), ValueError, "swiglu"),
     (rows(4, 32), rows(8, 32), bf(4, 4), dict(activation="swiglu", c=bf(4, 4)), ValueError, "swiglu"),
+    (rows(4, 32), rows(8, 32), bf(4, 4), dict(activation="swiglu", activation_clamp=-1.0), ValueError, "activation_clamp"),
+    (rows(4, 32), rows(8, 32), bf(4, 4), dict(activation="swiglu", activation_clamp=float("nan")), ValueError, "activation_clamp"),
     (rows(4, 32), rows(8, 32), bf(4, 8), {}, RuntimeError, "GPU"),
 ])
 def test_refusals(a, b, d, kw, err, what):

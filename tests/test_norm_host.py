@@ -23,6 +23,7 @@ def test_struct_sizes():
     (dict(x=torch.zeros(4, 8, dtype=torch.int8)), TypeError, "bf16, fp16 or fp32"),
     (dict(x=bf(1, 16385)), ValueError, "hidden 16385"),
     (dict(x=bf(4, 0)), ValueError, "hidden 0"),
+    (dict(x=bf(1, 1).expand(1 << 22, 1)), ValueError, "tokens 4194304"),
     (dict(x=bf(4, 8), residual=bf(4, 9)), TypeError, "rows of"),
     (dict(x=bf(4, 8), residual=torch.zeros(4, 8)), TypeError, "rows of"),
     (dict(x=bf(4, 8), pre_weight=bf(9)), TypeError, "norm weights"),
@@ -61,7 +62,7 @@ def test_c_entry_refusals():
     lib, p = _lib.load(), 4096          # (never dereferenced: refused first)
     base = dict(x=p, h=p, pre_weight=p, rows=4, hidden=64, x_stride=64, h_stride=64, residual_scale=1.0, eps=1e-6)
     for kw, what in ((dict(dtype=3), b"dtype"), (dict(hidden=0), b"hidden"), (dict(hidden=16385), b"hidden"),
-                     (dict(rows=-1), b"rows"), (dict(gate_mode=4), b"gate_mode"), (dict(gate_mode=1), b"gate and gate_mode"),
+                     (dict(rows=-1), b"rows"), (dict(rows=1 << 22), b"rows"), (dict(gate_mode=4), b"gate_mode"), (dict(gate_mode=1), b"gate and gate_mode"),
                      (dict(x=None), b"null x"), (dict(eps=-1.0), b"eps"), (dict(q=p), b"int8 rows"),
                      (dict(q=p, q_sf=p, dtype=2), b"int8 rows")):
         st = lib.dgm_rms_norm_residual(ctypes.byref(_lib.NormArgs(**{**base, **kw})), None)
