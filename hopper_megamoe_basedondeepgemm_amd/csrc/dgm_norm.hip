@@ -334,23 +334,25 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
   if (P.d_gate && F.gate_mode == GATE_CHANNEL) R::template store<T_F32>(P.workspace, 2 * set + off, H, dg);
 }
 
-// Column sums of partial[G][H]: a workgroup takes 64 columns, its wave i rows i, i + W, ...
-template <int T>
+// Column sums of partial[G][H]: a workgroup takes C columns, its thread groups of C the rows in turn.
+template <int T, int C>
 __global__ void __launch_bounds__(1024) k_norm_columns(const DgmNormGradArgs P, int groups) {
   const DgmNormArgs& F = P.forward;
-  __shared__ float lds[16][64];
-  const int H = F.hidden, col = blockIdx.x * 64 + (threadIdx.x & 63), wv = threadIdx.x >> 6, set = blockIdx.y;
+  constexpr int R = 1024 / C;
+  __shared__ float lds[R][C];
+  const int H = F.hidden, c = threadIdx.x % C, r = threadIdx.x / C, col = blockIdx.x * C + c, set = blockIdx.y;
   void* out = set == 0 ? P.d_pre_weight : set == 1 ? P.d_post_weight : F.gate_mode == GATE_CHANNEL ? P.d_gate : nullptr;
   if (!out) return;                               // (the whole workgroup)
   const float* src = (const float*)P.workspace + (int64_t)set * groups * H;
   float s = 0.f;
   if (col < H)
 #pragma unroll 8
-    for (int i = wv; i < groups; i += 16) s += src[(int64_t)i * H + col];
-  lds[wv][threadIdx.x & 63] = s;
+    for (int i = r; i < groups; i += R) s += src[(int64_t)i * H + col];
+  lds[r][c] = s;
   __syncthreads();
-  if (wv == 0 && col < H) {
-    for (int i = 1; i < 16; ++i) s += lds[i][threadIdx.x];
+  if (r == 0 && col < H) {
+#pragma unroll 8
+    for (int i = 1; i < R; ++i) s += lds[i][c];
     if (set < 2 && F.weights_f32) store1<T_F32>(out, col, s);
     else store1<T>(out, col, s);
   }
@@ -433,9 +435,11 @@ int dgm_rms_norm_residual(const DgmNormArgs* args, hipStream_t stream) {
   return dgm_last_launch_status();
 }
 
+// As many workgroups as the CUs hold (16 waves each), a row each at least: 32768 x 512 with 512 of them
+// took 174 us, 4096 x 7168 103 us.
 int dgm_rms_norm_residual_groups(int64_t rows, int hidden) {
-  (void)hidden;
-  const int64_t most = 512;
+  int64_t most = 4096;
+  dispatch_hidden(hidden, [&](auto, auto threads) { most = 4096 / (threads.value / 64); });
   return (int)(rows < 1 ? 1 : rows < most ? rows : most);
 }
 
@@ -468,8 +472,13 @@ int dgm_rms_norm_residual_backward(const DgmNormGradArgs* args, hipStream_t stre
       hipLaunchKernelGGL((k_norm_bwd<t.value, nv.value, threads.value, v.value>), dim3(groups), dim3(threads.value), 0,
                          stream, A);
     });
-    if (columns)
-      hipLaunchKernelGGL((k_norm_columns<t.value>), dim3((F.hidden + 63) / 64, 3), dim3(1024), 0, stream, A, groups);
+    if (columns) {
+      // (narrow rows have many groups: 16 columns a workgroup, so that there are enough of them)
+      if (groups > 1024)
+        hipLaunchKernelGGL((k_norm_columns<t.value, 16>), dim3((F.hidden + 15) / 16, 3), dim3(1024), 0, stream, A, groups);
+      else
+        hipLaunchKernelGGL((k_norm_columns<t.value, 64>), dim3((F.hidden + 63) / 64, 3), dim3(1024), 0, stream, A, groups);
+    }
   });
   return dgm_last_launch_status();
 }
