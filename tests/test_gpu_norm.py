@@ -110,7 +110,8 @@ def check_forward(x, r, w1, w2, gt, sigmoid, s, got_r, got_h):
 
 
 SHAPES = [(1, 1), (1, 8), (3, 7), (5, 64), (2, 100), (4, 512), (3, 513), (9, 1024), (2, 1032), (7, 2880), (2, 4096), (1, 4104),
-          (3, 8192), (2, 8200), (2, 12345), (1, 16384)]
+          (3, 8192), (2, 8200), (2, 12345), (1, 16384),
+          (300, 512), (257, 1000), (300, 2048), (258, 2880), (260, 7168), (257, 9000), (300, 33)]
 
 
 @pytest.mark.parametrize("T,H", SHAPES)
