@@ -7,8 +7,9 @@
 //   dl_te = alpha / (B' n_b) p_te (f_be - sum_j f_bj p_tj) (sigmoid: times 1 - sigmoid(l_te)) + 2 beta / N lse_t p_te
 // An expert masked with -inf has p = 0; a row of nothing else adds to the counts alone.
 //
-// A wave takes a token, its lanes the experts (up to 16 each); all passes read the logits once, so the bound
-// is HBM. Sums over tokens: a workgroup's waves add their tokens of one sequence in registers and leave one
+// Sixteen lanes take a token, in 16-byte pieces of its row (a whole wave per token spent most of its time on
+// the reductions and the scalar work of a token: 65536 x 256 bf16 76 us for loss and gradient, now 50); all
+// passes read the logits once, so the bound is HBM. Sums over tokens: a workgroup's waves add their tokens of one sequence in registers and leave one
 // row of sums per (chunk, sequence) at slot chunk + sequence (a walk that takes one step per slot, so slots
 // are distinct), which k_balance_columns adds up in a fixed order: no atomics on floats, no cleared memory.
 #include "dgm_common.hpp"
@@ -19,7 +20,8 @@ using namespace dgm;
 
 namespace {
 
-constexpr int WAVES = 16;                // of a workgroup over tokens
+// Waves of a workgroup over tokens: 16 while a lane's values fit the registers that this leaves (128).
+__host__ __device__ constexpr int waves_for(int values) { return values <= 24 ? 16 : 8; }
 
 // Row of the workspace: per slot E floats of p sums, E counts; then per slot lse^2 sum and n.
 struct Slots {
@@ -53,10 +55,10 @@ __host__ __device__ inline Slots slots_of(void* ws, int64_t slots, int seqs, int
   return s;
 }
 
-// Tokens of a chunk: about 512 chunks, 16 tokens at least.
+// Tokens of a chunk: whole rounds of a workgroup's waves (64 tokens), up to 512 chunks.
 __host__ __device__ inline int64_t chunk_tokens(int64_t tokens) {
-  const int64_t c = (tokens + 511) / 512;
-  return c < 16 ? 16 : c;
+  const int64_t c = (tokens + 64 * 512 - 1) / (64 * 512) * 64;
+  return c < 64 ? 64 : c;
 }
 
 DGM_DEV int64_t seq_begin(const DgmBalanceArgs& P, int b) {
@@ -86,102 +88,146 @@ DGM_DEV int slot_expert(const DgmBalanceArgs& P, int64_t t, int k) {
                               : (int64_t)reinterpret_cast<const int32_t*>(P.topk_idx)[at];
   return e >= 0 && e < P.experts ? (int)e : -1;
 }
-// What a wave reads of a token: its logits (lane: experts lane + 64 i, -inf behind the last) and whether it
-// is routed; `hit` its lane's slot (of the first 64).
-template <int T, int NE>
+// What sixteen lanes read of a token: its logits (-inf behind the last expert) and its slots; `hit` is the
+// lane's (of the first 16). VEC: rows of whole, aligned 16-byte pieces.
+template <int T, int NV, bool VEC>
 struct Token {
-  float l[NE];
+  static constexpr int V = T == T_F32 ? 4 : 8;             // experts of a piece
+  float l[NV];
   int hit;
-  DGM_DEV void load(const DgmBalanceArgs& P, int64_t t, int lane) {
-    hit = lane < P.topk ? slot_expert(P, t, lane) : -1;
+  static DGM_DEV int expert(int i) { return (i / V) * 16 * V + (int)(threadIdx.x & 15) * V + i % V; }
+  DGM_DEV void load(const DgmBalanceArgs& P, int64_t t) {
+    const int sub = threadIdx.x & 15;
+    hit = sub < P.topk ? slot_expert(P, t, sub) : -1;
+    const int64_t row = t * P.logits_stride;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      const int e = lane + 64 * i;
-      l[i] = e < P.experts ? load1<T>(P.logits, t * P.logits_stride + e) : -INFINITY;
+    for (int c = 0; c < NV; c += V) {
+      if constexpr (VEC) {
+        if (expert(c) < P.experts) {
+          if constexpr (T == T_F32) {
+            const f4 v = *reinterpret_cast<const f4*>(reinterpret_cast<const float*>(P.logits) + row + expert(c));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) l[c + i] = v[i];
+          } else {
+            load8<T>(P.logits, row + expert(c), l + c);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) l[c + i] = -INFINITY;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) l[c + i] = expert(c + i) < P.experts ? load1<T>(P.logits, row + expert(c + i)) : -INFINITY;
+      }
     }
   }
-  DGM_DEV bool routed(const DgmBalanceArgs& P, int64_t t, int lane) const {
+  DGM_DEV bool routed(const DgmBalanceArgs& P, int64_t t) const {
     bool any = hit >= 0;
-    for (int k = lane + 64; k < P.topk; k += 64) any |= slot_expert(P, t, k) >= 0;
-    return __ballot(any) != 0;
+    for (int k = (threadIdx.x & 15) + 16; k < P.topk; k += 16) any |= slot_expert(P, t, k) >= 0;
+    return ((__ballot(any) >> (threadIdx.x & 48)) & 0xffffu) != 0;
   }
 };
 
+DGM_DEV float sum_lanes16(float v) {
+  v += dpp_f32<0xB1>(v);        // quad_perm [1,0,3,2]
+  v += dpp_f32<0x4E>(v);        // quad_perm [2,3,0,1]
+  v += dpp_f32<0x141>(v);       // row_half_mirror
+  return v + dpp_f32<0x140>(v); // row_mirror
+}
+// over the four groups of sixteen lanes
+DGM_DEV float sum_groups(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
 // e^x by the hardware's exp2: within (2 + |x|) 2^-24 of the value, so a probability's error stays that of its
-// rounded fp32 exponent (a third of the instructions of expf, and these passes were bound by them).
+// rounded fp32 exponent (a third of the instructions of expf).
 DGM_DEV float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 
 // A token's probabilities and its log-sum-exp (softmax; 0 where nothing is left). A sum of zero (all masked)
 // gives zeros. sig: sigmoid(l), of the sigmoid form.
-template <int NE, bool SOFTMAX>
+template <int NV, bool SOFTMAX>
 DGM_DEV void probabilities(const float* l, float* p, float* sig, float& lse) {
   float s = 0.f;
   lse = 0.f;
   if constexpr (SOFTMAX) {
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) m = fmaxf(m, l[i]);
-    m = wave_max(m);
+    for (int i = 0; i < NV; ++i) m = fmaxf(m, l[i]);
+    m = max_lanes16(m);
     const float shift = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
+    for (int i = 0; i < NV; ++i) {
       p[i] = exp_fast(l[i] - shift);
       s += p[i];
     }
-    s = wave_sum(s);
+    s = sum_lanes16(s);
     if (s != 0.f) lse = m + logf(s);
   } else {
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
+    for (int i = 0; i < NV; ++i) {
       sig[i] = p[i] = __builtin_amdgcn_rcpf(1.0f + exp_fast(-l[i]));
       s += p[i];
     }
-    s = wave_sum(s);
+    s = sum_lanes16(s);
   }
   const float inv = s != 0.f ? 1.0f / s : 0.f;
 #pragma unroll
-  for (int i = 0; i < NE; ++i) p[i] *= inv;
+  for (int i = 0; i < NV; ++i) p[i] *= inv;
 }
 
-// Sums of tokens [lo, hi) by the workgroup's waves, into rows of E values (and counts in LDS).
-template <int T, int NE, bool SOFTMAX, int W>
-DGM_DEV void sum_tokens(const DgmBalanceArgs& P, int64_t lo, int64_t hi, float (*wave_p)[64 * NE], int* hist, float* wave_z,
+// Sums of tokens [lo, hi) by the workgroup's waves, four tokens at a time, into rows of the experts' values
+// (and counts in LDS).
+template <int T, int NV, bool VEC, bool SOFTMAX, int W>
+DGM_DEV void sum_tokens(const DgmBalanceArgs& P, int64_t lo, int64_t hi, float (*wave_p)[16 * NV], int* hist, float* wave_z,
                         int* wave_n) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float acc[NE], z = 0.f;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane & 15;
+  float acc[NV], z = 0.f;
   int n = 0;
 #pragma unroll
-  for (int i = 0; i < NE; ++i) acc[i] = 0.f;
-  // (the next token is requested before the current one is worked on)
-  Token<T, NE> cur, next;
-  if (lo + wave < hi) cur.load(P, lo + wave, lane);
-  for (int64_t t = lo + wave; t < hi; t += W, cur = next) {
-    next.load(P, t + W < hi ? t + W : t, lane);
-    if (cur.hit >= 0) atomicAdd(&hist[cur.hit], 1);
-    for (int k = lane + 64; k < P.topk; k += 64) {
-      const int e = slot_expert(P, t, k);
-      if (e >= 0) atomicAdd(&hist[e], 1);
+  for (int i = 0; i < NV; ++i) acc[i] = 0.f;
+  // (the next tokens are requested before the current ones are worked on; behind the last one it again)
+  auto token = [&](int64_t base) { return base + (lane >> 4) < hi ? base + (lane >> 4) : hi - 1; };
+  Token<T, NV, VEC> cur, next;
+  const int64_t first = lo + 4 * wave;
+  if (first < hi) cur.load(P, token(first));
+  for (int64_t base = first; base < hi; base += 4 * W, cur = next) {
+    if (base + 4 * W < hi) next.load(P, token(base + 4 * W));
+    const int64_t t = token(base);
+    const bool live = base + (lane >> 4) < hi, counted = cur.routed(P, t) && live;
+    if (live) {
+      if (cur.hit >= 0) atomicAdd(&hist[cur.hit], 1);
+      for (int k = sub + 16; k < P.topk; k += 16) {
+        const int e = slot_expert(P, t, k);
+        if (e >= 0) atomicAdd(&hist[e], 1);
+      }
     }
-    if (!cur.routed(P, t, lane)) continue;
-    float p[NE], sig[NE], lse;
-    probabilities<NE, SOFTMAX>(cur.l, p, sig, lse);
+    float p[NV], sig[NV], lse;
+    probabilities<NV, SOFTMAX>(cur.l, p, sig, lse);
 #pragma unroll
-    for (int i = 0; i < NE; ++i) acc[i] += p[i];
-    z += lse * lse;
-    ++n;
+    for (int i = 0; i < NV; ++i) acc[i] += counted ? p[i] : 0.f;      // (an unrouted row may hold anything)
+    z += counted ? lse * lse : 0.f;
+    n += counted;
   }
 #pragma unroll
-  for (int i = 0; i < NE; ++i) wave_p[wave][lane + 64 * i] = acc[i];
+  for (int i = 0; i < NV; ++i) {
+    const float v = sum_groups(acc[i]);
+    if (lane < 16) wave_p[wave][Token<T, NV, VEC>::expert(i)] = v;
+  }
+  z = sum_groups(z);
+  n += __shfl_xor(n, 16);
+  n += __shfl_xor(n, 32);
   if (lane == 0) {
     wave_z[wave] = z;
     wave_n[wave] = n;
   }
 }
 
-template <int T, int NE, bool SOFTMAX>
-__global__ void __launch_bounds__(64 * WAVES) k_balance_tokens(const DgmBalanceArgs P, int64_t chunk, int64_t slots) {
-  __shared__ float wave_p[WAVES][64 * NE];
-  __shared__ int hist[64 * NE];
+template <int T, int NV, bool VEC, bool SOFTMAX>
+__global__ void __launch_bounds__(64 * waves_for(NV)) k_balance_tokens(const DgmBalanceArgs P, int64_t chunk, int64_t slots) {
+  constexpr int WAVES = waves_for(NV);
+  __shared__ float wave_p[WAVES][16 * NV];
+  __shared__ int hist[16 * NV];
   __shared__ float wave_z[WAVES];
   __shared__ int wave_n[WAVES];
   const Slots S = slots_of(P.workspace, slots, P.seqs, P.experts);
@@ -192,9 +238,9 @@ __global__ void __launch_bounds__(64 * WAVES) k_balance_tokens(const DgmBalanceA
     lo = lo < c0 ? c0 : lo;
     hi = hi > c1 ? c1 : hi;
     if (lo >= hi) continue;                      // (the whole workgroup)
-    for (int e = threadIdx.x; e < 64 * NE; e += 64 * WAVES) hist[e] = 0;
+    for (int e = threadIdx.x; e < 16 * NV; e += 64 * WAVES) hist[e] = 0;
     __syncthreads();
-    sum_tokens<T, NE, SOFTMAX, WAVES>(P, lo, hi, wave_p, hist, wave_z, wave_n);
+    sum_tokens<T, NV, VEC, SOFTMAX, WAVES>(P, lo, hi, wave_p, hist, wave_z, wave_n);
     __syncthreads();
     const int64_t slot = (int64_t)blockIdx.x + b;
     for (int e = threadIdx.x; e < P.experts; e += 64 * WAVES) {
@@ -306,39 +352,39 @@ __global__ void __launch_bounds__(256) k_balance_loss(const DgmBalanceArgs P, in
   }
 }
 
-// One sequence of few tokens: all of it by one workgroup of 16 waves, in one launch.
-template <int T, int NE, bool SOFTMAX>
-__global__ void __launch_bounds__(1024) k_balance_small(const DgmBalanceArgs P) {
-  __shared__ float wave_p[16][64 * NE];
-  __shared__ int hist[64 * NE];
-  __shared__ float wave_z[16];
-  __shared__ int wave_n[16];
-  __shared__ double lds_cp[16];
-  __shared__ int lds_c[16];
-  for (int e = threadIdx.x; e < 64 * NE; e += 1024) hist[e] = 0;
+// One sequence of few tokens: all of it by one workgroup, in one launch.
+template <int T, int NV, bool VEC, bool SOFTMAX>
+__global__ void __launch_bounds__(64 * waves_for(NV)) k_balance_small(const DgmBalanceArgs P) {
+  constexpr int W = waves_for(NV);
+  __shared__ float wave_p[W][16 * NV];
+  __shared__ int hist[16 * NV];
+  __shared__ float wave_z[W];
+  __shared__ int wave_n[W];
+  __shared__ double lds_cp[W];
+  __shared__ int lds_c[W];
+  for (int e = threadIdx.x; e < 16 * NV; e += 64 * W) hist[e] = 0;
   __syncthreads();
-  const int64_t lo = seq_begin(P, 0), hi = seq_begin(P, 1);
-  sum_tokens<T, NE, SOFTMAX, 16>(P, lo, hi, wave_p, hist, wave_z, wave_n);
+  sum_tokens<T, NV, VEC, SOFTMAX, W>(P, seq_begin(P, 0), seq_begin(P, 1), wave_p, hist, wave_z, wave_n);
   __syncthreads();
-  const int e = threadIdx.x, wave = threadIdx.x >> 6;
+  const int wave = threadIdx.x >> 6;
   double cp = 0.0;
   int c = 0;
-  if (e < 64 * NE) {
+  for (int e = threadIdx.x; e < P.experts; e += 64 * W) {
     double p = 0.0;
-    for (int w = 0; w < 16; ++w) p += (double)wave_p[w][e];
-    c = hist[e];
-    cp = (double)c * p;
-    if (e < P.experts) P.counts[e] = c;
+    for (int w = 0; w < W; ++w) p += (double)wave_p[w][e];
+    c += hist[e];
+    cp += (double)hist[e] * p;
+    P.counts[e] = hist[e];
   }
   cp = wave_sum_f64(cp);
   c = wave_sum_i32(c);
-  if ((e & 63) == 0) lds_cp[wave] = cp, lds_c[wave] = c;
+  if ((threadIdx.x & 63) == 0) lds_cp[wave] = cp, lds_c[wave] = c;
   __syncthreads();
-  if (e == 0) {
+  if (threadIdx.x == 0) {
     double z = 0.0;
     int n = 0;
     cp = 0.0, c = 0;
-    for (int w = 0; w < 16; ++w) cp += lds_cp[w], c += lds_c[w], z += (double)wave_z[w], n += wave_n[w];
+    for (int w = 0; w < W; ++w) cp += lds_cp[w], c += lds_c[w], z += (double)wave_z[w], n += wave_n[w];
     P.seq_stats[0] = c;
     P.seq_stats[1] = n;
     P.seq_stats[2] = (int)__float_as_uint((float)z);
@@ -346,9 +392,11 @@ __global__ void __launch_bounds__(1024) k_balance_small(const DgmBalanceArgs P) 
   }
 }
 
-// Gradient of the logits: a wave takes `per` consecutive tokens; f of their sequence stays in registers.
-template <int T, int NE, bool SOFTMAX>
+// Gradient of the logits: a wave takes `per` consecutive tokens, four at a time; f of their sequence stays in
+// registers.
+template <int T, int NV, bool VEC, bool SOFTMAX>
 __global__ void __launch_bounds__(256) k_balance_grad(const DgmBalanceArgs P, int64_t per) {
+  using Tok = Token<T, NV, VEC>;
   const int lane = threadIdx.x & 63;
   const int64_t first = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * per;
   const int64_t last = first + per < P.tokens ? first + per : P.tokens;
@@ -356,15 +404,17 @@ __global__ void __launch_bounds__(256) k_balance_grad(const DgmBalanceArgs P, in
   const float g = *P.d_loss;
   const int live = P.totals[0], total = P.totals[1];
   const float zc = SOFTMAX && total > 0 ? 2.0f * P.z_coef / (float)total : 0.f;
-  int b = seq_of(P, first) - 1, n = 0;
-  int64_t begin = 0, end = first;          // (of the sequence whose f is held)
-  float f[NE], coef = 0.f;
+  int b = seq_of(P, first) - 1, n = 0;           // (per group of lanes from here on)
+  int64_t begin = 0, end = first;                // of the sequence whose f is held
+  float f[NV], coef = 0.f;
 #pragma unroll
-  for (int i = 0; i < NE; ++i) f[i] = 0.f;
-  Token<T, NE> cur, next;
-  cur.load(P, first, lane);
-  for (int64_t t = first; t < last; ++t, cur = next) {
-    next.load(P, t + 1 < last ? t + 1 : t, lane);
+  for (int i = 0; i < NV; ++i) f[i] = 0.f;
+  auto token = [&](int64_t base) { return base + (lane >> 4) < last ? base + (lane >> 4) : last - 1; };
+  Tok cur, next;
+  cur.load(P, token(first));
+  for (int64_t base = first; base < last; base += 4, cur = next) {
+    if (base + 4 < last) next.load(P, token(base + 4));
+    const int64_t t = token(base);
     if (t >= end) {
       do {
         ++b;
@@ -374,34 +424,49 @@ __global__ void __launch_bounds__(256) k_balance_grad(const DgmBalanceArgs P, in
       n = b < P.seqs ? P.seq_stats[4 * (int64_t)b + 1] : 0;
       if (n > 0) {
         const float scale = (float)P.experts / (float)P.seq_stats[4 * (int64_t)b];
+        const int* counts = P.counts + (int64_t)b * P.experts;
 #pragma unroll
-        for (int i = 0; i < NE; ++i) {
-          const int e = lane + 64 * i;
-          f[i] = e < P.experts ? (float)P.counts[(int64_t)b * P.experts + e] * scale : 0.f;
+        for (int c = 0; c < NV; c += 4) {
+          if constexpr (VEC) {
+            v4i v = {0, 0, 0, 0};
+            if (Tok::expert(c) < P.experts) v = *reinterpret_cast<const v4i*>(counts + Tok::expert(c));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[c + i] = (float)v[i] * scale;
+          } else {
+#pragma unroll
+            for (int i = c; i < c + 4; ++i) f[i] = Tok::expert(i) < P.experts ? (float)counts[Tok::expert(i)] * scale : 0.f;
+          }
         }
         coef = P.balance_coef / ((float)live * (float)n);
       }
     }
-    float d[NE];
-    if (n > 0 && t >= begin && cur.routed(P, t, lane)) {
-      float p[NE], sig[NE], lse, dot = 0.f;
-      probabilities<NE, SOFTMAX>(cur.l, p, sig, lse);
+    const bool counted = cur.routed(P, t) && n > 0 && t >= begin;
+    float p[NV], sig[NV], lse, dot = 0.f;
+    probabilities<NV, SOFTMAX>(cur.l, p, sig, lse);
 #pragma unroll
-      for (int i = 0; i < NE; ++i) dot += f[i] * p[i];
-      dot = wave_sum(dot);
+    for (int i = 0; i < NV; ++i) dot += f[i] * p[i];
+    dot = sum_lanes16(dot);
 #pragma unroll
-      for (int i = 0; i < NE; ++i) {
-        if constexpr (SOFTMAX) d[i] = g * (p[i] * (coef * (f[i] - dot) + zc * lse));
-        else d[i] = g * (p[i] * (coef * (f[i] - dot)) * (1.0f - sig[i]));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NE; ++i) d[i] = 0.f;
+    for (int i = 0; i < NV; ++i) {
+      const float d = SOFTMAX ? g * (p[i] * (coef * (f[i] - dot) + zc * lse)) : g * (p[i] * (coef * (f[i] - dot)) * (1.0f - sig[i]));
+      p[i] = counted ? d : 0.f;                  // (an unrouted row may hold anything)
     }
+    if (base + (lane >> 4) >= last) continue;
+    const int64_t row = t * P.d_logits_stride;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      const int e = lane + 64 * i;
-      if (e < P.experts) store1<T>(P.d_logits, t * P.d_logits_stride + e, d[i]);
+    for (int c = 0; c < NV; c += Tok::V) {
+      if constexpr (VEC) {
+        if (Tok::expert(c) < P.experts) {
+          if constexpr (T == T_F32)
+            *reinterpret_cast<f4*>(reinterpret_cast<float*>(P.d_logits) + row + Tok::expert(c)) = f4{p[c], p[c + 1], p[c + 2], p[c + 3]};
+          else
+            store8<T>(P.d_logits, row + Tok::expert(c), p + c);
+        }
+      } else {
+#pragma unroll
+        for (int i = c; i < c + Tok::V; ++i)
+          if (Tok::expert(i) < P.experts) store1<T>(P.d_logits, row + Tok::expert(i), p[i]);
+      }
     }
   }
 }
@@ -419,19 +484,28 @@ int check(const DgmBalanceArgs& A) {
   return 0;
 }
 
+// Values a lane holds (sixteen lanes a token), alignment and score as compile-time values.
 template <class F>
 void dispatch(const DgmBalanceArgs& A, F&& f) {
   using std::integral_constant;
-  auto score = [&](auto t, auto ne) {
-    if (A.score == 0) f(t, ne, std::true_type{});
-    else f(t, ne, std::false_type{});
+  const int e = A.dtype == DGM_SRC_F32 ? 4 : 2;
+  const bool vec = A.experts % (16 / e) == 0 &&
+                   (((uintptr_t)A.logits | (uintptr_t)A.d_logits | (uintptr_t)A.counts | (uint64_t)(A.logits_stride * e) |
+                     (uint64_t)(A.d_logits_stride * e)) & 15) == 0;
+  auto score = [&](auto t, auto nv, auto v) {
+    if (A.score == 0) f(t, nv, v, std::true_type{});
+    else f(t, nv, v, std::false_type{});
+  };
+  auto align = [&](auto t, auto nv) {
+    if (vec) score(t, nv, std::true_type{});
+    else score(t, nv, std::false_type{});
   };
   auto experts = [&](auto t) {
-    if (A.experts <= 64) score(t, integral_constant<int, 1>{});
-    else if (A.experts <= 128) score(t, integral_constant<int, 2>{});
-    else if (A.experts <= 256) score(t, integral_constant<int, 4>{});
-    else if (A.experts <= 512) score(t, integral_constant<int, 8>{});
-    else score(t, integral_constant<int, 16>{});
+    if (A.experts <= 128) align(t, integral_constant<int, 8>{});
+    else if (A.experts <= 256) align(t, integral_constant<int, 16>{});
+    else if (A.experts <= 384) align(t, integral_constant<int, 24>{});
+    else if (A.experts <= 512) align(t, integral_constant<int, 32>{});
+    else align(t, integral_constant<int, 64>{});
   };
   if (A.dtype == DGM_SRC_BF16) experts(integral_constant<int, T_BF16>{});
   else if (A.dtype == DGM_SRC_F16) experts(integral_constant<int, T_F16>{});
@@ -463,8 +537,9 @@ int dgm_router_balance_loss(const DgmBalanceArgs* args, hipStream_t stream) {
   if (int st = check(A)) return st;
   DGM_CHECK_ARG(A.loss, "null loss");
   if (A.seqs == 1 && A.tokens <= SMALL_TOKENS) {
-    dispatch(A, [&](auto t, auto ne, auto softmax) {
-      hipLaunchKernelGGL((k_balance_small<t.value, ne.value, softmax.value>), dim3(1), dim3(1024), 0, stream, A);
+    dispatch(A, [&](auto t, auto nv, auto v, auto softmax) {
+      hipLaunchKernelGGL((k_balance_small<t.value, nv.value, v.value, softmax.value>), dim3(1),
+                         dim3(64 * waves_for(nv.value)), 0, stream, A);
     });
     return dgm_last_launch_status();
   }
@@ -473,9 +548,9 @@ int dgm_router_balance_loss(const DgmBalanceArgs* args, hipStream_t stream) {
                 "workspace of dgm_router_balance_workspace_bytes, 16-byte aligned");
   const int64_t chunk = chunk_tokens(A.tokens), chunks = (A.tokens + chunk - 1) / chunk, slots = chunks + A.seqs;
   if (chunks > 0)
-    dispatch(A, [&](auto t, auto ne, auto softmax) {
-      hipLaunchKernelGGL((k_balance_tokens<t.value, ne.value, softmax.value>), dim3((unsigned)chunks), dim3(64 * WAVES), 0,
-                         stream, A, chunk, slots);
+    dispatch(A, [&](auto t, auto nv, auto v, auto softmax) {
+      hipLaunchKernelGGL((k_balance_tokens<t.value, nv.value, v.value, softmax.value>), dim3((unsigned)chunks),
+                         dim3(64 * waves_for(nv.value)), 0, stream, A, chunk, slots);
     });
   hipLaunchKernelGGL(k_balance_columns, dim3((unsigned)A.seqs, (unsigned)((A.experts + 63) / 64)), dim3(1024), 0, stream, A,
                      chunk, slots);
@@ -489,11 +564,11 @@ int dgm_router_balance_loss_backward(const DgmBalanceArgs* args, hipStream_t str
   if (int st = check(A)) return st;
   if (A.tokens == 0) return 0;
   DGM_CHECK_ARG(A.d_loss && A.d_logits, "null pointer");
-  // (consecutive tokens of a wave share their sequence's f: 8192 waves, a token each at least)
-  const int64_t per = (A.tokens + 8191) / 8192;
+  // (consecutive tokens of a wave share their sequence's f: 4096 waves, four tokens each at least)
+  const int64_t per = (A.tokens + 16383) / 16384 * 4;
   const int64_t waves = (A.tokens + per - 1) / per;
-  dispatch(A, [&](auto t, auto ne, auto softmax) {
-    hipLaunchKernelGGL((k_balance_grad<t.value, ne.value, softmax.value>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0,
+  dispatch(A, [&](auto t, auto nv, auto v, auto softmax) {
+    hipLaunchKernelGGL((k_balance_grad<t.value, nv.value, v.value, softmax.value>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0,
                        stream, A, per);
   });
   return dgm_last_launch_status();
