@@ -94,7 +94,7 @@ def _forward_args(x, residual, post_weight, pre_weight, gate, gate_sigmoid, resi
     T, H = x.shape
     w = post_weight if post_weight is not None else pre_weight
     args = _lib.NormArgs(x=x.data_ptr(), rows=T, x_stride=x.stride(0), hidden=H, dtype=_lib.SRC_DTYPES[x.dtype],
-                         residual_scale=residual_scale, eps=eps)
+                         residual_scale=float(residual_scale), eps=float(eps))
     # (the fields of absent parts stay at their zero: each one set costs time on a call that the GPU finishes in 3 us)
     if residual is not None:
         args.residual, args.residual_stride = residual.data_ptr(), residual.stride(0)

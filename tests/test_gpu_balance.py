@@ -97,7 +97,7 @@ def check(logits, idx, cuts, alpha, beta, score, cu=True, g=1.0):
     loss, counts, d = run(logits, idx, cuts, alpha, beta, score, g, cu)
     want, wc, wg, wm = formula(logits, idx, cuts, alpha, beta, score)
     assert torch.equal(counts.long().cpu().view(wc.shape), wc) and counts.dtype == torch.int32
-    assert loss.dtype == torch.float32 and abs(float(loss) - want) <= 300 * U * abs(want) + 1e-38
+    assert loss.dtype == torch.float32 and abs(float(loss.detach()) - want) <= 300 * U * abs(want) + 1e-38
     assert d.dtype == logits.dtype
     close(d, wg * g, wm * abs(g))
     return loss, counts, d
@@ -132,7 +132,7 @@ def test_no_tokens_and_nothing_routed():
         idx[:] = -1
         logits[:] = float("nan")                     # unrouted tokens' logits are not looked at
         loss, counts, d = run(logits, idx, cuts, 1.0, 0.1, "softmax")
-        assert float(loss) == 0.0 and not bool(counts.any()) and not bool(d.any()) and d.shape == logits.shape
+        assert float(loss.detach()) == 0.0 and not bool(counts.any()) and not bool(d.any()) and d.shape == logits.shape
 
 
 def test_masked_experts_and_bad_ids():
@@ -153,13 +153,33 @@ def test_masked_experts_and_bad_ids():
         for score, beta in (("softmax", 0.01), ("sigmoid", 0.0)):
             loss, counts, d = run(logits, idx, [0, 400], 1.0, beta, score)
             want, wc, wg, wm = formula(clean, idx, [0, 400], 1.0, beta, score)
-            assert torch.equal(counts.long().cpu(), wc) and abs(float(loss) - want) <= 300 * U * abs(want)
+            assert torch.equal(counts.long().cpu(), wc) and abs(float(loss.detach()) - want) <= 300 * U * abs(want)
             close(d, wg, wm)
             assert not bool(d[off].any()) and not bool(d[7].any()) and not bool(d[:, 50:].any())
         low = logits.masked_fill(torch.isinf(logits), torch.finfo(dtype).min)
         low[7, 0] = 0
         low[off] = 0
         check(low, idx, [0, 400], 1.0, 0.01, "softmax")
+
+
+def test_offsets_beyond_32_bits_and_refusals():
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    logits, idx = make(5, 64, 4, seed=2)
+    want = run(logits, idx, [0, 5], 1.0, 0.01, "softmax")
+    gap = (1 << 30) + 16
+    far = torch.empty(gap * 4 + 64, device="cuda").as_strided((5, 64), (gap, 1)).copy_(logits)
+    got = run(far, idx, [0, 5], 1.0, 0.01, "softmax")
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    leaf = logits.clone().requires_grad_()
+    loss, counts = dgm.router_balance_loss(leaf, idx)
+    assert not counts.requires_grad
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(loss, leaf, create_graph=True)
+    with pytest.raises(RuntimeError, match="cpu"):
+        dgm.router_balance_loss(logits, idx.cpu())
+    with pytest.raises(TypeError, match="stats of"):
+        dgm.router_balance_loss_backward(torch.ones((), device="cuda"), logits, idx, counts, counts)
 
 
 def test_gradient_against_differences():

@@ -164,6 +164,27 @@ def test_rows_of_another_call_do_not_matter():
         assert torch.equal(d, full[:m]), m
 
 
+@pytest.mark.parametrize("m", [3, 70])
+def test_offsets_beyond_32_bits(m):
+    """Rows of every operand more than 2^31 bytes from the first one, in the register and the tile kernels."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    n, k = 48, 256
+    a, b = make(m, n, k, seed=m)
+    d = torch.empty((m, n), dtype=torch.float32, device="cuda")
+    dgm.int8_gemm_nt(a, b, d)
+    far = {}
+    for name, rows, width, dt in (("a", m, k, torch.int8), ("b", n, k, torch.int8), ("d", m, n, torch.float32)):
+        gap = (5 << 30) // rows // dt.itemsize // 16 * 16
+        big = torch.empty(gap * (rows - 1) + width, dtype=dt, device="cuda")
+        far[name] = big.as_strided((rows, width), (gap, 1))
+    far["a"].copy_(a[0]), far["b"].copy_(b[0])
+    dgm.int8_gemm_nt((far["a"], a[1]), (far["b"], b[1]), far["d"])
+    assert torch.equal(far["d"], d)
+    dgm.int8_gemm_nt((far["a"], a[1]), (far["b"], b[1]), far["d"], c=far["d"])
+    assert torch.equal(far["d"], d + d)
+
+
 def test_streams_and_graph():
     need_gpu()
     import hopper_megamoe_basedondeepgemm_amd as dgm

@@ -292,6 +292,69 @@ def test_strides_alignment_and_places():
         dgm.rms_norm_residual(x.clone().requires_grad_(), r, w1, w2, gt, residual_out=ri)
 
 
+def test_shared_and_broadcast_leaves():
+    """One leaf in several places, expanded residual and gate: their gradients are the sums over the places."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    T, H = 12, 96
+    x, _, w1, _, _ = make(T, H, torch.float32, torch.float32, 1, 0, "none", 0, seed=4)
+    row, g = torch.randn(H, device="cuda"), torch.randn(1, 1, device="cuda")
+    leaves = [t.clone().requires_grad_() for t in (x, row, w1, g)]
+    lx, lr, lw, lg = leaves
+    got = dgm.rms_norm_residual(lx, lr.expand(T, H), lw, lw, lg.expand(T, 1), True, 0.5)
+    dr, dh = torch.randn_like(x), torch.randn_like(x)
+    gx, gr, gw, gg = torch.autograd.grad(got, leaves, (dr, dh))
+    want = Form(x, row.expand(T, H), w1, w1, g.expand(T, 1), True, 0.5).grads(dr, dh)
+    close(gx, *want["x"], 256)
+    close(gr, *(v.sum(0) for v in want["residual"]), 256 + T)
+    close(gw, want["post"][0] + want["pre"][0], want["post"][1] + want["pre"][1], 256 + 2 * T)
+    close(gg, *(v.sum(0, keepdim=True) for v in want["gate"]), 256 + H + T)
+    both = x.clone().requires_grad_()
+    r, h = dgm.rms_norm_residual(both, both, pre_weight=w1)
+    (gb,) = torch.autograd.grad((r, h), both, (dr, dh))
+    want = Form(x, x, None, w1, None, False, 1.0).grads(dr, dh)
+    close(gb, want["x"][0] + want["residual"][0], want["x"][1] + want["residual"][1], 257)
+
+
+def test_autograd_refusals():
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    x, _, _, w2, _ = make(4, 64, torch.float32, torch.float32, 0, 1, "none", 0)
+    leaf = x.clone().requires_grad_()
+    _, h = dgm.rms_norm_residual(leaf, pre_weight=w2)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(h.sum(), leaf, create_graph=True)
+    _, h = dgm.rms_norm_residual(leaf * 1, pre_weight=w2)
+    mid = leaf * 1
+    _, h = dgm.rms_norm_residual(mid, pre_weight=w2)
+    with torch.no_grad():
+        mid.zero_()                                       # (an input changed behind the forward pass)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(h.sum(), leaf)
+    with pytest.raises(RuntimeError, match="cpu"):
+        dgm.rms_norm_residual(x, x.cpu())
+
+
+def test_offsets_beyond_32_bits():
+    """Rows more than 2^31 elements apart, read and written."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    T, H, gap = 4, 512, (1 << 30) + 64
+    big = torch.empty(gap * (T - 1) + H, dtype=torch.bfloat16, device="cuda")
+    far = big.as_strided((T, H), (gap, 1))
+    x, r, w1, w2, gt = make(T, H, torch.bfloat16, torch.float32, 1, 1, "token", 1, seed=6)
+    far.copy_(x)
+    want = dgm.rms_norm_residual_forward(x, r, w1, w2, gt, True, 0.5)
+    got = dgm.rms_norm_residual_forward(far, r, w1, w2, gt, True, 0.5)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    dr, dh = torch.randn_like(x), torch.randn_like(x)
+    a = dgm.rms_norm_residual_backward(dr, dh, x, r, *want[2:], w1, w2, gt, True, 0.5)
+    b = dgm.rms_norm_residual_backward(dr, dh, far, r, *want[2:], w1, w2, gt, True, 0.5)
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+    dgm.rms_norm_residual(x, r, w1, w2, gt, True, 0.5, out=far)
+    assert torch.equal(far, want[1])
+
+
 def test_odd_values():
     """All-zero rows, rows of a large norm, infinities and NaN: as the formula has them, row by row."""
     need_gpu()
