@@ -50,7 +50,8 @@ def check_swiglu(d, ref, clamp):
 SHAPES = [(1, 1, 1), (1, 16, 64), (1, 4096, 2048), (2, 30, 16), (3, 7, 5), (5, 64, 48), (16, 16, 128), (17, 33, 80), (31, 100, 256),
           (33, 257, 112), (48, 512, 1024), (63, 130, 144), (64, 4096, 7168), (65, 128, 2048), (100, 384, 400), (128, 128, 128),
           (129, 320, 640), (200, 1000, 96), (255, 513, 272), (256, 256, 512), (300, 2880, 1024), (777, 640, 1296), (1000, 5120, 288),
-          (2049, 1040, 160)]
+          (2049, 1040, 160), (200, 1000, 512), (1000, 4000, 512), (2000, 4002, 528), (4000, 4000, 528), (3999, 4034, 400),
+          (3, 10, 5), (20, 34, 21), (50, 66, 37), (300, 66, 129)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
