@@ -3,6 +3,7 @@
 No counterpart in the reference, whose layer starts at the router: these are the row passes that a
 decoder block needs before ``fable_router_quant_topk_frontend`` and behind the layer's combine."""
 import ctypes
+import functools
 
 import torch
 
@@ -17,8 +18,9 @@ def _rows(t):
     return t if t.stride(1) == 1 or t.size(1) == 1 else t.contiguous()
 
 
-def _new_rows(x):
-    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+def _new_like(t):
+    """An uninitialised contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _gate_mode(gate, T, H):
@@ -89,120 +91,149 @@ def _check_outputs(outs, ins):
                 raise ValueError("an output overlaps an input other than as the same rows")
 
 
-def _forward_args(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, mode, r_out, h, q, sf,
-                  rstd_post, rstd_pre):
+def _forward_args(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, mode, rstd_post, rstd_pre):
+    """DgmNormArgs of a call's inputs. (The fields of absent parts stay at their zero: each one set costs time on
+    a call that the GPU finishes in 3 us.)"""
     T, H = x.shape
     w = post_weight if post_weight is not None else pre_weight
     args = _lib.NormArgs(x=x.data_ptr(), rows=T, x_stride=x.stride(0), hidden=H, dtype=_lib.SRC_DTYPES[x.dtype],
                          residual_scale=float(residual_scale), eps=float(eps))
-    # (the fields of absent parts stay at their zero: each one set costs time on a call that the GPU finishes in 3 us)
     if residual is not None:
         args.residual, args.residual_stride = residual.data_ptr(), residual.stride(0)
     if post_weight is not None:
-        args.post_weight = post_weight.data_ptr()
+        args.post_weight, args.rstd_post = post_weight.data_ptr(), rstd_post
     if pre_weight is not None:
-        args.pre_weight = pre_weight.data_ptr()
+        args.pre_weight, args.rstd_pre = pre_weight.data_ptr(), rstd_pre
     if w is not None and w.dtype == torch.float32:
         args.weights_f32 = 1
     if gate is not None:
         args.gate, args.gate_mode, args.gate_sigmoid = gate.data_ptr(), mode, int(bool(gate_sigmoid))
         if mode != GATE_CHANNEL:
             args.gate_stride = gate.stride(0)
-    if r_out is not None:
-        args.residual_out, args.residual_out_stride = r_out.data_ptr(), r_out.stride(0)
-    if h is not None:
-        args.h, args.h_stride = h.data_ptr(), h.stride(0)
-    if q is not None:
-        args.q, args.q_sf = q.data_ptr(), sf.data_ptr()
-    if rstd_post is not None:
-        args.rstd_post = rstd_post.data_ptr()
-    if rstd_pre is not None:
-        args.rstd_pre = rstd_pre.data_ptr()
     return args
 
 
-def _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, quant, residual_out, out, keep):
-    """The launch, after the checks: (residual rows, h, q, sf, rstd_post, rstd_pre)."""
-    T, H = x.shape
+def _readable(x, residual, post_weight, pre_weight, gate):
+    """The inputs as the kernels read them, and the gate's mode."""
     x = _rows(x)
-    residual = None if residual is None else _rows(residual)
+    if residual is not None:
+        residual = _rows(residual)
     if post_weight is not None and post_weight.stride(0) != 1:
         post_weight = post_weight.contiguous()
     if pre_weight is not None and pre_weight.stride(0) != 1:
         pre_weight = pre_weight.contiguous()
     mode = GATE_NONE
     if gate is not None:
-        mode = _gate_mode(gate, T, H)
-        gate = _rows(gate) if mode == GATE_FULL else gate.contiguous() if mode == GATE_CHANNEL else gate
+        mode = _gate_mode(gate, x.size(0), x.size(1))
+        if mode == GATE_FULL:
+            gate = _rows(gate)
+        elif mode == GATE_CHANNEL:
+            gate = gate.contiguous()
+    return x, residual, post_weight, pre_weight, gate, mode
+
+
+def _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, quant, residual_out, out, keep):
+    """The launch, after the checks: (residual rows, h, q, sf, rstd, args, read). ``keep``: rstd fp32 [norms,
+    tokens] for the backward pass; args: the launch's DgmNormArgs; read: the tensors whose memory it names."""
+    T = x.size(0)
+    read = _readable(x, residual, post_weight, pre_weight, gate)
+    x_, residual_, post_, pre_, gate_, mode = read
     same = residual is None and post_weight is None and gate is None and residual_scale == 1.0 and residual_out is None
-    r_out = None if same else residual_out if residual_out is not None else _new_rows(x)
-    h = None if pre_weight is None else out if out is not None else _new_rows(x)
-    q = sf = rstd_post = rstd_pre = None
+    r_out = None if same else residual_out if residual_out is not None else _new_like(x)
+    h = None if pre_weight is None else out if out is not None else _new_like(x)
+    q = sf = rstd = None
+    at = 0
+    if keep:
+        rstd = torch.empty(((post_weight is not None) + (pre_weight is not None), T), dtype=torch.float32, device=x.device)
+        at = rstd.data_ptr()
+    args = _forward_args(x_, residual_, post_, pre_, gate_, gate_sigmoid, residual_scale, eps, mode, at,
+                         at + 4 * T if at and post_weight is not None else at)
+    if r_out is not None:
+        args.residual_out, args.residual_out_stride = r_out.data_ptr(), r_out.stride(0)
+    if h is not None:
+        args.h, args.h_stride = h.data_ptr(), h.stride(0)
     if quant:
-        q = torch.empty((T, H), dtype=torch.int8, device=x.device)
+        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
         sf = torch.empty((T,), dtype=torch.float32, device=x.device)
-    if keep and post_weight is not None:
-        rstd_post = torch.empty((T,), dtype=torch.float32, device=x.device)
-    if keep and pre_weight is not None:
-        rstd_pre = torch.empty((T,), dtype=torch.float32, device=x.device)
+        args.q, args.q_sf = q.data_ptr(), sf.data_ptr()
     if (residual_out is not None or out is not None) and T > 0:
-        _check_outputs([t for t in (residual_out, out) if t is not None],
-                       [t for t in (x, residual, post_weight, pre_weight, gate) if t is not None])
+        _check_outputs([t for t in (residual_out, out) if t is not None], [t for t in read[:5] if t is not None])
     if T > 0 and not (same and h is None):
-        args = _forward_args(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, mode, r_out, h,
-                             q, sf, rstd_post, rstd_pre)
         _lib.check(_lib.load().dgm_rms_norm_residual(ctypes.byref(args), _lib.stream()))
-    return x if same else r_out, h, q, sf, rstd_post, rstd_pre
+    return x if same else r_out, h, q, sf, rstd, args, read
 
 
-def _backward(d_r, d_h, x, residual, rstd_post, rstd_pre, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps,
-              needs):
-    """The launches of the backward pass, after the checks."""
+@functools.lru_cache(maxsize=1024)
+def _groups(T, H):
+    return _lib.load().dgm_rms_norm_residual_groups(T, H)
+
+
+def _backward(d_r, d_h, x, residual, post_weight, pre_weight, gate, forward, needs):
+    """The launches of the backward pass, after the checks; forward: DgmNormArgs over the forward call's inputs
+    and rstd rows."""
     T, H = x.shape
-    x = _rows(x)
-    residual = None if residual is None else _rows(residual)
-    d_r = None if d_r is None else _rows(d_r)
-    d_h = None if d_h is None else _rows(d_h)
-    post_weight = None if post_weight is None else post_weight.contiguous()
-    pre_weight = None if pre_weight is None else pre_weight.contiguous()
-    mode = GATE_NONE
-    if gate is not None:
-        mode = _gate_mode(gate, T, H)
-        gate = _rows(gate) if mode == GATE_FULL else gate.contiguous() if mode == GATE_CHANNEL else gate
-    new = lambda t, need: torch.empty(t.shape, dtype=t.dtype, device=t.device) if need and t is not None else None
-    d_x, d_residual, d_post, d_pre, d_gate = (new(t, n) for t, n in zip((x, residual, post_weight, pre_weight, gate),
-                                                                        needs))
-    lib = _lib.load()
-    ws = None
-    if d_post is not None or d_pre is not None or (d_gate is not None and mode == GATE_CHANNEL):
-        ws = torch.empty((3, lib.dgm_rms_norm_residual_groups(T, H), H), dtype=torch.float32, device=x.device)
-    fwd = _forward_args(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, mode, None, None,
-                        None, None, rstd_post, rstd_pre)
-    p = lambda t: 0 if t is None else t.data_ptr()
-    s = lambda t: 0 if t is None else t.stride(0)
-    args = _lib.NormGradArgs(fwd, p(d_r), p(d_h), p(d_x), p(d_residual), p(d_gate), p(d_post), p(d_pre), p(ws),
-                             0 if ws is None else ws.nbytes, s(d_r), s(d_h), s(d_x), s(d_residual),
-                             s(d_gate) if mode in (GATE_TOKEN, GATE_FULL) else 0)
-    _lib.check(lib.dgm_rms_norm_residual_backward(ctypes.byref(args), _lib.stream()))
+    args = _lib.NormGradArgs(forward)
+    if d_r is not None:
+        d_r = _rows(d_r)
+        args.d_residual_out, args.d_residual_out_stride = d_r.data_ptr(), d_r.stride(0)
+    if d_h is not None:
+        d_h = _rows(d_h)
+        args.d_h, args.d_h_stride = d_h.data_ptr(), d_h.stride(0)
+    d_x = d_residual = d_post = d_pre = d_gate = None
+    columns = False                       # (a gradient that is a sum over rows)
+    if needs[0]:
+        d_x = _new_like(x)
+        args.d_x, args.d_x_stride = d_x.data_ptr(), H
+    if needs[1] and residual is not None:
+        d_residual = _new_like(x)
+        args.d_residual, args.d_residual_stride = d_residual.data_ptr(), H
+    if needs[2] and post_weight is not None:
+        d_post = _new_like(post_weight)
+        args.d_post_weight = d_post.data_ptr()
+        columns = True
+    if needs[3] and pre_weight is not None:
+        d_pre = _new_like(pre_weight)
+        args.d_pre_weight = d_pre.data_ptr()
+        columns = True
+    if needs[4] and gate is not None:
+        d_gate = _new_like(gate)
+        args.d_gate = d_gate.data_ptr()
+        if forward.gate_mode == GATE_CHANNEL:
+            columns = True
+        else:
+            args.d_gate_stride = d_gate.size(1)
+    if columns:
+        ws = torch.empty(3 * _groups(T, H) * H, dtype=torch.float32, device=x.device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), ws.nbytes
+    _lib.check(_lib.load().dgm_rms_norm_residual_backward(ctypes.byref(args), _lib.stream()))
     return d_x, d_residual, d_post, d_pre, d_gate
+
+
+_INPUTS = ("x", "residual", "post_weight", "pre_weight", "gate")
 
 
 class _RmsNormResidual(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps):
-        r, h, _, _, rstd_post, rstd_pre = _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale,
-                                                   eps, None, None, None, True)
-        ctx.save_for_backward(x, residual, post_weight, pre_weight, gate, rstd_post, rstd_pre)
-        ctx.options = gate_sigmoid, residual_scale, eps
+        r, h, _, _, rstd, args, read = _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps,
+                                                None, None, None, True)
+        ctx.save_for_backward(x, residual, post_weight, pre_weight, gate, rstd)
+        ctx.args = args
+        # (inputs that the kernels read as copies: those copies)
+        ctx.copies = [None if u is t else u for t, u in zip((x, residual, post_weight, pre_weight, gate), read)]
         ctx.set_materialize_grads(False)
         return (None if r is x else r), h
 
     @staticmethod
     def backward(ctx, d_r, d_h):
         _lib.no_second_derivative()
-        x, residual, post_weight, pre_weight, gate, rstd_post, rstd_pre = ctx.saved_tensors
-        return (*_backward(d_r, d_h, x, residual, rstd_post, rstd_pre, post_weight, pre_weight, gate, *ctx.options,
-                           ctx.needs_input_grad), None, None, None)
+        saved = ctx.saved_tensors
+        args = ctx.args
+        # (a tensor's memory may have moved since the forward pass)
+        for name, t, copy in zip(_INPUTS, saved, ctx.copies):
+            if t is not None:
+                setattr(args, name, (t if copy is None else copy).data_ptr())
+        return (*_backward(d_r, d_h, *saved[:5], args, ctx.needs_input_grad), None, None, None)
 
 
 def rms_norm_residual(x, residual=None, post_weight=None, pre_weight=None, gate=None, gate_sigmoid=False,
@@ -237,8 +268,8 @@ def rms_norm_residual(x, residual=None, post_weight=None, pre_weight=None, gate=
         r, h = _RmsNormResidual.apply(x, residual, post_weight, pre_weight, gate, bool(gate_sigmoid),
                                       float(residual_scale), float(eps))
         return (x if r is None else r), h
-    r, h, q, sf, _, _ = _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, quant,
-                                 residual_out, out, False)
+    r, h, q, sf, _, _, _ = _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, quant,
+                                    residual_out, out, False)
     return (r, h, (q, sf)) if quant else (r, h)
 
 
@@ -248,9 +279,9 @@ def rms_norm_residual_forward(x, residual=None, post_weight=None, pre_weight=Non
     (fp32 [tokens] each, None without that norm). Records no autograd graph."""
     _check(x, residual, post_weight, pre_weight, gate)
     _lib.require_one_device(x, residual, post_weight, pre_weight, gate)
-    r, h, _, _, rstd_post, rstd_pre = _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps,
-                                               None, None, None, True)
-    return r, h, rstd_post, rstd_pre
+    r, h, _, _, rstd, _, _ = _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, None,
+                                      None, None, True)
+    return r, h, rstd[0] if post_weight is not None else None, rstd[-1] if pre_weight is not None else None
 
 
 def rms_norm_residual_backward(d_r, d_h, x, residual, rstd_post, rstd_pre, post_weight=None, pre_weight=None, gate=None,
@@ -272,8 +303,11 @@ def rms_norm_residual_backward(d_r, d_h, x, residual, rstd_post, rstd_pre, post_
                               or not rstd.is_contiguous()):
             raise ValueError("rstd rows of rms_norm_residual_forward (fp32 [tokens]) expected")
     _lib.require_one_device(x, d_r, d_h, residual, post_weight, pre_weight, gate, rstd_post, rstd_pre)
-    return _backward(d_r, d_h, x, residual, rstd_post, rstd_pre, post_weight, pre_weight, gate, gate_sigmoid, residual_scale,
-                     eps, needs)
+    read = _readable(x, residual, post_weight, pre_weight, gate)
+    forward = _forward_args(*read[:5], gate_sigmoid, residual_scale, eps, read[5],
+                            rstd_post.data_ptr() if post_weight is not None else 0,
+                            rstd_pre.data_ptr() if pre_weight is not None else 0)
+    return _backward(d_r, d_h, x, residual, post_weight, pre_weight, gate, forward, needs)
 
 
 __all__ = ["rms_norm_residual", "rms_norm_residual_forward", "rms_norm_residual_backward"]

@@ -316,6 +316,30 @@ def test_shared_and_broadcast_leaves():
     close(gb, want["x"][0] + want["residual"][0], want["x"][1] + want["residual"][1], 257)
 
 
+def test_memory_that_moves_between_the_passes():
+    """Parameters and activations whose storage is replaced between forward and backward (as sharded training
+    does), and inputs that are read as copies."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    x, r, w1, w2, gt = make(9, 160, torch.bfloat16, torch.float32, 1, 1, "channel", 1, seed=8)
+    dr, dh = torch.randn_like(x), torch.randn_like(x)
+
+    def grads(move, turn):
+        t = lambda v: v.t().contiguous().t() if turn and v.dim() == 2 else v.clone()
+        leaves = [t(v).requires_grad_() for v in (x, r, w1, w2, gt)]
+        got = dgm.rms_norm_residual(*leaves, True, 0.5)
+        if move:
+            for v in leaves:
+                v.data = v.data.clone(memory_format=torch.preserve_format)
+            torch.cuda.synchronize()
+        return torch.autograd.grad(got, leaves, (dr, dh), retain_graph=True), torch.autograd.grad(got, leaves, (dr, dh))
+    want, again = grads(False, False)
+    for case in ((False, True), (True, False), (True, True)):
+        for got in grads(*case):
+            assert all(torch.equal(a, b) for a, b in zip(want, got)), case
+    assert all(torch.equal(a, b) for a, b in zip(want, again))
+
+
 def test_autograd_refusals():
     need_gpu()
     import hopper_megamoe_basedondeepgemm_amd as dgm
