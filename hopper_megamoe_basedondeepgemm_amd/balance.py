@@ -4,6 +4,7 @@ No counterpart in the reference, whose frontend stops at the top-k: this is what
 watching its balance in service, needs of the same logits and indices (``FusedSymmBuffer.logits`` and
 ``topk_idx`` as the frontend leaves them)."""
 import ctypes
+import functools
 
 import torch
 
@@ -37,31 +38,45 @@ def _check(logits, topk_idx, cu_seqlens, score, z_coef):
     _lib.require_one_device(logits, topk_idx, cu_seqlens)
 
 
-def _args(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score, counts, seq_stats, totals, loss=None, ws=None,
-          d_loss=None, d_logits=None):
-    p = lambda t: 0 if t is None else t.data_ptr()
-    return _lib.BalanceArgs(p(logits), p(topk_idx), p(cu_seqlens), p(loss), p(counts), p(seq_stats), p(totals), p(d_loss),
-                            p(d_logits), p(ws), 0 if ws is None else ws.nbytes, logits.size(0), logits.stride(0),
-                            topk_idx.stride(0), 0 if d_logits is None else d_logits.stride(0), logits.size(1),
-                            topk_idx.size(1), 1 if cu_seqlens is None else cu_seqlens.size(0) - 1,
-                            _lib.SRC_DTYPES[logits.dtype], int(topk_idx.dtype == torch.int64), SCORES[score],
-                            float(balance_coef), float(z_coef))
+def _args(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score, counts, stats):
+    """DgmBalanceArgs of a call's inputs (logits and topk_idx as rows), counts and statistics."""
+    T, E = logits.shape
+    at = stats.data_ptr()                 # (per sequence 4 int32, then the totals)
+    seqs = stats.size(0) // 4 - 1
+    args = _lib.BalanceArgs(logits=logits.data_ptr(), topk_idx=topk_idx.data_ptr(), counts=counts.data_ptr(), seq_stats=at,
+                            totals=at + 16 * seqs, tokens=T, logits_stride=logits.stride(0), idx_stride=topk_idx.stride(0),
+                            experts=E, topk=topk_idx.size(1), seqs=seqs, dtype=_lib.SRC_DTYPES[logits.dtype],
+                            idx_i64=int(topk_idx.dtype == torch.int64), score=SCORES[score],
+                            balance_coef=float(balance_coef), z_coef=float(z_coef))
+    if cu_seqlens is not None:
+        args.cu_seqlens = cu_seqlens.data_ptr()
+    return args
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(T, seqs, E):
+    return _lib.load().dgm_router_balance_workspace_bytes(T, seqs, E)
 
 
 def _forward(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score):
+    """The launches, after the checks."""
     dev = logits.device
     logits, topk_idx = _rows(logits), _rows(topk_idx)
-    cu_seqlens = None if cu_seqlens is None else cu_seqlens.contiguous()
-    seqs = 1 if cu_seqlens is None else cu_seqlens.size(0) - 1
-    E = logits.size(1)
+    T, E = logits.shape
+    seqs = 1
+    if cu_seqlens is not None:
+        cu_seqlens = cu_seqlens.contiguous()
+        seqs = cu_seqlens.size(0) - 1
     loss = torch.empty((), dtype=torch.float32, device=dev)
     counts = torch.empty((E,) if cu_seqlens is None else (seqs, E), dtype=torch.int32, device=dev)
-    stats = torch.empty(4 * seqs + 4, dtype=torch.int32, device=dev)       # per sequence, then the totals
-    lib = _lib.load()
-    need = lib.dgm_router_balance_workspace_bytes(logits.size(0), seqs, E)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    args = _args(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score, counts, stats, stats[-4:], loss, ws)
-    _lib.check(lib.dgm_router_balance_loss(ctypes.byref(args), _lib.stream()))
+    stats = torch.empty(4 * seqs + 4, dtype=torch.int32, device=dev)
+    args = _args(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score, counts, stats)
+    args.loss = loss.data_ptr()
+    need = _workspace_bytes(T, seqs, E)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need
+    _lib.check(_lib.load().dgm_router_balance_loss(ctypes.byref(args), _lib.stream()))
     return loss, counts, stats
 
 
@@ -70,8 +85,8 @@ def _backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, balance_coef,
     logits, topk_idx = _rows(logits), _rows(topk_idx)
     cu_seqlens = None if cu_seqlens is None else cu_seqlens.contiguous()
     d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    args = _args(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score, counts, stats, stats[-4:], d_loss=d_loss,
-                 d_logits=d_logits)
+    args = _args(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score, counts, stats)
+    args.d_loss, args.d_logits, args.d_logits_stride = d_loss.data_ptr(), d_logits.data_ptr(), logits.size(1)
     _lib.check(_lib.load().dgm_router_balance_loss_backward(ctypes.byref(args), _lib.stream()))
     return d_logits
 
