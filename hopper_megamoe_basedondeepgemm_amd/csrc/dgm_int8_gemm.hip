@@ -14,10 +14,6 @@ using namespace dgm;
 
 namespace {
 
-typedef int v16i __attribute__((ext_vector_type(16)));
-
-DGM_DEV v16i mfma_i8_32x32x32(v4i a, v4i b, v16i c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
-
 DGM_DEV float swiglu(float g, float u, float clamp, bool fast) {
   g = fminf(g, clamp);
   u = fminf(fmaxf(u, -clamp), clamp);
@@ -244,7 +240,9 @@ __device__ const uint4 k_zeros = {0u, 0u, 0u, 0u};
 // half lines, 64-byte steps, cost as many cycles of a CU's 64 B / clock). Both operands' rows go from HBM /
 // L2 straight into LDS, STAGES - 1 steps ahead of the one that is multiplied, with one barrier a step. A
 // row's eight 16-byte pieces lie permuted by the row's number, so that the lanes reading one piece of 16
-// rows meet 16 different bank groups (no conflicts counted).
+// rows meet 16 different bank groups (no conflicts counted). The 16 x 16 x 64 matrix instruction, whose
+// accumulators move half as often per product as those of 32 x 32 x 32: the large products run at the clock
+// that the card's power allows, and 8192 x 8192 x 4096 takes 246 us with it instead of 276.
 // SwiGLU: blocks of 32 channel rows alternate between gate and up rows, so that a wave holds both of a
 // channel.
 // Few tiles: gridDim.y workgroups share a tile, each a range of K, and leave their int32 sums in the
@@ -252,8 +250,8 @@ __device__ const uint4 k_zeros = {0u, 0u, 0u, 0u};
 template <int BM, int BN, int WM, int WN, int STAGES, bool SWIGLU>
 __global__ void __launch_bounds__(64 * WM * WN) k_int8_gemm_tiles(const DgmInt8GemmArgs P, int vec, int tiles_m, int tiles_n,
                                                                   int steps_per_split) {
-  constexpr int W = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, ROWS = BM + BN, LOADS = ROWS / (8 * W);
-  static_assert(ROWS % (8 * W) == 0 && BM % (8 * W) == 0 && W % 2 == 0 && (!SWIGLU || TN % 2 == 0), "whole loads per wave");
+  constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, ROWS = BM + BN, LOADS = ROWS / (8 * W);
+  static_assert(ROWS % (8 * W) == 0 && BM % (8 * W) == 0 && W % 2 == 0 && TM % 2 == 0 && (!SWIGLU || TN % 4 == 0), "whole loads per wave");
   __shared__ __attribute__((aligned(1024))) int8_t lds[STAGES][ROWS * 128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int split = blockIdx.y, k_begin = split * steps_per_split * 128;
@@ -301,26 +299,26 @@ __global__ void __launch_bounds__(64 * WM * WN) k_int8_gemm_tiles(const DgmInt8G
         load((const int8_t*)(k0 + 16 * piece < K ? (uint64_t)src[i] + (uint64_t)k0 : zeros), to + (i * W + wave) * 1024);
     }
   };
-  v16i acc[TN][TM];
+  v4i acc[TN][TM];
 #pragma unroll
   for (int n = 0; n < TN; ++n)
 #pragma unroll
-    for (int m = 0; m < TM; ++m) acc[n][m] = v16i{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  const int r = lane & 31, half = lane >> 5, wm = wave % WM, wn = wave / WM;
+    for (int m = 0; m < TM; ++m) acc[n][m] = v4i{0, 0, 0, 0};
+  const int r = lane & 15, g = lane >> 4, wm = wave % WM, wn = wave / WM;
   const int row_a = wm * (BM / WM) + r, row_b = BM + wn * (BN / WN) + r;
   auto multiply = [&](const int8_t* from) {
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      const int at = ((2 * kk + half) ^ ((r >> 1) & 7)) * 16;
+    for (int kk = 0; kk < 2; ++kk) {
+      const int at = ((4 * kk + g) ^ ((r >> 1) & 7)) * 16;
       v4i av[TM], bv[TN];
 #pragma unroll
-      for (int m = 0; m < TM; ++m) av[m] = *reinterpret_cast<const v4i*>(from + (row_a + 32 * m) * 128 + at);
+      for (int n = 0; n < TN; ++n) bv[n] = *reinterpret_cast<const v4i*>(from + (row_b + 16 * n) * 128 + at);
 #pragma unroll
-      for (int n = 0; n < TN; ++n) bv[n] = *reinterpret_cast<const v4i*>(from + (row_b + 32 * n) * 128 + at);
+      for (int m = 0; m < TM; ++m) av[m] = *reinterpret_cast<const v4i*>(from + (row_a + 16 * m) * 128 + at);
 #pragma unroll
-      for (int n = 0; n < TN; ++n)
+      for (int m = 0; m < TM; ++m)
 #pragma unroll
-        for (int m = 0; m < TM; ++m) acc[n][m] = mfma_i8_32x32x32(bv[n], av[m], acc[n][m]);
+        for (int n = 0; n < TN; ++n) acc[n][m] = mfma_i8_16x16x64(bv[n], av[m], acc[n][m]);
     }
   };
 #pragma unroll
@@ -338,7 +336,9 @@ __global__ void __launch_bounds__(64 * WM * WN) k_int8_gemm_tiles(const DgmInt8G
   // Results through LDS, 32 tokens of a wave at a time: from the lanes' four channels of 32 tokens to 16-byte
   // pieces of whole token rows (stored from the lanes, a 8192 x 8192 output took 80 us longer). Rows are
   // padded by 16 bytes, so that neither side meets bank conflicts.
-  constexpr int H = SWIGLU ? 2 : 1, CW = 32 * TN / H, PITCH = CW + 4;
+  constexpr int H = SWIGLU ? 2 : 1, CW = 16 * TN / H, PITCH = CW + 4;
+  // (SwiGLU: the wave's fragments of 16 channels are two of gate rows, two of up rows, ...)
+  auto frag = [](int n, int h) { return SWIGLU ? (n / 2) * 4 + n % 2 + 2 * h : n; };
   static_assert(W * 32 * PITCH * 4 <= (int)sizeof(lds), "the waves' parts fit");
   __syncthreads();
   float* part = reinterpret_cast<float*>(&lds[0][0]) + wave * 32 * PITCH;
@@ -346,16 +346,14 @@ __global__ void __launch_bounds__(64 * WM * WN) k_int8_gemm_tiles(const DgmInt8G
   if (gridDim.y > 1) {
     int* ws = P.workspace + (int64_t)split * P.m * P.n;
 #pragma unroll
-    for (int m = 0; m < TM; ++m)
+    for (int m = 0; m < TM / 2; ++m)
 #pragma unroll
       for (int h = 0; h < H; ++h) {
 #pragma unroll
-        for (int n = h; n < TN; n += H)
+        for (int n = 0; n < TN / H; ++n)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const v16i& x = acc[n][m];
-            *reinterpret_cast<v4i*>(part + r * PITCH + 32 * (n / H) + 8 * q + 4 * half) = v4i{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
-          }
+          for (int q = 0; q < 2; ++q)
+            *reinterpret_cast<v4i*>(part + (16 * q + r) * PITCH + 16 * n + 4 * g) = acc[frag(n, h)][2 * m + q];
         wave_sync();
         constexpr int L = CW / 4;
 #pragma unroll
@@ -375,31 +373,30 @@ __global__ void __launch_bounds__(64 * WM * WN) k_int8_gemm_tiles(const DgmInt8G
       }
     return;
   }
-  v4f sb[TN][4];
+  v4f sb[TN];
 #pragma unroll
-  for (int n = 0; n < TN; n += H)
+  for (int n = 0; n < TN / H; ++n) {
+    const int64_t c = c0 + 16 * n + 4 * g;
+    sb[frag(n, 0)] = load_scales(P, c, n_out);
+    if constexpr (SWIGLU) sb[frag(n, 1)] = load_scales(P, n_out + c, 2 * n_out);
+  }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int64_t c = c0 + 32 * n / H + 8 * q + 4 * half;
-      sb[n][q] = load_scales(P, c, n_out);
-      if constexpr (SWIGLU) sb[n + 1][q] = load_scales(P, n_out + c, 2 * n_out);
-    }
+  for (int m = 0; m < TM / 2; ++m) {
 #pragma unroll
-  for (int m = 0; m < TM; ++m) {
-    const int64_t token = t0 + 32 * m + r;
-    const float sa = P.sfa[(token < P.m ? token : P.m - 1) * P.sfa_stride];
+    for (int q = 0; q < 2; ++q) {
+      const int64_t token = t0 + 32 * m + 16 * q + r;
+      const float sa = P.sfa[(token < P.m ? token : P.m - 1) * P.sfa_stride];
 #pragma unroll
-    for (int n = 0; n < TN; n += H)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int n = 0; n < TN / H; ++n) {
         v4f v;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          v[i] = (float)acc[n][m][4 * q + i] * (sa * sb[n][q][i]);
-          if constexpr (SWIGLU) v[i] = swiglu(v[i], (float)acc[n + 1][m][4 * q + i] * (sa * sb[n + 1][q][i]), P.clamp, P.fast_math);
+          v[i] = (float)acc[frag(n, 0)][2 * m + q][i] * (sa * sb[frag(n, 0)][i]);
+          if constexpr (SWIGLU) v[i] = swiglu(v[i], (float)acc[frag(n, 1)][2 * m + q][i] * (sa * sb[frag(n, 1)][i]), P.clamp, P.fast_math);
         }
-        *reinterpret_cast<v4f*>(part + r * PITCH + 32 * n / H + 8 * q + 4 * half) = v;
+        *reinterpret_cast<v4f*>(part + (16 * q + r) * PITCH + 16 * n + 4 * g) = v;
       }
+    }
     wave_sync();
     with_epilogue(P, [&](auto t, auto add) {
       constexpr int E = t.value == DGM_SRC_F32 ? 4 : 8, L = CW / E;      // elements of a piece, pieces of a row
@@ -475,6 +472,7 @@ void launch_tiles(const DgmInt8GemmArgs& A, int vec, int splits, hipStream_t str
 //   128 x 128, 4 stages (one a CU):        0.77 us         (1024 x 4096: 27 us; 2 stages 35, 256 x 256 58)
 //   128 x 128, 2 stages:                   1.0 / 1.33 us   (2048 x 4096: 43 us; 4 stages 50, 256 x 256 59)
 //   256 x 256, 2 stages (one a CU):        2.0 us          (4096 x 4096: 70 us; 128 x 128 84 and 98)
+// (measured with the 32 x 32 x 32 instruction, which the ratios between the forms do not depend on)
 // The rows form takes 2 us and, per 1024 of K and 256 workgroups, 0.8 us up to 4 tokens, 1.0 up to 16, 1.4
 // up to 32 and 2.4 up to 64 (SwiGLU: 2.5 times the first two, 1.5 times the others): 16 x 4096, K 4096: 7 us
 // (tiles, 4 splits 11); 64 x 4096, K 7168: 22 us (tiles, 8 splits 16).
