@@ -59,39 +59,42 @@ def int8_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_m
     if m >= 1 << 20 or n >= 1 << 24:
         raise ValueError(f"m {m} and n {n}: below 2^20 and 2^24")
     n_out = n // 2 if swiglu else n
-    if d.dtype not in _lib.SRC_DTYPES or tuple(d.shape) != (m, n_out):
+    if d.dtype not in _lib.SRC_DTYPES or d.dim() != 2 or d.size(0) != m or d.size(1) != n_out:
         raise TypeError(f"d: bf16, fp16 or fp32 [{m}, {n_out}] expected, got {d.dtype} {tuple(d.shape)}")
-    if d.numel() and ((n_out > 1 and d.stride(1) != 1) or (m > 1 and d.stride(0) < n_out)):
+    d_stride = d.stride(0)
+    if m and n_out and ((n_out > 1 and d.stride(1) != 1) or (m > 1 and d_stride < n_out)):
         raise ValueError("d: rows must be contiguous and must not overlap")
     if c is not None and (c.dtype != d.dtype or tuple(c.shape) not in ((m, n_out), (n_out,))):
         raise TypeError(f"c: {d.dtype} [{m}, {n_out}] or [{n_out}] expected, got {c.dtype} {tuple(c.shape)}")
     _lib.require_one_device(d, aq, asf, bq, bsf, c)
-    if torch.is_grad_enabled() and (d.requires_grad or (c is not None and c.requires_grad)):
+    if (d.requires_grad or (c is not None and c.requires_grad)) and torch.is_grad_enabled():
         raise RuntimeError("int8_gemm_nt has no gradient: call it under torch.no_grad()")
     if m == 0 or n_out == 0:
         return d
     aq, bq = _rows(aq), _rows(bq)
-    lo, hi = d.data_ptr(), d.data_ptr() + ((m - 1) * d.stride(0) + n_out) * d.element_size()
-    pa, pb = aq.data_ptr(), bq.data_ptr()
-    if (pa < hi and lo < pa + (m - 1) * aq.stride(0) + k) or (pb < hi and lo < pb + (n - 1) * bq.stride(0) + k):
+    size = d.element_size()
+    pa, pb, lo, a_stride, b_stride = aq.data_ptr(), bq.data_ptr(), d.data_ptr(), aq.stride(0), bq.stride(0)
+    hi = lo + ((m - 1) * d_stride + n_out) * size
+    if (pa < hi and lo < pa + (m - 1) * a_stride + k) or (pb < hi and lo < pb + (n - 1) * b_stride + k):
         raise ValueError("d overlaps an operand")
-    c_stride = 0
+    args = _lib.Int8GemmArgs(pa, asf.data_ptr(), pb, bsf.data_ptr(), 0, lo, m, n, k, a_stride, asf.stride(0), b_stride,
+                             bsf.stride(0), 0, d_stride, _lib.SRC_DTYPES[d.dtype], swiglu,
+                             3.0e38 if activation_clamp is None else float(activation_clamp), 1 if fast_math else 0)
     if c is not None:
         if c.dim() == 1:
-            c = c.contiguous()
+            c, c_stride, end = c.contiguous(), 0, n_out
         else:
             c = _rows(c)
             c_stride = c.stride(0)
-        end = c.data_ptr() + (n_out if c.dim() == 1 else (m - 1) * c_stride + n_out) * c.element_size()
-        if c.data_ptr() < hi and lo < end and not (c.dim() == 2 and c.data_ptr() == lo and (m == 1 or c_stride == d.stride(0))):
+            end = (m - 1) * c_stride + n_out
+        pc = c.data_ptr()
+        if pc < hi and lo < pc + end * size and not (pc == lo and c.dim() == 2 and (m == 1 or c_stride == d_stride)):
             raise ValueError("c overlaps d other than as the same rows")
+        args.c, args.c_stride = pc, c_stride
     need = _workspace_bytes(m, n, k, swiglu)
-    ws = torch.empty(need, dtype=torch.uint8, device=d.device) if need else None
-    args = _lib.Int8GemmArgs(pa, asf.data_ptr(), pb, bsf.data_ptr(), 0 if c is None else c.data_ptr(),
-                             lo, m, n, k, aq.stride(0), asf.stride(0), bq.stride(0), bsf.stride(0), c_stride,
-                             d.stride(0), _lib.SRC_DTYPES[d.dtype], int(swiglu),
-                             float(activation_clamp if activation_clamp is not None else 3.0e38), int(bool(fast_math)),
-                             0 if ws is None else ws.data_ptr(), need)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=d.device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need
     _lib.check(_lib.load().dgm_int8_gemm_nt(ctypes.byref(args), _lib.stream()))
     return d
 
