@@ -209,7 +209,8 @@ def _backward(d_r, d_h, x, residual, post_weight, pre_weight, gate, forward, nee
     return d_x, d_residual, d_post, d_pre, d_gate
 
 
-_INPUTS = ("x", "residual", "post_weight", "pre_weight", "gate")
+def _places(tensors):
+    return [None if t is None else (t.data_ptr(), t.stride()) for t in tensors]
 
 
 class _RmsNormResidual(torch.autograd.Function):
@@ -217,10 +218,11 @@ class _RmsNormResidual(torch.autograd.Function):
     def forward(ctx, x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps):
         r, h, _, _, rstd, args, read = _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps,
                                                 None, None, None, True)
-        ctx.save_for_backward(x, residual, post_weight, pre_weight, gate, rstd)
-        ctx.args = args
-        # (inputs that the kernels read as copies: those copies)
-        ctx.copies = [None if u is t else u for t, u in zip((x, residual, post_weight, pre_weight, gate), read)]
+        saved = x, residual, post_weight, pre_weight, gate, rstd
+        ctx.save_for_backward(*saved)
+        ctx.options = gate_sigmoid, residual_scale, eps
+        # (the launch's arguments, those copies that the kernels read for inputs, and where the saved tensors were)
+        ctx.args, ctx.copies, ctx.places = args, [None if u is t else u for t, u in zip(saved, read[:5])], _places(saved)
         ctx.set_materialize_grads(False)
         return (None if r is x else r), h
 
@@ -229,10 +231,13 @@ class _RmsNormResidual(torch.autograd.Function):
         _lib.no_second_derivative()
         saved = ctx.saved_tensors
         args = ctx.args
-        # (a tensor's memory may have moved since the forward pass)
-        for name, t, copy in zip(_INPUTS, saved, ctx.copies):
-            if t is not None:
-                setattr(args, name, (t if copy is None else copy).data_ptr())
+        if _places(saved) != ctx.places:
+            # Other memory since the forward pass: storage replaced, or tensors that saved-tensor hooks brought
+            # back (offloading, recomputation), the rstd rows among them and in strides of their own.
+            read = _readable(*saved[:5])
+            rstd = saved[5].contiguous()
+            at = rstd.data_ptr()
+            args = _forward_args(*read[:5], *ctx.options, read[5], at, at if saved[2] is None else at + 4 * rstd.size(1))
         return (*_backward(d_r, d_h, *saved[:5], args, ctx.needs_input_grad), None, None, None)
 
 

@@ -340,6 +340,44 @@ def test_memory_that_moves_between_the_passes():
     assert all(torch.equal(a, b) for a, b in zip(want, again))
 
 
+@pytest.mark.parametrize("way", ["offload", "recompute", "moved"])
+@pytest.mark.parametrize("post,pre", [(1, 1), (0, 1), (1, 0), (0, 0)])
+def test_saved_tensors_that_hooks_bring_back(way, post, pre):
+    """Tensors saved for the backward pass that come back in other memory and other strides, the rstd rows among them:
+    the gradients are those of the plain call, bit for bit."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    from torch.utils.checkpoint import checkpoint
+    x, r, w1, w2, gt = make(37, 200, torch.bfloat16, torch.float32, post, pre, "full", 1, seed=9)
+    wide = torch.randn((37, 320), device="cuda").to(torch.bfloat16)
+    wide[:, 40:240] = x
+    dr, dh = torch.randn_like(x), torch.randn_like(x)
+
+    def grads(how):
+        base, leaves = wide.clone().requires_grad_(), [v if v is None else v.clone().requires_grad_() for v in (r, w1, w2, gt)]
+
+        def run(base, *rest):
+            return dgm.rms_norm_residual(base[:, 40:240], *rest, True, 0.5)
+        if how == "offload":
+            with torch.autograd.graph.save_on_cpu():
+                got = run(base, *leaves)
+        elif how == "recompute":
+            got = checkpoint(run, base, *leaves, use_reentrant=False)
+        elif how == "moved":
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2
+                                                          else t.clone()):
+                got = run(base, *leaves)
+        else:
+            got = run(base, *leaves)
+        keep = [torch.full((2, 37), 7.0, device="cuda") for _ in range(64)]     # (over rows that were given up)
+        pairs = [(o, d) for o, d in zip(got, (dr, dh)) if o is not None]
+        out = torch.autograd.grad([o for o, _ in pairs], [base] + [v for v in leaves if v is not None], [d for _, d in pairs])
+        del keep
+        return out
+    for a, b in zip(grads("plain"), grads(way)):
+        assert torch.equal(a, b)
+
+
 def test_autograd_refusals():
     need_gpu()
     import hopper_megamoe_basedondeepgemm_amd as dgm
