@@ -26,8 +26,8 @@ def mega_moe_block(x, norm_weight, router_weight, l1, l2, sym_buffer, residual=N
     Returns ``(r, h)``: the new residual stream and, with ``next_weight``, the next norm's output (else
     None). Inference only: under autograd it raises."""
     weights = () if shared_expert is None else tuple(t for pair in shared_expert for t in pair)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, residual, norm_weight, router_weight, post_weight, gate, next_weight)):
+    leaves = (x, residual, norm_weight, router_weight, post_weight, gate, next_weight) + weights
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves):
         raise RuntimeError("mega_moe_block has no gradient: call it under torch.no_grad()")
     if x.dim() != 2 or x.dtype != torch.bfloat16 or x.size(1) != sym_buffer.hidden:
         raise TypeError(f"x must be bf16 [tokens, {sym_buffer.hidden}], got {x.dtype} {tuple(x.shape)}")

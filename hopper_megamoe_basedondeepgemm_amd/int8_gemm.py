@@ -66,9 +66,10 @@ def int8_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_m
         raise ValueError("d: rows must be contiguous and must not overlap")
     if c is not None and (c.dtype != d.dtype or tuple(c.shape) not in ((m, n_out), (n_out,))):
         raise TypeError(f"c: {d.dtype} [{m}, {n_out}] or [{n_out}] expected, got {c.dtype} {tuple(c.shape)}")
-    _lib.require_one_device(d, aq, asf, bq, bsf, c)
-    if (d.requires_grad or (c is not None and c.requires_grad)) and torch.is_grad_enabled():
+    if (d.requires_grad or asf.requires_grad or bsf.requires_grad
+            or (c is not None and c.requires_grad)) and torch.is_grad_enabled():
         raise RuntimeError("int8_gemm_nt has no gradient: call it under torch.no_grad()")
+    _lib.require_one_device(d, aq, asf, bq, bsf, c)
     if m == 0 or n_out == 0:
         return d
     aq, bq = _rows(aq), _rows(bq)

@@ -47,6 +47,20 @@ def test_refusals(a, b, d, kw, err, what):
         dgm.int8_gemm_nt(a, b, d, **kw)
 
 
+@pytest.mark.parametrize("leaf", ["sfa", "sfb", "c", "d"])
+def test_no_gradient_is_dropped(leaf):
+    """A product, or a block, over leaves that ask for a gradient is refused, their scales among them."""
+    a, b, d, c = rows(4, 32), rows(8, 32), torch.zeros(4, 8), torch.zeros(4, 8)
+    {"sfa": a[1], "sfb": b[1], "c": c, "d": d}[leaf].requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        dgm.int8_gemm_nt(a, b, d, c=c)
+    with pytest.raises(RuntimeError, match="GPU"), torch.no_grad():
+        dgm.int8_gemm_nt(a, b, d, c=c)
+    if leaf == "sfb":
+        with pytest.raises(RuntimeError, match="no gradient"):
+            dgm.mega_moe_block(bf(4, 32), bf(32), bf(2, 32), None, None, None, shared_expert=(b, a))
+
+
 def test_c_entry_refusals():
     lib, p = _lib.load(), 4096          # (never dereferenced: refused first)
     base = dict(a=p, sfa=p, b=p, sfb=p, d=p, m=4, n=8, k=32, a_stride=32, b_stride=32, d_stride=8, sfa_stride=1, sfb_stride=1)
