@@ -9,9 +9,10 @@
 //
 // Sixteen lanes take a token, in 16-byte pieces of its row (a whole wave per token spent most of its time on
 // the reductions and the scalar work of a token: 65536 x 256 bf16 76 us for loss and gradient, now 50); all
-// passes read the logits once, so the bound is HBM. Sums over tokens: a workgroup's waves add their tokens of one sequence in registers and leave one
-// row of sums per (chunk, sequence) at slot chunk + sequence (a walk that takes one step per slot, so slots
-// are distinct), which k_balance_columns adds up in a fixed order: no atomics on floats, no cleared memory.
+// passes read the logits once, so the bound is HBM. Sums over tokens: a workgroup's waves add their tokens of
+// one sequence in registers and leave one row of sums per (chunk, sequence) at slot chunk + sequence (a walk
+// that takes one step per slot, so slots are distinct), which k_balance_columns adds up in a fixed order: no
+// atomics on floats, no cleared memory.
 #include "dgm_common.hpp"
 #include "dgm_abi_internal.hpp"
 #include "dgm_rows.hpp"

@@ -241,3 +241,29 @@ def test_strides_frontend_buffer_and_streams():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(held, both())), i
+
+
+@pytest.mark.parametrize("way", ["offload", "recompute"])
+def test_saved_tensors_that_hooks_bring_back(way):
+    """Tensors saved for the backward pass that come back in other memory and strides: the same gradient, bit for bit."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    from torch.utils.checkpoint import checkpoint
+    logits, idx = make(300, 64, 4, seed=6)
+    cu = torch.tensor([0, 100, 290], dtype=torch.int32, device="cuda")
+
+    def grad(how):
+        leaf = logits.t().contiguous().requires_grad_()
+
+        def run(v):
+            return dgm.router_balance_loss(v.t(), idx, cu, 1.0, 0.01)[0]
+        if how == "offload":
+            with torch.autograd.graph.save_on_cpu():
+                loss = run(leaf)
+        else:
+            loss = checkpoint(run, leaf, use_reentrant=False) if how == "recompute" else run(leaf)
+        keep = [torch.full((12,), 7, dtype=torch.int32, device="cuda") for _ in range(64)]      # (over given up memory)
+        out = torch.autograd.grad(loss, leaf)[0]
+        del keep
+        return out
+    assert torch.equal(grad("plain"), grad(way))
