@@ -243,7 +243,7 @@ __device__ const uint4 k_zeros = {0u, 0u, 0u, 0u};
 // rows meet 16 different bank groups (no conflicts counted). The 16 x 16 x 64 matrix instruction, whose
 // accumulators move half as often per product as those of 32 x 32 x 32: the large products run at the clock
 // that the card's power allows, and 8192 x 8192 x 4096 takes 246 us with it instead of 276.
-// SwiGLU: blocks of 32 channel rows alternate between gate and up rows, so that a wave holds both of a
+// SwiGLU: blocks of 16 channel rows alternate between gate and up rows, so that a wave holds both of a
 // channel.
 // Few tiles: gridDim.y workgroups share a tile, each a range of K, and leave their int32 sums in the
 // workspace [split][token][channel] for k_int8_gemm_join.
@@ -251,7 +251,7 @@ template <int BM, int BN, int WM, int WN, int STAGES, bool SWIGLU>
 __global__ void __launch_bounds__(64 * WM * WN) k_int8_gemm_tiles(const DgmInt8GemmArgs P, int vec, int tiles_m, int tiles_n,
                                                                   int steps_per_split) {
   constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, ROWS = BM + BN, LOADS = ROWS / (8 * W);
-  static_assert(ROWS % (8 * W) == 0 && BM % (8 * W) == 0 && W % 2 == 0 && TM % 2 == 0 && (!SWIGLU || TN % 4 == 0), "whole loads per wave");
+  static_assert(ROWS % (8 * W) == 0 && BM % (8 * W) == 0 && W % 2 == 0 && TM % 2 == 0 && (!SWIGLU || TN % 2 == 0), "whole loads per wave");
   __shared__ __attribute__((aligned(1024))) int8_t lds[STAGES][ROWS * 128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int split = blockIdx.y, k_begin = split * steps_per_split * 128;
@@ -275,9 +275,9 @@ __global__ void __launch_bounds__(64 * WM * WN) k_int8_gemm_tiles(const DgmInt8G
       src[i] = P.a + (m < P.m ? m : P.m - 1) * P.a_stride + 16 * piece;
     } else {
       const int rb = row - BM;
-      int64_t n = SWIGLU ? n0 + (rb >> 6) * 32 + (rb & 31) : n0 + rb;
+      int64_t n = SWIGLU ? n0 + (rb >> 5) * 16 + (rb & 15) : n0 + rb;
       n = n < n_out ? n : n_out - 1;
-      if (SWIGLU && (rb & 32)) n += n_out;
+      if (SWIGLU && (rb & 16)) n += n_out;
       src[i] = P.b + n * P.b_stride + 16 * piece;
     }
   }
@@ -337,8 +337,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_int8_gemm_tiles(const DgmInt8G
   // pieces of whole token rows (stored from the lanes, a 8192 x 8192 output took 80 us longer). Rows are
   // padded by 16 bytes, so that neither side meets bank conflicts.
   constexpr int H = SWIGLU ? 2 : 1, CW = 16 * TN / H, PITCH = CW + 4;
-  // (SwiGLU: the wave's fragments of 16 channels are two of gate rows, two of up rows, ...)
-  auto frag = [](int n, int h) { return SWIGLU ? (n / 2) * 4 + n % 2 + 2 * h : n; };
+  // (SwiGLU: the wave's fragments of 16 channels are gate and up rows in turn)
+  auto frag = [](int n, int h) { return SWIGLU ? 2 * n + h : n; };
   static_assert(W * 32 * PITCH * 4 <= (int)sizeof(lds), "the waves' parts fit");
   __syncthreads();
   float* part = reinterpret_cast<float*>(&lds[0][0]) + wave * 32 * PITCH;
@@ -464,28 +464,35 @@ void launch_tiles(const DgmInt8GemmArgs& A, int vec, int splits, hipStream_t str
   else hipLaunchKernelGGL(k_int8_gemm_join<false>, join, dim3(256), 0, stream, A, vec, splits);
 }
 
-// Which kernel takes an aligned product, from estimates of its time in us (256 CUs). A tile form takes
-// `alone` us per K step while every workgroup has a CU to itself, `full` us when the CUs hold as many as
-// fit (2 or 1), and 4 us around it; splitting K costs a second launch and the sums' way through memory
-// (3.5 TB/s). The step times were measured with K = 4096:
-//   64 x 128 tokens x channels, 3 stages:  0.60 / 0.97 us  (256 x 4096: 20 us; the 128 x 128 forms 24 and 32)
-//   128 x 128, 4 stages (one a CU):        0.77 us         (1024 x 4096: 27 us; 2 stages 35, 256 x 256 58)
-//   128 x 128, 2 stages:                   1.0 / 1.33 us   (2048 x 4096: 43 us; 4 stages 50, 256 x 256 59)
-//   256 x 256, 2 stages (one a CU):        2.0 us          (4096 x 4096: 70 us; 128 x 128 84 and 98)
-// (measured with the 32 x 32 x 32 instruction, which the ratios between the forms do not depend on)
+// Which kernel takes an aligned product, from estimates of its time in us (256 CUs). A tile form takes `alone`
+// us per K step while every workgroup has a CU to itself, `full` us when the CUs hold as many as fit, and 4.2 us
+// around it; splitting K costs a second launch and the sums' way through memory (2.9 TB/s). The step times are
+// fitted to 137 products of 17 to 8192 tokens with every form and split, none warm in the caches: the estimates'
+// choice takes 0.5 % longer than the best form on average. Where each form is the best (us; next best):
+//   64 x 64, 4 stages:    256 x 4096, K 2048: 8.8 (64 x 128 9.7);    200 x 2880, K 2880: 10.6 (12.1)
+//   64 x 128, 3 stages:   300 x 5120, K 2880: 12.7 (64 x 64 15.9);   512 x 4096, K 2048: 10.4 (11.5)
+//   128 x 128, 4 stages:  1024 x 4096, K 7168: 38.8 (192 x 128 46);  512 x 8192, K 4096: 25.4 (30)
+//   128 x 128, 2 stages:  2048 x 4096, K 2048: 23.2 (128 x 256 24.3); 777 x 7168, K 2048: 20.8 (64 x 128 22)
+//   192 x 128:            1000 x 5120, K 2880: 25.1 (128 x 128 28);  1536 x 4096, K 7168: 52 (58)
+//   128 x 256:            512 x 16384, K 4096: 40 (128 x 128 45);    4096 x 2048, K 4096: 38 (41)
+//   192 x 256:            1536 x 8192, K 4096: 53 (256 x 256 61);    4096 x 5120, K 2880: 82 (256 x 192 93)
+//   256 x 192:            8192 x 2880, K 2880: 88 (192 x 128 98);    4096 x 2880, K 2880: 45 (256 x 256 50)
+//   256 x 256:            8192 x 8192, K 4096: 243 (192 x 256 266);  2048 x 8192, K 4096: 69 (128 x 128 82)
+// Up to 192 x 128 the steps are bound by the loads that a CU keeps in flight (more stages: no faster).
 // The rows form takes 2 us and, per 1024 of K and 256 workgroups, 0.8 us up to 4 tokens, 1.0 up to 16, 1.4
-// up to 32 and 2.4 up to 64 (SwiGLU: 2.5 times the first two, 1.5 times the others): 16 x 4096, K 4096: 7 us
-// (tiles, 4 splits 11); 64 x 4096, K 7168: 22 us (tiles, 8 splits 16).
+// up to 32 and 3.0 up to 64 (SwiGLU: 2.5 times the first two, 1.5 times the others): 16 x 4096, K 4096: 7 us
+// (64 x 64, 4 splits 11); 64 x 5120, K 2880: 14.8 us (64 x 64: 10.1).
 struct Form { int kind, splits; };
-enum { ROWS = 0, T64, T128_DEEP, T128, T256 };
+enum { ROWS = 0, T64, T64_128, T128_DEEP, T128, T192_128, T128_256, T192_256, T256_192, T256 };
 Form choose(int64_t m, int64_t n, int64_t k, bool swiglu, int64_t workspace_bytes) {
   static const struct { int bm, bn, per_cu; double alone, full; } tiles[] = {
-      {0, 0, 0, 0, 0}, {64, 128, 2, 0.60, 0.97}, {128, 128, 1, 0.77, 0.77}, {128, 128, 2, 1.0, 1.33}, {256, 256, 1, 2.0, 2.0}};
+      {0, 0, 0, 0, 0},           {64, 64, 2, 0.36, 0.64},  {64, 128, 2, 0.55, 0.88}, {128, 128, 1, 0.67, 0.67}, {128, 128, 2, 0.86, 1.14},
+      {192, 128, 1, 0.85, 0.85}, {128, 256, 1, 1.1, 1.1},  {192, 256, 1, 1.28, 1.28}, {256, 192, 1, 1.35, 1.5},  {256, 256, 1, 1.65, 1.65}};
   const int64_t steps = (k + 127) / 128;
   Form best = {ROWS, 1};
   double least = 1e30;
   if (m <= 64) {
-    const double c = (m <= 4 ? 0.8 : m <= 16 ? 1.0 : m <= 32 ? 1.4 : 2.4) * (!swiglu ? 1.0 : m <= 16 ? 2.5 : 1.5);
+    const double c = (m <= 4 ? 0.8 : m <= 16 ? 1.0 : m <= 32 ? 1.4 : 3.0) * (!swiglu ? 1.0 : m <= 16 ? 2.5 : 1.5);
     const double wgs = (double)((n / (swiglu ? 2 : 1) + 15) / 16) / 256;
     least = 2 + (double)((k + 1023) / 1024) * c * (wgs < 1 ? 1 : wgs);
   }
@@ -494,8 +501,8 @@ Form choose(int64_t m, int64_t n, int64_t k, bool swiglu, int64_t workspace_byte
       if (s > 1 && (steps < 2 * s || (int64_t)s * m * n * 4 > workspace_bytes)) break;
       const int64_t wgs = ((m + tiles[t].bm - 1) / tiles[t].bm) * ((n + tiles[t].bn - 1) / tiles[t].bn) * s;
       const int64_t rounds = (wgs + 256 * tiles[t].per_cu - 1) / (256 * tiles[t].per_cu);
-      double us = 4 + (double)((steps + s - 1) / s) * (wgs <= 256 ? tiles[t].alone : tiles[t].full * (double)rounds);
-      if (s > 1) us += 3 + 8e-6 / 3.5 * (double)s * (double)m * (double)n;
+      double us = 4.2 + (double)((steps + s - 1) / s) * (wgs <= 256 ? tiles[t].alone : tiles[t].full * (double)rounds);
+      if (s > 1) us += 3.8 + 8e-6 / 2.9 * (double)s * (double)m * (double)n;
       if (us < least) least = us, best = {t, s};
     }
   return best;
@@ -536,10 +543,15 @@ int dgm_int8_gemm_nt(const DgmInt8GemmArgs* args, hipStream_t stream) {
   const int vec = (((uintptr_t)A.d | (uintptr_t)A.c | (uint64_t)(A.d_stride * e) | (uint64_t)(A.c_stride * e)) & 15) == 0;
   const int64_t held = A.workspace && ((uintptr_t)A.workspace & 15) == 0 ? A.workspace_bytes : 0;
   const Form f = aligned ? choose(A.m, A.n, A.k, A.swiglu != 0, held < MOST_WORKSPACE ? held : MOST_WORKSPACE) : Form{ROWS, 1};
-  if (f.kind == T256) launch_tiles<256, 256, 2, 4, 2>(A, vec, f.splits, stream);
-  else if (f.kind == T128) launch_tiles<128, 128, 2, 2, 2>(A, vec, f.splits, stream);
-  else if (f.kind == T128_DEEP) launch_tiles<128, 128, 2, 2, 4>(A, vec, f.splits, stream);
-  else if (f.kind == T64) launch_tiles<64, 128, 2, 2, 3>(A, vec, f.splits, stream);
+  if (f.kind == T64) launch_tiles<64, 64, 2, 2, 4>(A, vec, f.splits, stream);
+  else if (f.kind == T64_128) launch_tiles<64, 128, 2, 4, 3>(A, vec, f.splits, stream);
+  else if (f.kind == T128_DEEP) launch_tiles<128, 128, 2, 4, 4>(A, vec, f.splits, stream);
+  else if (f.kind == T128) launch_tiles<128, 128, 2, 4, 2>(A, vec, f.splits, stream);
+  else if (f.kind == T192_128) launch_tiles<192, 128, 2, 4, 3>(A, vec, f.splits, stream);
+  else if (f.kind == T128_256) launch_tiles<128, 256, 2, 4, 3>(A, vec, f.splits, stream);
+  else if (f.kind == T192_256) launch_tiles<192, 256, 2, 4, 2>(A, vec, f.splits, stream);
+  else if (f.kind == T256_192) launch_tiles<256, 192, 4, 2, 2>(A, vec, f.splits, stream);
+  else if (f.kind == T256) launch_tiles<256, 256, 2, 4, 2>(A, vec, f.splits, stream);
   else if (A.m <= 16) launch_rows<1>(A, aligned, vec, stream);
   else if (A.m <= 32) launch_rows<2>(A, aligned, vec, stream);
   else launch_rows<4>(A, aligned, vec, stream);

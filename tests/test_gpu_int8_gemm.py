@@ -77,6 +77,27 @@ def test_shapes(m, n, k):
             check_swiglu(d, ref, clamp)
 
 
+@pytest.mark.parametrize("m,n,k", [(69, 8278, 144), (200, 8242, 160), (392, 8206, 144), (586, 8292, 144), (4100, 1830, 144),
+                                   (1025, 7226, 144), (1732, 6474, 144), (1543, 7174, 144), (50, 4246, 4112), (18, 7758, 4112),
+                                   (65, 8270, 7184), (67, 4354, 7184), (133, 5502, 7184), (67, 8222, 10256), (135, 8284, 10256),
+                                   (225, 8230, 10256), (585, 4106, 16400)])
+def test_ragged_tiles(m, n, k):
+    """The tile sizes that wide outputs and long sums take, whole and in ranges of K, with edges in every direction."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    a, b = make(m, n, k, seed=m + k)
+    ref = product(a, b)
+    d = torch.full((m + 1, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    bias = torch.randn(n, device="cuda").to(torch.bfloat16)
+    check(dgm.int8_gemm_nt(a, b, d[:m], c=bias), ref + bias.double(), ref.abs() + bias.double().abs())
+    f = torch.full((m, n + 3), 7.0, device="cuda")
+    check(dgm.int8_gemm_nt(a, b, f[:, :n]), ref, ref.abs())
+    assert bool((d[m:] == 7).all()) and bool((f[:, n:] == 7).all())
+    d = torch.full((m + 1, n // 2), 7.0, dtype=torch.bfloat16, device="cuda")
+    check_swiglu(dgm.int8_gemm_nt(a, b, d[:m], activation="swiglu", activation_clamp=2.0), ref, 2.0)
+    assert bool((d[m:] == 7).all())
+
+
 @pytest.mark.parametrize("m", [1, 7, 40, 130, 400])
 def test_extreme_values(m):
     """Codes over all of int8, -128 included; the largest k with every product 128 * 128; zero scales."""
