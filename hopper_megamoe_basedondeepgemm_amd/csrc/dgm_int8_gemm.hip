@@ -468,7 +468,8 @@ void launch_tiles(const DgmInt8GemmArgs& A, int vec, int splits, hipStream_t str
 // us per K step while every workgroup has a CU to itself, `full` us when the CUs hold as many as fit, and 4.2 us
 // around it; splitting K costs a second launch and the sums' way through memory (2.9 TB/s). The step times are
 // fitted to 137 products of 17 to 8192 tokens with every form and split, none warm in the caches: the estimates'
-// choice takes 0.5 % longer than the best form on average. Where each form is the best (us; next best):
+// choice takes 0.5 % longer than the best form on average, and 2 % on 88 other products of 1 to 12000 tokens.
+// Where each form is the best (us; next best):
 //   64 x 64, 4 stages:    256 x 4096, K 2048: 8.8 (64 x 128 9.7);    200 x 2880, K 2880: 10.6 (12.1)
 //   64 x 128, 3 stages:   300 x 5120, K 2880: 12.7 (64 x 64 15.9);   512 x 4096, K 2048: 10.4 (11.5)
 //   128 x 128, 4 stages:  1024 x 4096, K 7168: 38.8 (192 x 128 46);  512 x 8192, K 4096: 25.4 (30)
@@ -480,7 +481,7 @@ void launch_tiles(const DgmInt8GemmArgs& A, int vec, int splits, hipStream_t str
 //   256 x 256:            8192 x 8192, K 4096: 243 (192 x 256 266);  2048 x 8192, K 4096: 69 (128 x 128 82)
 // Up to 192 x 128 the steps are bound by the loads that a CU keeps in flight (more stages: no faster).
 // The rows form takes 2 us and, per 1024 of K and 256 workgroups, 0.8 us up to 4 tokens, 1.0 up to 16, 1.4
-// up to 32 and 3.0 up to 64 (SwiGLU: 2.5 times the first two, 1.5 times the others): 16 x 4096, K 4096: 7 us
+// up to 32 and 3.0 up to 64 (SwiGLU: 1.8 times the first two, 1.5 times the others): 16 x 4096, K 4096: 7 us
 // (64 x 64, 4 splits 11); 64 x 5120, K 2880: 14.8 us (64 x 64: 10.1).
 struct Form { int kind, splits; };
 enum { ROWS = 0, T64, T64_128, T128_DEEP, T128, T192_128, T128_256, T192_256, T256_192, T256 };
@@ -492,7 +493,7 @@ Form choose(int64_t m, int64_t n, int64_t k, bool swiglu, int64_t workspace_byte
   Form best = {ROWS, 1};
   double least = 1e30;
   if (m <= 64) {
-    const double c = (m <= 4 ? 0.8 : m <= 16 ? 1.0 : m <= 32 ? 1.4 : 3.0) * (!swiglu ? 1.0 : m <= 16 ? 2.5 : 1.5);
+    const double c = (m <= 4 ? 0.8 : m <= 16 ? 1.0 : m <= 32 ? 1.4 : 3.0) * (!swiglu ? 1.0 : m <= 16 ? 1.8 : 1.5);
     const double wgs = (double)((n / (swiglu ? 2 : 1) + 15) / 16) / 256;
     least = 2 + (double)((k + 1023) / 1024) * c * (wgs < 1 ? 1 : wgs);
   }
