@@ -170,32 +170,38 @@ DGM_DEV v4i load16(const int8_t* row, int k, int K) {
 }
 
 // Few tokens, or rows off 16-byte alignment (16 MT tokens per workgroup): the weights are read once per
-// workgroup row, straight into registers. A workgroup takes 16 channels (SwiGLU: their gate and up rows),
-// its eight waves the K blocks of 128 in turn (lane l: 32 bytes of row l % 16, so a block's rows are read in
-// whole 128-byte lines); the waves' int32 sums meet in LDS. One token, 4096 x 2048: 4.2 us, 2.0 TB/s. (Two or
-// four K blocks requested at once: no faster, or slower.)
-template <int MT, bool SWIGLU, bool ALIGNED>
+// workgroup row, straight into registers. A workgroup's eight waves take K blocks of 128 in turn (lane l: 32
+// bytes of row l % 16, so a block's rows are read in whole 128-byte lines); the waves' int32 sums meet in LDS.
+// KP parts of K share a fragment: its 16 rows are 16 / KP weight rows in each part, its 16 token columns 16 / KP
+// tokens in each, and of the products those of a part with itself count. A workgroup has CH channels; SwiGLU with
+// CH below the rows of a part holds gate and up rows in one fragment, else in one each.
+// One token, 4096 x 2048: 4.2 us, 2.0 TB/s. (Two or four K blocks requested at once: no faster, or slower.)
+template <int MT, int KP, int CH, bool SWIGLU, bool ALIGNED>
 __global__ void __launch_bounds__(512) k_int8_gemm_rows(const DgmInt8GemmArgs P, int vec) {
-  constexpr int W = 8, H = SWIGLU ? 2 : 1;
+  constexpr int W = 8, ROWS = 16 / KP, H = SWIGLU && CH == ROWS ? 2 : 1;
+  static_assert(KP == 1 || MT == 1, "parts of K share the token columns");
+  static_assert(CH % 4 == 0 && (CH == ROWS || (SWIGLU && 2 * CH == ROWS)), "four channels a lane");
   __shared__ v4i sums[W][H * MT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4, K = (int)P.k;
-  const int64_t n_out = SWIGLU ? P.n / 2 : P.n, m0 = (int64_t)blockIdx.y * (16 * MT), n0 = (int64_t)blockIdx.x * 16;
+  const int64_t n_out = SWIGLU ? P.n / 2 : P.n, m0 = (int64_t)blockIdx.y * (ROWS * MT), n0 = (int64_t)blockIdx.x * CH;
+  const int part = (K + 128 * KP - 1) / (128 * KP) * 128;      // of K
   const int8_t* a[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
-    const int64_t m = m0 + 16 * t + r;
+    const int64_t m = m0 + 16 * t + r % ROWS;
     a[t] = P.a + (m < P.m ? m : P.m - 1) * P.a_stride;
   }
   const int8_t* b[H];
-  b[0] = P.b + (n0 + r < n_out ? n0 + r : n_out - 1) * P.b_stride;
-  if constexpr (SWIGLU) b[1] = b[0] + n_out * P.b_stride;
+  const int64_t n_row = n0 + r % CH < n_out ? n0 + r % CH : n_out - 1;
+  b[0] = P.b + (r % ROWS < CH ? n_row : n_out + n_row) * P.b_stride;
+  if constexpr (H == 2) b[1] = b[0] + n_out * P.b_stride;
   v4i acc[H][MT];
 #pragma unroll
   for (int h = 0; h < H; ++h)
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[h][t] = v4i{0, 0, 0, 0};
-  for (int k0 = wave * 128; k0 < K; k0 += W * 128) {
-    const int k = k0 + 32 * g;
+  for (int k0 = wave * 128; k0 < part; k0 += W * 128) {
+    const int k = r / ROWS * part + k0 + 32 * g;
     v4i bv[H][2], av[MT][2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -216,14 +222,19 @@ __global__ void __launch_bounds__(512) k_int8_gemm_rows(const DgmInt8GemmArgs P,
 #pragma unroll
     for (int t = 0; t < MT; ++t) sums[wave][h * MT + t][lane] = acc[h][t];
   __syncthreads();
-  if (wave >= MT) return;
+  if (wave >= MT || g >= CH / 4 || r >= ROWS) return;
   const int64_t m = m0 + 16 * wave + r;
   if (m >= P.m) return;
+  // (part q: rows 4 g .. behind ROWS q, token column r behind ROWS q)
   v4i s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-  for (int h = 0; h < H; ++h)
+  for (int w = 0; w < W; ++w)
 #pragma unroll
-    for (int w = 0; w < W; ++w) s[h] += sums[w][h * MT + wave][lane];
+    for (int q = 0; q < KP; ++q) {
+      const int at = lane + q * (ROWS / 4 * 16 + ROWS);
+      s[0] += sums[w][wave][at];
+      if constexpr (SWIGLU) s[1] += H == 2 ? sums[w][MT + wave][at] : sums[w][wave][at + CH / 4 * 16];
+    }
   const int64_t n = n0 + 4 * g;
   if (n >= n_out) return;
   const float sa = P.sfa[m * P.sfa_stride];
@@ -439,14 +450,35 @@ __global__ void __launch_bounds__(256) k_int8_gemm_join(const DgmInt8GemmArgs P,
   });
 }
 
+// Parts of K and channels of a workgroup of the rows kernel (us, neighbour first).
+// Two parts: half the rows a workgroup, twice the workgroups. Where 16 channels each leave CUs without one, or up
+// to 2 tokens (whose rows cost nothing): 1 x 1024, K 8192 7.2 -> 5.3; 8 x 2048, K 4096 5.9 -> 5.0; 1 x 14336, K 4096
+// 15.2 -> 13.2; but 4 x 8192, K 8192 16 -> 20 and, with too little K for the waves, 1 x 4096, K 2048 4.2 -> 4.5.
+// SwiGLU with gate and up rows in one fragment: up to 8 tokens, or where it is needed to fill the CUs: 1 x 4096,
+// K 7168 15.4 -> 10.4; 16 x 4096, K 7168 16.6 -> 12.1; but 16 x 8192, K 4096 12.8 -> 14.1 (token rows are read twice
+// as often).
+struct Rows { int parts, channels; };
+Rows rows_form(int64_t m, int64_t n, int64_t k, bool swiglu) {
+  const int parts = (m <= 8 && n <= 2048 && k >= 2048) || (m <= 2 && k >= 4096) ? 2 : 1;
+  const bool one = swiglu && (parts == 2 || m <= 8 || n <= 4096);
+  return {parts, 16 / parts / (one ? 2 : 1)};
+}
+
+template <int MT, int KP, int CH, bool SWIGLU>
+void launch_rows(const DgmInt8GemmArgs& A, bool aligned, int vec, hipStream_t stream) {
+  const int64_t n_out = SWIGLU ? A.n / 2 : A.n, tokens = 16 / KP * MT;
+  const dim3 grid((unsigned)((n_out + CH - 1) / CH), (unsigned)((A.m + tokens - 1) / tokens));
+  if (aligned) hipLaunchKernelGGL((k_int8_gemm_rows<MT, KP, CH, SWIGLU, true>), grid, dim3(512), 0, stream, A, vec);
+  else hipLaunchKernelGGL((k_int8_gemm_rows<MT, KP, CH, SWIGLU, false>), grid, dim3(512), 0, stream, A, vec);
+}
 template <int MT>
 void launch_rows(const DgmInt8GemmArgs& A, bool aligned, int vec, hipStream_t stream) {
-  const int64_t n_out = A.swiglu ? A.n / 2 : A.n;
-  const dim3 grid((unsigned)((n_out + 15) / 16), (unsigned)((A.m + 16 * MT - 1) / (16 * MT)));
-  if (A.swiglu && aligned) hipLaunchKernelGGL((k_int8_gemm_rows<MT, true, true>), grid, dim3(512), 0, stream, A, vec);
-  else if (A.swiglu) hipLaunchKernelGGL((k_int8_gemm_rows<MT, true, false>), grid, dim3(512), 0, stream, A, vec);
-  else if (aligned) hipLaunchKernelGGL((k_int8_gemm_rows<MT, false, true>), grid, dim3(512), 0, stream, A, vec);
-  else hipLaunchKernelGGL((k_int8_gemm_rows<MT, false, false>), grid, dim3(512), 0, stream, A, vec);
+  const Rows f = rows_form(A.m, A.n, A.k, A.swiglu != 0);
+  if constexpr (MT == 1)
+    if (f.parts == 2) return A.swiglu ? launch_rows<1, 2, 4, true>(A, aligned, vec, stream) : launch_rows<1, 2, 8, false>(A, aligned, vec, stream);
+  if (!A.swiglu) launch_rows<MT, 1, 16, false>(A, aligned, vec, stream);
+  else if (f.channels == 8) launch_rows<MT, 1, 8, true>(A, aligned, vec, stream);
+  else launch_rows<MT, 1, 16, true>(A, aligned, vec, stream);
 }
 
 template <int BM, int BN, int WM, int WN, int STAGES>
@@ -466,9 +498,9 @@ void launch_tiles(const DgmInt8GemmArgs& A, int vec, int splits, hipStream_t str
 
 // Which kernel takes an aligned product, from estimates of its time in us (256 CUs). A tile form takes `alone`
 // us per K step while every workgroup has a CU to itself, `full` us when the CUs hold as many as fit, and 4.2 us
-// around it; splitting K costs a second launch and the sums' way through memory (2.9 TB/s). The step times are
-// fitted to 137 products of 17 to 8192 tokens with every form and split, none warm in the caches: the estimates'
-// choice takes 0.5 % longer than the best form on average, and 2 % on 88 other products of 1 to 12000 tokens.
+// around it; splitting K costs a second launch, 0.35 us a split and the sums' way through memory (3.2 TB/s). The times are
+// fitted to 300 products of 1 to 12000 tokens with every form and split, none warm in the caches: the estimates'
+// choice takes 0.5 % longer than the best form on average.
 // Where each form is the best (us; next best):
 //   64 x 64, 4 stages:    256 x 4096, K 2048: 8.8 (64 x 128 9.7);    200 x 2880, K 2880: 10.6 (12.1)
 //   64 x 128, 3 stages:   300 x 5120, K 2880: 12.7 (64 x 64 15.9);   512 x 4096, K 2048: 10.4 (11.5)
@@ -480,9 +512,10 @@ void launch_tiles(const DgmInt8GemmArgs& A, int vec, int splits, hipStream_t str
 //   256 x 192:            8192 x 2880, K 2880: 88 (192 x 128 98);    4096 x 2880, K 2880: 45 (256 x 256 50)
 //   256 x 256:            8192 x 8192, K 4096: 243 (192 x 256 266);  2048 x 8192, K 4096: 69 (128 x 128 82)
 // Up to 192 x 128 the steps are bound by the loads that a CU keeps in flight (more stages: no faster).
-// The rows form takes 2 us and, per 1024 of K and 256 workgroups, 0.8 us up to 4 tokens, 1.0 up to 16, 1.4
-// up to 32 and 3.0 up to 64 (SwiGLU: 1.8 times the first two, 1.5 times the others): 16 x 4096, K 4096: 7 us
-// (64 x 64, 4 splits 11); 64 x 5120, K 2880: 14.8 us (64 x 64: 10.1).
+// The rows form takes 2 us and, per 1024 of a part of K and round of 256 workgroups, 0.75 us up to 4 tokens, 1.25
+// up to 16, 1.65 up to 32 and 2.8 up to 64 (SwiGLU with a fragment each for gate and up rows 1.75 times the first
+// two and twice the others): 16 x 4096, K 7168: 11.5 us (64 x 64, 4 splits 13); 32 x 8192, K 4096: 16.5 us (64 x 64,
+// 2 splits 13.7).
 struct Form { int kind, splits; };
 enum { ROWS = 0, T64, T64_128, T128_DEEP, T128, T192_128, T128_256, T192_256, T256_192, T256 };
 Form choose(int64_t m, int64_t n, int64_t k, bool swiglu, int64_t workspace_bytes) {
@@ -493,9 +526,11 @@ Form choose(int64_t m, int64_t n, int64_t k, bool swiglu, int64_t workspace_byte
   Form best = {ROWS, 1};
   double least = 1e30;
   if (m <= 64) {
-    const double c = (m <= 4 ? 0.8 : m <= 16 ? 1.0 : m <= 32 ? 1.4 : 3.0) * (!swiglu ? 1.0 : m <= 16 ? 1.8 : 1.5);
-    const double wgs = (double)((n / (swiglu ? 2 : 1) + 15) / 16) / 256;
-    least = 2 + (double)((k + 1023) / 1024) * c * (wgs < 1 ? 1 : wgs);
+    const Rows f = rows_form(m, n, k, swiglu);
+    const double c = (m <= 4 ? 0.75 : m <= 16 ? 1.25 : m <= 32 ? 1.65 : 2.8) *
+                     (!swiglu || f.channels < 16 / f.parts ? 1.0 : m <= 16 ? 1.75 : 2.0);
+    const int64_t wgs = (n / (swiglu ? 2 : 1) + f.channels - 1) / f.channels;
+    least = 2 + (double)((k + 1024 * f.parts - 1) / (1024 * f.parts)) * c * (double)((wgs + 255) / 256);
   }
   for (int t = T64; t <= T256; ++t)
     for (int s = 1; s <= 8; s *= 2) {
@@ -503,7 +538,7 @@ Form choose(int64_t m, int64_t n, int64_t k, bool swiglu, int64_t workspace_byte
       const int64_t wgs = ((m + tiles[t].bm - 1) / tiles[t].bm) * ((n + tiles[t].bn - 1) / tiles[t].bn) * s;
       const int64_t rounds = (wgs + 256 * tiles[t].per_cu - 1) / (256 * tiles[t].per_cu);
       double us = 4.2 + (double)((steps + s - 1) / s) * (wgs <= 256 ? tiles[t].alone : tiles[t].full * (double)rounds);
-      if (s > 1) us += 3.8 + 8e-6 / 2.9 * (double)s * (double)m * (double)n;
+      if (s > 1) us += 2.4 + 0.35 * s + 8e-6 / 3.2 * (double)s * (double)m * (double)n;
       if (us < least) least = us, best = {t, s};
     }
   return best;

@@ -77,6 +77,26 @@ def test_shapes(m, n, k):
             check_swiglu(d, ref, clamp)
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 10, 2048), (1, 34, 4097), (2, 4098, 4112), (3, 2046, 2064), (5, 18, 7001), (7, 1030, 2192),
+                                   (8, 2048, 4224), (8, 2050, 2064), (9, 2048, 2048), (2, 8206, 4109), (4, 8206, 4112),
+                                   (16, 4090, 1040), (16, 4098, 1040), (31, 4096, 528), (50, 1026, 400)])
+def test_few_tokens(m, n, k):
+    """The forms that few tokens take: parts of K in a fragment, gate and up rows in one or two, edges in every direction."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    for full in (False, True):
+        a, b = make(m, n, k, seed=m + n + k, full=full)
+        ref = product(a, b)
+        f = torch.full((m + 1, n + 3), 7.0, device="cuda")
+        check(dgm.int8_gemm_nt(a, b, f[:m, :n]), ref, ref.abs())
+        assert bool((f[:, n:] == 7).all()) and bool((f[m:] == 7).all())
+        c = torch.randn((m, n), device="cuda").to(torch.bfloat16)
+        check(dgm.int8_gemm_nt(a, b, c.clone(), c=c), ref + c.double(), ref.abs() + c.double().abs())
+        d = torch.full((m + 1, n // 2), 7.0, dtype=torch.bfloat16, device="cuda")
+        check_swiglu(dgm.int8_gemm_nt(a, b, d[:m], activation="swiglu", activation_clamp=3.0), ref, 3.0)
+        assert bool((d[m:] == 7).all())
+
+
 @pytest.mark.parametrize("m,n,k", [(69, 8278, 144), (200, 8242, 160), (392, 8206, 144), (586, 8292, 144), (4100, 1830, 144),
                                    (1025, 7226, 144), (1732, 6474, 144), (1543, 7174, 144), (50, 4246, 4112), (18, 7758, 4112),
                                    (65, 8270, 7184), (67, 4354, 7184), (133, 5502, 7184), (67, 8222, 10256), (135, 8284, 10256),
