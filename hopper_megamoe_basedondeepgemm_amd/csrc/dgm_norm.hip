@@ -120,6 +120,35 @@ struct Held {
   }
 };
 
+// The same of any type T.
+struct HeldRow {
+  u4 a, b;
+  template <int T>
+  DGM_DEV void load(const void* p, int64_t off, int H) {
+    const int i = (int)threadIdx.x * 8;
+    a = b = u4{0u, 0u, 0u, 0u};
+    if (i >= H) return;
+    if constexpr (T == T_F32) {
+      const u4* q = reinterpret_cast<const u4*>(reinterpret_cast<const float*>(p) + off + i);
+      a = q[0], b = q[1];
+    } else {
+      a = *reinterpret_cast<const u4*>(reinterpret_cast<const uint16_t*>(p) + off + i);
+    }
+  }
+  template <int T>
+  DGM_DEV void unpack(float* v) const {
+    if constexpr (T == T_F32) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t lo = a[k], hi = b[k];
+        v[k] = __uint_as_float(lo), v[4 + k] = __uint_as_float(hi);
+      }
+    } else {
+      unpack8<T>(a, v);
+    }
+  }
+};
+
 // Gates: the hardware's exp2 and reciprocal, within (4 + |g|) 2^-24 of the value (with IEEE expf and division
 // 8192 x 4096 under a channel gate took 64 us, so 55).
 DGM_DEV float gate_sigmoid(float g) { return sigmoid<true>(g); }
@@ -137,9 +166,38 @@ __global__ void __launch_bounds__(THREADS) k_norm_fwd(const DgmNormArgs P) {
   const bool wf = P.weights_f32;
   const float inv_h = 1.0f / (float)H;
   float t[N], w[N];
-  R::template load<T>(P.x, row * P.x_stride, H, t);
+  // Rows of eight elements a thread: everything is requested at the start, so that a row waits for memory once
+  // (64 x 4096 3.3 -> 3.0 us, 4096 x 4096 fp32 under a full gate 62.6 -> 60.7).
+  constexpr bool EARLY = VEC && NV == 1;
+  HeldRow hx, h1, hg, hr, h2;
+  if constexpr (EARLY) {
+    hx.load<T>(P.x, row * P.x_stride, H);
+    if (P.residual) hr.load<T>(P.residual, row * P.residual_stride, H);
+    if (P.post_weight) {
+      if (wf) h1.load<T_F32>(P.post_weight, 0, H);
+      else h1.load<T>(P.post_weight, 0, H);
+    }
+    if (P.gate_mode == GATE_CHANNEL || P.gate_mode == GATE_FULL) hg.load<T>(P.gate, P.gate_mode == GATE_FULL ? row * P.gate_stride : 0, H);
+    if (P.pre_weight) {
+      if (wf) h2.load<T_F32>(P.pre_weight, 0, H);
+      else h2.load<T>(P.pre_weight, 0, H);
+    }
+  }
+  auto get = [&](const HeldRow& held, const void* p, int64_t off, float* v) {
+    if constexpr (EARLY) held.unpack<T>(v);
+    else R::template load<T>(p, off, H, v);
+  };
+  auto get_weight = [&](const HeldRow& held, const void* p) {
+    if constexpr (EARLY) {
+      if (wf) held.unpack<T_F32>(w);
+      else held.unpack<T>(w);
+    } else {
+      R::template weight<T>(p, wf, H, w);
+    }
+  };
+  get(hx, P.x, row * P.x_stride, t);
   if (P.post_weight) {
-    R::template weight<T>(P.post_weight, wf, H, w);
+    get_weight(h1, P.post_weight);
     float ss = 0.f;
 #pragma unroll
     for (int k = 0; k < N; ++k) ss += t[k] * t[k];
@@ -156,13 +214,13 @@ __global__ void __launch_bounds__(THREADS) k_norm_fwd(const DgmNormArgs P) {
 #pragma unroll
       for (int k = 0; k < N; ++k) t[k] *= a;
     } else {
-      R::template load<T>(P.gate, P.gate_mode == GATE_FULL ? row * P.gate_stride : 0, H, w);
+      get(hg, P.gate, P.gate_mode == GATE_FULL ? row * P.gate_stride : 0, w);
 #pragma unroll
       for (int k = 0; k < N; ++k) t[k] *= P.gate_sigmoid ? gate_sigmoid(w[k]) : w[k];
     }
   }
   if (P.residual) {
-    R::template load<T>(P.residual, row * P.residual_stride, H, w);
+    get(hr, P.residual, row * P.residual_stride, w);
 #pragma unroll
     for (int k = 0; k < N; ++k) t[k] = w[k] + P.residual_scale * t[k];
   } else {
@@ -171,7 +229,7 @@ __global__ void __launch_bounds__(THREADS) k_norm_fwd(const DgmNormArgs P) {
   }
   if (P.residual_out) R::template store<T>(P.residual_out, row * P.residual_out_stride, H, t);
   if (!P.pre_weight) return;
-  R::template weight<T>(P.pre_weight, wf, H, w);
+  get_weight(h2, P.pre_weight);
   float ss = 0.f;
 #pragma unroll
   for (int k = 0; k < N; ++k)
