@@ -253,8 +253,15 @@ __global__ void __launch_bounds__(THREADS) k_norm_fwd(const DgmNormArgs P) {
     red.template run<true>(amax);
     const float s = fmaxf(amax, 1e-30f) / 127.0f;
     if (threadIdx.x == 0) P.q_sf[row] = s;
+    // h / s by the reciprocal and one correction: rounded to a whole number it is the quotient's for every bf16
+    // amax and every bf16 h up to it (all 5.3e8 pairs compared on the CPU; the reciprocal alone misses 5464).
+    // amax infinite: step 0 leaves 0, and NaN for the infinite ones. (A division each: 1024 x 7168 17.4 us.)
+    const float inv = 1.0f / s, step = s == INFINITY ? 0.f : s;
 #pragma unroll
-    for (int k = 0; k < N; ++k) t[k] = fminf(fmaxf(rintf(t[k] / s), -127.f), 127.f);
+    for (int k = 0; k < N; ++k) {
+      const float quotient = t[k] * inv;
+      t[k] = fminf(fmaxf(rintf(fmaf(fmaf(-quotient, step, t[k]), inv, quotient)), -127.f), 127.f);
+    }
     int8_t* q = P.q + row * (int64_t)H;
     if constexpr (VEC) {
 #pragma unroll

@@ -254,6 +254,28 @@ def test_int8_rows(H):
     assert not bool(q[4].any()) and q.dtype == torch.int8 and sf.shape == (9,)
 
 
+def test_int8_rows_of_any_value():
+    """Rows over all of bf16: each magnitude as a row's largest with all kinds of values below it, denormal, infinite and
+    NaN ones included, cast as per_token_cast_to_int8 casts them."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    cast = dgm.quantization_qoq_fused.per_token_cast_to_int8
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.ones((1, 1024), device="cuda").bfloat16()
+    x[0, 1::2] = -1                                       # (mean square 1, eps 0: h is the weight)
+    for top in [0.0] + [2.0 ** e * (1 + f / 128) for e in range(-133, 128, 3) for f in (0, 37, 126, 127)] + [float("inf"), float("nan")]:
+        scale = top if 0 < top < float("inf") else 3.0
+        w = scale * torch.rand(1024, generator=g, device="cuda", dtype=torch.float64)
+        w[:512] *= torch.linspace(0, 1, 512, device="cuda", dtype=torch.float64)
+        w[512:640] = (torch.arange(128, device="cuda") - 0.5) / 127 * scale          # (halves of a step)
+        w[5] = top
+        w = w.float().bfloat16()
+        _, h, (q, sf) = dgm.rms_norm_residual(x, pre_weight=w, eps=0.0, quant="int8")
+        assert torch.equal(h.abs().nan_to_num(7.0), w[None].abs().nan_to_num(7.0)), top
+        want, want_sf = cast(h)
+        assert torch.equal(sf, want_sf[:, 0]) and torch.equal(q, want), top
+
+
 def test_strides_alignment_and_places():
     """Row strides, misaligned rows, transposed and expanded inputs, outputs over the inputs' rows: the
     same values as from plain inputs, and nothing beside the rows written."""
