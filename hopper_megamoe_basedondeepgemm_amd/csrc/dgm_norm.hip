@@ -588,6 +588,8 @@ int dgm_rms_norm_residual_backward(const DgmNormGradArgs* args, hipStream_t stre
   DGM_CHECK_ARG(!A.d_pre_weight || F.pre_weight, "d_pre_weight without its weight");
   DGM_CHECK_ARG(!A.d_post_weight || F.post_weight, "d_post_weight without its weight");
   DGM_CHECK_ARG(!A.d_gate || F.gate_mode != GATE_NONE, "d_gate without a gate");
+  // (read before the first row is, so also where there is none)
+  DGM_CHECK_ARG(F.gate_mode != GATE_CHANNEL || F.gate, "gate and gate_mode");
   DGM_CHECK_ARG(!columns || (A.workspace && A.workspace_bytes >= (int64_t)groups * F.hidden * 12 &&
                              ((uintptr_t)A.workspace & 15) == 0),
                 "workspace of 3 x groups x hidden floats, 16-byte aligned");

@@ -82,3 +82,13 @@ def test_c_entry_refusals():
                           ({}, dict(d_post_weight=p), b"d_post_weight")):
         st, msg = grad(fwd, **kw)
         assert st == -1 and what in msg, (fwd, kw, msg)
+
+
+def test_c_backward_without_rows():
+    """No rows: a channel gate is read all the same, so a null one is refused."""
+    lib, p = _lib.load(), 4096          # (never dereferenced: refused first)
+    for hidden in (64, 9000):
+        fwd = _lib.NormArgs(rows=0, hidden=hidden, gate_mode=1, residual_scale=1.0, eps=1e-6)
+        a = _lib.NormGradArgs(forward=fwd, d_gate=p, workspace=p, workspace_bytes=hidden * 12)
+        assert lib.dgm_rms_norm_residual_backward(ctypes.byref(a), None) == -1
+        assert b"gate and gate_mode" in lib.dgm_last_error()
