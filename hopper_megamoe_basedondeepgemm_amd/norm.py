@@ -209,6 +209,20 @@ def _backward(d_r, d_h, x, residual, post_weight, pre_weight, gate, forward, nee
     return d_x, d_residual, d_post, d_pre, d_gate
 
 
+def _check_backward(d_r, d_h, x, residual, post_weight, pre_weight, gate, rstd_post, rstd_pre):
+    _check(x, residual, post_weight, pre_weight, gate)
+    for d in (d_r, d_h):
+        if d is not None and (d.dtype != x.dtype or d.shape != x.shape):
+            raise TypeError(f"gradient rows of {x.dtype} {tuple(x.shape)} expected, got {d.dtype} {tuple(d.shape)}")
+    if d_h is not None and pre_weight is None:
+        raise ValueError("d_h without a pre_weight")
+    for w, rstd in ((post_weight, rstd_post), (pre_weight, rstd_pre)):
+        if w is not None and (rstd is None or rstd.dtype != torch.float32 or tuple(rstd.shape) != (x.size(0),)
+                              or not rstd.is_contiguous()):
+            raise ValueError("rstd rows of rms_norm_residual_forward (fp32 [tokens]) expected")
+    _lib.require_one_device(x, d_r, d_h, residual, post_weight, pre_weight, gate, rstd_post, rstd_pre)
+
+
 def _places(tensors):
     return [None if t is None else (t.data_ptr(), t.stride()) for t in tensors]
 
@@ -233,11 +247,16 @@ class _RmsNormResidual(torch.autograd.Function):
         args = ctx.args
         if _places(saved) != ctx.places:
             # Other memory since the forward pass: storage replaced, or tensors that saved-tensor hooks brought
-            # back (offloading, recomputation), the rstd rows among them and in strides of their own.
-            read = _readable(*saved[:5])
+            # back (offloading, recomputation), the rstd rows among them and in strides of their own. What a hook
+            # returns is checked as an argument is: the kernels read it by address.
             rstd = saved[5].contiguous()
+            post, pre = saved[2] is not None, saved[3] is not None
+            if rstd.dim() != 2 or rstd.size(0) != post + pre:
+                raise ValueError(f"saved rstd rows came back as {tuple(rstd.shape)}")
+            _check_backward(d_r, d_h, *saved[:5], rstd[0] if post else None, rstd[-1] if pre else None)
+            read = _readable(*saved[:5])
             at = rstd.data_ptr()
-            args = _forward_args(*read[:5], *ctx.options, read[5], at, at if saved[2] is None else at + 4 * rstd.size(1))
+            args = _forward_args(*read[:5], *ctx.options, read[5], at, at + 4 * rstd.size(1) if post else at)
         return (*_backward(d_r, d_h, *saved[:5], args, ctx.needs_input_grad), None, None, None)
 
 
@@ -296,18 +315,7 @@ def rms_norm_residual_backward(d_r, d_h, x, residual, rstd_post, rstd_pre, post_
     ``rms_norm_residual_forward``; None for an absent input or one that ``needs`` leaves out. r is
     recomputed in fp32 from x and residual. Sums over tokens (the weights, a channel gate) are taken in
     fp32 in a fixed order."""
-    _check(x, residual, post_weight, pre_weight, gate)
-    T, H = x.shape
-    for d in (d_r, d_h):
-        if d is not None and (d.dtype != x.dtype or d.shape != x.shape):
-            raise TypeError(f"gradient rows of {x.dtype} {tuple(x.shape)} expected, got {d.dtype} {tuple(d.shape)}")
-    if d_h is not None and pre_weight is None:
-        raise ValueError("d_h without a pre_weight")
-    for w, rstd in ((post_weight, rstd_post), (pre_weight, rstd_pre)):
-        if w is not None and (rstd is None or rstd.dtype != torch.float32 or tuple(rstd.shape) != (T,)
-                              or not rstd.is_contiguous()):
-            raise ValueError("rstd rows of rms_norm_residual_forward (fp32 [tokens]) expected")
-    _lib.require_one_device(x, d_r, d_h, residual, post_weight, pre_weight, gate, rstd_post, rstd_pre)
+    _check_backward(d_r, d_h, x, residual, post_weight, pre_weight, gate, rstd_post, rstd_pre)
     read = _readable(x, residual, post_weight, pre_weight, gate)
     forward = _forward_args(*read[:5], gate_sigmoid, residual_scale, eps, read[5],
                             rstd_post.data_ptr() if post_weight is not None else 0,
