@@ -490,3 +490,16 @@ def test_repeats_streams_and_graph():
         torch.cuda.synchronize()
         now = both()
         assert all(torch.equal(a, b) for a, b in zip(held, now)), i
+
+
+def test_saved_tensors_that_stay_on_the_cpu():
+    """A hook that leaves a tensor on the CPU: refused before its address is read."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    x, r, w1, w2, gt = make(6, 96, torch.bfloat16, torch.float32, 1, 1, "token", 1, seed=4)
+    for part in ((6, 96), (96,), (6, 1), (2, 6)):
+        leaf = x.clone().requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.cpu() if t.shape == part else t):
+            got = dgm.rms_norm_residual(leaf, r, w1, w2, gt)
+        with pytest.raises(RuntimeError, match="cpu|GPU"):
+            torch.autograd.grad(got, leaf, (torch.ones_like(x), torch.ones_like(x)))
