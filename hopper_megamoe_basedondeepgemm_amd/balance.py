@@ -91,12 +91,23 @@ def _backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, balance_coef,
     return d_logits
 
 
+def _check_backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, score, z_coef):
+    _check(logits, topk_idx, cu_seqlens, score, z_coef)
+    seqs = 1 if cu_seqlens is None else cu_seqlens.size(0) - 1
+    E = logits.size(1)
+    if (d_loss.dtype != torch.float32 or d_loss.numel() != 1 or counts.dtype != torch.int32 or counts.numel() != seqs * E
+            or stats.dtype != torch.int32 or stats.numel() != 4 * seqs + 4 or not counts.is_contiguous()
+            or not stats.is_contiguous()):
+        raise TypeError("d_loss fp32 scalar, counts and stats of router_balance_loss_forward expected")
+    _lib.require_one_device(logits, d_loss, counts, stats)
+
+
 class _RouterBalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, topk_idx, cu_seqlens, balance_coef, z_coef, score):
         loss, counts, stats = _forward(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score)
         ctx.save_for_backward(logits, topk_idx, cu_seqlens, counts, stats)
-        ctx.options = balance_coef, z_coef, score
+        ctx.options, ctx.rows = (balance_coef, z_coef, score), (logits.dtype, logits.shape)
         ctx.mark_non_differentiable(counts)
         return loss, counts
 
@@ -104,6 +115,11 @@ class _RouterBalanceLoss(torch.autograd.Function):
     def backward(ctx, d_loss, _):
         _lib.no_second_derivative()
         logits, topk_idx, cu_seqlens, counts, stats = ctx.saved_tensors
+        # (saved-tensor hooks may bring anything back: checked as arguments are, the kernel reads it by address)
+        if (logits.dtype, logits.shape) != ctx.rows:
+            raise TypeError(f"saved logits came back as {logits.dtype} {tuple(logits.shape)}")
+        counts, stats = counts.contiguous(), stats.contiguous()
+        _check_backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, ctx.options[2], ctx.options[1])
         return _backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, *ctx.options), None, None, None, None, None
 
 
@@ -141,14 +157,7 @@ def router_balance_loss_backward(d_loss, logits, topk_idx, counts, stats, cu_seq
                                  score="softmax"):
     """The logits' gradient (logits' type) from d_loss (fp32 scalar tensor), the forward call's inputs and the
     counts and stats of ``router_balance_loss_forward``; zeros for tokens that add nothing."""
-    _check(logits, topk_idx, cu_seqlens, score, z_coef)
-    seqs = 1 if cu_seqlens is None else cu_seqlens.size(0) - 1
-    E = logits.size(1)
-    if (d_loss.dtype != torch.float32 or d_loss.numel() != 1 or counts.dtype != torch.int32 or counts.numel() != seqs * E
-            or stats.dtype != torch.int32 or stats.numel() != 4 * seqs + 4 or not counts.is_contiguous()
-            or not stats.is_contiguous()):
-        raise TypeError("d_loss fp32 scalar, counts and stats of router_balance_loss_forward expected")
-    _lib.require_one_device(logits, d_loss, counts, stats)
+    _check_backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, score, z_coef)
     return _backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, balance_coef, z_coef, score)
 
 

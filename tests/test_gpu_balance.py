@@ -267,3 +267,22 @@ def test_saved_tensors_that_hooks_bring_back(way):
         del keep
         return out
     assert torch.equal(grad("plain"), grad(way))
+
+
+def test_saved_tensors_that_come_back_strided_or_elsewhere():
+    """Counts in other strides are read as such; tensors left on the CPU are refused, not read."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    logits, idx = make(300, 64, 4, seed=7)
+    cu = torch.tensor([0, 100, 290], dtype=torch.int32, device="cuda")
+
+    def grad(unpack):
+        leaf = logits.clone().requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            loss = dgm.router_balance_loss(leaf, idx, cu, 1.0, 0.01)[0]
+        return torch.autograd.grad(loss, leaf)[0]
+    want = grad(lambda t: t)
+    assert torch.equal(want, grad(lambda t: t.t().contiguous().t() if t.dim() == 2 else t.clone()))
+    for part in ((300, 64), (300, 4), (3,), (2, 64), (12,)):
+        with pytest.raises(RuntimeError, match="cpu|GPU"):
+            grad(lambda t: t.cpu() if t.shape == part else t)

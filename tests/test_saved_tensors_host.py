@@ -38,3 +38,33 @@ def test_norm(no_launch, change):  # noqa: F811
     with pytest.raises((TypeError, ValueError)):
         norm(change)
     assert no_launch.calls == ["dgm_rms_norm_residual"]
+
+
+def balance(change):
+    logits = torch.randn(300, 8, requires_grad=True)
+    with hooks(change):
+        loss, _ = dgm.router_balance_loss(logits, torch.zeros((300, 2), dtype=torch.int64),
+                                          torch.tensor([0, 100, 200, 300], dtype=torch.int32))
+    return torch.autograd.grad(loss, logits)[0]
+
+
+@pytest.mark.parametrize("change", [
+    lambda t: t.bfloat16() if t.shape == (300, 8) else t,          # logits, at half the bytes
+    lambda t: t[:, :4] if t.shape == (300, 8) else t,
+    lambda t: t[:200] if t.shape == (300, 8) else t,
+    lambda t: t.short() if t.shape == (300, 2) else t,             # topk_idx
+    lambda t: t[:200] if t.shape == (300, 2) else t,
+    lambda t: t.short() if t.shape == (4,) else t,                 # cu_seqlens
+    lambda t: t[:3] if t.shape == (4,) else t,
+    lambda t: t.short() if t.shape == (3, 8) else t,               # counts
+    lambda t: t[:2] if t.shape == (3, 8) else t,
+    lambda t: t.short() if t.shape == (16,) else t,                # stats
+    lambda t: t[:12] if t.shape == (16,) else t,
+])
+def test_balance(no_launch, change):  # noqa: F811
+    assert balance(lambda t: t).shape == (300, 8)
+    assert no_launch.calls == ["dgm_router_balance_loss", "dgm_router_balance_loss_backward"]
+    no_launch.calls.clear()
+    with pytest.raises((TypeError, ValueError)):
+        balance(change)
+    assert no_launch.calls == ["dgm_router_balance_loss"]
