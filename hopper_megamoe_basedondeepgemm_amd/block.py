@@ -23,6 +23,8 @@ def mega_moe_block(x, norm_weight, router_weight, l1, l2, sym_buffer, residual=N
     down, each as ``per_token_cast_to_int8`` packs bf16 weights (one scale per channel, I a multiple of
     128); its products are int8 (``int8_gemm_nt``) on the rows that the first norm writes beside h and on
     the cast of the SwiGLU output, and the down product adds to the experts' output in fp32, rounded once.
+    ``sym_buffer`` holds every expert: on an expert-parallel share y is this rank's part of a sum, so such a
+    buffer is refused (the parts called one by one, with the sum behind the layer, serve it).
     Returns ``(r, h)``: the new residual stream and, with ``next_weight``, the next norm's output (else
     None). Inference only: under autograd it raises."""
     weights = () if shared_expert is None else tuple(t for pair in shared_expert for t in pair)
@@ -31,6 +33,9 @@ def mega_moe_block(x, norm_weight, router_weight, l1, l2, sym_buffer, residual=N
         raise RuntimeError("mega_moe_block has no gradient: call it under torch.no_grad()")
     if x.dim() != 2 or x.dtype != torch.bfloat16 or x.size(1) != sym_buffer.hidden:
         raise TypeError(f"x must be bf16 [tokens, {sym_buffer.hidden}], got {x.dtype} {tuple(x.shape)}")
+    if sym_buffer.num_local_experts != sym_buffer.num_experts:
+        raise ValueError(f"mega_moe_block needs every expert: this buffer's layer computes {sym_buffer.num_local_experts} of "
+                         f"{sym_buffer.num_experts}, and what follows it here belongs behind the sum over ranks")
     if weights:
         inner = weights[2].size(1)
         if weights[0].size(0) != 2 * inner or inner % 128:
