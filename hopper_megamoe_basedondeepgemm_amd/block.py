@@ -10,11 +10,13 @@ from .quantization_qoq_fused import per_token_cast_to_int8
 
 def mega_moe_block(x, norm_weight, router_weight, l1, l2, sym_buffer, residual=None, shared_expert=None, post_weight=None,
                    gate=None, gate_sigmoid=False, residual_scale=1.0, next_weight=None, eps=1e-6,
-                   cumulative_local_expert_recv_stats=None, activation_clamp=10.0, **layer):
+                   cumulative_local_expert_recv_stats=None, activation_clamp=10.0, force_balanced=None, token_offset=0,
+                   phase_stamps=None, one_launch=None, fast_math=True):
     """Norm, MoE layer with an optional dense expert beside it, and the way back into the residual stream:
 
         s, h  = rms_norm_residual(x, residual, pre_weight=norm_weight)       (s = residual + x, or x)
-        y     = mxfp4_mega_moe_from_bf16(h, ...) on ``sym_buffer`` (its other options through ``layer``)
+        y     = mxfp4_mega_moe_from_bf16(h, ...) on ``sym_buffer`` (with the options from activation_clamp to
+                one_launch; its SwiGLU, like the dense expert's, is the fast_math one, so False is refused)
         y    += down(swiglu(gate_up(h)))                                      (shared_expert)
         return rms_norm_residual(y, s, post_weight, next_weight, gate, gate_sigmoid, residual_scale)
 
@@ -36,6 +38,8 @@ def mega_moe_block(x, norm_weight, router_weight, l1, l2, sym_buffer, residual=N
     if sym_buffer.num_local_experts != sym_buffer.num_experts:
         raise ValueError(f"mega_moe_block needs every expert: this buffer's layer computes {sym_buffer.num_local_experts} of "
                          f"{sym_buffer.num_experts}, and what follows it here belongs behind the sum over ranks")
+    if not fast_math:
+        raise ValueError("fast_math=False: the layer's call from bf16 rows has no IEEE SwiGLU")
     if weights:
         inner = weights[2].size(1)
         if weights[0].size(0) != 2 * inner or inner % 128:
@@ -48,7 +52,7 @@ def mega_moe_block(x, norm_weight, router_weight, l1, l2, sym_buffer, residual=N
             s, h = rms_norm_residual(x, residual, pre_weight=norm_weight, eps=eps)
         y = torch.empty_like(h)
         mxfp4_mega_moe_from_bf16(y, h, router_weight, l1, l2, sym_buffer, cumulative_local_expert_recv_stats,
-                                 activation_clamp, **layer)
+                                 activation_clamp, force_balanced, token_offset, phase_stamps, one_launch)
         if weights and x.size(0):
             act = torch.empty((x.size(0), inner), dtype=torch.bfloat16, device=x.device)
             int8_gemm_nt(rows, shared_expert[0], act, activation="swiglu", activation_clamp=activation_clamp)
