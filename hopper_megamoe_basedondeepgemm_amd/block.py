@@ -2,9 +2,10 @@
 whose calls start at the router and end at the combine)."""
 import torch
 
-from .int8_gemm import int8_gemm_nt
+from . import _lib
+from .int8_gemm import MAX_K, _operand, int8_gemm_nt
 from .mega import mxfp4_mega_moe_from_bf16
-from .norm import rms_norm_residual
+from .norm import _check as _check_norm, rms_norm_residual
 from .quantization_qoq_fused import per_token_cast_to_int8
 
 
@@ -40,11 +41,19 @@ def mega_moe_block(x, norm_weight, router_weight, l1, l2, sym_buffer, residual=N
                          f"{sym_buffer.num_experts}, and what follows it here belongs behind the sum over ranks")
     if not fast_math:
         raise ValueError("fast_math=False: the layer's call from bf16 rows has no IEEE SwiGLU")
+    # (all of the block's own arguments: the layer counts its tokens, so nothing may be refused behind it)
+    residual_scale = float(residual_scale)
+    _check_norm(x, residual, None, norm_weight, None)
+    _check_norm(x, None, post_weight, next_weight, gate)
     if weights:
-        inner = weights[2].size(1)
-        if weights[0].size(0) != 2 * inner or inner % 128:
-            raise ValueError(f"shared_expert: gate and up rows [2 I, hidden] for down [hidden, I], I a multiple of 128; got "
-                             f"{tuple(weights[0].shape)} and {tuple(weights[2].shape)}")
+        gate_up, down = _operand("gate and up", shared_expert[0])[0], _operand("down", shared_expert[1])[0]
+        inner = down.size(1)
+        if tuple(gate_up.shape) != (2 * inner, x.size(1)) or down.size(0) != x.size(1) or inner % 128 or not 0 < inner <= MAX_K:
+            raise ValueError(f"shared_expert: gate and up rows [2 I, {x.size(1)}] for down [{x.size(1)}, I], I a multiple of 128 "
+                             f"up to {MAX_K}; got {tuple(gate_up.shape)} and {tuple(down.shape)}")
+        if activation_clamp is not None and not activation_clamp >= 0:
+            raise ValueError(f"activation_clamp {activation_clamp}: at least 0, or None")
+    _lib.require_one_device(*leaves)
     with torch.no_grad():
         if weights:
             s, h, rows = rms_norm_residual(x, residual, pre_weight=norm_weight, eps=eps, quant="int8")
