@@ -7,6 +7,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libdgm_megamoe.so")
@@ -264,6 +265,15 @@ def no_graph_under_capture():
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("no autograd under graph capture: call with torch.no_grad() and capture the explicit "
                            "*_backward call")
+
+
+def no_tangents(*tensors):
+    """Refuses forward-mode tangents: the kernels would compute from the values and drop them without a word."""
+    if getattr(forward_ad, "_current_level", 0) < 0:          # (outside every dual_level no tensor has one)
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("this operator has no forward-mode derivative: an argument carries a tangent")
 
 
 def no_second_derivative():

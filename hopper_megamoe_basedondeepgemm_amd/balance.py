@@ -35,6 +35,7 @@ def _check(logits, topk_idx, cu_seqlens, score, z_coef):
         raise ValueError(f"score {score!r}: one of {sorted(SCORES)}")
     if score == "sigmoid" and z_coef:
         raise ValueError("z_coef belongs to score='softmax'")
+    _lib.no_tangents(logits)
     _lib.require_one_device(logits, topk_idx, cu_seqlens)
 
 
@@ -99,6 +100,7 @@ def _check_backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, score, 
             or stats.dtype != torch.int32 or stats.numel() != 4 * seqs + 4 or not counts.is_contiguous()
             or not stats.is_contiguous()):
         raise TypeError("d_loss fp32 scalar, counts and stats of router_balance_loss_forward expected")
+    _lib.no_tangents(d_loss)
     _lib.require_one_device(logits, d_loss, counts, stats)
 
 

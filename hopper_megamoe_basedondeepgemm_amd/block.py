@@ -34,6 +34,7 @@ def mega_moe_block(x, norm_weight, router_weight, l1, l2, sym_buffer, residual=N
     leaves = (x, residual, norm_weight, router_weight, post_weight, gate, next_weight) + weights
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves):
         raise RuntimeError("mega_moe_block has no gradient: call it under torch.no_grad()")
+    _lib.no_tangents(*leaves)
     if x.dim() != 2 or x.dtype != torch.bfloat16 or x.size(1) != sym_buffer.hidden:
         raise TypeError(f"x must be bf16 [tokens, {sym_buffer.hidden}], got {x.dtype} {tuple(x.shape)}")
     if sym_buffer.num_local_experts != sym_buffer.num_experts:

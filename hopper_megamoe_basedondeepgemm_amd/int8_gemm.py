@@ -69,6 +69,7 @@ def int8_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_m
     if (d.requires_grad or asf.requires_grad or bsf.requires_grad
             or (c is not None and c.requires_grad)) and torch.is_grad_enabled():
         raise RuntimeError("int8_gemm_nt has no gradient: call it under torch.no_grad()")
+    _lib.no_tangents(d, asf, bsf, c)
     _lib.require_one_device(d, aq, asf, bq, bsf, c)
     if m == 0 or n_out == 0:
         return d

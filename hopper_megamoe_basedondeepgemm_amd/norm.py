@@ -244,6 +244,7 @@ class _RmsNormResidual(torch.autograd.Function):
     def backward(ctx, d_r, d_h):
         _lib.no_second_derivative()
         saved = ctx.saved_tensors
+        _lib.no_tangents(d_r, d_h, *saved)
         args = ctx.args
         if _places(saved) != ctx.places:
             # Other memory since the forward pass: storage replaced, or tensors that saved-tensor hooks brought
@@ -281,6 +282,7 @@ def rms_norm_residual(x, residual=None, post_weight=None, pre_weight=None, gate=
     capture use ``rms_norm_residual_forward`` and ``rms_norm_residual_backward``). Work runs on the
     current stream of the tensors' device, which has to be the current one."""
     _check(x, residual, post_weight, pre_weight, gate, quant, residual_out, out)
+    _lib.no_tangents(x, residual, post_weight, pre_weight, gate, residual_out, out)
     _lib.require_one_device(x, residual, post_weight, pre_weight, gate, residual_out, out)
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)
                                     or (post_weight is not None and post_weight.requires_grad)
@@ -302,6 +304,7 @@ def rms_norm_residual_forward(x, residual=None, post_weight=None, pre_weight=Non
     """``rms_norm_residual`` with what its explicit backward call needs: ``(r, h, rstd_post, rstd_pre)``
     (fp32 [tokens] each, None without that norm). Records no autograd graph."""
     _check(x, residual, post_weight, pre_weight, gate)
+    _lib.no_tangents(x, residual, post_weight, pre_weight, gate)
     _lib.require_one_device(x, residual, post_weight, pre_weight, gate)
     r, h, _, _, rstd, _, _ = _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_scale, eps, None,
                                       None, None, True)
@@ -316,6 +319,7 @@ def rms_norm_residual_backward(d_r, d_h, x, residual, rstd_post, rstd_pre, post_
     recomputed in fp32 from x and residual. Sums over tokens (the weights, a channel gate) are taken in
     fp32 in a fixed order."""
     _check_backward(d_r, d_h, x, residual, post_weight, pre_weight, gate, rstd_post, rstd_pre)
+    _lib.no_tangents(d_r, d_h, x, residual, post_weight, pre_weight, gate)
     read = _readable(x, residual, post_weight, pre_weight, gate)
     forward = _forward_args(*read[:5], gate_sigmoid, residual_scale, eps, read[5],
                             rstd_post.data_ptr() if post_weight is not None else 0,
