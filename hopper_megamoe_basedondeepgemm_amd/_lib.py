@@ -276,6 +276,12 @@ def no_tangents(*tensors):
             raise RuntimeError("this operator has no forward-mode derivative: an argument carries a tangent")
 
 
+def written(*tensors):
+    """Tells autograd that a launch has written these tensors' own memory: a graph that saved one of them raises in its
+    backward pass, as behind torch's in-place operations, instead of reading the new values."""
+    torch.autograd.graph.increment_version(tensors)
+
+
 def no_second_derivative():
     """In a backward pass: refuses create_graph=True (the gradients are not differentiable themselves)."""
     if torch.is_grad_enabled():

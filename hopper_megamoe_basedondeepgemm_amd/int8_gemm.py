@@ -98,6 +98,7 @@ def int8_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_m
         ws = torch.empty(need, dtype=torch.uint8, device=d.device)
         args.workspace, args.workspace_bytes = ws.data_ptr(), need
     _lib.check(_lib.load().dgm_int8_gemm_nt(ctypes.byref(args), _lib.stream()))
+    _lib.written(d)
     return d
 
 

@@ -160,6 +160,8 @@ def _forward(x, residual, post_weight, pre_weight, gate, gate_sigmoid, residual_
         _check_outputs([t for t in (residual_out, out) if t is not None], [t for t in read[:5] if t is not None])
     if T > 0 and not (same and h is None):
         _lib.check(_lib.load().dgm_rms_norm_residual(ctypes.byref(args), _lib.stream()))
+        if residual_out is not None or out is not None:
+            _lib.written(*(t for t in (residual_out, out) if t is not None))
     return x if same else r_out, h, q, sf, rstd, args, read
 
 

@@ -1,0 +1,55 @@
+"""Outputs that a caller gives (CPU, launches left out): autograd learns of the write, or the call is refused."""
+import pytest
+import torch
+
+import hopper_megamoe_basedondeepgemm_amd as dgm
+from tests.no_launch import no_launch  # noqa: F401
+
+
+def saved():
+    """(a tensor that an earlier graph needs in its backward pass, that graph's result)"""
+    leaf = torch.randn(4, 16, requires_grad=True)
+    mid = leaf * 2
+    return leaf, mid, (mid * mid).sum()
+
+
+@pytest.mark.parametrize("name", ["residual_out", "out"])
+@pytest.mark.parametrize("part", [False, True])
+def test_norm_rows_that_a_graph_has_saved(no_launch, name, part):  # noqa: F811
+    leaf, mid, loss = saved()
+    with torch.no_grad():
+        rows = mid[1:3] if part else mid
+        dgm.rms_norm_residual(torch.randn(rows.shape), pre_weight=torch.ones(16), **{name: rows})
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(loss, leaf)
+
+
+@pytest.mark.parametrize("add", [False, True])
+def test_product_rows_that_a_graph_has_saved(no_launch, add):  # noqa: F811
+    leaf, mid, loss = saved()
+    a, b = (torch.zeros((4, 32), dtype=torch.int8), torch.ones(4)), (torch.zeros((16, 32), dtype=torch.int8), torch.ones(16))
+    with torch.no_grad():
+        dgm.int8_gemm_nt(a, b, mid, c=mid if add else None)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(loss, leaf)
+
+
+def test_under_inference_mode(no_launch):  # noqa: F811
+    with torch.inference_mode():
+        x = torch.randn(4, 16)
+        dgm.rms_norm_residual(x, pre_weight=torch.ones(16), out=x, residual_out=torch.empty(4, 16))
+        dgm.int8_gemm_nt((torch.zeros((4, 32), dtype=torch.int8), torch.ones(4)),
+                         (torch.zeros((16, 32), dtype=torch.int8), torch.ones(16)), x)
+    assert len(no_launch.calls) == 2
+
+
+def test_nothing_written_is_nothing_changed(no_launch):  # noqa: F811
+    """A call that is refused, or has no rows, leaves the version."""
+    x = torch.randn(4, 16)
+    with pytest.raises(ValueError, match="overlaps an input"):
+        dgm.rms_norm_residual(x[:3], pre_weight=torch.ones(16), out=x[1:])
+    dgm.rms_norm_residual(x[:0], pre_weight=torch.ones(16), out=x[:0])
+    no_launch.status = -1
+    with pytest.raises(RuntimeError, match="dgm error"):
+        dgm.rms_norm_residual(torch.randn(4, 16), pre_weight=torch.ones(16), out=x)
+    assert x._version == 0
