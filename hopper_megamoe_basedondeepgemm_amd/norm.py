@@ -289,7 +289,9 @@ def rms_norm_residual(x, residual=None, post_weight=None, pre_weight=None, gate=
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)
                                     or (post_weight is not None and post_weight.requires_grad)
                                     or (pre_weight is not None and pre_weight.requires_grad)
-                                    or (gate is not None and gate.requires_grad)):
+                                    or (gate is not None and gate.requires_grad)
+                                    or (residual_out is not None and residual_out.requires_grad)
+                                    or (out is not None and out.requires_grad)):
         _lib.no_graph_under_capture()
         if quant or residual_out is not None or out is not None:
             raise ValueError("quant, residual_out and out have no gradient: call under torch.no_grad()")

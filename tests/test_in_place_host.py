@@ -53,3 +53,15 @@ def test_nothing_written_is_nothing_changed(no_launch):  # noqa: F811
     with pytest.raises(RuntimeError, match="dgm error"):
         dgm.rms_norm_residual(torch.randn(4, 16), pre_weight=torch.ones(16), out=x)
     assert x._version == 0
+
+
+@pytest.mark.parametrize("name", ["residual_out", "out"])
+def test_an_output_that_asks_for_a_gradient(no_launch, name):  # noqa: F811
+    x, w = torch.randn(4, 16), torch.ones(16)
+    for rows in (torch.zeros(4, 16, requires_grad=True), torch.zeros(4, 16, requires_grad=True) * 1):
+        with pytest.raises(ValueError, match="no gradient"):
+            dgm.rms_norm_residual(x, pre_weight=w, **{name: rows})
+        assert not no_launch.calls
+        with torch.no_grad():
+            dgm.rms_norm_residual(x, pre_weight=w, **{name: rows})
+        no_launch.calls.clear()
