@@ -76,11 +76,12 @@ def int8_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_m
     aq, bq = _rows(aq), _rows(bq)
     size = d.element_size()
     pa, pb, lo, a_stride, b_stride = aq.data_ptr(), bq.data_ptr(), d.data_ptr(), aq.stride(0), bq.stride(0)
+    psa, psb, sa_stride, sb_stride = asf.data_ptr(), bsf.data_ptr(), asf.stride(0), bsf.stride(0)
     hi = lo + ((m - 1) * d_stride + n_out) * size
-    if (pa < hi and lo < pa + (m - 1) * a_stride + k) or (pb < hi and lo < pb + (n - 1) * b_stride + k):
+    if ((pa < hi and lo < pa + (m - 1) * a_stride + k) or (pb < hi and lo < pb + (n - 1) * b_stride + k)
+            or (psa < hi and lo < psa + 4 * (m - 1) * sa_stride + 4) or (psb < hi and lo < psb + 4 * (n - 1) * sb_stride + 4)):
         raise ValueError("d overlaps an operand")
-    args = _lib.Int8GemmArgs(pa, asf.data_ptr(), pb, bsf.data_ptr(), 0, lo, m, n, k, a_stride, asf.stride(0), b_stride,
-                             bsf.stride(0), 0, d_stride, _lib.SRC_DTYPES[d.dtype], swiglu,
+    args = _lib.Int8GemmArgs(pa, psa, pb, psb, 0, lo, m, n, k, a_stride, sa_stride, b_stride, sb_stride, 0, d_stride, _lib.SRC_DTYPES[d.dtype], swiglu,
                              3.0e38 if activation_clamp is None else float(activation_clamp), 1 if fast_math else 0)
     if c is not None:
         if c.dim() == 1:

@@ -65,3 +65,21 @@ def test_an_output_that_asks_for_a_gradient(no_launch, name):  # noqa: F811
         with torch.no_grad():
             dgm.rms_norm_residual(x, pre_weight=w, **{name: rows})
         no_launch.calls.clear()
+
+
+@pytest.mark.parametrize("which,scales,apart", [
+    ("a", slice(46, 50), True), ("a", slice(47, 51), False), ("a", slice(113, 117), False), ("a", slice(114, 118), True),
+    ("a", slice(40, 47, 2), True), ("a", slice(45, 52, 2), False), ("b", slice(34, 50), True), ("b", slice(35, 51), False),
+    ("b", slice(113, 129), False), ("b", slice(114, 130), True), ("b", slice(20, 51, 2), False), ("b", slice(18, 49, 2), True)])
+def test_a_product_over_its_own_scales(no_launch, which, scales, apart):  # noqa: F811
+    """d is written while other workgroups still read the scales."""
+    memory = torch.ones(200)
+    d, mine = memory[50:114].view(4, 16), memory[scales]
+    a = torch.zeros((4, 32), dtype=torch.int8), mine if which == "a" else torch.ones(4)
+    b = torch.zeros((16, 32), dtype=torch.int8), mine if which == "b" else torch.ones(16)
+    if apart:
+        dgm.int8_gemm_nt(a, b, d)
+    else:
+        with pytest.raises(ValueError, match="d overlaps"):
+            dgm.int8_gemm_nt(a, b, d)
+    assert len(no_launch.calls) == apart
