@@ -320,7 +320,8 @@ DGM_DEV void finish_loss(const DgmBalanceArgs& P, double f, double z, int live, 
   P.totals[0] = live;
   P.totals[1] = total;
   const double a = live > 0 ? (double)P.balance_coef * f / (double)live : 0.0;
-  const double b = total > 0 ? (double)P.z_coef * z / (double)total : 0.0;
+  // (without a z loss lse^2 may be beyond fp32: a row at its type's lowest value)
+  const double b = total > 0 && P.z_coef != 0.f ? (double)P.z_coef * z / (double)total : 0.0;
   *P.loss = (float)(a + b);
 }
 __global__ void __launch_bounds__(256) k_balance_loss(const DgmBalanceArgs P, int64_t slots) {
