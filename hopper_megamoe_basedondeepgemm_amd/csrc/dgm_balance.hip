@@ -146,9 +146,10 @@ DGM_DEV float sum_groups(float v) {
 DGM_DEV float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 
 // A token's probabilities and its log-sum-exp (softmax; 0 where nothing is left). A sum of zero (all masked)
-// gives zeros. sig: sigmoid(l), of the sigmoid form.
+// gives zeros. rest: 1 - sigmoid(l), of the sigmoid form, from the same exponential (a difference from 1 has no bits
+// of it left beyond l = 17).
 template <int NV, bool SOFTMAX>
-DGM_DEV void probabilities(const float* l, float* p, float* sig, float& lse) {
+DGM_DEV void probabilities(const float* l, float* p, float* rest, float& lse) {
   float s = 0.f;
   lse = 0.f;
   if constexpr (SOFTMAX) {
@@ -167,7 +168,9 @@ DGM_DEV void probabilities(const float* l, float* p, float* sig, float& lse) {
   } else {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      sig[i] = p[i] = __builtin_amdgcn_rcpf(1.0f + exp_fast(-l[i]));
+      const float e = exp_fast(-fabsf(l[i])), r = __builtin_amdgcn_rcpf(1.0f + e);
+      p[i] = l[i] < 0.f ? e * r : r;
+      rest[i] = l[i] < 0.f ? r : e * r;
       s += p[i];
     }
     s = sum_lanes16(s);
@@ -203,8 +206,8 @@ DGM_DEV void sum_tokens(const DgmBalanceArgs& P, int64_t lo, int64_t hi, float (
         if (e >= 0) atomicAdd(&hist[e], 1);
       }
     }
-    float p[NV], sig[NV], lse;
-    probabilities<NV, SOFTMAX>(cur.l, p, sig, lse);
+    float p[NV], rest[NV], lse;
+    probabilities<NV, SOFTMAX>(cur.l, p, rest, lse);
 #pragma unroll
     for (int i = 0; i < NV; ++i) acc[i] += counted ? p[i] : 0.f;      // (an unrouted row may hold anything)
     z += counted ? lse * lse : 0.f;
@@ -443,14 +446,14 @@ __global__ void __launch_bounds__(256) k_balance_grad(const DgmBalanceArgs P, in
       }
     }
     const bool counted = cur.routed(P, t) && n > 0 && t >= begin;
-    float p[NV], sig[NV], lse, dot = 0.f;
-    probabilities<NV, SOFTMAX>(cur.l, p, sig, lse);
+    float p[NV], rest[NV], lse, dot = 0.f;
+    probabilities<NV, SOFTMAX>(cur.l, p, rest, lse);
 #pragma unroll
     for (int i = 0; i < NV; ++i) dot += f[i] * p[i];
     dot = sum_lanes16(dot);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const float d = SOFTMAX ? g * (p[i] * (coef * (f[i] - dot) + zc * lse)) : g * (p[i] * (coef * (f[i] - dot)) * (1.0f - sig[i]));
+      const float d = SOFTMAX ? g * (p[i] * (coef * (f[i] - dot) + zc * lse)) : g * (p[i] * (coef * (f[i] - dot)) * rest[i]);
       p[i] = counted ? d : 0.f;                  // (an unrouted row may hold anything)
     }
     if (base + (lane >> 4) >= last) continue;

@@ -25,3 +25,22 @@ def test_rows_at_the_lowest_value(T, dtype):
         want, wc, wg, wm = formula(even, idx, cuts, 1.0, 0.0, "softmax")
         assert torch.equal(counts.long().cpu(), wc) and abs(float(loss.detach()) - want) <= 300 * U * abs(want)
         close(d, wg, wm)
+
+
+@pytest.mark.parametrize("T", [40, 700])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradient_of_large_sigmoid_scores(T, dtype):
+    """Logits up to 30: the factor 1 - sigmoid(l) = sigmoid(-l) relative to itself, (6 + |l|) 2^-24 more than the
+    170 of the other factors."""
+    need_gpu()
+    logits, idx = make(T, 72, 4, dtype, seed=T + 1)
+    logits = (logits.float() + torch.linspace(-20, 22, T, device="cuda")[:, None]).clamp(-30, 30).to(dtype)
+    _, counts, d = run(logits, idx, [0, T], 1.0, 0.0, "sigmoid")
+    l = logits.double().cpu()
+    sg, rest = torch.sigmoid(l), torch.sigmoid(-l)
+    p = sg / sg.sum(1, keepdim=True)
+    routed = ((idx >= 0) & (idx < 72)).any(1).cpu()
+    f = 72 * counts.double().cpu() / counts.sum().cpu()
+    dot = (p * f).sum(1, keepdim=True)
+    c = routed[:, None] / routed.sum() * p * rest
+    close(d, c * (f - dot), c * (f + dot), 210)
