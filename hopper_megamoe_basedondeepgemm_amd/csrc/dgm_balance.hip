@@ -150,13 +150,12 @@ DGM_DEV float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408
 // of it left beyond l = 17).
 template <int NV, bool SOFTMAX>
 DGM_DEV void probabilities(const float* l, float* p, float* rest, float& lse) {
-  float s = 0.f;
+  float s = 0.f, m = -INFINITY;
   lse = 0.f;
-  if constexpr (SOFTMAX) {
-    float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) m = fmaxf(m, l[i]);
-    m = max_lanes16(m);
+  for (int i = 0; i < NV; ++i) m = fmaxf(m, l[i]);
+  m = max_lanes16(m);
+  if constexpr (SOFTMAX) {
     const float shift = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -166,9 +165,12 @@ DGM_DEV void probabilities(const float* l, float* p, float* rest, float& lse) {
     s = sum_lanes16(s);
     if (s != 0.f) lse = m + logf(s);
   } else {
+    // A row below -64: sigmoid(l) is e^l to the last bit there, and the shares are those of e^(l - m), which do not
+    // leave fp32's range with it (from l = -88 on every sigmoid would be 0).
+    const bool low = m < -64.f && m != -INFINITY;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const float e = exp_fast(-fabsf(l[i])), r = __builtin_amdgcn_rcpf(1.0f + e);
+      const float e = exp_fast(low ? l[i] - m : -fabsf(l[i])), r = low ? 1.0f : __builtin_amdgcn_rcpf(1.0f + e);
       p[i] = l[i] < 0.f ? e * r : r;
       rest[i] = l[i] < 0.f ? r : e * r;
       s += p[i];

@@ -44,3 +44,14 @@ def test_gradient_of_large_sigmoid_scores(T, dtype):
     dot = (p * f).sum(1, keepdim=True)
     c = routed[:, None] / routed.sum() * p * rest
     close(d, c * (f - dot), c * (f + dot), 210)
+
+
+@pytest.mark.parametrize("T", [40, 700])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_vanishing_sigmoid_scores(T, dtype):
+    """Rows of logits from -250 to -50: each sigmoid may lie below the least fp32 number, their shares do not."""
+    need_gpu()
+    logits, idx = make(T, 48, 4, dtype, seed=T + 2)
+    logits = (logits.float().clamp(-12, 12) - torch.linspace(0, 238, T, device="cuda")[:, None]).to(dtype)
+    check(logits, idx, [0, T], 1.0, 0.0, "sigmoid")
+    check(logits, idx, [0, 11, 30, T], 1.0, 0.0, "sigmoid", g=-2.0)
