@@ -152,6 +152,14 @@ struct HeldRow {
 // Gates: the hardware's exp2 and reciprocal, within (4 + |g|) 2^-24 of the value (with IEEE expf and division
 // 8192 x 4096 under a channel gate took 64 us, so 55).
 DGM_DEV float gate_sigmoid(float g) { return sigmoid<true>(g); }
+// For the gradient, sigmoid(g) by its side of one half: q = sigmoid(-|g|) with g's sign. The gate is q or 1 - q, its
+// derivative |q| (1 - |q|), to full precision on both sides (from a sigmoid near 1 the difference a (1 - a) keeps no
+// bits beyond g = 17).
+DGM_DEV float gate_side(float g) {
+  const float e = __builtin_amdgcn_exp2f(fabsf(g) * -1.4426950408889634f);
+  return copysignf(e * __builtin_amdgcn_rcpf(1.0f + e), g);
+}
+DGM_DEV float side_value(float q) { return __float_as_int(q) < 0 ? -q : 1.0f - q; }
 
 enum { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_TOKEN = 2, GATE_FULL = 3 };
 
@@ -349,7 +357,9 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
     } else {
       R::template load<T>(F.x, row * F.x_stride, H, x);
     }
-    // z (kept in x), a, t
+    // z (kept in x), t, and a: the gate, or its side of one half under a sigmoid
+    const bool sig = F.gate_mode != GATE_NONE && F.gate_sigmoid;
+    auto gate = [&](float v) { return sig ? side_value(v) : v; };
 #pragma unroll
     for (int k = 0; k < N; ++k) { x[k] *= rstd1; t[k] = x[k]; a[k] = 1.f; }
     if (F.post_weight) {
@@ -358,16 +368,16 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
       for (int k = 0; k < N; ++k) t[k] *= w[k];
     }
     if (F.gate_mode == GATE_TOKEN) {
-      const float v = F.gate_sigmoid ? gate_sigmoid(token_gate) : token_gate;
+      const float v = sig ? gate_side(token_gate) : token_gate;
 #pragma unroll
       for (int k = 0; k < N; ++k) a[k] = v;
     } else if (F.gate_mode != GATE_NONE) {
       if (F.gate_mode == GATE_CHANNEL) weight(F.gate, false, 2, a);
       else if constexpr (AHEAD) unpack8<T>(ca.w, a);
       else R::template load<T>(F.gate, row * F.gate_stride, H, a);
-      if (F.gate_sigmoid)
+      if (sig)
 #pragma unroll
-        for (int k = 0; k < N; ++k) a[k] = gate_sigmoid(a[k]);
+        for (int k = 0; k < N; ++k) a[k] = gate_side(a[k]);
     }
     // g = R' = the gradient of t
     if (P.d_residual_out) {
@@ -390,7 +400,7 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
       float dot = 0.f;
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        u[k] = (u[k] + F.residual_scale * a[k] * t[k]) * rstd2;
+        u[k] = (u[k] + F.residual_scale * gate(a[k]) * t[k]) * rstd2;
         dw2[k] += d[k] * u[k];
         d[k] *= w[k];
         dot += d[k] * u[k];
@@ -408,8 +418,8 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
     if (F.gate_mode != GATE_NONE) {
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const float da = g[k] * t[k] * (F.gate_sigmoid ? a[k] * (1.f - a[k]) : 1.f);
-        g[k] *= a[k];
+        const float da = g[k] * t[k] * (sig ? fabsf(a[k]) * (1.f - fabsf(a[k])) : 1.f);
+        g[k] *= gate(a[k]);
         a[k] = da;
       }
       if (F.gate_mode == GATE_TOKEN) {
