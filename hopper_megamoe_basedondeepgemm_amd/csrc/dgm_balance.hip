@@ -145,42 +145,50 @@ DGM_DEV float sum_groups(float v) {
 // rounded fp32 exponent (a third of the instructions of expf).
 DGM_DEV float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 
-// A token's probabilities and its log-sum-exp (softmax; 0 where nothing is left). A sum of zero (all masked)
-// gives zeros. rest: 1 - sigmoid(l), of the sigmoid form, from the same exponential (a difference from 1 has no bits
-// of it left beyond l = 17).
-template <int NV, bool SOFTMAX>
-DGM_DEV void probabilities(const float* l, float* p, float* rest, float& lse) {
-  float s = 0.f, m = -INFINITY;
-  lse = 0.f;
+template <int NV>
+DGM_DEV float highest(const float* l) {
+  float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NV; ++i) m = fmaxf(m, l[i]);
-  m = max_lanes16(m);
-  if constexpr (SOFTMAX) {
-    const float shift = m == -INFINITY ? 0.f : m;
+  return max_lanes16(m);
+}
+DGM_DEV float inverse(float s) { return s != 0.f ? 1.0f / s : 0.f; }
+
+// A token's softmax and its log-sum-exp (0 where nothing is left). A sum of zero (all masked) gives zeros.
+template <int NV>
+DGM_DEV void softmax(const float* l, float* p, float& lse) {
+  float s = 0.f;
+  const float m = highest<NV>(l), shift = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      p[i] = exp_fast(l[i] - shift);
-      s += p[i];
-    }
-    s = sum_lanes16(s);
-    if (s != 0.f) lse = m + logf(s);
-  } else {
-    // A row below -64: sigmoid(l) is e^l to the last bit there, and the shares are those of e^(l - m), which do not
-    // leave fp32's range with it (from l = -88 on every sigmoid would be 0).
-    const bool low = m < -64.f && m != -INFINITY;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const float e = exp_fast(low ? l[i] - m : -fabsf(l[i])), r = low ? 1.0f : __builtin_amdgcn_rcpf(1.0f + e);
-      p[i] = l[i] < 0.f ? e * r : r;
-      rest[i] = l[i] < 0.f ? r : e * r;
-      s += p[i];
-    }
-    s = sum_lanes16(s);
+  for (int i = 0; i < NV; ++i) {
+    p[i] = exp_fast(l[i] - shift);
+    s += p[i];
   }
-  const float inv = s != 0.f ? 1.0f / s : 0.f;
+  s = sum_lanes16(s);
+  lse = s != 0.f ? m + logf(s) : 0.f;
+  const float inv = inverse(s);
 #pragma unroll
   for (int i = 0; i < NV; ++i) p[i] *= inv;
 }
+
+// Sigmoid scores of a token, 1 / (1 + e^-l). Below -17 each is e^l to the last bit, and from -88 on out of fp32's range,
+// which their shares are not: the scores of a row that lies there are taken times e^-m, as 1 / (0 + e^(m - l)).
+// (A constant and a shift for each row, so that no element pays for it.)
+struct Sigmoid {
+  float one, shift;                              // shift: m log2 e
+  template <int NV>
+  DGM_DEV static Sigmoid of(const float* l) {
+    const float m = highest<NV>(l);
+    const bool low = m < -17.5f && m != -INFINITY;
+    return {low ? 0.f : 1.0f, low ? m * 1.4426950408889634f : 0.f};
+  }
+  // e^(m - l); score: the scaled one
+  DGM_DEV float exponential(float l) const { return __builtin_amdgcn_exp2f(fmaf(l, -1.4426950408889634f, shift)); }
+  DGM_DEV float score(float e) const { return __builtin_amdgcn_rcpf(one + e); }
+  // 1 - score, without a difference, which keeps no bits of it beyond l = 17 (from e = 2^25 on it is 1, and the score
+  // may have left the range)
+  DGM_DEV float rest(float e, float score) const { return e >= 0x1p25f ? 1.0f : e * score; }
+};
 
 // Sums of tokens [lo, hi) by the workgroup's waves, four tokens at a time, into rows of the experts' values
 // (and counts in LDS).
@@ -208,8 +216,18 @@ DGM_DEV void sum_tokens(const DgmBalanceArgs& P, int64_t lo, int64_t hi, float (
         if (e >= 0) atomicAdd(&hist[e], 1);
       }
     }
-    float p[NV], rest[NV], lse;
-    probabilities<NV, SOFTMAX>(cur.l, p, rest, lse);
+    float p[NV], lse = 0.f;
+    if constexpr (SOFTMAX) {
+      softmax<NV>(cur.l, p, lse);
+    } else {
+      const Sigmoid f = Sigmoid::of<NV>(cur.l);
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) s += p[i] = f.score(f.exponential(cur.l[i]));
+      const float inv = inverse(sum_lanes16(s));
+#pragma unroll
+      for (int i = 0; i < NV; ++i) p[i] *= inv;
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) acc[i] += counted ? p[i] : 0.f;      // (an unrouted row may hold anything)
     z += counted ? lse * lse : 0.f;
@@ -448,16 +466,33 @@ __global__ void __launch_bounds__(256) k_balance_grad(const DgmBalanceArgs P, in
       }
     }
     const bool counted = cur.routed(P, t) && n > 0 && t >= begin;
-    float p[NV], rest[NV], lse, dot = 0.f;
-    probabilities<NV, SOFTMAX>(cur.l, p, rest, lse);
+    float p[NV], dot = 0.f;
+    if constexpr (SOFTMAX) {
+      float lse;
+      softmax<NV>(cur.l, p, lse);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) dot += f[i] * p[i];
-    dot = sum_lanes16(dot);
+      for (int i = 0; i < NV; ++i) dot += f[i] * p[i];
+      dot = sum_lanes16(dot);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const float d = SOFTMAX ? g * (p[i] * (coef * (f[i] - dot) + zc * lse)) : g * (p[i] * (coef * (f[i] - dot)) * rest[i]);
-      p[i] = counted ? d : 0.f;                  // (an unrouted row may hold anything)
+      for (int i = 0; i < NV; ++i) p[i] = g * (p[i] * (coef * (f[i] - dot) + zc * lse));
+    } else {
+      // (p: score times 1 - score, which is all that is left to use of them behind the sums)
+      const Sigmoid of = Sigmoid::of<NV>(cur.l);
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const float e = of.exponential(cur.l[i]), score = of.score(e);
+        s += score;
+        dot += f[i] * score;
+        p[i] = score * of.rest(e, score);
+      }
+      const float inv = inverse(sum_lanes16(s)), scale = g * (coef * inv);
+      dot = sum_lanes16(dot) * inv;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) p[i] *= scale * (f[i] - dot);
     }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) p[i] = counted ? p[i] : 0.f;          // (an unrouted row may hold anything)
     if (base + (lane >> 4) >= last) continue;
     const int64_t row = t * P.d_logits_stride;
 #pragma unroll
