@@ -152,14 +152,6 @@ struct HeldRow {
 // Gates: the hardware's exp2 and reciprocal, within (4 + |g|) 2^-24 of the value (with IEEE expf and division
 // 8192 x 4096 under a channel gate took 64 us, so 55).
 DGM_DEV float gate_sigmoid(float g) { return sigmoid<true>(g); }
-// For the gradient, sigmoid(g) by its side of one half: q = sigmoid(-|g|) with g's sign. The gate is q or 1 - q, its
-// derivative |q| (1 - |q|), to full precision on both sides (from a sigmoid near 1 the difference a (1 - a) keeps no
-// bits beyond g = 17).
-DGM_DEV float gate_side(float g) {
-  const float e = __builtin_amdgcn_exp2f(fabsf(g) * -1.4426950408889634f);
-  return copysignf(e * __builtin_amdgcn_rcpf(1.0f + e), g);
-}
-DGM_DEV float side_value(float q) { return __float_as_int(q) < 0 ? -q : 1.0f - q; }
 
 enum { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_TOKEN = 2, GATE_FULL = 3 };
 
@@ -304,10 +296,10 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
 #pragma unroll
   for (int k = 0; k < N; ++k) dw2[k] = dw1[k] = dg[k] = 0.f;
   // 16-bit rows of eight elements a thread: the next row, with its rstd and token gate, is requested before
-  // the current one is worked on, and the weights and a channel gate wait in LDS (each thread's own): loads are awaited in
+  // the current one is worked on, and the weights and a channel gate (sigmoid and derivative taken) wait in LDS (each thread's own): loads are awaited in
   // their order, so weights read from memory in the loop would wait for the next row first.
   constexpr bool AHEAD = VEC && T != T_F32 && NV == 1;
-  __shared__ f4 held_w[AHEAD ? 3 : 1][2][AHEAD ? THREADS : 1];
+  __shared__ f4 held_w[AHEAD ? 4 : 1][2][AHEAD ? THREADS : 1];
   Held hx, hr, hd, hg, ha;
   float next_rstd1 = 1.f, next_rstd2 = 0.f, next_gate = 1.f;
   auto scalars = [&](int64_t row) {
@@ -323,11 +315,14 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
     if (F.gate_mode == GATE_FULL) ha.load(F.gate, row * F.gate_stride, H);
     scalars(row);
   };
+  auto keep = [&](const float* v, int set) {
+    held_w[set][0][threadIdx.x] = f4{v[0], v[1], v[2], v[3]};
+    held_w[set][1][threadIdx.x] = f4{v[4], v[5], v[6], v[7]};
+  };
   auto keep_weight = [&](const void* p, bool f32, int set) {
     float v[N];
     R::template weight<T>(p, f32, H, v);
-    held_w[set][0][threadIdx.x] = f4{v[0], v[1], v[2], v[3]};
-    held_w[set][1][threadIdx.x] = f4{v[4], v[5], v[6], v[7]};
+    keep(v, set);
   };
   auto weight = [&](const void* p, bool f32, int set, float* v) {
     if constexpr (AHEAD) {
@@ -341,14 +336,29 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
   if constexpr (AHEAD) {
     if (F.post_weight) keep_weight(F.post_weight, F.weights_f32, 0);
     if (F.pre_weight) keep_weight(F.pre_weight, F.weights_f32, 1);
-    if (F.gate_mode == GATE_CHANNEL) keep_weight(F.gate, false, 2);
+    if (F.gate_mode == GATE_CHANNEL) {
+      float v[N], d[N];
+      R::template load<T>(F.gate, 0, H, v);
+      if (F.gate_sigmoid) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const float rest = gate_sigmoid(-v[k]);
+          v[k] = gate_sigmoid(v[k]);
+          d[k] = v[k] * rest;
+        }
+        keep(d, 3);
+      }
+      keep(v, 2);
+    }
     if ((int64_t)blockIdx.x < F.rows) request(blockIdx.x);
   }
   for (int64_t row = blockIdx.x; row < F.rows; row += gridDim.x) {
     float x[N], t[N], a[N], w[N], g[N];
     Held cx, cr, cd, cg, ca;
     if constexpr (!AHEAD) scalars(row);
-    const float rstd1 = next_rstd1, rstd2 = next_rstd2, token_gate = next_gate;
+    // (the same in every lane: scalar registers, as the vector ones are short)
+    auto scalar = [](float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); };
+    const float rstd1 = scalar(next_rstd1), rstd2 = scalar(next_rstd2), token_gate = scalar(next_gate);
     if constexpr (AHEAD) {
       cx = hx, cr = hr, cd = hd, cg = hg, ca = ha;
       const int64_t next = row + gridDim.x;
@@ -357,9 +367,7 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
     } else {
       R::template load<T>(F.x, row * F.x_stride, H, x);
     }
-    // z (kept in x), t, and a: the gate, or its side of one half under a sigmoid
-    const bool sig = F.gate_mode != GATE_NONE && F.gate_sigmoid;
-    auto gate = [&](float v) { return sig ? side_value(v) : v; };
+    // z (kept in x), n (in t), a
 #pragma unroll
     for (int k = 0; k < N; ++k) { x[k] *= rstd1; t[k] = x[k]; a[k] = 1.f; }
     if (F.post_weight) {
@@ -368,16 +376,18 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
       for (int k = 0; k < N; ++k) t[k] *= w[k];
     }
     if (F.gate_mode == GATE_TOKEN) {
-      const float v = sig ? gate_side(token_gate) : token_gate;
+      const float v = F.gate_sigmoid ? gate_sigmoid(token_gate) : token_gate;
 #pragma unroll
       for (int k = 0; k < N; ++k) a[k] = v;
     } else if (F.gate_mode != GATE_NONE) {
-      if (F.gate_mode == GATE_CHANNEL) weight(F.gate, false, 2, a);
-      else if constexpr (AHEAD) unpack8<T>(ca.w, a);
-      else R::template load<T>(F.gate, row * F.gate_stride, H, a);
-      if (sig)
+      if (F.gate_mode == GATE_CHANNEL) weight(F.gate, false, 2, a);       // (AHEAD: behind the sigmoid)
+      else if constexpr (AHEAD) {
+        unpack8<T>(ca.w, a);
+        if (F.gate_sigmoid) keep(a, 2);            // (the row's gate, for its derivative)
+      } else R::template load<T>(F.gate, row * F.gate_stride, H, a);
+      if (F.gate_sigmoid && !(AHEAD && F.gate_mode == GATE_CHANNEL))
 #pragma unroll
-        for (int k = 0; k < N; ++k) a[k] = gate_side(a[k]);
+        for (int k = 0; k < N; ++k) a[k] = gate_sigmoid(a[k]);
     }
     // g = R' = the gradient of t
     if (P.d_residual_out) {
@@ -400,7 +410,7 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
       float dot = 0.f;
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        u[k] = (u[k] + F.residual_scale * gate(a[k]) * t[k]) * rstd2;
+        u[k] = (u[k] + F.residual_scale * a[k] * t[k]) * rstd2;
         dw2[k] += d[k] * u[k];
         d[k] *= w[k];
         dot += d[k] * u[k];
@@ -416,10 +426,28 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
 #pragma unroll
     for (int k = 0; k < N; ++k) g[k] *= F.residual_scale;
     if (F.gate_mode != GATE_NONE) {
+      if (F.gate_sigmoid) {
+        // the gate's derivative a (1 - a), with 1 - a = sigmoid(-gate): a difference keeps no bits of it beyond a gate
+        // of 17 (computed here: held from above, or by the smaller of the two, every row would pay for it)
+        if (F.gate_mode == GATE_TOKEN) {
+          const float rest = gate_sigmoid(-token_gate);
+#pragma unroll
+          for (int k = 0; k < N; ++k) t[k] *= a[k] * rest;
+        } else if (AHEAD && F.gate_mode == GATE_CHANNEL) {
+          weight(F.gate, false, 3, w);
+#pragma unroll
+          for (int k = 0; k < N; ++k) t[k] *= w[k];
+        } else {
+          if constexpr (AHEAD) weight(F.gate, false, 2, w);
+          else R::template load<T>(F.gate, F.gate_mode == GATE_FULL ? row * F.gate_stride : 0, H, w);
+#pragma unroll
+          for (int k = 0; k < N; ++k) t[k] *= a[k] * gate_sigmoid(-w[k]);
+        }
+      }
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const float da = g[k] * t[k] * (sig ? fabsf(a[k]) * (1.f - fabsf(a[k])) : 1.f);
-        g[k] *= gate(a[k]);
+        const float da = g[k] * t[k];
+        g[k] *= a[k];
         a[k] = da;
       }
       if (F.gate_mode == GATE_TOKEN) {
