@@ -149,9 +149,21 @@ struct HeldRow {
   }
 };
 
-// Gates: the hardware's exp2 and reciprocal, within (4 + |g|) 2^-24 of the value (with IEEE expf and division
-// 8192 x 4096 under a channel gate took 64 us, so 55).
-DGM_DEV float gate_sigmoid(float g) { return sigmoid<true>(g); }
+// Gates. 16-bit rows: the hardware's exp2 and reciprocal, within (4 + |g|) 2^-24 of the value, far below half a step of
+// their type (with IEEE expf and division 8192 x 4096 bf16 under a channel gate took 64 us, so 55). fp32 rows: the
+// exponent's rounding put back, within 8 2^-24 (the exponential 4, the reciprocal 2, the sum and the product 1 each).
+template <int T>
+DGM_DEV float gate_sigmoid(float g) {
+  if constexpr (T != T_F32) return sigmoid<true>(g);
+  float x = -fabsf(g);
+  x = x < -126.0f ? -126.0f : x;                 // (0 there; a gate that is no number stays one)
+  const float h = x * 1.4426950408889634f;
+  const float low = fmaf(x, 1.925963033500569e-8f, fmaf(x, 1.4426950408889634f, -h));
+  float e = __builtin_amdgcn_exp2f(h);
+  e = fmaf(e, low * 0.6931471805599453f, e);
+  const float r = __builtin_amdgcn_rcpf(1.0f + e);
+  return g < 0.f ? e * r : r;
+}
 
 enum { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_TOKEN = 2, GATE_FULL = 3 };
 
@@ -210,13 +222,13 @@ __global__ void __launch_bounds__(THREADS) k_norm_fwd(const DgmNormArgs P) {
   if (P.gate_mode != GATE_NONE) {
     if (P.gate_mode == GATE_TOKEN) {
       float a = load1<T>(P.gate, row * P.gate_stride);
-      if (P.gate_sigmoid) a = gate_sigmoid(a);
+      if (P.gate_sigmoid) a = gate_sigmoid<T>(a);
 #pragma unroll
       for (int k = 0; k < N; ++k) t[k] *= a;
     } else {
       get(hg, P.gate, P.gate_mode == GATE_FULL ? row * P.gate_stride : 0, w);
 #pragma unroll
-      for (int k = 0; k < N; ++k) t[k] *= P.gate_sigmoid ? gate_sigmoid(w[k]) : w[k];
+      for (int k = 0; k < N; ++k) t[k] *= P.gate_sigmoid ? gate_sigmoid<T>(w[k]) : w[k];
     }
   }
   if (P.residual) {
@@ -299,7 +311,10 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
   // the current one is worked on, and the weights and a channel gate (sigmoid and derivative taken) wait in LDS (each thread's own): loads are awaited in
   // their order, so weights read from memory in the loop would wait for the next row first.
   constexpr bool AHEAD = VEC && T != T_F32 && NV == 1;
-  __shared__ f4 held_w[AHEAD ? 4 : 1][2][AHEAD ? THREADS : 1];
+  // (a channel gate waits in LDS in fp32 too: its sigmoid and derivative are one row's work, not every row's)
+  constexpr bool HELD_GATE = VEC && NV == 1;
+  constexpr int GATE = AHEAD ? 2 : 0;            // the gate's two sets, behind the weights'
+  __shared__ f4 held_w[AHEAD ? 4 : HELD_GATE ? 2 : 1][2][HELD_GATE ? THREADS : 1];
   Held hx, hr, hd, hg, ha;
   float next_rstd1 = 1.f, next_rstd2 = 0.f, next_gate = 1.f;
   auto scalars = [&](int64_t row) {
@@ -324,32 +339,36 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
     R::template weight<T>(p, f32, H, v);
     keep(v, set);
   };
-  auto weight = [&](const void* p, bool f32, int set, float* v) {
-    if constexpr (AHEAD) {
-      const f4 lo = held_w[set][0][threadIdx.x], hi = held_w[set][1][threadIdx.x];
+  auto held = [&](int set, float* v) {
+    const f4 lo = held_w[set][0][threadIdx.x], hi = held_w[set][1][threadIdx.x];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = lo[k], v[4 + k] = hi[k];
-    } else {
-      R::template weight<T>(p, f32, H, v);
-    }
+    for (int k = 0; k < 4; ++k) v[k] = lo[k], v[4 + k] = hi[k];
+  };
+  auto weight = [&](const void* p, bool f32, int set, float* v) {
+    if constexpr (AHEAD) held(set, v);
+    else R::template weight<T>(p, f32, H, v);
   };
   if constexpr (AHEAD) {
     if (F.post_weight) keep_weight(F.post_weight, F.weights_f32, 0);
     if (F.pre_weight) keep_weight(F.pre_weight, F.weights_f32, 1);
+  }
+  if constexpr (HELD_GATE) {
     if (F.gate_mode == GATE_CHANNEL) {
       float v[N], d[N];
       R::template load<T>(F.gate, 0, H, v);
       if (F.gate_sigmoid) {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-          const float rest = gate_sigmoid(-v[k]);
-          v[k] = gate_sigmoid(v[k]);
+          const float rest = gate_sigmoid<T>(-v[k]);
+          v[k] = gate_sigmoid<T>(v[k]);
           d[k] = v[k] * rest;
         }
-        keep(d, 3);
+        keep(d, GATE + 1);
       }
-      keep(v, 2);
+      keep(v, GATE);
     }
+  }
+  if constexpr (AHEAD) {
     if ((int64_t)blockIdx.x < F.rows) request(blockIdx.x);
   }
   for (int64_t row = blockIdx.x; row < F.rows; row += gridDim.x) {
@@ -376,18 +395,22 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
       for (int k = 0; k < N; ++k) t[k] *= w[k];
     }
     if (F.gate_mode == GATE_TOKEN) {
-      const float v = F.gate_sigmoid ? gate_sigmoid(token_gate) : token_gate;
+      const float v = F.gate_sigmoid ? gate_sigmoid<T>(token_gate) : token_gate;
 #pragma unroll
       for (int k = 0; k < N; ++k) a[k] = v;
     } else if (F.gate_mode != GATE_NONE) {
-      if (F.gate_mode == GATE_CHANNEL) weight(F.gate, false, 2, a);       // (AHEAD: behind the sigmoid)
-      else if constexpr (AHEAD) {
+      if (F.gate_mode == GATE_CHANNEL) {
+        if constexpr (HELD_GATE) held(GATE, a);    // (behind the sigmoid)
+        else R::template load<T>(F.gate, 0, H, a);
+      } else if constexpr (AHEAD) {
         unpack8<T>(ca.w, a);
-        if (F.gate_sigmoid) keep(a, 2);            // (the row's gate, for its derivative)
-      } else R::template load<T>(F.gate, row * F.gate_stride, H, a);
-      if (F.gate_sigmoid && !(AHEAD && F.gate_mode == GATE_CHANNEL))
+        if (F.gate_sigmoid) keep(a, GATE);         // (the row's gate, for its derivative)
+      } else {
+        R::template load<T>(F.gate, row * F.gate_stride, H, a);
+      }
+      if (F.gate_sigmoid && !(HELD_GATE && F.gate_mode == GATE_CHANNEL))
 #pragma unroll
-        for (int k = 0; k < N; ++k) a[k] = gate_sigmoid(a[k]);
+        for (int k = 0; k < N; ++k) a[k] = gate_sigmoid<T>(a[k]);
     }
     // g = R' = the gradient of t
     if (P.d_residual_out) {
@@ -430,18 +453,18 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
         // the gate's derivative a (1 - a), with 1 - a = sigmoid(-gate): a difference keeps no bits of it beyond a gate
         // of 17 (computed here: held from above, or by the smaller of the two, every row would pay for it)
         if (F.gate_mode == GATE_TOKEN) {
-          const float rest = gate_sigmoid(-token_gate);
+          const float rest = gate_sigmoid<T>(-token_gate);
 #pragma unroll
           for (int k = 0; k < N; ++k) t[k] *= a[k] * rest;
-        } else if (AHEAD && F.gate_mode == GATE_CHANNEL) {
-          weight(F.gate, false, 3, w);
+        } else if (HELD_GATE && F.gate_mode == GATE_CHANNEL) {
+          held(GATE + 1, w);
 #pragma unroll
           for (int k = 0; k < N; ++k) t[k] *= w[k];
         } else {
-          if constexpr (AHEAD) weight(F.gate, false, 2, w);
+          if constexpr (AHEAD) held(GATE, w);
           else R::template load<T>(F.gate, F.gate_mode == GATE_FULL ? row * F.gate_stride : 0, H, w);
 #pragma unroll
-          for (int k = 0; k < N; ++k) t[k] *= a[k] * gate_sigmoid(-w[k]);
+          for (int k = 0; k < N; ++k) t[k] *= a[k] * gate_sigmoid<T>(-w[k]);
         }
       }
 #pragma unroll

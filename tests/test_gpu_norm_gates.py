@@ -34,3 +34,21 @@ def test_gradient_of_a_wide_open_gate(gate, dtype, H):
     off = (got.double() - value).abs()
     tol = value.abs() * (fi.eps / 2) + (256 + 72 + over) * U * mag * (1 + fi.eps) + fi.tiny * fi.eps
     assert bool((off <= tol).all()), float((off / tol).max())
+
+
+@pytest.mark.parametrize("gate", ["channel", "token", "full"])
+def test_small_gates_of_fp32_rows(gate):
+    """fp32 rows: sigmoid within 8 2^-24 of itself wherever it is a normal number (the hardware's exponential and
+    reciprocal within a unit, 2 2^-24, each; the exponential's correction, the sum and the product half a unit each; 1
+    for the exponent's last bits)."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    T, H = 64, 64
+    x = torch.ones((T, H), device="cuda")
+    shape = {"channel": (H,), "token": (T, 1), "full": (T, H)}[gate]
+    n = T * H if gate == "full" else 64
+    for lo, hi in ((-86, -40), (-40, 0), (0, 90)):
+        g = torch.linspace(lo, hi, n, device="cuda").view(shape)
+        r, _ = dgm.rms_norm_residual(x, gate=g, gate_sigmoid=True)
+        want = torch.sigmoid(g.double()).expand(T, H)
+        assert bool(((r.double() - want).abs() <= 8 * U * want).all()), float(((r.double() - want).abs() / want).max() / U)
