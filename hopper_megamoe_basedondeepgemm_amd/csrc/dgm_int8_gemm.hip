@@ -14,9 +14,10 @@ using namespace dgm;
 
 namespace {
 
+// (compared, not fminf / fmaxf, which put the clamp in the place of what is no number)
 DGM_DEV float swiglu(float g, float u, float clamp, bool fast) {
-  g = fminf(g, clamp);
-  u = fminf(fmaxf(u, -clamp), clamp);
+  g = g > clamp ? clamp : g;
+  u = u > clamp ? clamp : u < -clamp ? -clamp : u;
   return g * (fast ? sigmoid<true>(g) : sigmoid<false>(g)) * u;
 }
 

@@ -2,6 +2,7 @@
 the routed ones, on the int8 rows that ``per_token_cast_to_int8`` and ``rms_norm_residual`` write."""
 import ctypes
 import functools
+import math
 
 import torch
 
@@ -40,7 +41,8 @@ def int8_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_m
     ``per_token_cast_to_int8`` returns them (it also packs the weights: one scale per channel). c has d's
     type and may be d itself. ``activation="swiglu"``: b holds gate rows, then up rows, and d [m, n / 2] =
     silu(min(gate, clamp)) * clamp(up, -clamp, clamp), the layer's SwiGLU (``activation_clamp`` None: no
-    clamp; ``fast_math`` as in ``mxfp4_mega_moe_fused``). Sums are exact in int32 (k <= 131071), the rest is
+    clamp; ``fast_math`` as in ``mxfp4_mega_moe_fused``; unlike the layer's it keeps NaN, of scales that are
+    infinite or NaN). Sums are exact in int32 (k <= 131071), the rest is
     fp32, rounded once. 16-byte aligned rows (k a multiple of 16) take the fast kernels. No gradient. Work
     runs on the current stream of the tensors' device, which has to be the current one. Returns d."""
     aq, asf = _operand("a", a)
@@ -82,7 +84,7 @@ def int8_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_m
             or (psa < hi and lo < psa + 4 * (m - 1) * sa_stride + 4) or (psb < hi and lo < psb + 4 * (n - 1) * sb_stride + 4)):
         raise ValueError("d overlaps an operand")
     args = _lib.Int8GemmArgs(pa, psa, pb, psb, 0, lo, m, n, k, a_stride, sa_stride, b_stride, sb_stride, 0, d_stride, _lib.SRC_DTYPES[d.dtype], swiglu,
-                             3.0e38 if activation_clamp is None else float(activation_clamp), 1 if fast_math else 0)
+                             math.inf if activation_clamp is None else float(activation_clamp), 1 if fast_math else 0)
     if c is not None:
         if c.dim() == 1:
             c, c_stride, end = c.contiguous(), 0, n_out

@@ -453,7 +453,7 @@ typedef struct DgmInt8GemmArgs {
   int64_t a_stride, sfa_stride, b_stride, sfb_stride, c_stride, d_stride;
   int32_t dtype;
   int32_t swiglu;
-  float clamp;
+  float clamp;       /* INFINITY: none; NaN stays NaN */
   int32_t fast_math; /* SwiGLU's sigmoid: 1 hardware exp2 and reciprocal, 0 IEEE */
   int32_t* workspace; /* of this call until it has run; without it (NULL) K is not split */
   int64_t workspace_bytes;
