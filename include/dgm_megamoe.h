@@ -438,7 +438,8 @@ int dgm_norm_struct_sizes(size_t* norm_args, size_t* norm_grad_args);
  *   d[m][n] = sfa[m] sfb[n] sum_k a[m][k] b[n][k] (+ c[m][n]; c_stride 0: one row c[n] for every token)
  * or with `swiglu` over b's gate rows [0, n/2) and up rows [n/2, n), as the layer's:
  *   d[m][i] = silu(min(gate, clamp)) * clamp(up, -clamp, clamp)
- * Sums exact in int32 (k 1 to 131071), the rest fp32, one rounding to dtype (DGM_SRC_*), which c shares.
+ * Sums exact in int32 (k 1 to 131071), the rest fp32 (sfa sfb first, which has to be zero or a normal number), one
+ * rounding to dtype (DGM_SRC_*), which c shares.
  * Rows of k (a, b) and n (c, d) contiguous elements at strides in elements; scales at their strides.
  * c may be d at the same stride. m below 2^20, n below 2^24. No counterpart in the reference. */
 #define DGM_INT8_GEMM_MAX_K 131071
