@@ -39,6 +39,11 @@ def _check(logits, topk_idx, cu_seqlens, score, z_coef):
     _lib.require_one_device(logits, topk_idx, cu_seqlens)
 
 
+def _readable(logits, topk_idx, cu_seqlens):
+    """The inputs as the kernels read them."""
+    return _rows(logits), _rows(topk_idx), None if cu_seqlens is None else cu_seqlens.contiguous()
+
+
 def _args(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score, counts, stats):
     """DgmBalanceArgs of a call's inputs (logits and topk_idx as rows), counts and statistics."""
     T, E = logits.shape
@@ -60,14 +65,12 @@ def _workspace_bytes(T, seqs, E):
 
 
 def _forward(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score):
-    """The launches, after the checks."""
+    """The launches, after the checks: (loss, counts, stats, args, read). args: the launch's DgmBalanceArgs; read: the
+    tensors whose memory it names."""
     dev = logits.device
-    logits, topk_idx = _rows(logits), _rows(topk_idx)
+    logits, topk_idx, cu_seqlens = _readable(logits, topk_idx, cu_seqlens)
     T, E = logits.shape
-    seqs = 1
-    if cu_seqlens is not None:
-        cu_seqlens = cu_seqlens.contiguous()
-        seqs = cu_seqlens.size(0) - 1
+    seqs = 1 if cu_seqlens is None else cu_seqlens.size(0) - 1
     loss = torch.empty((), dtype=torch.float32, device=dev)
     counts = torch.empty((E,) if cu_seqlens is None else (seqs, E), dtype=torch.int32, device=dev)
     stats = torch.empty(4 * seqs + 4, dtype=torch.int32, device=dev)
@@ -78,15 +81,12 @@ def _forward(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score):
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         args.workspace, args.workspace_bytes = ws.data_ptr(), need
     _lib.check(_lib.load().dgm_router_balance_loss(ctypes.byref(args), _lib.stream()))
-    return loss, counts, stats
+    return loss, counts, stats, args, (logits, topk_idx, cu_seqlens)
 
 
-def _backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, balance_coef, z_coef, score):
-    """The launch of the backward pass, after the checks."""
-    logits, topk_idx = _rows(logits), _rows(topk_idx)
-    cu_seqlens = None if cu_seqlens is None else cu_seqlens.contiguous()
+def _backward(d_loss, logits, args):
+    """The launch of the backward pass, after the checks; args: DgmBalanceArgs of the forward call's inputs and results."""
     d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    args = _args(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score, counts, stats)
     args.d_loss, args.d_logits, args.d_logits_stride = d_loss.data_ptr(), d_logits.data_ptr(), logits.size(1)
     _lib.check(_lib.load().dgm_router_balance_loss_backward(ctypes.byref(args), _lib.stream()))
     return d_logits
@@ -104,25 +104,39 @@ def _check_backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, score, 
     _lib.require_one_device(logits, d_loss, counts, stats)
 
 
+def _places(tensors):
+    return [None if t is None else (t.data_ptr(), t.stride()) for t in tensors]
+
+
 class _RouterBalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, topk_idx, cu_seqlens, balance_coef, z_coef, score):
-        loss, counts, stats = _forward(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score)
-        ctx.save_for_backward(logits, topk_idx, cu_seqlens, counts, stats)
+        loss, counts, stats, args, read = _forward(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score)
+        saved = logits, topk_idx, cu_seqlens, counts, stats
+        ctx.save_for_backward(*saved)
         ctx.options, ctx.rows = (balance_coef, z_coef, score), (logits.dtype, logits.shape)
+        # (the launch's arguments, those copies that the kernels read for inputs, and where the saved tensors were)
+        ctx.args, ctx.copies, ctx.places = args, [None if u is t else u for t, u in zip(saved, read)], _places(saved)
         ctx.mark_non_differentiable(counts)
         return loss, counts
 
     @staticmethod
     def backward(ctx, d_loss, _):
         _lib.no_second_derivative()
-        logits, topk_idx, cu_seqlens, counts, stats = ctx.saved_tensors
-        # (saved-tensor hooks may bring anything back: checked as arguments are, the kernel reads it by address)
-        if (logits.dtype, logits.shape) != ctx.rows:
-            raise TypeError(f"saved logits came back as {logits.dtype} {tuple(logits.shape)}")
-        counts, stats = counts.contiguous(), stats.contiguous()
-        _check_backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, ctx.options[2], ctx.options[1])
-        return _backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, *ctx.options), None, None, None, None, None
+        saved = ctx.saved_tensors
+        logits, args = saved[0], ctx.args
+        if _places(saved) != ctx.places:
+            # Other memory since the forward pass, of saved-tensor hooks, which may bring anything back: checked as
+            # arguments are, the kernel reads it by address.
+            _, topk_idx, cu_seqlens, counts, stats = saved
+            if (logits.dtype, logits.shape) != ctx.rows:
+                raise TypeError(f"saved logits came back as {logits.dtype} {tuple(logits.shape)}")
+            counts, stats = counts.contiguous(), stats.contiguous()
+            _check_backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, ctx.options[2], ctx.options[1])
+            held = _readable(logits, topk_idx, cu_seqlens)
+            args = _args(*held, *ctx.options, counts, stats)
+        _lib.no_tangents(d_loss, logits)
+        return _backward(d_loss, logits, args), None, None, None, None, None
 
 
 def router_balance_loss(logits, topk_idx, cu_seqlens=None, balance_coef=1.0, z_coef=0.0, score="softmax"):
@@ -152,7 +166,7 @@ def router_balance_loss_forward(logits, topk_idx, cu_seqlens=None, balance_coef=
     """``router_balance_loss`` with what its explicit backward call needs: ``(loss, counts, stats)``. Records
     no autograd graph."""
     _check(logits, topk_idx, cu_seqlens, score, z_coef)
-    return _forward(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score)
+    return _forward(logits, topk_idx, cu_seqlens, balance_coef, z_coef, score)[:3]
 
 
 def router_balance_loss_backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens=None, balance_coef=1.0, z_coef=0.0,
@@ -160,7 +174,8 @@ def router_balance_loss_backward(d_loss, logits, topk_idx, counts, stats, cu_seq
     """The logits' gradient (logits' type) from d_loss (fp32 scalar tensor), the forward call's inputs and the
     counts and stats of ``router_balance_loss_forward``; zeros for tokens that add nothing."""
     _check_backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, score, z_coef)
-    return _backward(d_loss, logits, topk_idx, counts, stats, cu_seqlens, balance_coef, z_coef, score)
+    held = _readable(logits, topk_idx, cu_seqlens)
+    return _backward(d_loss, logits, _args(*held, balance_coef, z_coef, score, counts, stats))
 
 
 __all__ = ["router_balance_loss", "router_balance_loss_forward", "router_balance_loss_backward"]
