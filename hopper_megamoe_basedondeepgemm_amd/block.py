@@ -5,7 +5,7 @@ import torch
 from . import _lib
 from .int8_gemm import MAX_K, _operand, int8_gemm_nt
 from .mega import mxfp4_mega_moe_from_bf16
-from .norm import _check as _check_norm, rms_norm_residual
+from .norm import _check as _check_norm, _forward as _norm
 from .quantization_qoq_fused import per_token_cast_to_int8
 
 
@@ -44,6 +44,8 @@ def mega_moe_block(x, norm_weight, router_weight, l1, l2, sym_buffer, residual=N
         raise ValueError("fast_math=False: the layer's call from bf16 rows has no IEEE SwiGLU")
     # (all of the block's own arguments: the layer counts its tokens, so nothing may be refused behind it)
     residual_scale = float(residual_scale)
+    if norm_weight is None:
+        raise TypeError("norm_weight: [hidden] expected, got None")
     _check_norm(x, residual, None, norm_weight, None)
     _check_norm(x, None, post_weight, next_weight, gate)
     if weights:
@@ -56,18 +58,16 @@ def mega_moe_block(x, norm_weight, router_weight, l1, l2, sym_buffer, residual=N
             raise ValueError(f"activation_clamp {activation_clamp}: at least 0, or None")
     _lib.require_one_device(*leaves)
     with torch.no_grad():
-        if weights:
-            s, h, rows = rms_norm_residual(x, residual, pre_weight=norm_weight, eps=eps, quant="int8")
-        else:
-            s, h = rms_norm_residual(x, residual, pre_weight=norm_weight, eps=eps)
+        s, h, q, sf, *_ = _norm(x, residual, None, norm_weight, None, False, 1.0, eps, "int8" if weights else None, None, None,
+                                False)
         y = torch.empty_like(h)
         mxfp4_mega_moe_from_bf16(y, h, router_weight, l1, l2, sym_buffer, cumulative_local_expert_recv_stats,
                                  activation_clamp, force_balanced, token_offset, phase_stamps, one_launch)
         if weights and x.size(0):
             act = torch.empty((x.size(0), inner), dtype=torch.bfloat16, device=x.device)
-            int8_gemm_nt(rows, shared_expert[0], act, activation="swiglu", activation_clamp=activation_clamp)
+            int8_gemm_nt((q, sf), shared_expert[0], act, activation="swiglu", activation_clamp=activation_clamp)
             int8_gemm_nt(per_token_cast_to_int8(act), shared_expert[1], y, c=y)
-        return rms_norm_residual(y, s, post_weight, next_weight, gate, gate_sigmoid, residual_scale, eps)
+        return _norm(y, s, post_weight, next_weight, gate, gate_sigmoid, residual_scale, eps, None, None, None, False)[:2]
 
 
 __all__ = ["mega_moe_block"]

@@ -16,7 +16,7 @@ def buffer(ep_size=1, hidden=32, experts=4):
 
 
 def block(sym_buffer=None, **kw):
-    return dgm.mega_moe_block(bf(4, 32), bf(32), bf(4, 32), None, None, sym_buffer or buffer(), **kw)
+    return dgm.mega_moe_block(bf(4, 32), kw.pop("norm_weight", bf(32)), bf(4, 32), None, None, sym_buffer or buffer(), **kw)
 
 
 def test_an_expert_parallel_share_is_refused():
@@ -51,7 +51,7 @@ def test_the_layer_gets_its_options(monkeypatch):
         seen.update(stats=cumulative_local_expert_recv_stats, clamp=activation_clamp, balanced=force_balanced,
                     offset=token_offset, stamps=phase_stamps, one=one_launch)
     monkeypatch.setattr(module, "mxfp4_mega_moe_from_bf16", layer)
-    monkeypatch.setattr(module, "rms_norm_residual", lambda x, residual=None, *a, **kw: (x, x))
+    monkeypatch.setattr(module, "_norm", lambda x, *a: (x, x, None, None, None, None, None))
     monkeypatch.setattr("hopper_megamoe_basedondeepgemm_amd._lib.require_one_device", lambda *tensors: None)
     block(cumulative_local_expert_recv_stats=1, activation_clamp=2.0, force_balanced=True, token_offset=3, phase_stamps=4,
           one_launch=False)
@@ -64,6 +64,7 @@ def expert(inner=128, hidden=32, up=None, out=None, dtype=torch.int8):
 
 
 @pytest.mark.parametrize("kw, err, what", [
+    (dict(norm_weight=None), TypeError, "norm_weight"),
     (dict(residual=bf(4, 33)), TypeError, "rows of"),
     (dict(post_weight=bf(33)), TypeError, "norm weights"),
     (dict(next_weight=bf(31)), TypeError, "norm weights"),
@@ -91,7 +92,7 @@ def test_refusals_come_before_the_layer(kw, err, what, monkeypatch):
 
 def test_refusals_do_not_wait_for_the_first_norm(monkeypatch):
     from hopper_megamoe_basedondeepgemm_amd import block as module
-    monkeypatch.setattr(module, "rms_norm_residual", lambda *a, **k: pytest.fail("a norm has run"))
+    monkeypatch.setattr(module, "_norm", lambda *a, **k: pytest.fail("a norm has run"))
     for kw in (dict(post_weight=bf(33)), dict(gate=bf(4)), dict(shared_expert=expert(out=48)), dict(shared_expert=expert())):
         with pytest.raises((TypeError, ValueError, RuntimeError)):
             block(**kw)
