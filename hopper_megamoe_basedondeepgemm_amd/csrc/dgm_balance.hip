@@ -175,15 +175,15 @@ DGM_DEV void softmax(const float* l, float* p, float& lse) {
 // which their shares are not: the scores of a row that lies there are taken times e^-m, as 1 / (0 + e^(m - l)).
 // (A constant and a shift for each row, so that no element pays for it.)
 struct Sigmoid {
-  float one, shift;                              // shift: m log2 e
+  float one, shift;
   template <int NV>
   DGM_DEV static Sigmoid of(const float* l) {
     const float m = highest<NV>(l);
     const bool low = m < -17.5f && m != -INFINITY;
-    return {low ? 0.f : 1.0f, low ? m * 1.4426950408889634f : 0.f};
+    return {low ? 0.f : 1.0f, low ? m : 0.f};
   }
-  // e^(m - l); score: the scaled one
-  DGM_DEV float exponential(float l) const { return __builtin_amdgcn_exp2f(fmaf(l, -1.4426950408889634f, shift)); }
+  // e^(m - l) (the difference first: m log2 e may be beyond fp32); score: the scaled one
+  DGM_DEV float exponential(float l) const { return exp_fast(shift - l); }
   DGM_DEV float score(float e) const { return __builtin_amdgcn_rcpf(one + e); }
   // 1 - score, without a difference, which keeps no bits of it beyond l = 17 (from e = 2^25 on it is 1, and the score
   // may have left the range)

@@ -55,3 +55,28 @@ def test_rows_of_vanishing_sigmoid_scores(T, dtype):
     logits = (logits.float().clamp(-12, 12) - torch.linspace(0, 238, T, device="cuda")[:, None]).to(dtype)
     check(logits, idx, [0, T], 1.0, 0.0, "sigmoid")
     check(logits, idx, [0, 11, 30, T], 1.0, 0.0, "sigmoid", g=-2.0)
+
+
+@pytest.mark.parametrize("T", [40, 700])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_sigmoid_rows_at_the_lowest_value(T, dtype):
+    """Rows of the type's lowest value alone, or with masked experts beside it: the others share alike, and 1 - sigmoid
+    is 1."""
+    need_gpu()
+    E = 24
+    logits, idx = make(T, E, 2, dtype, seed=T)
+    logits[3:6] = torch.finfo(dtype).min
+    logits[5, 10:] = float("-inf")
+    idx[3:6, 0] = torch.arange(3, device="cuda")
+    loss, counts, d = run(logits, idx, [0, T], 1.0, 0.0, "sigmoid")
+    l = logits.double().cpu()
+    p, rest = torch.sigmoid(l), torch.sigmoid(-l)
+    p[3:5], p[5] = 1.0, (torch.arange(E) < 10).double()
+    p = p / p.sum(1, keepdim=True)
+    routed = ((idx >= 0) & (idx < E)).any(1).cpu()
+    f = E * counts.double().cpu() / counts.sum().cpu()
+    want = float((f * p[routed].mean(0)).sum())
+    assert abs(float(loss.detach()) - want) <= 300 * U * want
+    dot = (p * f).sum(1, keepdim=True)
+    c = routed[:, None] / routed.sum() * p * rest
+    close(d, c * (f - dot), c * (f + dot), 210)
