@@ -31,10 +31,18 @@ struct Row {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int i = (j * THREADS + (int)threadIdx.x) * 8;
-        if (i < H) load8<T>(p, off + i, v + 8 * j);
-        else
+        if constexpr (T == T_F32) {
+          if (i < H) load8<T>(p, off + i, v + 8 * j);
+          else
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[8 * j + k] = 0.f;
+            for (int k = 0; k < 8; ++k) v[8 * j + k] = 0.f;
+        } else {
+          // (converted behind the branch: with the conversion in it the fp16 values of two chunks met through scratch
+          // memory, 8192 x 4096 78 us instead of 52)
+          u4 w = {0u, 0u, 0u, 0u};
+          if (i < H) w = *reinterpret_cast<const u4*>(reinterpret_cast<const uint16_t*>(p) + off + i);
+          unpack8<T>(w, v + 8 * j);
+        }
       }
     } else {
 #pragma unroll
