@@ -303,7 +303,9 @@ __global__ void __launch_bounds__(THREADS) k_norm_fwd(const DgmNormArgs P) {
 // Gradients: workgroup g takes rows g, g + G, ...; the columns' sums over its rows stay in registers and
 // go to partial[set][g][H] (set 0 pre weight, 1 post weight, 2 channel gate), which k_norm_columns adds up
 // in a fixed order.
-template <int T, int NV, int THREADS, bool VEC>
+// SIG: a gate, under a sigmoid (a kernel of its own: with it in the others' way, those that spill take up to 17 % longer
+// for rows without one).
+template <int T, int NV, int THREADS, bool VEC, bool SIG>
 __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
   using R = Row<NV, THREADS, VEC>;
   constexpr int N = R::N;
@@ -316,11 +318,12 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
 #pragma unroll
   for (int k = 0; k < N; ++k) dw2[k] = dw1[k] = dg[k] = 0.f;
   // 16-bit rows of eight elements a thread: the next row, with its rstd and token gate, is requested before
-  // the current one is worked on, and the weights and a channel gate (sigmoid and derivative taken) wait in LDS (each thread's own): loads are awaited in
+  // the current one is worked on, and the weights wait in LDS (each thread's own): loads are awaited in
   // their order, so weights read from memory in the loop would wait for the next row first.
   constexpr bool AHEAD = VEC && T != T_F32 && NV == 1;
-  // (a channel gate waits in LDS in fp32 too: its sigmoid and derivative are one row's work, not every row's)
-  constexpr bool HELD_GATE = VEC && NV == 1;
+  // A channel gate waits in LDS in all rows of eight elements a thread: its sigmoid and derivative are one row's work,
+  // not every row's.
+  constexpr bool HELD_GATE = NV == 1;
   constexpr int GATE = AHEAD ? 2 : 0;            // the gate's two sets, behind the weights'
   __shared__ f4 held_w[AHEAD ? 4 : HELD_GATE ? 2 : 1][2][HELD_GATE ? THREADS : 1];
   Held hx, hr, hd, hg, ha;
@@ -364,7 +367,7 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
     if (F.gate_mode == GATE_CHANNEL) {
       float v[N], d[N];
       R::template load<T>(F.gate, 0, H, v);
-      if (F.gate_sigmoid) {
+      if constexpr (SIG) {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
           const float rest = gate_sigmoid<T>(-v[k]);
@@ -403,7 +406,7 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
       for (int k = 0; k < N; ++k) t[k] *= w[k];
     }
     if (F.gate_mode == GATE_TOKEN) {
-      const float v = F.gate_sigmoid ? gate_sigmoid<T>(token_gate) : token_gate;
+      const float v = SIG ? gate_sigmoid<T>(token_gate) : token_gate;
 #pragma unroll
       for (int k = 0; k < N; ++k) a[k] = v;
     } else if (F.gate_mode != GATE_NONE) {
@@ -412,11 +415,11 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
         else R::template load<T>(F.gate, 0, H, a);
       } else if constexpr (AHEAD) {
         unpack8<T>(ca.w, a);
-        if (F.gate_sigmoid) keep(a, GATE);         // (the row's gate, for its derivative)
+        if constexpr (SIG) keep(a, GATE);         // (the row's gate, for its derivative)
       } else {
         R::template load<T>(F.gate, row * F.gate_stride, H, a);
       }
-      if (F.gate_sigmoid && !(HELD_GATE && F.gate_mode == GATE_CHANNEL))
+      if (SIG && !(HELD_GATE && F.gate_mode == GATE_CHANNEL))
 #pragma unroll
         for (int k = 0; k < N; ++k) a[k] = gate_sigmoid<T>(a[k]);
     }
@@ -457,7 +460,7 @@ __global__ void __launch_bounds__(THREADS) k_norm_bwd(const DgmNormGradArgs P) {
 #pragma unroll
     for (int k = 0; k < N; ++k) g[k] *= F.residual_scale;
     if (F.gate_mode != GATE_NONE) {
-      if (F.gate_sigmoid) {
+      if constexpr (SIG) {
         // the gate's derivative a (1 - a), with 1 - a = sigmoid(-gate): a difference keeps no bits of it beyond a gate
         // of 17 (computed here: held from above, or by the smaller of the two, every row would pay for it)
         if (F.gate_mode == GATE_TOKEN) {
@@ -670,8 +673,12 @@ int dgm_rms_norm_residual_backward(const DgmNormGradArgs* args, hipStream_t stre
   // (no rows: the partial sums of the one group are written as zeros)
   dispatch_type(F.dtype, vec, [&](auto t, auto v) {
     dispatch_hidden(F.hidden, [&](auto nv, auto threads) {
-      hipLaunchKernelGGL((k_norm_bwd<t.value, nv.value, threads.value, v.value>), dim3(groups), dim3(threads.value), 0,
-                         stream, A);
+      if (F.gate_mode != GATE_NONE && F.gate_sigmoid)
+        hipLaunchKernelGGL((k_norm_bwd<t.value, nv.value, threads.value, v.value, true>), dim3(groups), dim3(threads.value), 0,
+                           stream, A);
+      else
+        hipLaunchKernelGGL((k_norm_bwd<t.value, nv.value, threads.value, v.value, false>), dim3(groups), dim3(threads.value), 0,
+                           stream, A);
     });
     if (columns) {
       // (narrow rows have many groups: 16 columns a workgroup, so that there are enough of them)
