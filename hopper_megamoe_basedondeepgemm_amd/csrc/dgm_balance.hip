@@ -173,7 +173,7 @@ DGM_DEV void softmax(const float* l, float* p, float& lse) {
 
 // Sigmoid scores of a token, 1 / (1 + e^-l). Below -17 each is e^l to the last bit, and from -88 on out of fp32's range,
 // which their shares are not: the scores of a row that lies there are taken times e^-m, as 1 / (0 + e^(m - l)).
-// (A constant and a shift for each row, so that no element pays for it.)
+// (A constant and a shift for each row: a select for each element and a branch for such rows both cost more.)
 struct Sigmoid {
   float one, shift;
   template <int NV>

@@ -512,7 +512,8 @@ void launch_tiles(const DgmInt8GemmArgs& A, int vec, int splits, hipStream_t str
 //   192 x 256:            1536 x 8192, K 4096: 53 (256 x 256 61);    4096 x 5120, K 2880: 82 (256 x 192 93)
 //   256 x 192:            8192 x 2880, K 2880: 88 (192 x 128 98);    4096 x 2880, K 2880: 45 (256 x 256 50)
 //   256 x 256:            8192 x 8192, K 4096: 243 (192 x 256 266);  2048 x 8192, K 4096: 69 (128 x 128 82)
-// Up to 192 x 128 the steps are bound by the loads that a CU keeps in flight (more stages: no faster).
+// Up to 192 x 128 a step takes 2.5 to 3 times what the matrix instructions need; more stages, so more loads in flight,
+// are no faster, and the cause is not known.
 // The rows form takes 2 us and, per 1024 of a part of K and round of 256 workgroups, 0.75 us up to 4 tokens, 1.25
 // up to 16, 1.65 up to 32 and 2.8 up to 64 (SwiGLU with a fragment each for gate and up rows 1.75 times the first
 // two and twice the others): 16 x 4096, K 7168: 11.5 us (64 x 64, 4 splits 13); 32 x 8192, K 4096: 16.5 us (64 x 64,

@@ -38,7 +38,7 @@ struct Row {
             for (int k = 0; k < 8; ++k) v[8 * j + k] = 0.f;
         } else {
           // (converted behind the branch: with the conversion in it the fp16 values of two chunks met through scratch
-          // memory, 8192 x 4096 78 us instead of 52)
+          // memory, 8192 x 4096 78 us instead of 46)
           u4 w = {0u, 0u, 0u, 0u};
           if (i < H) w = *reinterpret_cast<const u4*>(reinterpret_cast<const uint16_t*>(p) + off + i);
           unpack8<T>(w, v + 8 * j);
@@ -560,7 +560,10 @@ int check_forward(const DgmNormArgs* A) {
   return 0;
 }
 
-// Threads of a row's workgroup: eight elements each up to 8192, then sixteen (unaligned rows alike).
+// Threads of a row's workgroup: eight elements each up to 8192, then sixteen (unaligned rows alike). Backward, sixteen
+// elements with their column sums do not fit the 128 registers that 1024 threads leave: 106 to 144 of them are kept in
+// scratch memory (aligned; unaligned 196 to 266, and 14 to 50 for rows of 4097 to 8192), and 2048 x 16384 bf16 takes 264
+// us, 1.5 TB/s.
 template <class F>
 void dispatch_hidden(int H, F&& f) {
   using std::integral_constant;
@@ -571,8 +574,8 @@ void dispatch_hidden(int H, F&& f) {
   else if (H <= 8192) f(integral_constant<int, 1>{}, integral_constant<int, 1024>{});
   else f(integral_constant<int, 2>{}, integral_constant<int, 1024>{});
 }
-// Forward rows of 16 bits, many of them: half the threads with sixteen elements each (8192 x 4096: 57 -> 51
-// us, 4096 x 7168: 52 -> 46 us; one row of 4096 takes 5.4 us the other way and 5.8 this one, fp32 rows 48 and
+// Forward rows of 16 bits, many of them: half the threads with sixteen elements each (bf16, 8192 x 4096: 57 -> 51
+// us, 4096 x 7168: 52 -> 46 us; fp16 takes bf16's time; one row of 4096 takes 5.4 us the other way and 5.8 this one, fp32 rows 48 and
 // 49 us at 4096 x 4096).
 template <class F>
 void dispatch_hidden_pairs(int H, F&& f) {
