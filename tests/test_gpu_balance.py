@@ -286,3 +286,28 @@ def test_saved_tensors_that_come_back_strided_or_elsewhere():
     for part in ((300, 64), (300, 4), (3,), (2, 64), (12,)):
         with pytest.raises(RuntimeError, match="cpu|GPU"):
             grad(lambda t: t.cpu() if t.shape == part else t)
+
+
+@pytest.mark.parametrize("turned", [False, True])
+def test_several_backward_passes_and_moved_memory(turned):
+    """The same graph run twice with other incoming gradients, two graphs alive at once, inputs that are read as copies
+    and inputs whose memory is replaced between the passes: the plain call's gradient each time."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    logits, idx = make(700, 96, 4, torch.bfloat16, seed=12)
+    cu = torch.tensor([0, 100, 101, 650], dtype=torch.int32, device="cuda")
+    every = torch.stack([cu, cu + 7], 1)[:, 0]                   # (strided: read as a copy)
+    turn = lambda t: t.t().contiguous().t() if turned else t.clone()
+    want = run(logits, idx, cu.tolist(), 1.0, 0.01, "softmax")[2]
+    twice = run(logits, idx, cu.tolist(), 1.0, 0.01, "softmax", g=-2.0)[2]
+    a, b = turn(logits).requires_grad_(), turn(logits + 1).requires_grad_()
+    la, _ = dgm.router_balance_loss(a, turn(idx), every, 1.0, 0.01)
+    lb, _ = dgm.router_balance_loss(b, turn(idx), every, 1.0, 0.01)
+    keep = [torch.full((700 * 96,), 7, dtype=torch.int32, device="cuda") for _ in range(8)]      # (over given up memory)
+    other = torch.autograd.grad(lb, b)[0]
+    assert torch.equal(torch.autograd.grad(la * -2.0, a, retain_graph=True)[0], twice)
+    assert torch.equal(torch.autograd.grad(la, a, retain_graph=True)[0], want)
+    a.data = a.data.clone()
+    assert torch.equal(torch.autograd.grad(la, a)[0], want)
+    assert torch.equal(other, run(logits + 1, idx, cu.tolist(), 1.0, 0.01, "softmax")[2])
+    del keep
