@@ -9,30 +9,11 @@
 // registers hold consecutive channels of one token.
 #include "dgm_common.hpp"
 #include "dgm_abi_internal.hpp"
+#include "dgm_epilogue.hpp"
 
 using namespace dgm;
 
 namespace {
-
-// (compared, not fminf / fmaxf, which put the clamp in the place of what is no number)
-DGM_DEV float swiglu(float g, float u, float clamp, bool fast) {
-  g = g > clamp ? clamp : g;
-  u = u > clamp ? clamp : u < -clamp ? -clamp : u;
-  return g * (fast ? sigmoid<true>(g) : sigmoid<false>(g)) * u;
-}
-
-// Type of D (and C) and what is added, as compile-time values: f(integral_constant dtype, bool_constant add).
-template <class F>
-DGM_DEV void with_epilogue(const DgmInt8GemmArgs& P, F&& f) {
-  using std::integral_constant;
-  auto add = [&](auto t) {
-    if (P.c) f(t, std::true_type{});
-    else f(t, std::false_type{});
-  };
-  if (P.dtype == DGM_SRC_F32) add(integral_constant<int, DGM_SRC_F32>{});
-  else if (P.dtype == DGM_SRC_F16) add(integral_constant<int, DGM_SRC_F16>{});
-  else add(integral_constant<int, DGM_SRC_BF16>{});
-}
 
 // scales of channels n .. n + 3 (behind the last: its own)
 DGM_DEV v4f load_scales(const DgmInt8GemmArgs& P, int64_t n, int64_t end) {
@@ -42,114 +23,16 @@ DGM_DEV v4f load_scales(const DgmInt8GemmArgs& P, int64_t n, int64_t end) {
   return s;
 }
 
-template <int T>
-DGM_DEV float c_value(const void* p, int64_t i) {
-  if constexpr (T == DGM_SRC_F32) return reinterpret_cast<const float*>(p)[i];
-  else if constexpr (T == DGM_SRC_F16) return (float)reinterpret_cast<const _Float16*>(p)[i];
-  else return bf16_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
-}
-
-// Orders a wave's LDS accesses before and after it, between its lanes.
-DGM_DEV void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-// A 16-byte piece of token m's row from channel n on (eight channels, fp32: four), from LDS: C added, rounded,
-// stored. vec: rows of D (and C) are 16-byte aligned.
-template <int T, bool ADD>
-DGM_DEV void put_piece(const DgmInt8GemmArgs& P, int64_t m, int64_t n, int64_t n_out, int vec, const float* from) {
-  constexpr int E = T == DGM_SRC_F32 ? 4 : 8;
-  if (n >= n_out) return;
-  float v[E];
-#pragma unroll
-  for (int i = 0; i < E; i += 4) {
-    const v4f f = *reinterpret_cast<const v4f*>(from + i);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[i + k] = f[k];
-  }
-  const int64_t at = m * P.d_stride + n, ct = m * P.c_stride + n;
-  if (vec && n + E <= n_out) {
-    if constexpr (T == DGM_SRC_F32) {
-      if constexpr (ADD) {
-        const v4f c = *reinterpret_cast<const v4f*>(reinterpret_cast<const float*>(P.c) + ct);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += c[i];
-      }
-      *reinterpret_cast<v4f*>(reinterpret_cast<float*>(P.d) + at) = v4f{v[0], v[1], v[2], v[3]};
-    } else {
-      if constexpr (ADD) {
-        const v4i c = *reinterpret_cast<const v4i*>(reinterpret_cast<const uint16_t*>(P.c) + ct);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint16_t w[1] = {(uint16_t)((uint32_t)c[i >> 1] >> (16 * (i & 1)))};
-          v[i] += c_value<T>(w, 0);
-        }
-      }
-      v4i o;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t lo = T == DGM_SRC_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[2 * i]) : __builtin_bit_cast(uint16_t, (__bf16)v[2 * i]);
-        const uint32_t hi = T == DGM_SRC_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[2 * i + 1]) : __builtin_bit_cast(uint16_t, (__bf16)v[2 * i + 1]);
-        o[i] = (int)(lo | hi << 16);
-      }
-      *reinterpret_cast<v4i*>(reinterpret_cast<uint16_t*>(P.d) + at) = o;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      if (n + i >= n_out) continue;
-      if constexpr (ADD) v[i] += c_value<T>(P.c, ct + i);
-      if constexpr (T == DGM_SRC_F32) reinterpret_cast<float*>(P.d)[at + i] = v[i];
-      else if constexpr (T == DGM_SRC_F16) reinterpret_cast<_Float16*>(P.d)[at + i] = (_Float16)v[i];
-      else reinterpret_cast<__bf16*>(P.d)[at + i] = (__bf16)v[i];
-    }
-  }
-}
-
-// Channels n .. n + 3 of token m; WHOLE: all four exist and one store (one load of C) takes them.
+// Channels n .. n + 3 of token m with their scales.
 template <int T, bool ADD, bool SWIGLU, bool WHOLE>
-DGM_DEV void put4(const DgmInt8GemmArgs& P, int64_t m, int64_t n, int64_t n_out, float sa, v4f sb, v4f su, v4i acc, v4i up) {
+DGM_DEV void put4_scaled(const DgmInt8GemmArgs& P, int64_t m, int64_t n, int64_t n_out, float sa, v4f sb, v4f su, v4i acc, v4i up) {
   float v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     v[i] = (float)acc[i] * (sa * sb[i]);
     if constexpr (SWIGLU) v[i] = swiglu(v[i], (float)up[i] * (sa * su[i]), P.clamp, P.fast_math);
   }
-  const int64_t at = m * P.d_stride + n, ct = m * P.c_stride + n;
-  if constexpr (WHOLE) {
-    if constexpr (ADD) {
-      if constexpr (T == DGM_SRC_F32) {
-        const v4f c = *reinterpret_cast<const v4f*>(reinterpret_cast<const float*>(P.c) + ct);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += c[i];
-      } else {
-        const uint2 c = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(P.c) + ct);
-        const uint16_t w[4] = {(uint16_t)c.x, (uint16_t)(c.x >> 16), (uint16_t)c.y, (uint16_t)(c.y >> 16)};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += c_value<T>(w, i);
-      }
-    }
-    if constexpr (T == DGM_SRC_F32) {
-      *reinterpret_cast<v4f*>(reinterpret_cast<float*>(P.d) + at) = v4f{v[0], v[1], v[2], v[3]};
-    } else {
-      uint32_t h[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        h[i] = T == DGM_SRC_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[i]) : __builtin_bit_cast(uint16_t, (__bf16)v[i]);
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(P.d) + at) = uint2{h[0] | h[1] << 16, h[2] | h[3] << 16};
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (n + i >= n_out) continue;
-      if constexpr (ADD) v[i] += c_value<T>(P.c, ct + i);
-      if constexpr (T == DGM_SRC_F32) reinterpret_cast<float*>(P.d)[at + i] = v[i];
-      else if constexpr (T == DGM_SRC_F16) reinterpret_cast<_Float16*>(P.d)[at + i] = (_Float16)v[i];
-      else reinterpret_cast<__bf16*>(P.d)[at + i] = (__bf16)v[i];
-    }
-  }
+  put4<T, ADD, WHOLE>(P, m, n, n_out, v);
 }
 
 // 16 bytes of a row from k on. ALIGNED: K is a multiple of 16 and rows are 16-byte aligned. Behind K: zeros
@@ -241,8 +124,8 @@ __global__ void __launch_bounds__(512) k_int8_gemm_rows(const DgmInt8GemmArgs P,
   const float sa = P.sfa[m * P.sfa_stride];
   const v4f sb = load_scales(P, n, n_out), su = SWIGLU ? load_scales(P, n_out + n, 2 * n_out) : sb;
   with_epilogue(P, [&](auto t, auto add) {
-    if (vec && n + 3 < n_out) put4<t.value, add.value, SWIGLU, true>(P, m, n, n_out, sa, sb, su, s[0], s[1]);
-    else put4<t.value, add.value, SWIGLU, false>(P, m, n, n_out, sa, sb, su, s[0], s[1]);
+    if (vec && n + 3 < n_out) put4_scaled<t.value, add.value, SWIGLU, true>(P, m, n, n_out, sa, sb, su, s[0], s[1]);
+    else put4_scaled<t.value, add.value, SWIGLU, false>(P, m, n, n_out, sa, sb, su, s[0], s[1]);
   });
 }
 
@@ -446,8 +329,8 @@ __global__ void __launch_bounds__(256) k_int8_gemm_join(const DgmInt8GemmArgs P,
   const float sa = P.sfa[m * P.sfa_stride];
   const v4f sb = load_scales(P, n, n_out), su = SWIGLU ? load_scales(P, n_out + n, 2 * n_out) : sb;
   with_epilogue(P, [&](auto t, auto add) {
-    if (vec && n + 3 < n_out) put4<t.value, add.value, SWIGLU, true>(P, m, n, n_out, sa, sb, su, s[0], s[1]);
-    else put4<t.value, add.value, SWIGLU, false>(P, m, n, n_out, sa, sb, su, s[0], s[1]);
+    if (vec && n + 3 < n_out) put4_scaled<t.value, add.value, SWIGLU, true>(P, m, n, n_out, sa, sb, su, s[0], s[1]);
+    else put4_scaled<t.value, add.value, SWIGLU, false>(P, m, n, n_out, sa, sb, su, s[0], s[1]);
   });
 }
 
