@@ -20,6 +20,9 @@ from .utils import per_token_cast_to_fp4, per_token_cast_to_fp8, ceil_div, align
 from .balance import router_balance_loss, router_balance_loss_backward, router_balance_loss_forward
 from .int8_gemm import int8_gemm_nt
 from .norm import rms_norm_residual, rms_norm_residual_backward, rms_norm_residual_forward
+from .mxfp4 import (mxfp4_gemm_nt, mxfp4_linear, mxfp4_linear_backward, mxfp4_linear_forward, mxfp4_quantize,
+                    mxfp4_quantize_both)
+from .layer_norm import layer_norm_residual, layer_norm_residual_backward, layer_norm_residual_forward
 from .block import mega_moe_block
 from . import checkpoint
 from .checkpoint import (mxfp4_checkpoint_to_mega_moe, nvfp4_checkpoint_to_mega_moe, mega_moe_to_mxfp4_checkpoint,
@@ -46,4 +49,6 @@ __all__ = [
     "get_nvfp4_mega_moe_sm90_weight_layout",
     "router_balance_loss", "router_balance_loss_forward", "router_balance_loss_backward",
     "mega_moe_block", "int8_gemm_nt", "rms_norm_residual", "rms_norm_residual_forward", "rms_norm_residual_backward",
+    "mxfp4_quantize", "mxfp4_quantize_both", "mxfp4_gemm_nt", "mxfp4_linear", "mxfp4_linear_forward", "mxfp4_linear_backward",
+    "layer_norm_residual", "layer_norm_residual_forward", "layer_norm_residual_backward",
 ]

@@ -36,6 +36,9 @@ EXPORTS = [
     "dgm_norm_struct_sizes", "dgm_int8_gemm_nt", "dgm_int8_gemm_struct_size",
     "dgm_int8_gemm_workspace_bytes", "dgm_router_balance_loss", "dgm_router_balance_loss_backward",
     "dgm_router_balance_workspace_bytes", "dgm_balance_struct_size",
+    "dgm_layer_norm_residual", "dgm_layer_norm_residual_groups", "dgm_layer_norm_residual_backward",
+    "dgm_layer_norm_struct_sizes", "dgm_mxfp4_quantize", "dgm_mxfp4_quant_struct_size", "dgm_mxfp4_gemm_nt",
+    "dgm_mxfp4_gemm_struct_size", "dgm_mxfp4_gemm_workspace_bytes",
 ]
 # source element types of the weight packers (DGM_SRC_*)
 SRC_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -98,6 +101,35 @@ class NormGradArgs(ctypes.Structure):
                                                 "d_pre_weight", "workspace")] +
                 [(n, ctypes.c_int64) for n in ("workspace_bytes", "d_residual_out_stride", "d_h_stride", "d_x_stride",
                                                "d_residual_stride", "d_gate_stride")])
+
+
+class LayerNormArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "residual", "weight", "bias", "residual_out", "h", "codes", "scales",
+                                                "mean", "rstd")] +
+                [(n, ctypes.c_int64) for n in ("rows", "x_stride", "residual_stride", "residual_out_stride", "h_stride")] +
+                [(n, ctypes.c_int32) for n in ("hidden", "dtype", "weights_f32")] +
+                [("residual_scale", ctypes.c_float), ("eps", ctypes.c_float)])
+
+
+class LayerNormGradArgs(ctypes.Structure):
+    _fields_ = ([("forward", LayerNormArgs)] +
+                [(n, ctypes.c_void_p) for n in ("d_residual_out", "d_h", "d_x", "d_residual", "d_weight", "d_bias", "workspace")] +
+                [(n, ctypes.c_int64) for n in ("workspace_bytes", "d_residual_out_stride", "d_h_stride", "d_x_stride",
+                                               "d_residual_stride")])
+
+
+class Mxfp4QuantArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "codes", "scales", "t_codes", "t_scales")] +
+                [(n, ctypes.c_int64) for n in ("rows", "cols", "x_stride")] +
+                [("dtype", ctypes.c_int32), ("amax_floor", ctypes.c_float)])
+
+
+class Mxfp4GemmArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("a", "sfa", "b", "sfb", "c", "d")] +
+                [(n, ctypes.c_int64) for n in ("m", "n", "k", "a_stride", "sfa_stride", "b_stride", "sfb_stride",
+                                               "c_stride", "d_stride")] +
+                [("dtype", ctypes.c_int32), ("swiglu", ctypes.c_int32), ("clamp", ctypes.c_float),
+                 ("fast_math", ctypes.c_int32), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)])
 
 
 class Int8GemmArgs(ctypes.Structure):
@@ -179,6 +211,15 @@ def load():
     sig["dgm_norm_struct_sizes"] = ([ctypes.POINTER(ctypes.c_size_t)] * 2, i32)
     sig["dgm_rms_norm_residual_groups"] = ([i64, i32], i32)
     sig["dgm_rms_norm_residual_backward"] = ([ctypes.POINTER(NormGradArgs), vp], i32)
+    sig["dgm_layer_norm_residual"] = ([ctypes.POINTER(LayerNormArgs), vp], i32)
+    sig["dgm_layer_norm_residual_groups"] = ([i64, i32], i32)
+    sig["dgm_layer_norm_residual_backward"] = ([ctypes.POINTER(LayerNormGradArgs), vp], i32)
+    sig["dgm_layer_norm_struct_sizes"] = ([ctypes.POINTER(ctypes.c_size_t)] * 2, i32)
+    sig["dgm_mxfp4_quantize"] = ([ctypes.POINTER(Mxfp4QuantArgs), vp], i32)
+    sig["dgm_mxfp4_quant_struct_size"] = ([ctypes.POINTER(ctypes.c_size_t)], i32)
+    sig["dgm_mxfp4_gemm_nt"] = ([ctypes.POINTER(Mxfp4GemmArgs), vp], i32)
+    sig["dgm_mxfp4_gemm_workspace_bytes"] = ([i64, i64, i64, i32], i64)
+    sig["dgm_mxfp4_gemm_struct_size"] = ([ctypes.POINTER(ctypes.c_size_t)], i32)
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
         fn.argtypes = args

@@ -1,0 +1,279 @@
+// Residual add and layer norm (gfx950) in one pass over the rows, and the gradients of both.
+//
+// Row of H elements: t = residual + s x (t = s x without residual), mu = mean t, rstd = rsqrt(mean (t - mu)^2 + eps),
+// u = (t - mu) rstd, h = u w + b (w, b: 1 and 0 if absent). Everything between the loads and the stores is fp32; t
+// enters the norm unrounded and stays in registers, so that the variance is that of the differences from the mean (no
+// cancellation) and each input is read once. A workgroup owns a row; the bound is HBM.
+// Gradients, with R = dL/dt (of the stored t) and D = dL/dh:
+//   du = D w, R' = R + rstd (du - mean du - u mean(du u)), dresidual = R', dx = s R', dw = sum D u, db = sum D.
+#include "dgm_abi_internal.hpp"
+#include "dgm_mxfp4.hpp"
+#include "dgm_row_tiles.hpp"
+
+using namespace dgm;
+
+namespace {
+
+// t, in fp32 and in this order wherever it is computed: forward and backward see the same bits.
+DGM_DEV float total(float r, float s, float x) { return fmaf(s, x, r); }
+
+template <int T, int NV, int THREADS, bool VEC>
+__global__ void __launch_bounds__(THREADS) k_layer_norm_fwd(const DgmLayerNormArgs P) {
+  using R = Row<NV, THREADS, VEC>;
+  constexpr int N = R::N;
+  __shared__ float lds[2][THREADS / 64][2];
+  Reduce<THREADS> red{lds};
+  const int H = P.hidden;
+  const int64_t row = blockIdx.x;
+  const bool wf = P.weights_f32;
+  const float inv_h = 1.0f / (float)H;
+  float t[N], w[N];
+  R::template load<T>(P.x, row * P.x_stride, H, t);
+  if (P.residual) {
+    R::template load<T>(P.residual, row * P.residual_stride, H, w);
+#pragma unroll
+    for (int k = 0; k < N; ++k) t[k] = total(w[k], P.residual_scale, t[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) t[k] *= P.residual_scale;
+  }
+  if (P.residual_out) R::template store<T>(P.residual_out, row * P.residual_out_stride, H, t);
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) sum += t[k];       // (zeros behind H)
+  red.run(sum);
+  const float mean = sum / (float)H;              // (by 1 / H, a row of equal elements would not have them for its mean)
+  float ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    t[k] = R::index(k) < H ? t[k] - mean : 0.f;
+    ss += t[k] * t[k];
+  }
+  red.run(ss);
+  const float rstd = 1.0f / sqrtf(ss * inv_h + P.eps);
+  if (P.mean && threadIdx.x == 0) P.mean[row] = mean, P.rstd[row] = rstd;
+#pragma unroll
+  for (int k = 0; k < N; ++k) t[k] *= rstd;
+  if (P.weight) {
+    R::template weight<T>(P.weight, wf, H, w);
+#pragma unroll
+    for (int k = 0; k < N; ++k) t[k] *= w[k];
+  }
+  if (P.bias) {
+    R::template weight<T>(P.bias, wf, H, w);
+#pragma unroll
+    for (int k = 0; k < N; ++k) t[k] += w[k];
+  }
+  if (P.h) R::template store<T>(P.h, row * P.h_stride, H, t);
+  if constexpr (T == T_BF16 && VEC) {
+    if (!P.codes) return;
+    // MXFP4 rows of the rounded h: a thread's eight elements are a quarter of a block (zeros behind H)
+    const int64_t blocks = (H + 31) / 32;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t[8 * j + k] = round_bf16(t[8 * j + k]);
+      const uint32_t code = mx_scale_code(max_u32_lanes4(magnitude8(t + 8 * j)), __float_as_uint(1e-30f));
+      const int64_t piece = j * THREADS + (int)threadIdx.x;
+      if (piece >= 4 * blocks) continue;
+      reinterpret_cast<uint32_t*>(P.codes)[row * blocks * 4 + piece] = e2m1_codes8<T>(t + 8 * j, code);
+      if ((piece & 3) == 0) P.scales[row * blocks + (piece >> 2)] = (uint8_t)code;
+    }
+  }
+}
+
+// Gradients: workgroup g takes rows g, g + G, ...; the columns' sums over its rows stay in registers and go to
+// partial[set][g][H] (set 0 weight, 1 bias), which k_layer_norm_columns adds up in a fixed order.
+template <int T, int NV, int THREADS, bool VEC>
+__global__ void __launch_bounds__(THREADS) k_layer_norm_bwd(const DgmLayerNormGradArgs P) {
+  using R = Row<NV, THREADS, VEC>;
+  constexpr int N = R::N;
+  __shared__ float lds[2][THREADS / 64][2];
+  Reduce<THREADS> red{lds};
+  const DgmLayerNormArgs& F = P.forward;
+  const int H = F.hidden;
+  const float inv_h = 1.0f / (float)H;
+  float dw[N], db[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) dw[k] = db[k] = 0.f;
+  for (int64_t row = blockIdx.x; row < F.rows; row += gridDim.x) {
+    float g[N];
+    if (P.d_residual_out) R::template load<T>(P.d_residual_out, row * P.d_residual_out_stride, H, g);
+    else
+#pragma unroll
+      for (int k = 0; k < N; ++k) g[k] = 0.f;
+    if (P.d_h) {
+      float u[N], d[N], w[N];
+      R::template load<T>(F.x, row * F.x_stride, H, u);
+      if (F.residual) {
+        R::template load<T>(F.residual, row * F.residual_stride, H, w);
+#pragma unroll
+        for (int k = 0; k < N; ++k) u[k] = total(w[k], F.residual_scale, u[k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) u[k] *= F.residual_scale;
+      }
+      R::template load<T>(P.d_h, row * P.d_h_stride, H, d);
+      const float mean = F.mean[row], rstd = F.rstd[row];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        u[k] = (u[k] - mean) * rstd;
+        dw[k] += d[k] * u[k];
+        db[k] += d[k];
+      }
+      if (F.weight) {
+        R::template weight<T>(F.weight, F.weights_f32, H, w);
+#pragma unroll
+        for (int k = 0; k < N; ++k) d[k] *= w[k];
+      }
+      float sum = 0.f, dot = 0.f;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {          // (d is zero behind H)
+        sum += d[k];
+        dot += d[k] * u[k];
+      }
+      red.run(sum, dot);
+      sum *= inv_h;
+      dot *= inv_h;
+#pragma unroll
+      for (int k = 0; k < N; ++k) g[k] += rstd * (d[k] - sum - u[k] * dot);
+    }
+    if (P.d_residual) R::template store<T>(P.d_residual, row * P.d_residual_stride, H, g);
+    if (P.d_x) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) g[k] *= F.residual_scale;
+      R::template store<T>(P.d_x, row * P.d_x_stride, H, g);
+    }
+  }
+  const int64_t set = (int64_t)gridDim.x * H, off = (int64_t)blockIdx.x * H;
+  if (P.d_weight) R::template store<T_F32>(P.workspace, off, H, dw);
+  if (P.d_bias) R::template store<T_F32>(P.workspace, set + off, H, db);
+}
+
+// Column sums of partial[G][H]: a workgroup takes C columns, its thread groups of C the rows in turn.
+template <int T, int C>
+__global__ void __launch_bounds__(1024) k_layer_norm_columns(const DgmLayerNormGradArgs P, int groups) {
+  const DgmLayerNormArgs& F = P.forward;
+  constexpr int R = 1024 / C;
+  __shared__ float lds[R][C];
+  const int H = F.hidden, c = threadIdx.x % C, r = threadIdx.x / C, col = blockIdx.x * C + c, set = blockIdx.y;
+  void* out = set == 0 ? P.d_weight : P.d_bias;
+  if (!out) return;                               // (the whole workgroup)
+  const float* src = (const float*)P.workspace + (int64_t)set * groups * H;
+  float s = 0.f;
+  if (col < H)
+#pragma unroll 8
+    for (int i = r; i < groups; i += R) s += src[(int64_t)i * H + col];
+  lds[r][c] = s;
+  __syncthreads();
+  if (r == 0 && col < H) {
+#pragma unroll 8
+    for (int i = 1; i < R; ++i) s += lds[i][c];
+    if (F.weights_f32) store1<T_F32>(out, col, s);
+    else store1<T>(out, col, s);
+  }
+}
+
+// Threads of a row's workgroup: eight elements each up to 8192, then sixteen.
+template <class F>
+void dispatch_hidden(int H, F&& f) {
+  using std::integral_constant;
+  if (H <= 512) f(integral_constant<int, 1>{}, integral_constant<int, 64>{});
+  else if (H <= 1024) f(integral_constant<int, 1>{}, integral_constant<int, 128>{});
+  else if (H <= 2048) f(integral_constant<int, 1>{}, integral_constant<int, 256>{});
+  else if (H <= 4096) f(integral_constant<int, 1>{}, integral_constant<int, 512>{});
+  else if (H <= 8192) f(integral_constant<int, 1>{}, integral_constant<int, 1024>{});
+  else f(integral_constant<int, 2>{}, integral_constant<int, 1024>{});
+}
+
+int check_forward(const DgmLayerNormArgs* A) {
+  DGM_CHECK_ARG(A->dtype >= DGM_SRC_BF16 && A->dtype <= DGM_SRC_F32, "dtype 0 bf16, 1 fp16, 2 fp32");
+  // (a launch has fewer than 2^32 threads, a row up to 1024 of them)
+  DGM_CHECK_ARG(A->rows >= 0 && A->rows < (1 << 22), "rows below 2^22");
+  DGM_CHECK_ARG(A->hidden > 0 && A->hidden <= DGM_NORM_MAX_HIDDEN, "hidden 1 to 16384");
+  DGM_CHECK_ARG(A->eps >= 0.f, "eps >= 0");
+  DGM_CHECK_ARG(A->rows == 0 || A->x, "null x");
+  return 0;
+}
+
+bool forward_aligned(const DgmLayerNormArgs* A) {
+  const int e = element_size(A->dtype);
+  return A->hidden % 8 == 0 && aligned(A->x, A->x_stride, e) && aligned(A->residual, A->residual_stride, e) &&
+         aligned(A->weight, 0, e) && aligned(A->bias, 0, e) && aligned(A->residual_out, A->residual_out_stride, e) &&
+         aligned(A->h, A->h_stride, e);
+}
+
+}  // namespace
+
+extern "C" {
+
+int dgm_layer_norm_struct_sizes(size_t* norm_args, size_t* norm_grad_args) {
+  DGM_CHECK_ARG(norm_args && norm_grad_args, "null pointer");
+  *norm_args = sizeof(DgmLayerNormArgs);
+  *norm_grad_args = sizeof(DgmLayerNormGradArgs);
+  return 0;
+}
+
+int dgm_layer_norm_residual(const DgmLayerNormArgs* args, hipStream_t stream) {
+  DGM_CHECK_ARG(args, "null arguments");
+  if (int st = check_forward(args)) return st;
+  const DgmLayerNormArgs A = *args;
+  const bool vec = forward_aligned(&A);
+  DGM_CHECK_ARG((A.codes != nullptr) == (A.scales != nullptr), "codes with their scales");
+  DGM_CHECK_ARG((A.mean != nullptr) == (A.rstd != nullptr), "mean with rstd");
+  DGM_CHECK_ARG(!A.codes || (A.dtype == DGM_SRC_BF16 && vec && ((uintptr_t)A.codes & 3) == 0), "MXFP4 rows: of 16-byte aligned bf16 rows of whole eights");
+  if (A.rows == 0) return 0;
+  dispatch_type(A.dtype, vec, [&](auto t, auto v) {
+    dispatch_hidden(A.hidden, [&](auto nv, auto threads) {
+      hipLaunchKernelGGL((k_layer_norm_fwd<t.value, nv.value, threads.value, v.value>), dim3((unsigned)A.rows),
+                         dim3(threads.value), 0, stream, A);
+    });
+  });
+  return dgm_last_launch_status();
+}
+
+// As many workgroups as the CUs hold (16 waves each), a row each at least.
+int dgm_layer_norm_residual_groups(int64_t rows, int hidden) {
+  int64_t most = 4096;
+  dispatch_hidden(hidden, [&](auto, auto threads) { most = 4096 / (threads.value / 64); });
+  return (int)(rows < 1 ? 1 : rows < most ? rows : most);
+}
+
+int dgm_layer_norm_residual_backward(const DgmLayerNormGradArgs* args, hipStream_t stream) {
+  DGM_CHECK_ARG(args, "null arguments");
+  const DgmLayerNormGradArgs A = *args;
+  const DgmLayerNormArgs& F = A.forward;
+  if (int st = check_forward(&F)) return st;
+  const bool columns = A.d_weight || A.d_bias;
+  const int groups = dgm_layer_norm_residual_groups(F.rows, F.hidden);
+  if (F.rows > 0) {
+    DGM_CHECK_ARG(!A.d_h || (F.mean && F.rstd), "mean and rstd of the forward pass");
+    DGM_CHECK_ARG(!A.d_residual || F.residual, "d_residual without a residual");
+  }
+  DGM_CHECK_ARG(!A.d_weight || F.weight, "d_weight without its weight");
+  DGM_CHECK_ARG(!A.d_bias || F.bias, "d_bias without its bias");
+  DGM_CHECK_ARG(!columns || (A.workspace && A.workspace_bytes >= (int64_t)groups * F.hidden * 8 &&
+                             ((uintptr_t)A.workspace & 15) == 0),
+                "workspace of 2 x groups x hidden floats, 16-byte aligned");
+  const int e = element_size(F.dtype);
+  const bool vec = forward_aligned(&F) && aligned(A.d_residual_out, A.d_residual_out_stride, e) &&
+                   aligned(A.d_h, A.d_h_stride, e) && aligned(A.d_x, A.d_x_stride, e) &&
+                   aligned(A.d_residual, A.d_residual_stride, e);
+  // (no rows: the partial sums of the one group are written as zeros)
+  dispatch_type(F.dtype, vec, [&](auto t, auto v) {
+    dispatch_hidden(F.hidden, [&](auto nv, auto threads) {
+      hipLaunchKernelGGL((k_layer_norm_bwd<t.value, nv.value, threads.value, v.value>), dim3(groups), dim3(threads.value), 0,
+                         stream, A);
+    });
+    if (columns) {
+      // (narrow rows have many groups: 16 columns a workgroup, so that there are enough of them)
+      if (groups > 1024)
+        hipLaunchKernelGGL((k_layer_norm_columns<t.value, 16>), dim3((F.hidden + 15) / 16, 2), dim3(1024), 0, stream, A, groups);
+      else
+        hipLaunchKernelGGL((k_layer_norm_columns<t.value, 64>), dim3((F.hidden + 63) / 64, 2), dim3(1024), 0, stream, A, groups);
+    }
+  });
+  return dgm_last_launch_status();
+}
+
+}  // extern "C"

@@ -1,0 +1,143 @@
+// Rows, or columns, of a matrix as MXFP4 (gfx950): blocks of 32 values along a row (column) become E2M1 codes, two a
+// byte, under one E8M0 scale,
+//   e = least integer with max(amax, floor) <= 6 2^e (at least -126),  code = nearest E2M1 of x / 2^e,
+// midpoints to the smaller magnitude; a block that holds an infinity or NaN gets scale 255 and zeros. Behind the last
+// element a block holds zeros. About ten operations a value: the bound is HBM, at 2 (fp32 4) bytes read and 17 / 32
+// written a value (both ways: twice 17 / 32).
+#include "dgm_abi_internal.hpp"
+#include "dgm_mxfp4.hpp"
+#include "dgm_row_tiles.hpp"
+
+using namespace dgm;
+
+namespace {
+
+// eight elements of row `row` from column c on, zeros behind the last
+template <int T, bool VEC>
+DGM_DEV void load_piece(const DgmMxfp4QuantArgs& P, int64_t row, int64_t c, float* v) {
+  if constexpr (VEC) {
+    if (c < P.cols) load8<T>(P.x, row * P.x_stride + c, v);
+    else
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < P.cols ? load1<T>(P.x, row * P.x_stride + c + i) : 0.f;
+  }
+}
+
+// Rows: a thread takes eight values, four neighbours a block. 2^log_row threads a row of the workgroup, `runs`
+// workgroups along a row.
+template <int T, bool VEC>
+__global__ void __launch_bounds__(256) k_mxfp4_rows(const DgmMxfp4QuantArgs P, int log_row, int runs) {
+  const int64_t group = blockIdx.x / (unsigned)runs;
+  const int run = (int)(blockIdx.x - group * runs);
+  const int64_t row = (group << (8 - log_row)) + (threadIdx.x >> log_row);
+  const int64_t piece = ((int64_t)run << log_row) + (threadIdx.x & ((1 << log_row) - 1));
+  const int64_t blocks = (P.cols + 31) / 32;
+  if (row >= P.rows || piece >= 4 * blocks) return;           // (whole blocks: four lanes share one)
+  float v[8];
+  load_piece<T, VEC>(P, row, piece * 8, v);
+  const uint32_t code = mx_scale_code(max_u32_lanes4(magnitude8(v)), __float_as_uint(P.amax_floor));
+  reinterpret_cast<uint32_t*>(P.codes)[row * blocks * 4 + piece] = e2m1_codes8<T>(v, code);
+  if ((piece & 3) == 0) P.scales[row * blocks + (piece >> 2)] = (uint8_t)code;
+}
+
+// Columns, and rows with them (BOTH): a tile of R rows x 128 columns is read once, its rows' codes are made on the
+// way into LDS, and a thread then takes 32 rows of a column.
+template <int T, bool VEC, bool BOTH>
+__global__ void __launch_bounds__(256) k_mxfp4_columns(const DgmMxfp4QuantArgs P, int tiles_c) {
+  constexpr int R = T == T_F32 ? 64 : 128, C = 128;
+  using E = std::conditional_t<T == T_F32, uint32_t, uint16_t>;
+  __shared__ __attribute__((aligned(16))) E tile[R][C];
+  const int64_t r0 = (int64_t)(blockIdx.x / (unsigned)tiles_c) * R, c0 = (int64_t)(blockIdx.x % (unsigned)tiles_c) * C;
+  const int64_t row_blocks = (P.cols + 31) / 32, col_blocks = (P.rows + 31) / 32;
+  const uint32_t floor_bits = __float_as_uint(P.amax_floor);
+  const int at = (threadIdx.x & 15) * 8;
+#pragma unroll
+  for (int i = 0; i < R / 16; ++i) {
+    const int r = i * 16 + (threadIdx.x >> 4);
+    float v[8];
+    if (r0 + r < P.rows) load_piece<T, VEC>(P, r0 + r, c0 + at, v);
+    else
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = 0.f;
+    store8<T>(&tile[r][0], at, v);              // (exact: the values are of type T)
+    if constexpr (BOTH) {
+      const uint32_t code = mx_scale_code(max_u32_lanes4(magnitude8(v)), floor_bits);
+      const int64_t piece = (c0 + at) / 8;
+      if (r0 + r < P.rows && piece < 4 * row_blocks) {
+        reinterpret_cast<uint32_t*>(P.codes)[(r0 + r) * row_blocks * 4 + piece] = e2m1_codes8<T>(v, code);
+        if ((piece & 3) == 0) P.scales[(r0 + r) * row_blocks + (piece >> 2)] = (uint8_t)code;
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < C * (R / 32); i += 256) {
+    const int c = i % C, b = i / C;
+    if (c0 + c >= P.cols || r0 / 32 + b >= col_blocks) continue;
+    float v[32];
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      v[k] = load1<T>(&tile[32 * b + k][c], 0);
+      m = max_u32(m, magnitude(v[k]));
+    }
+    const uint32_t code = mx_scale_code(m, floor_bits);
+    u4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = e2m1_codes8<T>(v + 8 * k, code);
+    const int64_t block = (c0 + c) * col_blocks + r0 / 32 + b;
+    reinterpret_cast<u4*>(P.t_codes)[block] = w;
+    P.t_scales[block] = (uint8_t)code;
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int dgm_mxfp4_quant_struct_size(size_t* args) {
+  DGM_CHECK_ARG(args, "null pointer");
+  *args = sizeof(DgmMxfp4QuantArgs);
+  return 0;
+}
+
+int dgm_mxfp4_quantize(const DgmMxfp4QuantArgs* args, hipStream_t stream) {
+  DGM_CHECK_ARG(args, "null arguments");
+  const DgmMxfp4QuantArgs A = *args;
+  DGM_CHECK_ARG(A.dtype >= DGM_SRC_BF16 && A.dtype <= DGM_SRC_F32, "dtype 0 bf16, 1 fp16, 2 fp32");
+  DGM_CHECK_ARG(A.rows >= 0 && A.rows < (1 << 24) && A.cols >= 0 && A.cols < (1 << 24), "rows and columns below 2^24");
+  DGM_CHECK_ARG(A.x_stride >= 0, "stride >= 0");
+  DGM_CHECK_ARG(A.amax_floor >= 0.f && A.amax_floor < INFINITY, "amax_floor a number, at least 0");
+  DGM_CHECK_ARG((A.codes != nullptr) == (A.scales != nullptr) && (A.t_codes != nullptr) == (A.t_scales != nullptr),
+                "codes with their scales");
+  if (A.rows == 0 || A.cols == 0) return 0;
+  DGM_CHECK_ARG(A.x && (A.codes || A.t_codes), "null pointer");
+  DGM_CHECK_ARG((((uintptr_t)A.codes | (uintptr_t)A.t_codes) & 15) == 0, "codes on 16 bytes");
+  const bool vec = A.cols % 8 == 0 && aligned(A.x, A.x_stride, element_size(A.dtype));
+  const int64_t pieces = (A.cols + 31) / 32 * 4;
+  // threads a row: the most that leave few without a piece
+  int log_row = 2, runs = 1;
+  double best = 0;
+  for (int l = 2; l <= 8; ++l) {
+    const int64_t n = (pieces + (1 << l) - 1) >> l;
+    const double used = (double)pieces / (double)(n << l);
+    if (used >= best - 0.05) log_row = l, runs = (int)n, best = used > best ? used : best;
+  }
+  const int64_t groups = (A.rows + (256 >> log_row) - 1) >> (8 - log_row);
+  const int tile_rows = A.dtype == DGM_SRC_F32 ? 64 : 128;
+  const int64_t tiles_c = (A.cols + 127) / 128, tiles_r = (A.rows + tile_rows - 1) / tile_rows;
+  DGM_CHECK_ARG((A.t_codes ? tiles_c * tiles_r : groups * runs) < (1 << 24), "a launch has fewer than 2^32 threads");
+  dispatch_type(A.dtype, vec, [&](auto t, auto v) {
+    if (!A.t_codes)
+      hipLaunchKernelGGL((k_mxfp4_rows<t.value, v.value>), dim3((unsigned)(groups * runs)), dim3(256), 0, stream, A, log_row, runs);
+    else if (A.codes)
+      hipLaunchKernelGGL((k_mxfp4_columns<t.value, v.value, true>), dim3((unsigned)(tiles_c * tiles_r)), dim3(256), 0, stream, A, (int)tiles_c);
+    else
+      hipLaunchKernelGGL((k_mxfp4_columns<t.value, v.value, false>), dim3((unsigned)(tiles_c * tiles_r)), dim3(256), 0, stream, A, (int)tiles_c);
+  });
+  return dgm_last_launch_status();
+}
+
+}  // extern "C"

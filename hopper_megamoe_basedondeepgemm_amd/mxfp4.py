@@ -1,0 +1,297 @@
+"""MXFP4 (E2M1 codes with an E8M0 scale for each 32) outside the routed experts, on the GPU: rows and columns of any
+matrix quantised, products of such rows, and a linear layer trained on them.
+
+No counterpart in the reference, whose MXFP4 lives in the experts' weights and the activations between them
+(deep_gemm/utils/math.py:85 ``per_token_cast_to_fp4`` is the rule of the codes and scales here too)."""
+import ctypes
+import functools
+import math
+
+import torch
+
+from . import _lib
+
+MAX_DIM = 1 << 24
+
+
+def _rows(t):
+    return t if t.stride(1) == 1 or t.size(1) == 1 else t.contiguous()
+
+
+def _check_quantize(x, amax_floor):
+    if x.dtype not in _lib.SRC_DTYPES or x.dim() != 2:
+        raise TypeError(f"x must be bf16, fp16 or fp32 [rows, cols], got {x.dtype} {tuple(x.shape)}")
+    if x.size(0) >= MAX_DIM or x.size(1) >= MAX_DIM:
+        raise ValueError(f"x {tuple(x.shape)}: below 2^24 each way")
+    if not 0 <= amax_floor < math.inf:
+        raise ValueError(f"amax_floor {amax_floor}: a number, at least 0")
+
+
+def _new(rows, cols, like):
+    """Uninitialised (codes, scales) of rows of cols elements."""
+    blocks = (cols + 31) // 32
+    return (torch.empty((rows, 16 * blocks), dtype=torch.uint8, device=like.device),
+            torch.empty((rows, blocks), dtype=torch.uint8, device=like.device))
+
+
+def _quantize(x, amax_floor, rows, columns):
+    """((codes, scales) of x's rows, the same of its columns), each if wanted, after the checks."""
+    if x.stride(1) != 1 and x.stride(0) == 1:             # (a transposed view: its rows are the memory's columns)
+        by_column, by_row = _quantize(x.t(), amax_floor, columns, rows)
+        return by_row, by_column
+    x = _rows(x)
+    m, n = x.shape
+    by_row = _new(m, n, x) if rows else None
+    by_column = _new(n, m, x) if columns else None
+    args = _lib.Mxfp4QuantArgs(x=x.data_ptr(), rows=m, cols=n, x_stride=x.stride(0), dtype=_lib.SRC_DTYPES[x.dtype],
+                               amax_floor=amax_floor)
+    if rows:
+        args.codes, args.scales = by_row[0].data_ptr(), by_row[1].data_ptr()
+    if columns:
+        args.t_codes, args.t_scales = by_column[0].data_ptr(), by_column[1].data_ptr()
+    if m and n:
+        _lib.check(_lib.load().dgm_mxfp4_quantize(ctypes.byref(args), _lib.stream()))
+    return by_row, by_column
+
+
+def _refuse_gradient(*tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError("codes and scales have no gradient: call under torch.no_grad(), or mxfp4_linear")
+    _lib.no_tangents(*tensors)
+
+
+def mxfp4_quantize(x, transpose=False, amax_floor=1e-30):
+    """``(codes, scales)`` of x's rows, or with ``transpose`` of its columns, as ``mxfp4_gemm_nt`` takes them:
+
+        block of 32 along a row: e = least integer with max(|block|, amax_floor) <= 6 2^e (at least -126),
+        codes = nearest E2M1 of block / 2^e (midpoints to the smaller magnitude), scale byte e + 127
+
+    x: bf16, fp16 or fp32 [rows, cols], any strides, each size below 2^24. codes uint8 [rows, 16 ceil(cols / 32)], two a
+    byte, the first in the low half; scales uint8 [rows, ceil(cols / 32)]; behind the last column a block holds zeros.
+    (The codes and scale bytes of ``per_token_cast_to_fp4(x, amax_floor=...)``, which takes bf16 rows of whole blocks.)
+    A block with an infinity or NaN has scale 255 (NaN) and zeros, so that a product with it is NaN.
+    No gradient. Work runs on the current stream of x's device, which has to be the current one."""
+    _check_quantize(x, amax_floor)
+    _refuse_gradient(x)
+    _lib.require_one_device(x)
+    return _quantize(x, amax_floor, not transpose, transpose)[1 if transpose else 0]
+
+
+def mxfp4_quantize_both(x, amax_floor=1e-30):
+    """``(mxfp4_quantize(x), mxfp4_quantize(x, transpose=True))`` from one pass over x: what a product along x's columns
+    and one along its rows take (a weight in the forward pass and for its input's gradient)."""
+    _check_quantize(x, amax_floor)
+    _refuse_gradient(x)
+    _lib.require_one_device(x)
+    return _quantize(x, amax_floor, True, True)
+
+
+def _operand(name, pair):
+    """(codes, scale bytes) of a product's operand."""
+    q, sf = pair
+    if q.dtype != torch.uint8 or q.dim() != 2:
+        raise TypeError(f"{name}: uint8 codes [rows, k / 2] expected, got {q.dtype} {tuple(q.shape)}")
+    if sf.dtype == torch.int32 and sf.dim() == 2:         # (per_token_cast_to_fp4(use_packed_ue8m0=True))
+        sf = sf.contiguous().view(torch.uint8)
+    if sf.dtype != torch.uint8 or sf.dim() != 2 or sf.size(0) != q.size(0) or q.size(1) != 16 * sf.size(1):
+        raise TypeError(f"{name}: uint8 scales [{q.size(0)}, {q.size(1) / 16:g}] (a byte for 16 bytes of codes) expected, got "
+                        f"{sf.dtype} {tuple(sf.shape)}")
+    return q, sf
+
+
+def _readable(q, sf):
+    """An operand as the kernels read it: code rows on 16 bytes, scale rows of contiguous bytes."""
+    if q.stride(1) != 1 or q.stride(0) % 16 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    return q, _rows(sf)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(m, n, k, swiglu):
+    return _lib.load().dgm_mxfp4_gemm_workspace_bytes(m, n, k, int(swiglu))
+
+
+def mxfp4_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_math=True):
+    """d = a @ b.T over MXFP4 rows, into d (bf16, fp16 or fp32 [m, n], any row stride):
+
+        d[m, n] = sum over blocks 2^(sa + sb - 254) sum of code products (+ c[m, n], or c[n] for a 1-D c)
+
+    a = (codes [m, k / 2], scales [m, k / 32]) and b of n rows, as ``mxfp4_quantize`` returns them for tokens and
+    weights (or ``per_token_cast_to_fp4`` with ``use_packed_ue8m0``; the two halves of a byte have to be in one order in
+    both). c has d's type and may be d itself. ``activation="swiglu"``: b holds gate rows, then up rows, and
+    d [m, n / 2] = silu(min(gate, clamp)) * clamp(up, -clamp, clamp), the layer's SwiGLU (``activation_clamp`` None: no
+    clamp; ``fast_math`` as in ``int8_gemm_nt``). Sums in fp32, one rounding; a scale of 255 makes its row NaN. k a
+    multiple of 32. m, n and k below 2^24, ceil(m / 64) ceil(n / 64) below 2^23. No gradient (``mxfp4_linear`` has
+    one). Work runs on the current stream of the tensors' device, which has to be the current one. Returns d."""
+    aq, asf = _operand("a", a)
+    bq, bsf = _operand("b", b)
+    m, k = aq.size(0), 2 * aq.size(1)
+    n = bq.size(0)
+    if 2 * bq.size(1) != k or not 32 <= k < MAX_DIM:
+        raise ValueError(f"k of a {k} and of b {2 * bq.size(1)}: equal, 32 to 2^24")
+    if activation not in (None, "swiglu"):
+        raise ValueError(f"activation {activation!r}: None or 'swiglu'")
+    swiglu = activation is not None
+    if swiglu and (n % 2 or c is not None):
+        raise ValueError("swiglu takes a gate and an up half of b's rows, and no c")
+    if activation_clamp is not None and not activation_clamp >= 0:
+        raise ValueError(f"activation_clamp {activation_clamp}: at least 0, or None")
+    if m >= MAX_DIM or n >= MAX_DIM or ((m + 63) // 64) * ((n + 63) // 64) >= 1 << 23:
+        raise ValueError(f"m {m} and n {n}: below 2^24, and ceil(m / 64) ceil(n / 64) below 2^23")
+    n_out = n // 2 if swiglu else n
+    if d.dtype not in _lib.SRC_DTYPES or d.dim() != 2 or d.size(0) != m or d.size(1) != n_out:
+        raise TypeError(f"d: bf16, fp16 or fp32 [{m}, {n_out}] expected, got {d.dtype} {tuple(d.shape)}")
+    d_stride = d.stride(0)
+    if m and n_out and ((n_out > 1 and d.stride(1) != 1) or (m > 1 and d_stride < n_out)):
+        raise ValueError("d: rows must be contiguous and must not overlap")
+    if c is not None and (c.dtype != d.dtype or tuple(c.shape) not in ((m, n_out), (n_out,))):
+        raise TypeError(f"c: {d.dtype} [{m}, {n_out}] or [{n_out}] expected, got {c.dtype} {tuple(c.shape)}")
+    if (d.requires_grad or (c is not None and c.requires_grad)) and torch.is_grad_enabled():
+        raise RuntimeError("mxfp4_gemm_nt has no gradient: call it under torch.no_grad(), or mxfp4_linear")
+    _lib.no_tangents(d, c)
+    _lib.require_one_device(d, aq, asf, bq, bsf, c)
+    if m == 0 or n_out == 0:
+        return d
+    aq, asf = _readable(aq, asf)
+    bq, bsf = _readable(bq, bsf)
+    size = d.element_size()
+    pa, pb, lo, a_stride, b_stride = aq.data_ptr(), bq.data_ptr(), d.data_ptr(), aq.stride(0), bq.stride(0)
+    psa, psb, sa_stride, sb_stride = asf.data_ptr(), bsf.data_ptr(), asf.stride(0), bsf.stride(0)
+    hi = lo + ((m - 1) * d_stride + n_out) * size
+    if ((pa < hi and lo < pa + (m - 1) * a_stride + k // 2) or (pb < hi and lo < pb + (n - 1) * b_stride + k // 2)
+            or (psa < hi and lo < psa + (m - 1) * sa_stride + k // 32) or (psb < hi and lo < psb + (n - 1) * sb_stride + k // 32)):
+        raise ValueError("d overlaps an operand")
+    args = _lib.Mxfp4GemmArgs(pa, psa, pb, psb, 0, lo, m, n, k, a_stride, sa_stride, b_stride, sb_stride, 0, d_stride,
+                              _lib.SRC_DTYPES[d.dtype], swiglu, math.inf if activation_clamp is None else float(activation_clamp),
+                              1 if fast_math else 0)
+    if c is not None:
+        if c.dim() == 1:
+            c, c_stride, end = c.contiguous(), 0, n_out
+        else:
+            c = _rows(c)
+            c_stride = c.stride(0)
+            end = (m - 1) * c_stride + n_out
+        pc = c.data_ptr()
+        if pc < hi and lo < pc + end * size and not (pc == lo and c.dim() == 2 and (m == 1 or c_stride == d_stride)):
+            raise ValueError("c overlaps d other than as the same rows")
+        args.c, args.c_stride = pc, c_stride
+    need = _workspace_bytes(m, n, k, swiglu)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=d.device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need
+    _lib.check(_lib.load().dgm_mxfp4_gemm_nt(ctypes.byref(args), _lib.stream()))
+    _lib.written(d)
+    return d
+
+
+def _check_linear(x, weight):
+    _check_quantize(x, 0.0)
+    if weight.dtype not in _lib.SRC_DTYPES or weight.dim() != 2 or weight.size(1) != x.size(1):
+        raise TypeError(f"weight must be bf16, fp16 or fp32 [out, {x.size(1)}], got {weight.dtype} {tuple(weight.shape)}")
+    if x.size(1) == 0 or weight.size(0) == 0:
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)}: no feature")
+    if weight.size(0) >= MAX_DIM:
+        raise ValueError(f"weight {tuple(weight.shape)}: below 2^24 each way")
+
+
+def _product(a, b, dtype):
+    d = torch.empty((a[0].size(0), b[0].size(0)), dtype=dtype, device=a[0].device)
+    if a[0].size(1) == 0:
+        return d.zero_()                   # (a sum over no tokens)
+    return mxfp4_gemm_nt(a, b, d)
+
+
+def _linear_forward(x, weight, keep_x, keep_weight):
+    """y, what the weight's gradient needs (x's columns) and what x's needs (the weight's columns), if wanted."""
+    xq, xt = _quantize(x, 1e-30, True, keep_x)
+    wq, wt = _quantize(weight, 1e-30, True, keep_weight)
+    return _product(xq, wq, x.dtype), xt, wt
+
+
+def _linear_backward(d_y, xt, wt, x_dtype, w_dtype):
+    """(d_x, d_weight), each where its operand is given."""
+    by_row, by_column = _quantize(d_y, 1e-30, wt is not None, xt is not None)
+    return (_product(by_row, wt, x_dtype) if wt is not None else None,
+            _product(by_column, xt, w_dtype) if xt is not None else None)
+
+
+class _Mxfp4Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight):
+        y, xt, wt = _linear_forward(x, weight, ctx.needs_input_grad[1], ctx.needs_input_grad[0])
+        ctx.save_for_backward(*(xt or (None, None)), *(wt or (None, None)))
+        ctx.shapes = x.shape, weight.shape, x.dtype, weight.dtype
+        return y
+
+    @staticmethod
+    def backward(ctx, d_y):
+        _lib.no_second_derivative()
+        saved = ctx.saved_tensors
+        _lib.no_tangents(d_y, *saved)
+        return _backward_of(d_y, saved[:2], saved[2:], *ctx.shapes, ctx.needs_input_grad)
+
+
+def _backward_of(d_y, xt, wt, x_shape, w_shape, x_dtype, w_dtype, needs):
+    """The backward pass after its checks (what comes back from saved-tensor hooks is checked as an argument is)."""
+    (m, k), n = x_shape, w_shape[0]
+    if d_y.dtype != x_dtype or tuple(d_y.shape) != (m, n):
+        raise TypeError(f"d_y of {x_dtype} [{m}, {n}] expected, got {d_y.dtype} {tuple(d_y.shape)}")
+    kept = []
+    for name, pair, wanted, inner in (("columns of x", xt, needs[1], m), ("columns of the weight", wt, needs[0], n)):
+        if not wanted:
+            kept.append(None)
+            continue
+        blocks = (inner + 31) // 32
+        if pair is None or any(t is None or t.dtype != torch.uint8 for t in pair) or \
+                tuple(pair[0].shape) != (k, 16 * blocks) or tuple(pair[1].shape) != (k, blocks):
+            raise ValueError(f"saved {name}: uint8 codes [{k}, {16 * blocks}] and scales [{k}, {blocks}] expected, as "
+                             "mxfp4_linear_forward returns them")
+        kept.append(pair)
+    _lib.require_one_device(d_y, *(t for pair in kept if pair is not None for t in pair))
+    return _linear_backward(d_y, *kept, x_dtype, w_dtype)
+
+
+def mxfp4_linear(x, weight):
+    """y = x @ weight.T with all three products of a training step in MXFP4:
+
+        y = q(x) q(weight)^T,  d_x = q(d_y) q(weight^T)^T,  d_weight = q(d_y^T) q(x^T)^T
+
+    q as ``mxfp4_quantize`` along the dimension that its product sums over; the gradients pass straight through the
+    roundings. x: bf16, fp16 or fp32 [tokens, in], weight: any of them [out, in] (fp32 master weights); y and d_x have
+    x's type, d_weight the weight's; any strides, each size below 2^24, products within ``mxfp4_gemm_nt``'s limits.
+    The backward pass keeps the codes of x's and the weight's columns (17 / 32 byte a value), not the inputs. Under graph capture use ``mxfp4_linear_forward`` and
+    ``mxfp4_linear_backward``. Work runs on the current stream of the tensors' device, which has to be the current one."""
+    _check_linear(x, weight)
+    _lib.no_tangents(x, weight)
+    _lib.require_one_device(x, weight)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        _lib.no_graph_under_capture()
+        return _Mxfp4Linear.apply(x, weight)
+    return _linear_forward(x, weight, False, False)[0]
+
+
+def mxfp4_linear_forward(x, weight, needs=(True, True)):
+    """``mxfp4_linear`` with what its explicit backward call needs: ``(y, x_columns, weight_columns)`` (each
+    ``mxfp4_quantize(..., transpose=True)`` of its input; None where ``needs`` of (d_x, d_weight) does not want it).
+    Records no autograd graph."""
+    _check_linear(x, weight)
+    _lib.no_tangents(x, weight)
+    _lib.require_one_device(x, weight)
+    return _linear_forward(x, weight, bool(needs[1]), bool(needs[0]))
+
+
+def mxfp4_linear_backward(d_y, x_columns, weight_columns, x_shape, weight_shape, weight_dtype=None, needs=(True, True)):
+    """Gradients of ``mxfp4_linear``: ``(d_x, d_weight)`` from d_y = dL/dy and what ``mxfp4_linear_forward`` returned for
+    x of x_shape and the weight of weight_shape; d_x has d_y's type, d_weight ``weight_dtype`` (None: d_y's). None for
+    what ``needs`` leaves out."""
+    weight_dtype = weight_dtype or d_y.dtype
+    if d_y.dtype not in _lib.SRC_DTYPES or weight_dtype not in _lib.SRC_DTYPES:
+        raise TypeError(f"d_y and the weight are bf16, fp16 or fp32, got {d_y.dtype} and {weight_dtype}")
+    if len(x_shape) != 2 or len(weight_shape) != 2 or x_shape[1] != weight_shape[1]:
+        raise ValueError(f"x {tuple(x_shape)} and weight {tuple(weight_shape)}: [tokens, in] and [out, in]")
+    _lib.no_tangents(d_y)
+    return _backward_of(d_y, x_columns, weight_columns, tuple(x_shape), tuple(weight_shape), d_y.dtype, weight_dtype, needs)
+
+
+__all__ = ["mxfp4_quantize", "mxfp4_quantize_both", "mxfp4_gemm_nt", "mxfp4_linear", "mxfp4_linear_forward",
+           "mxfp4_linear_backward"]

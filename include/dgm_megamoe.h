@@ -464,6 +464,101 @@ int64_t dgm_int8_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int swigl
 int dgm_int8_gemm_nt(const DgmInt8GemmArgs* args, hipStream_t stream);
 int dgm_int8_gemm_struct_size(size_t* args);
 
+/* dgm_layer_norm_residual: the scaled residual add and the layer norm behind it, one pass:
+ *   t = residual + residual_scale x (t = residual_scale x without residual),
+ *   h = (t - mean t) rsqrt(mean (t - mean t)^2 + eps) weight + bias.
+ * All arithmetic in fp32, t unrounded into the norm. Rows, types, strides and limits as in DgmNormArgs; weight and bias
+ * [hidden] of the rows' type or fp32, NULL: 1 and 0. residual_out may be residual, or x, at the same stride; h may be
+ * x or residual. codes / scales: MXFP4 rows of the rounded h as dgm_mxfp4_quantize writes them (amax_floor 1e-30), of
+ * bf16 rows with hidden a multiple of 8 and everything 16-byte aligned. mean / rstd [rows] fp32 are what the backward
+ * pass needs of the forward one. No counterpart in the reference. */
+typedef struct DgmLayerNormArgs {
+  const void* x;
+  const void* residual;
+  const void* weight;
+  const void* bias;
+  void* residual_out;
+  void* h;
+  uint8_t* codes;
+  uint8_t* scales;
+  float* mean;
+  float* rstd;
+  int64_t rows;
+  int64_t x_stride, residual_stride, residual_out_stride, h_stride;
+  int32_t hidden;
+  int32_t dtype;
+  int32_t weights_f32;
+  float residual_scale;
+  float eps;
+} DgmLayerNormArgs;
+int dgm_layer_norm_residual(const DgmLayerNormArgs* args, hipStream_t stream);
+
+/* Its gradients, from d_residual_out = dL/dt and d_h = dL/dh (each may be NULL: zero), as
+ * dgm_rms_norm_residual_backward's. workspace: 2 x dgm_layer_norm_residual_groups(rows, hidden) x hidden floats for
+ * d_weight and d_bias. */
+typedef struct DgmLayerNormGradArgs {
+  DgmLayerNormArgs forward;
+  const void* d_residual_out;
+  const void* d_h;
+  void* d_x;
+  void* d_residual;
+  void* d_weight;
+  void* d_bias;
+  float* workspace;
+  int64_t workspace_bytes;
+  int64_t d_residual_out_stride, d_h_stride, d_x_stride, d_residual_stride;
+} DgmLayerNormGradArgs;
+int dgm_layer_norm_residual_groups(int64_t rows, int hidden);
+int dgm_layer_norm_residual_backward(const DgmLayerNormGradArgs* args, hipStream_t stream);
+int dgm_layer_norm_struct_sizes(size_t* norm_args, size_t* norm_grad_args);
+
+/* Rows of x [rows, cols] (type DGM_SRC_*, contiguous elements at a row stride) as MXFP4, and / or its columns: blocks
+ * of 32 along a row (column), zeros behind the last element, each with an E8M0 scale byte e + 127, e the least integer
+ * with max(amax, amax_floor) <= 6 2^e (at least -126), and E2M1 codes of x / 2^e, two a byte, the first in the low
+ * half: the nearest, midpoints to the smaller magnitude, no negative zero. A block with an infinity or NaN: scale 255
+ * (E8M0's NaN), zeros. codes [rows, 16 ceil(cols / 32)] and scales [rows, ceil(cols / 32)], contiguous, NULL: not
+ * wanted; t_codes [cols, 16 ceil(rows / 32)] and t_scales [cols, ceil(rows / 32)] of the columns. Codes on 16 bytes.
+ * rows and cols below 2^24. Finite rows: dgm_cast_fp4_rows's result. */
+typedef struct DgmMxfp4QuantArgs {
+  const void* x;
+  uint8_t* codes;
+  uint8_t* scales;
+  uint8_t* t_codes;
+  uint8_t* t_scales;
+  int64_t rows, cols, x_stride;
+  int32_t dtype;
+  float amax_floor;
+} DgmMxfp4QuantArgs;
+int dgm_mxfp4_quantize(const DgmMxfp4QuantArgs* args, hipStream_t stream);
+int dgm_mxfp4_quant_struct_size(size_t* args);
+
+/* MXFP4 x MXFP4 product of rows (a token each) with weight rows (a channel each), as dgm_mxfp4_quantize writes them:
+ *   d[m][n] = sum_k a[m][k] b[n][k] (+ c[m][n]; c_stride 0: one row c[n] for every token), with each block's scales,
+ * or with `swiglu` over b's gate rows [0, n/2) and up rows [n/2, n) as dgm_int8_gemm_nt's. k (a multiple of 32) counts
+ * elements, a_stride and b_stride bytes (multiples of 16), sfa_stride and sfb_stride bytes of E8M0 scales (any). Sums
+ * in fp32, one rounding to dtype (DGM_SRC_*), which c shares; c may be d at the same stride. m, n and k below 2^24,
+ * ceil(m / 64) ceil(n / 64) below 2^23. No counterpart in the reference. */
+typedef struct DgmMxfp4GemmArgs {
+  const uint8_t* a;
+  const uint8_t* sfa;
+  const uint8_t* b;
+  const uint8_t* sfb;
+  const void* c;
+  void* d;
+  int64_t m, n, k;
+  int64_t a_stride, sfa_stride, b_stride, sfb_stride, c_stride, d_stride;
+  int32_t dtype;
+  int32_t swiglu;
+  float clamp;       /* INFINITY: none; NaN stays NaN */
+  int32_t fast_math; /* SwiGLU's sigmoid: 1 hardware exp2 and reciprocal, 0 IEEE */
+  float* workspace;  /* of this call until it has run; without it (NULL) K is not split */
+  int64_t workspace_bytes;
+} DgmMxfp4GemmArgs;
+/* bytes of workspace a call of this size uses (0: none), 16-byte aligned */
+int64_t dgm_mxfp4_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int swiglu);
+int dgm_mxfp4_gemm_nt(const DgmMxfp4GemmArgs* args, hipStream_t stream);
+int dgm_mxfp4_gemm_struct_size(size_t* args);
+
 /* The router's balance loss over logits [tokens, experts] (rows at logits_stride, type DGM_SRC_*) and the
  * chosen experts topk_idx [tokens, topk] (rows at idx_stride; int64 or int32; ids outside [0, experts) are
  * no slot, a token without a slot is unrouted and adds nothing). Sequences: tokens [cu_seqlens[b],
