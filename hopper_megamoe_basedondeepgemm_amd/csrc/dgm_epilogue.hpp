@@ -41,8 +41,8 @@ DGM_DEV void wave_sync() {
 }
 
 // A 16-byte piece of token m's row from channel n on (eight channels, fp32: four), from LDS: C added, rounded,
-// stored. vec: rows of D (and C) are 16-byte aligned.
-template <int T, bool ADD, class Args>
+// stored. vec: rows of D (and C) are 16-byte aligned; STREAM: 2 = and stored past the caches.
+template <int T, bool ADD, bool STREAM = false, class Args>
 DGM_DEV void put_piece(const Args& P, int64_t m, int64_t n, int64_t n_out, int vec, const float* from) {
   constexpr int E = T == DGM_SRC_F32 ? 4 : 8;
   if (n >= n_out) return;
@@ -61,7 +61,10 @@ DGM_DEV void put_piece(const Args& P, int64_t m, int64_t n, int64_t n_out, int v
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] += c[i];
       }
-      *reinterpret_cast<v4f*>(reinterpret_cast<float*>(P.d) + at) = v4f{v[0], v[1], v[2], v[3]};
+      v4f* to = reinterpret_cast<v4f*>(reinterpret_cast<float*>(P.d) + at);
+      const v4f o = {v[0], v[1], v[2], v[3]};
+      if (STREAM && vec == 2) __builtin_nontemporal_store(o, to);
+      else *to = o;
     } else {
       if constexpr (ADD) {
         const v4i c = *reinterpret_cast<const v4i*>(reinterpret_cast<const uint16_t*>(P.c) + ct);
@@ -78,7 +81,9 @@ DGM_DEV void put_piece(const Args& P, int64_t m, int64_t n, int64_t n_out, int v
         const uint32_t hi = T == DGM_SRC_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[2 * i + 1]) : __builtin_bit_cast(uint16_t, (__bf16)v[2 * i + 1]);
         o[i] = (int)(lo | hi << 16);
       }
-      *reinterpret_cast<v4i*>(reinterpret_cast<uint16_t*>(P.d) + at) = o;
+      v4i* to = reinterpret_cast<v4i*>(reinterpret_cast<uint16_t*>(P.d) + at);
+      if (STREAM && vec == 2) __builtin_nontemporal_store(o, to);
+      else *to = o;
     }
   } else {
 #pragma unroll

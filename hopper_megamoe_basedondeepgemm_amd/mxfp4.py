@@ -100,8 +100,8 @@ def _operand(name, pair):
 
 
 def _readable(q, sf):
-    """An operand as the kernels read it: code rows on 16 bytes, scale rows of contiguous bytes."""
-    if q.stride(1) != 1 or q.stride(0) % 16 or q.data_ptr() % 16:
+    """An operand as the kernels read it: code rows on 16 bytes and less than 2^23 apart, scale rows of contiguous bytes."""
+    if q.stride(1) != 1 or q.stride(0) % 16 or q.stride(0) >= 1 << 23 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
     return q, _rows(sf)
 

@@ -535,7 +535,7 @@ int dgm_mxfp4_quant_struct_size(size_t* args);
 /* MXFP4 x MXFP4 product of rows (a token each) with weight rows (a channel each), as dgm_mxfp4_quantize writes them:
  *   d[m][n] = sum_k a[m][k] b[n][k] (+ c[m][n]; c_stride 0: one row c[n] for every token), with each block's scales,
  * or with `swiglu` over b's gate rows [0, n/2) and up rows [n/2, n) as dgm_int8_gemm_nt's. k (a multiple of 32) counts
- * elements, a_stride and b_stride bytes (multiples of 16), sfa_stride and sfb_stride bytes of E8M0 scales (any). Sums
+ * elements, a_stride and b_stride bytes (multiples of 16 below 2^23), sfa_stride and sfb_stride bytes of E8M0 scales (any). Sums
  * in fp32, one rounding to dtype (DGM_SRC_*), which c shares; c may be d at the same stride. m, n and k below 2^24,
  * ceil(m / 64) ceil(n / 64) below 2^23. No counterpart in the reference. */
 typedef struct DgmMxfp4GemmArgs {
