@@ -38,7 +38,8 @@ EXPORTS = [
     "dgm_router_balance_workspace_bytes", "dgm_balance_struct_size",
     "dgm_layer_norm_residual", "dgm_layer_norm_residual_groups", "dgm_layer_norm_residual_backward",
     "dgm_layer_norm_struct_sizes", "dgm_mxfp4_quantize", "dgm_mxfp4_quant_struct_size", "dgm_mxfp4_gemm_nt",
-    "dgm_mxfp4_gemm_struct_size", "dgm_mxfp4_gemm_workspace_bytes",
+    "dgm_mxfp4_gemm_struct_size", "dgm_mxfp4_gemm_workspace_bytes", "dgm_mxfp4_linear", "dgm_mxfp4_linear_backward",
+    "dgm_mxfp4_linear_workspace_bytes", "dgm_mxfp4_linear_struct_size",
 ]
 # source element types of the weight packers (DGM_SRC_*)
 SRC_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -132,6 +133,13 @@ class Mxfp4GemmArgs(ctypes.Structure):
                  ("fast_math", ctypes.c_int32), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)])
 
 
+class Mxfp4LinearArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "w", "y", "d_y", "d_x", "d_w", "x_columns", "x_column_scales",
+                                                "w_columns", "w_column_scales", "workspace")] +
+                [(n, ctypes.c_int64) for n in ("workspace_bytes", "m", "n", "k", "x_stride", "w_stride", "d_y_stride")] +
+                [("x_dtype", ctypes.c_int32), ("w_dtype", ctypes.c_int32)])
+
+
 class Int8GemmArgs(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("a", "sfa", "b", "sfb", "c", "d")] +
                 [(n, ctypes.c_int64) for n in ("m", "n", "k", "a_stride", "sfa_stride", "b_stride", "sfb_stride",
@@ -220,6 +228,10 @@ def load():
     sig["dgm_mxfp4_gemm_nt"] = ([ctypes.POINTER(Mxfp4GemmArgs), vp], i32)
     sig["dgm_mxfp4_gemm_workspace_bytes"] = ([i64, i64, i64, i32], i64)
     sig["dgm_mxfp4_gemm_struct_size"] = ([ctypes.POINTER(ctypes.c_size_t)], i32)
+    sig["dgm_mxfp4_linear"] = ([ctypes.POINTER(Mxfp4LinearArgs), vp], i32)
+    sig["dgm_mxfp4_linear_backward"] = ([ctypes.POINTER(Mxfp4LinearArgs), vp], i32)
+    sig["dgm_mxfp4_linear_workspace_bytes"] = ([i64, i64, i64, i32], i64)
+    sig["dgm_mxfp4_linear_struct_size"] = ([ctypes.POINTER(ctypes.c_size_t)], i32)
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
         fn.argtypes = args

@@ -14,7 +14,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdgm_megamoe.so")
 PROBE_LIB = os.path.join(HERE, "libdgm_probe.so")
 SOURCES = ["dgm_megamoe.hip", "dgm_fused.hip", "dgm_packers.hip", "dgm_noalloc.hip", "dgm_norm.hip",
-           "dgm_int8_gemm.hip", "dgm_balance.hip", "dgm_layer_norm.hip", "dgm_mxfp4_quant.hip", "dgm_mxfp4_gemm.hip"]
+           "dgm_int8_gemm.hip", "dgm_balance.hip", "dgm_layer_norm.hip", "dgm_mxfp4_quant.hip", "dgm_mxfp4_gemm.hip",
+           "dgm_mxfp4_linear.hip"]
 PROBE_SOURCES = ["dgm_probe.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

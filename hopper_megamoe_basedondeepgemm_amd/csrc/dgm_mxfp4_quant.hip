@@ -44,12 +44,15 @@ __global__ void __launch_bounds__(256) k_mxfp4_rows(const DgmMxfp4QuantArgs P, i
 }
 
 // Columns, and rows with them (BOTH): a tile of R rows x 128 columns is read once, its rows' codes are made on the
-// way into LDS, and a thread then takes 32 rows of a column.
+// way into LDS, and a thread then takes 32 rows of a column (16 bits: of two, a dword a row). The columns' codes meet in
+// LDS again, so that what is stored for a column lies together (64 bytes; fp32 32).
 template <int T, bool VEC, bool BOTH>
 __global__ void __launch_bounds__(256) k_mxfp4_columns(const DgmMxfp4QuantArgs P, int tiles_c) {
-  constexpr int R = T == T_F32 ? 64 : 128, C = 128;
+  constexpr int R = T == T_F32 ? 64 : 128, C = 128, B = R / 32, PAIR = T == T_F32 ? 1 : 2;
   using E = std::conditional_t<T == T_F32, uint32_t, uint16_t>;
   __shared__ __attribute__((aligned(16))) E tile[R][C];
+  __shared__ u4 codes[B][C + 1];
+  __shared__ uint8_t scales[C][B];
   const int64_t r0 = (int64_t)(blockIdx.x / (unsigned)tiles_c) * R, c0 = (int64_t)(blockIdx.x % (unsigned)tiles_c) * C;
   const int64_t row_blocks = (P.cols + 31) / 32, col_blocks = (P.rows + 31) / 32;
   const uint32_t floor_bits = __float_as_uint(P.amax_floor);
@@ -73,23 +76,39 @@ __global__ void __launch_bounds__(256) k_mxfp4_columns(const DgmMxfp4QuantArgs P
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < C * (R / 32); i += 256) {
-    const int c = i % C, b = i / C;
-    if (c0 + c >= P.cols || r0 / 32 + b >= col_blocks) continue;
-    float v[32];
-    uint32_t m = 0;
+  {
+    const int c = threadIdx.x % (C / PAIR) * PAIR, b = threadIdx.x / (C / PAIR);
+    static_assert(C / PAIR * B == 256, "a thread for each");
+    uint32_t w[32];
 #pragma unroll
-    for (int k = 0; k < 32; ++k) {
-      v[k] = load1<T>(&tile[32 * b + k][c], 0);
-      m = max_u32(m, magnitude(v[k]));
+    for (int k = 0; k < 32; ++k) w[k] = *reinterpret_cast<const uint32_t*>(&tile[32 * b + k][c]);
+#pragma unroll
+    for (int h = 0; h < PAIR; ++h) {
+      float v[32];
+      uint32_t m = 0;
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        if constexpr (T == T_F32) v[k] = __uint_as_float(w[k]);
+        else if constexpr (T == T_F16) v[k] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[k] >> (16 * h)));
+        else v[k] = __uint_as_float(h ? w[k] & 0xffff0000u : w[k] << 16);
+        m = max_u32(m, magnitude(v[k]));
+      }
+      const uint32_t code = mx_scale_code(m, floor_bits);
+      u4 q;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) q[k] = e2m1_codes8<T>(v + 8 * k, code);
+      codes[b][c + h] = q;
+      scales[c + h][b] = (uint8_t)code;
     }
-    const uint32_t code = mx_scale_code(m, floor_bits);
-    u4 w;
+  }
+  __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = e2m1_codes8<T>(v + 8 * k, code);
+  for (int i = threadIdx.x; i < C * B; i += 256) {
+    const int c = i / B, b = i % B;
+    if (c0 + c >= P.cols || r0 / 32 + b >= col_blocks) continue;
     const int64_t block = (c0 + c) * col_blocks + r0 / 32 + b;
-    reinterpret_cast<u4*>(P.t_codes)[block] = w;
-    P.t_scales[block] = (uint8_t)code;
+    reinterpret_cast<u4*>(P.t_codes)[block] = codes[b][c];
+    P.t_scales[block] = scales[c][b];
   }
 }
 

@@ -184,43 +184,98 @@ def mxfp4_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_
     return d
 
 
+def _fits(m, n):
+    return ((m + 63) // 64) * ((n + 63) // 64) < 1 << 23
+
+
 def _check_linear(x, weight):
     _check_quantize(x, 0.0)
     if weight.dtype not in _lib.SRC_DTYPES or weight.dim() != 2 or weight.size(1) != x.size(1):
         raise TypeError(f"weight must be bf16, fp16 or fp32 [out, {x.size(1)}], got {weight.dtype} {tuple(weight.shape)}")
-    if x.size(1) == 0 or weight.size(0) == 0:
+    (m, k), n = x.shape, weight.size(0)
+    if k == 0 or n == 0:
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)}: no feature")
-    if weight.size(0) >= MAX_DIM:
-        raise ValueError(f"weight {tuple(weight.shape)}: below 2^24 each way")
+    if n >= MAX_DIM or not (_fits(m, n) and _fits(m, k) and _fits(n, k)):
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)}: sizes below 2^24, and ceil(a / 64) ceil(b / 64) below "
+                         "2^23 for each two of tokens, in and out")
 
 
-def _product(a, b, dtype):
-    d = torch.empty((a[0].size(0), b[0].size(0)), dtype=dtype, device=a[0].device)
-    if a[0].size(1) == 0:
-        return d.zero_()                   # (a sum over no tokens)
-    return mxfp4_gemm_nt(a, b, d)
+@functools.lru_cache(maxsize=1024)
+def _linear_workspace_bytes(m, n, k, backward):
+    return _lib.load().dgm_mxfp4_linear_workspace_bytes(m, n, k, backward)
+
+
+def _code_bytes(rows, cols):
+    return rows * 16 * ((cols + 31) // 32)
+
+
+def _columns_memory(rows, cols, like):
+    """One piece of memory for the codes and scales of rows of cols elements."""
+    return torch.empty(_code_bytes(rows, cols) // 16 * 17, dtype=torch.uint8, device=like.device)
+
+
+def _as_pair(memory, rows, cols):
+    codes, blocks = _code_bytes(rows, cols), (cols + 31) // 32
+    return memory[:codes].view(rows, 16 * blocks), memory[codes:].view(rows, blocks)
 
 
 def _linear_forward(x, weight, keep_x, keep_weight):
     """y, what the weight's gradient needs (x's columns) and what x's needs (the weight's columns), if wanted."""
-    xq, xt = _quantize(x, 1e-30, True, keep_x)
-    wq, wt = _quantize(weight, 1e-30, True, keep_weight)
-    return _product(xq, wq, x.dtype), xt, wt
+    x, weight = _rows(x), _rows(weight)
+    (m, k), n = x.shape, weight.size(0)
+    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    args = _lib.Mxfp4LinearArgs(x=x.data_ptr(), w=weight.data_ptr(), y=y.data_ptr(), m=m, n=n, k=k, x_stride=x.stride(0),
+                                w_stride=weight.stride(0), x_dtype=_lib.SRC_DTYPES[x.dtype], w_dtype=_lib.SRC_DTYPES[weight.dtype])
+    xt = wt = None
+    if keep_x:
+        xt = _columns_memory(k, m, x)
+        if m:
+            at = xt.data_ptr()
+            args.x_columns, args.x_column_scales = at, at + _code_bytes(k, m)
+    if keep_weight:
+        wt = _columns_memory(k, n, x)
+        at = wt.data_ptr()
+        args.w_columns, args.w_column_scales = at, at + _code_bytes(k, n)
+    if m:
+        need = _linear_workspace_bytes(m, n, k, 0)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need
+    _lib.check(_lib.load().dgm_mxfp4_linear(ctypes.byref(args), _lib.stream()))
+    return y, xt, wt
 
 
-def _linear_backward(d_y, xt, wt, x_dtype, w_dtype):
-    """(d_x, d_weight), each where its operand is given."""
-    by_row, by_column = _quantize(d_y, 1e-30, wt is not None, xt is not None)
-    return (_product(by_row, wt, x_dtype) if wt is not None else None,
-            _product(by_column, xt, w_dtype) if xt is not None else None)
+def _linear_backward(d_y, xt, wt, k, x_dtype, w_dtype):
+    """(d_x, d_weight), each where its operand (addresses of codes and scales) is given."""
+    d_y = _rows(d_y)
+    m, n = d_y.shape
+    args = _lib.Mxfp4LinearArgs(d_y=d_y.data_ptr(), m=m, n=n, k=k, d_y_stride=d_y.stride(0), x_dtype=_lib.SRC_DTYPES[x_dtype],
+                                w_dtype=_lib.SRC_DTYPES[w_dtype])
+    d_x = d_w = None
+    if wt is not None:
+        d_x = torch.empty((m, k), dtype=x_dtype, device=d_y.device)
+        args.d_x = d_x.data_ptr()
+        args.w_columns, args.w_column_scales = wt
+    if xt is not None:
+        d_w = torch.empty((n, k), dtype=w_dtype, device=d_y.device)
+        if m == 0:
+            d_w.zero_()                    # (a sum over no tokens)
+        else:
+            args.d_w = d_w.data_ptr()
+            args.x_columns, args.x_column_scales = xt
+    if m:
+        need = _linear_workspace_bytes(m, n, k, 1)
+        ws = torch.empty(need, dtype=torch.uint8, device=d_y.device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need
+        _lib.check(_lib.load().dgm_mxfp4_linear_backward(ctypes.byref(args), _lib.stream()))
+    return d_x, d_w
 
 
 class _Mxfp4Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight):
         y, xt, wt = _linear_forward(x, weight, ctx.needs_input_grad[1], ctx.needs_input_grad[0])
-        ctx.save_for_backward(*(xt or (None, None)), *(wt or (None, None)))
-        ctx.shapes = x.shape, weight.shape, x.dtype, weight.dtype
+        ctx.save_for_backward(xt, wt)
+        ctx.shape = x.size(0), weight.size(0), x.size(1), x.dtype, weight.dtype
         return y
 
     @staticmethod
@@ -228,27 +283,20 @@ class _Mxfp4Linear(torch.autograd.Function):
         _lib.no_second_derivative()
         saved = ctx.saved_tensors
         _lib.no_tangents(d_y, *saved)
-        return _backward_of(d_y, saved[:2], saved[2:], *ctx.shapes, ctx.needs_input_grad)
-
-
-def _backward_of(d_y, xt, wt, x_shape, w_shape, x_dtype, w_dtype, needs):
-    """The backward pass after its checks (what comes back from saved-tensor hooks is checked as an argument is)."""
-    (m, k), n = x_shape, w_shape[0]
-    if d_y.dtype != x_dtype or tuple(d_y.shape) != (m, n):
-        raise TypeError(f"d_y of {x_dtype} [{m}, {n}] expected, got {d_y.dtype} {tuple(d_y.shape)}")
-    kept = []
-    for name, pair, wanted, inner in (("columns of x", xt, needs[1], m), ("columns of the weight", wt, needs[0], n)):
-        if not wanted:
-            kept.append(None)
-            continue
-        blocks = (inner + 31) // 32
-        if pair is None or any(t is None or t.dtype != torch.uint8 for t in pair) or \
-                tuple(pair[0].shape) != (k, 16 * blocks) or tuple(pair[1].shape) != (k, blocks):
-            raise ValueError(f"saved {name}: uint8 codes [{k}, {16 * blocks}] and scales [{k}, {blocks}] expected, as "
-                             "mxfp4_linear_forward returns them")
-        kept.append(pair)
-    _lib.require_one_device(d_y, *(t for pair in kept if pair is not None for t in pair))
-    return _linear_backward(d_y, *kept, x_dtype, w_dtype)
+        m, n, k, x_dtype, w_dtype = ctx.shape
+        kept = []
+        for memory, wanted, inner in ((saved[0], ctx.needs_input_grad[1], m), (saved[1], ctx.needs_input_grad[0], n)):
+            if not wanted:
+                kept.append(None)
+                continue
+            # (what saved-tensor hooks bring back is checked as an argument is: the kernels read it by address)
+            size = _code_bytes(k, inner)
+            if memory.dtype != torch.uint8 or tuple(memory.shape) != (size // 16 * 17,):
+                raise ValueError(f"saved columns came back as {memory.dtype} {tuple(memory.shape)}")
+            kept.append((_contiguous16(memory), size))
+        _lib.require_one_device(d_y, *(p[0] for p in kept if p is not None))
+        at = [None if p is None else (p[0].data_ptr(), p[0].data_ptr() + p[1]) for p in kept]
+        return _linear_backward(d_y, *at, k, x_dtype, w_dtype)
 
 
 def mxfp4_linear(x, weight):
@@ -259,8 +307,9 @@ def mxfp4_linear(x, weight):
     q as ``mxfp4_quantize`` along the dimension that its product sums over; the gradients pass straight through the
     roundings. x: bf16, fp16 or fp32 [tokens, in], weight: any of them [out, in] (fp32 master weights); y and d_x have
     x's type, d_weight the weight's; any strides, each size below 2^24, products within ``mxfp4_gemm_nt``'s limits.
-    The backward pass keeps the codes of x's and the weight's columns (17 / 32 byte a value), not the inputs. Under graph capture use ``mxfp4_linear_forward`` and
-    ``mxfp4_linear_backward``. Work runs on the current stream of the tensors' device, which has to be the current one."""
+    The backward pass keeps the codes of x's and the weight's columns (17 / 32 byte a value), not the inputs. Under graph
+    capture use ``mxfp4_linear_forward`` and ``mxfp4_linear_backward``. Work runs on the current stream of the tensors'
+    device, which has to be the current one."""
     _check_linear(x, weight)
     _lib.no_tangents(x, weight)
     _lib.require_one_device(x, weight)
@@ -277,7 +326,10 @@ def mxfp4_linear_forward(x, weight, needs=(True, True)):
     _check_linear(x, weight)
     _lib.no_tangents(x, weight)
     _lib.require_one_device(x, weight)
-    return _linear_forward(x, weight, bool(needs[1]), bool(needs[0]))
+    with torch.no_grad():
+        y, xt, wt = _linear_forward(x, weight, bool(needs[1]), bool(needs[0]))
+    k = x.size(1)
+    return y, None if xt is None else _as_pair(xt, k, x.size(0)), None if wt is None else _as_pair(wt, k, weight.size(0))
 
 
 def mxfp4_linear_backward(d_y, x_columns, weight_columns, x_shape, weight_shape, weight_dtype=None, needs=(True, True)):
@@ -287,10 +339,35 @@ def mxfp4_linear_backward(d_y, x_columns, weight_columns, x_shape, weight_shape,
     weight_dtype = weight_dtype or d_y.dtype
     if d_y.dtype not in _lib.SRC_DTYPES or weight_dtype not in _lib.SRC_DTYPES:
         raise TypeError(f"d_y and the weight are bf16, fp16 or fp32, got {d_y.dtype} and {weight_dtype}")
-    if len(x_shape) != 2 or len(weight_shape) != 2 or x_shape[1] != weight_shape[1]:
+    if len(x_shape) != 2 or len(weight_shape) != 2 or x_shape[1] != weight_shape[1] or x_shape[1] < 1 or weight_shape[0] < 1:
         raise ValueError(f"x {tuple(x_shape)} and weight {tuple(weight_shape)}: [tokens, in] and [out, in]")
+    (m, k), n = x_shape, weight_shape[0]
+    if max(m, n, k) >= MAX_DIM or not (_fits(m, k) and _fits(n, k)):
+        raise ValueError(f"x {tuple(x_shape)} and weight {tuple(weight_shape)}: sizes below 2^24, and ceil(a / 64) ceil(b / 64) below 2^23")
+    if tuple(d_y.shape) != (m, n):
+        raise TypeError(f"d_y [{m}, {n}] expected, got {tuple(d_y.shape)}")
+    kept = []
+    for name, pair, wanted, inner in (("x_columns", x_columns, needs[1], m), ("weight_columns", weight_columns, needs[0], n)):
+        if not wanted:
+            kept.append(None)
+            continue
+        blocks = (inner + 31) // 32
+        if pair is None or any(t.dtype != torch.uint8 for t in pair) or tuple(pair[0].shape) != (k, 16 * blocks) \
+                or tuple(pair[1].shape) != (k, blocks):
+            raise ValueError(f"{name}: uint8 codes [{k}, {16 * blocks}] and scales [{k}, {blocks}] expected, as mxfp4_linear_forward "
+                             "returns them")
+        kept.append(pair)
     _lib.no_tangents(d_y)
-    return _backward_of(d_y, x_columns, weight_columns, tuple(x_shape), tuple(weight_shape), d_y.dtype, weight_dtype, needs)
+    _lib.require_one_device(d_y, *(t for pair in kept if pair is not None for t in pair))
+    # (the tensors are held until the launches are enqueued)
+    kept = [None if p is None else (_contiguous16(p[0]), p[1].contiguous()) for p in kept]
+    at = [None if p is None else (p[0].data_ptr(), p[1].data_ptr()) for p in kept]
+    with torch.no_grad():
+        return _linear_backward(d_y, *at, k, d_y.dtype, weight_dtype)
+
+
+def _contiguous16(t):
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 __all__ = ["mxfp4_quantize", "mxfp4_quantize_both", "mxfp4_gemm_nt", "mxfp4_linear", "mxfp4_linear_forward",

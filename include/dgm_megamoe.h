@@ -559,6 +559,36 @@ int64_t dgm_mxfp4_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int swig
 int dgm_mxfp4_gemm_nt(const DgmMxfp4GemmArgs* args, hipStream_t stream);
 int dgm_mxfp4_gemm_struct_size(size_t* args);
 
+/* A linear layer whose three products are MXFP4, each pass as one call over the two operators above. Forward:
+ * y [m, n] (x_dtype) = q(x) q(w)^T for x [m, k] (x_dtype) and w [n, k] (w_dtype), rows at strides in elements; the
+ * columns of x and w are quantised in the same pass where x_columns (x_column_scales), w_columns (...) are given, as
+ * dgm_mxfp4_quantize's t_codes (t_scales). Backward: from d_y [m, n] (x_dtype), d_x [m, k] (x_dtype) = q(d_y) q(w^T)^T
+ * with w's columns, and d_w [n, k] (w_dtype) = q(d_y^T) q(x^T)^T with x's columns, each if given (m > 0 for both).
+ * y, d_x and d_w are contiguous. amax_floor 1e-30. workspace: dgm_mxfp4_linear_workspace_bytes, of this call until it
+ * has run, 16-byte aligned; column codes on 16 bytes. m, n and k below 2^24, products within dgm_mxfp4_gemm_nt's
+ * limits. */
+typedef struct DgmMxfp4LinearArgs {
+  const void* x;
+  const void* w;
+  void* y;
+  const void* d_y;
+  void* d_x;
+  void* d_w;
+  uint8_t* x_columns;
+  uint8_t* x_column_scales;
+  uint8_t* w_columns;
+  uint8_t* w_column_scales;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t m, n, k;
+  int64_t x_stride, w_stride, d_y_stride;
+  int32_t x_dtype, w_dtype;
+} DgmMxfp4LinearArgs;
+int64_t dgm_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int backward);
+int dgm_mxfp4_linear(const DgmMxfp4LinearArgs* args, hipStream_t stream);
+int dgm_mxfp4_linear_backward(const DgmMxfp4LinearArgs* args, hipStream_t stream);
+int dgm_mxfp4_linear_struct_size(size_t* args);
+
 /* The router's balance loss over logits [tokens, experts] (rows at logits_stride, type DGM_SRC_*) and the
  * chosen experts topk_idx [tokens, topk] (rows at idx_stride; int64 or int32; ids outside [0, experts) are
  * no slot, a token without a slot is unrouted and adds nothing). Sequences: tokens [cu_seqlens[b],
