@@ -26,6 +26,32 @@ DGM_DEV void load_piece(const DgmMxfp4QuantArgs& P, int64_t row, int64_t c, floa
   }
 }
 
+// The same as loaded, without a branch (a load in one is awaited at its end): outside the matrix another place of it.
+template <int T>
+struct RawPiece {
+  u4 w[T == T_F32 ? 2 : 1];
+  bool some;
+  DGM_DEV void load(const DgmMxfp4QuantArgs& P, int64_t row, int64_t c) {
+    some = row < P.rows && c < P.cols;
+    const int64_t at = (row < P.rows ? row : P.rows - 1) * P.x_stride + (c < P.cols ? c : 0);
+    const u4* p = reinterpret_cast<const u4*>(reinterpret_cast<const char*>(P.x) + at * (T == T_F32 ? 4 : 2));
+    w[0] = p[0];
+    if constexpr (T == T_F32) w[1] = p[1];
+  }
+  DGM_DEV void unpack(float* v) const {
+    if constexpr (T == T_F32) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t d = w[k / 4][k % 4];
+        v[k] = some ? __uint_as_float(d) : 0.f;
+      }
+    } else {
+      const u4 none = {0u, 0u, 0u, 0u};
+      unpack8<T>(some ? w[0] : none, v);
+    }
+  }
+};
+
 // Rows: a thread takes eight values, four neighbours a block. 2^log_row threads a row of the workgroup, `runs`
 // workgroups along a row.
 template <int T, bool VEC>
@@ -50,21 +76,30 @@ template <int T, bool VEC, bool BOTH>
 __global__ void __launch_bounds__(256) k_mxfp4_columns(const DgmMxfp4QuantArgs P, int tiles_c) {
   constexpr int R = T == T_F32 ? 64 : 128, C = 128, B = R / 32, PAIR = T == T_F32 ? 1 : 2;
   using E = std::conditional_t<T == T_F32, uint32_t, uint16_t>;
-  __shared__ __attribute__((aligned(16))) E tile[R][C];
-  __shared__ u4 codes[B][C + 1];
-  __shared__ uint8_t scales[C][B];
+  // (the columns' codes and scales take the tile's place: five workgroups a CU)
+  __shared__ __attribute__((aligned(16))) uint8_t memory[R * C * sizeof(E)];
+  E(*tile)[C] = reinterpret_cast<E(*)[C]>(memory);
+  u4(*codes)[C + 1] = reinterpret_cast<u4(*)[C + 1]>(memory);
+  uint8_t(*scales)[B] = reinterpret_cast<uint8_t(*)[B]>(memory + B * (C + 1) * 16);
+  static_assert(B * (C + 1) * 16 + C * B <= (int)sizeof(memory), "they fit");
   const int64_t r0 = (int64_t)(blockIdx.x / (unsigned)tiles_c) * R, c0 = (int64_t)(blockIdx.x % (unsigned)tiles_c) * C;
   const int64_t row_blocks = (P.cols + 31) / 32, col_blocks = (P.rows + 31) / 32;
   const uint32_t floor_bits = __float_as_uint(P.amax_floor);
   const int at = (threadIdx.x & 15) * 8;
+  RawPiece<T> raw[VEC ? R / 16 : 1];             // (all requested before the first is used)
+  if constexpr (VEC)
+#pragma unroll
+    for (int i = 0; i < R / 16; ++i) raw[i].load(P, r0 + i * 16 + (threadIdx.x >> 4), c0 + at);
 #pragma unroll
   for (int i = 0; i < R / 16; ++i) {
     const int r = i * 16 + (threadIdx.x >> 4);
     float v[8];
-    if (r0 + r < P.rows) load_piece<T, VEC>(P, r0 + r, c0 + at, v);
-    else
+    if constexpr (VEC) {
+      raw[i].unpack(v);
+    } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = 0.f;
+      for (int k = 0; k < 8; ++k) v[k] = r0 + r < P.rows && c0 + at + k < P.cols ? load1<T>(P.x, (r0 + r) * P.x_stride + c0 + at + k) : 0.f;
+    }
     store8<T>(&tile[r][0], at, v);              // (exact: the values are of type T)
     if constexpr (BOTH) {
       const uint32_t code = mx_scale_code(max_u32_lanes4(magnitude8(v)), floor_bits);
@@ -82,6 +117,7 @@ __global__ void __launch_bounds__(256) k_mxfp4_columns(const DgmMxfp4QuantArgs P
     uint32_t w[32];
 #pragma unroll
     for (int k = 0; k < 32; ++k) w[k] = *reinterpret_cast<const uint32_t*>(&tile[32 * b + k][c]);
+    __syncthreads();
 #pragma unroll
     for (int h = 0; h < PAIR; ++h) {
       float v[32];
