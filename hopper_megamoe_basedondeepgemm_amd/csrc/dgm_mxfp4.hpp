@@ -20,6 +20,17 @@ DGM_DEV uint32_t magnitude8(const float* v) {
   for (int i = 0; i < 8; ++i) m = max_u32(m, magnitude(v[i]));
   return m;
 }
+// Magnitudes of two 16-bit elements in a dword, and the larger of each half: bf16 and fp16 order as their bits do.
+typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+DGM_DEV uint32_t max_pairs(uint32_t m, uint32_t w) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, m), __builtin_bit_cast(us2, w & 0x7fff7fffu)));
+}
+// the fp32 bits of a 16-bit magnitude (an infinity or NaN stays one)
+template <int T>
+DGM_DEV uint32_t magnitude_bits(uint32_t half) {
+  if constexpr (T == T_F16) return __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)half));
+  else return half << 16;
+}
 // maximum over aligned groups of four lanes (all active), in each of them
 DGM_DEV uint32_t max_u32_lanes4(uint32_t v) {
   v = max_u32(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));      // quad_perm [1,0,3,2]

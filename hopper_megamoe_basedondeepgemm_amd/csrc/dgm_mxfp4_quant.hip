@@ -12,45 +12,54 @@ using namespace dgm;
 
 namespace {
 
-// eight elements of row `row` from column c on, zeros behind the last
-template <int T, bool VEC>
+// eight elements of row `row` from column c on, zeros outside the matrix
+template <int T>
 DGM_DEV void load_piece(const DgmMxfp4QuantArgs& P, int64_t row, int64_t c, float* v) {
-  if constexpr (VEC) {
-    if (c < P.cols) load8<T>(P.x, row * P.x_stride + c, v);
-    else
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < P.cols ? load1<T>(P.x, row * P.x_stride + c + i) : 0.f;
-  }
+  for (int i = 0; i < 8; ++i) v[i] = row < P.rows && c + i < P.cols ? load1<T>(P.x, row * P.x_stride + c + i) : 0.f;
 }
 
-// The same as loaded, without a branch (a load in one is awaited at its end): outside the matrix another place of it.
+// The same as loaded, without a branch (a load in one is awaited at its end): at `p`, which is inside the matrix, and
+// zeros if !some.
 template <int T>
 struct RawPiece {
   u4 w[T == T_F32 ? 2 : 1];
-  bool some;
-  DGM_DEV void load(const DgmMxfp4QuantArgs& P, int64_t row, int64_t c) {
-    some = row < P.rows && c < P.cols;
-    const int64_t at = (row < P.rows ? row : P.rows - 1) * P.x_stride + (c < P.cols ? c : 0);
-    const u4* p = reinterpret_cast<const u4*>(reinterpret_cast<const char*>(P.x) + at * (T == T_F32 ? 4 : 2));
-    w[0] = p[0];
-    if constexpr (T == T_F32) w[1] = p[1];
+  DGM_DEV void load(const char* p) {
+    w[0] = reinterpret_cast<const u4*>(p)[0];
+    if constexpr (T == T_F32) w[1] = reinterpret_cast<const u4*>(p)[1];
+  }
+  DGM_DEV void clear_unless(bool some) {
+    const u4 none = {0u, 0u, 0u, 0u};
+    w[0] = some ? w[0] : none;
+    if constexpr (T == T_F32) w[1] = some ? w[1] : none;
   }
   DGM_DEV void unpack(float* v) const {
     if constexpr (T == T_F32) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const uint32_t d = w[k / 4][k % 4];
-        v[k] = some ? __uint_as_float(d) : 0.f;
+        v[k] = __uint_as_float(d);
       }
     } else {
-      const u4 none = {0u, 0u, 0u, 0u};
-      unpack8<T>(some ? w[0] : none, v);
+      unpack8<T>(w[0], v);
+    }
+  }
+  // the largest magnitude's fp32 bits
+  DGM_DEV uint32_t magnitude() const {
+    if constexpr (T == T_F32) {
+      float v[8];
+      unpack(v);
+      return magnitude8(v);
+    } else {
+      uint32_t m = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m = max_pairs(m, w[0][k]);
+      return magnitude_bits<T>(max_u32(m & 0xffffu, m >> 16));
     }
   }
 };
+template <int T>
+constexpr int SIZE = T == T_F32 ? 4 : 2;
 
 // Rows: a thread takes eight values, four neighbours a block. 2^log_row threads a row of the workgroup, `runs`
 // workgroups along a row.
@@ -63,8 +72,19 @@ __global__ void __launch_bounds__(256) k_mxfp4_rows(const DgmMxfp4QuantArgs P, i
   const int64_t blocks = (P.cols + 31) / 32;
   if (row >= P.rows || piece >= 4 * blocks) return;           // (whole blocks: four lanes share one)
   float v[8];
-  load_piece<T, VEC>(P, row, piece * 8, v);
-  const uint32_t code = mx_scale_code(max_u32_lanes4(magnitude8(v)), __float_as_uint(P.amax_floor));
+  uint32_t m;
+  if constexpr (VEC) {
+    RawPiece<T> raw;
+    const bool some = piece * 8 < P.cols;
+    raw.load(reinterpret_cast<const char*>(P.x) + (row * P.x_stride + (some ? piece * 8 : 0)) * SIZE<T>);
+    raw.clear_unless(some);
+    raw.unpack(v);
+    m = raw.magnitude();
+  } else {
+    load_piece<T>(P, row, piece * 8, v);
+    m = magnitude8(v);
+  }
+  const uint32_t code = mx_scale_code(max_u32_lanes4(m), __float_as_uint(P.amax_floor));
   reinterpret_cast<uint32_t*>(P.codes)[row * blocks * 4 + piece] = e2m1_codes8<T>(v, code);
   if ((piece & 3) == 0) P.scales[row * blocks + (piece >> 2)] = (uint8_t)code;
 }
@@ -85,28 +105,42 @@ __global__ void __launch_bounds__(256) k_mxfp4_columns(const DgmMxfp4QuantArgs P
   const int64_t r0 = (int64_t)(blockIdx.x / (unsigned)tiles_c) * R, c0 = (int64_t)(blockIdx.x % (unsigned)tiles_c) * C;
   const int64_t row_blocks = (P.cols + 31) / 32, col_blocks = (P.rows + 31) / 32;
   const uint32_t floor_bits = __float_as_uint(P.amax_floor);
-  const int at = (threadIdx.x & 15) * 8;
+  const int at = (threadIdx.x & 15) * 8, first = threadIdx.x >> 4;
+  const int most = (int)min(P.rows - r0, (int64_t)R) - 1;              // last row of the tile
+  const bool inside = c0 + at < P.cols;
   RawPiece<T> raw[VEC ? R / 16 : 1];             // (all requested before the first is used)
-  if constexpr (VEC)
+  if constexpr (VEC) {
+    const char* from = reinterpret_cast<const char*>(P.x) + (r0 * P.x_stride + (inside ? c0 + at : 0)) * SIZE<T>;
 #pragma unroll
-    for (int i = 0; i < R / 16; ++i) raw[i].load(P, r0 + i * 16 + (threadIdx.x >> 4), c0 + at);
+    for (int i = 0; i < R / 16; ++i) raw[i].load(from + (int64_t)min(i * 16 + first, most) * P.x_stride * SIZE<T>);
+  }
+  const int64_t piece = (c0 + at) / 8;
+  uint32_t* const row_codes = reinterpret_cast<uint32_t*>(P.codes) + r0 * row_blocks * 4 + piece;
+  uint8_t* const row_scales = P.scales + r0 * row_blocks + (piece >> 2);
 #pragma unroll
   for (int i = 0; i < R / 16; ++i) {
-    const int r = i * 16 + (threadIdx.x >> 4);
+    const int r = i * 16 + first;
     float v[8];
+    uint32_t m;
     if constexpr (VEC) {
-      raw[i].unpack(v);
+      raw[i].clear_unless(inside && r <= most);
+      u4* to = reinterpret_cast<u4*>(&tile[r][at]);
+      to[0] = raw[i].w[0];
+      if constexpr (T == T_F32) to[1] = raw[i].w[1];
+      if constexpr (BOTH) {
+        raw[i].unpack(v);
+        m = raw[i].magnitude();
+      }
     } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = r0 + r < P.rows && c0 + at + k < P.cols ? load1<T>(P.x, (r0 + r) * P.x_stride + c0 + at + k) : 0.f;
+      load_piece<T>(P, r0 + r, c0 + at, v);
+      store8<T>(&tile[r][0], at, v);              // (exact: the values are of type T)
+      m = magnitude8(v);
     }
-    store8<T>(&tile[r][0], at, v);              // (exact: the values are of type T)
     if constexpr (BOTH) {
-      const uint32_t code = mx_scale_code(max_u32_lanes4(magnitude8(v)), floor_bits);
-      const int64_t piece = (c0 + at) / 8;
-      if (r0 + r < P.rows && piece < 4 * row_blocks) {
-        reinterpret_cast<uint32_t*>(P.codes)[(r0 + r) * row_blocks * 4 + piece] = e2m1_codes8<T>(v, code);
-        if ((piece & 3) == 0) P.scales[(r0 + r) * row_blocks + (piece >> 2)] = (uint8_t)code;
+      const uint32_t code = mx_scale_code(max_u32_lanes4(m), floor_bits);
+      if (r <= most && piece < 4 * row_blocks) {
+        row_codes[(int64_t)r * row_blocks * 4] = e2m1_codes8<T>(v, code);
+        if ((piece & 3) == 0) row_scales[(int64_t)r * row_blocks] = (uint8_t)code;
       }
     }
   }
@@ -118,16 +152,20 @@ __global__ void __launch_bounds__(256) k_mxfp4_columns(const DgmMxfp4QuantArgs P
 #pragma unroll
     for (int k = 0; k < 32; ++k) w[k] = *reinterpret_cast<const uint32_t*>(&tile[32 * b + k][c]);
     __syncthreads();
+    uint32_t pairs = 0;                            // 16 bits: both columns' magnitudes
+    if constexpr (PAIR == 2)
+#pragma unroll
+      for (int k = 0; k < 32; ++k) pairs = max_pairs(pairs, w[k]);
 #pragma unroll
     for (int h = 0; h < PAIR; ++h) {
       float v[32];
       uint32_t m = 0;
+      if constexpr (PAIR == 2) m = magnitude_bits<T>(h ? pairs >> 16 : pairs & 0xffffu);
 #pragma unroll
       for (int k = 0; k < 32; ++k) {
-        if constexpr (T == T_F32) v[k] = __uint_as_float(w[k]);
+        if constexpr (T == T_F32) v[k] = __uint_as_float(w[k]), m = max_u32(m, magnitude(v[k]));
         else if constexpr (T == T_F16) v[k] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[k] >> (16 * h)));
         else v[k] = __uint_as_float(h ? w[k] & 0xffff0000u : w[k] << 16);
-        m = max_u32(m, magnitude(v[k]));
       }
       const uint32_t code = mx_scale_code(m, floor_bits);
       u4 q;
