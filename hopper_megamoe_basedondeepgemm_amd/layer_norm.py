@@ -40,20 +40,13 @@ def _check(x, residual, weight, bias, quant=None, residual_out=None, out=None):
 
 
 def _forward_args(x, residual, weight, bias, residual_scale, eps):
-    """DgmLayerNormArgs of a call's inputs (absent parts stay at their zero)."""
+    """DgmLayerNormArgs of a call's inputs (its outputs at their zero)."""
     T, H = x.shape
-    args = _lib.LayerNormArgs(x=x.data_ptr(), rows=T, x_stride=x.stride(0), hidden=H, dtype=_lib.SRC_DTYPES[x.dtype],
-                              residual_scale=residual_scale, eps=eps)
-    if residual is not None:
-        args.residual, args.residual_stride = residual.data_ptr(), residual.stride(0)
-    if weight is not None:
-        args.weight = weight.data_ptr()
-    if bias is not None:
-        args.bias = bias.data_ptr()
     w = weight if weight is not None else bias
-    if w is not None and w.dtype == torch.float32:
-        args.weights_f32 = 1
-    return args
+    r, r_stride = (0, 0) if residual is None else (residual.data_ptr(), residual.stride(0))
+    return _lib.LayerNormArgs(x.data_ptr(), r, 0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                              0, 0, 0, 0, 0, 0, T, x.stride(0), r_stride, 0, 0, H, _lib.SRC_DTYPES[x.dtype],
+                              w is not None and w.dtype == torch.float32, residual_scale, eps)
 
 
 def _readable(x, residual, weight, bias):
@@ -92,7 +85,7 @@ def _forward(x, residual, weight, bias, residual_scale, eps, quant, residual_out
     args.h, args.h_stride = h.data_ptr(), h.stride(0)
     fused = quant and H % 8 == 0 and _aligned(*read, r_out, h)
     if fused:
-        rows = _new_mxfp4(T, H, x)
+        rows = _new_mxfp4(T, H, x.device)
         args.codes, args.scales = rows[0].data_ptr(), rows[1].data_ptr()
     if T > 0:
         if residual_out is not None or out is not None:

@@ -18,38 +18,48 @@ def _rows(t):
     return t if t.stride(1) == 1 or t.size(1) == 1 else t.contiguous()
 
 
+def _fits(m, n):
+    return ((m + 63) // 64) * ((n + 63) // 64) < 1 << 23
+
+
 def _check_quantize(x, amax_floor):
-    if x.dtype not in _lib.SRC_DTYPES or x.dim() != 2:
-        raise TypeError(f"x must be bf16, fp16 or fp32 [rows, cols], got {x.dtype} {tuple(x.shape)}")
-    if x.size(0) >= MAX_DIM or x.size(1) >= MAX_DIM:
-        raise ValueError(f"x {tuple(x.shape)}: below 2^24 each way")
+    shape = x.shape
+    if x.dtype not in _lib.SRC_DTYPES or len(shape) != 2:
+        raise TypeError(f"x must be bf16, fp16 or fp32 [rows, cols], got {x.dtype} {tuple(shape)}")
+    if shape[0] >= MAX_DIM or shape[1] >= MAX_DIM:
+        raise ValueError(f"x {tuple(shape)}: below 2^24 each way")
     if not 0 <= amax_floor < math.inf:
         raise ValueError(f"amax_floor {amax_floor}: a number, at least 0")
 
 
-def _new(rows, cols, like):
+def _new(rows, cols, device):
     """Uninitialised (codes, scales) of rows of cols elements."""
     blocks = (cols + 31) // 32
-    return (torch.empty((rows, 16 * blocks), dtype=torch.uint8, device=like.device),
-            torch.empty((rows, blocks), dtype=torch.uint8, device=like.device))
+    return (torch.empty((rows, 16 * blocks), dtype=torch.uint8, device=device),
+            torch.empty((rows, blocks), dtype=torch.uint8, device=device))
 
 
 def _quantize(x, amax_floor, rows, columns):
     """((codes, scales) of x's rows, the same of its columns), each if wanted, after the checks."""
-    if x.stride(1) != 1 and x.stride(0) == 1:             # (a transposed view: its rows are the memory's columns)
-        by_column, by_row = _quantize(x.t(), amax_floor, columns, rows)
-        return by_row, by_column
-    x = _rows(x)
+    stride, one = x.stride()
+    if one != 1:
+        if stride == 1:                                   # (a transposed view: its rows are the memory's columns)
+            by_column, by_row = _quantize(x.t(), amax_floor, columns, rows)
+            return by_row, by_column
+        if x.size(1) != 1:
+            x = x.contiguous()
+            stride = x.stride(0)
     m, n = x.shape
-    by_row = _new(m, n, x) if rows else None
-    by_column = _new(n, m, x) if columns else None
-    args = _lib.Mxfp4QuantArgs(x=x.data_ptr(), rows=m, cols=n, x_stride=x.stride(0), dtype=_lib.SRC_DTYPES[x.dtype],
-                               amax_floor=amax_floor)
+    by_row = by_column = None
+    r = r_sf = c = c_sf = 0
     if rows:
-        args.codes, args.scales = by_row[0].data_ptr(), by_row[1].data_ptr()
+        by_row = _new(m, n, x.device)
+        r, r_sf = by_row[0].data_ptr(), by_row[1].data_ptr()
     if columns:
-        args.t_codes, args.t_scales = by_column[0].data_ptr(), by_column[1].data_ptr()
+        by_column = _new(n, m, x.device)
+        c, c_sf = by_column[0].data_ptr(), by_column[1].data_ptr()
     if m and n:
+        args = _lib.Mxfp4QuantArgs(x.data_ptr(), r, r_sf, c, c_sf, m, n, stride, _lib.SRC_DTYPES[x.dtype], amax_floor)
         _lib.check(_lib.load().dgm_mxfp4_quantize(ctypes.byref(args), _lib.stream()))
     return by_row, by_column
 
@@ -87,23 +97,34 @@ def mxfp4_quantize_both(x, amax_floor=1e-30):
 
 
 def _operand(name, pair):
-    """(codes, scale bytes) of a product's operand."""
+    """(codes, scale bytes, rows, bytes of a code row) of a product's operand."""
     q, sf = pair
-    if q.dtype != torch.uint8 or q.dim() != 2:
-        raise TypeError(f"{name}: uint8 codes [rows, k / 2] expected, got {q.dtype} {tuple(q.shape)}")
-    if sf.dtype == torch.int32 and sf.dim() == 2:         # (per_token_cast_to_fp4(use_packed_ue8m0=True))
+    shape, sf_shape = q.shape, sf.shape
+    if q.dtype != torch.uint8 or len(shape) != 2:
+        raise TypeError(f"{name}: uint8 codes [rows, k / 2] expected, got {q.dtype} {tuple(shape)}")
+    if sf.dtype == torch.int32 and len(sf_shape) == 2:         # (per_token_cast_to_fp4(use_packed_ue8m0=True))
         sf = sf.contiguous().view(torch.uint8)
-    if sf.dtype != torch.uint8 or sf.dim() != 2 or sf.size(0) != q.size(0) or q.size(1) != 16 * sf.size(1):
-        raise TypeError(f"{name}: uint8 scales [{q.size(0)}, {q.size(1) / 16:g}] (a byte for 16 bytes of codes) expected, got "
-                        f"{sf.dtype} {tuple(sf.shape)}")
-    return q, sf
+        sf_shape = sf.shape
+    rows, size = shape
+    if sf.dtype != torch.uint8 or len(sf_shape) != 2 or sf_shape[0] != rows or size != 16 * sf_shape[1]:
+        raise TypeError(f"{name}: uint8 scales [{rows}, {size / 16:g}] (a byte for 16 bytes of codes) expected, got "
+                        f"{sf.dtype} {tuple(sf_shape)}")
+    return q, sf, rows, size
 
 
 def _readable(q, sf):
-    """An operand as the kernels read it: code rows on 16 bytes and less than 2^23 apart, scale rows of contiguous bytes."""
-    if q.stride(1) != 1 or q.stride(0) % 16 or q.stride(0) >= 1 << 23 or q.data_ptr() % 16:
+    """An operand as the kernels read it, code rows on 16 bytes and less than 2^23 apart, scale rows of contiguous bytes:
+    (codes, scales, their addresses, their row strides)."""
+    stride, one = q.stride()
+    at = q.data_ptr()
+    if one != 1 or stride % 16 or stride >= 1 << 23 or at % 16:
         q = q.clone(memory_format=torch.contiguous_format)
-    return q, _rows(sf)
+        stride, at = q.stride(0), q.data_ptr()
+    sf_stride, one = sf.stride()
+    if one != 1 and sf.size(1) != 1:
+        sf = sf.contiguous()
+        sf_stride = sf.stride(0)
+    return q, sf, at, sf.data_ptr(), stride, sf_stride
 
 
 @functools.lru_cache(maxsize=1024)
@@ -123,12 +144,11 @@ def mxfp4_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_
     clamp; ``fast_math`` as in ``int8_gemm_nt``). Sums in fp32, one rounding; a scale of 255 makes its row NaN. k a
     multiple of 32. m, n and k below 2^24, ceil(m / 64) ceil(n / 64) below 2^23. No gradient (``mxfp4_linear`` has
     one). Work runs on the current stream of the tensors' device, which has to be the current one. Returns d."""
-    aq, asf = _operand("a", a)
-    bq, bsf = _operand("b", b)
-    m, k = aq.size(0), 2 * aq.size(1)
-    n = bq.size(0)
-    if 2 * bq.size(1) != k or not 32 <= k < MAX_DIM:
-        raise ValueError(f"k of a {k} and of b {2 * bq.size(1)}: equal, 32 to 2^24")
+    aq, asf, m, size_a = _operand("a", a)
+    bq, bsf, n, size_b = _operand("b", b)
+    k = 2 * size_a
+    if size_a != size_b or not 32 <= k < MAX_DIM:
+        raise ValueError(f"k of a {k} and of b {2 * size_b}: equal, 32 to 2^24")
     if activation not in (None, "swiglu"):
         raise ValueError(f"activation {activation!r}: None or 'swiglu'")
     swiglu = activation is not None
@@ -136,13 +156,14 @@ def mxfp4_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_
         raise ValueError("swiglu takes a gate and an up half of b's rows, and no c")
     if activation_clamp is not None and not activation_clamp >= 0:
         raise ValueError(f"activation_clamp {activation_clamp}: at least 0, or None")
-    if m >= MAX_DIM or n >= MAX_DIM or ((m + 63) // 64) * ((n + 63) // 64) >= 1 << 23:
+    if m >= MAX_DIM or n >= MAX_DIM or not _fits(m, n):
         raise ValueError(f"m {m} and n {n}: below 2^24, and ceil(m / 64) ceil(n / 64) below 2^23")
     n_out = n // 2 if swiglu else n
-    if d.dtype not in _lib.SRC_DTYPES or d.dim() != 2 or d.size(0) != m or d.size(1) != n_out:
+    dtype = _lib.SRC_DTYPES.get(d.dtype)
+    if dtype is None or d.shape != (m, n_out):
         raise TypeError(f"d: bf16, fp16 or fp32 [{m}, {n_out}] expected, got {d.dtype} {tuple(d.shape)}")
-    d_stride = d.stride(0)
-    if m and n_out and ((n_out > 1 and d.stride(1) != 1) or (m > 1 and d_stride < n_out)):
+    d_stride, one = d.stride()
+    if m and n_out and ((n_out > 1 and one != 1) or (m > 1 and d_stride < n_out)):
         raise ValueError("d: rows must be contiguous and must not overlap")
     if c is not None and (c.dtype != d.dtype or tuple(c.shape) not in ((m, n_out), (n_out,))):
         raise TypeError(f"c: {d.dtype} [{m}, {n_out}] or [{n_out}] expected, got {c.dtype} {tuple(c.shape)}")
@@ -152,17 +173,15 @@ def mxfp4_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_
     _lib.require_one_device(d, aq, asf, bq, bsf, c)
     if m == 0 or n_out == 0:
         return d
-    aq, asf = _readable(aq, asf)
-    bq, bsf = _readable(bq, bsf)
-    size = d.element_size()
-    pa, pb, lo, a_stride, b_stride = aq.data_ptr(), bq.data_ptr(), d.data_ptr(), aq.stride(0), bq.stride(0)
-    psa, psb, sa_stride, sb_stride = asf.data_ptr(), bsf.data_ptr(), asf.stride(0), bsf.stride(0)
-    hi = lo + ((m - 1) * d_stride + n_out) * size
-    if ((pa < hi and lo < pa + (m - 1) * a_stride + k // 2) or (pb < hi and lo < pb + (n - 1) * b_stride + k // 2)
-            or (psa < hi and lo < psa + (m - 1) * sa_stride + k // 32) or (psb < hi and lo < psb + (n - 1) * sb_stride + k // 32)):
+    aq, asf, pa, psa, a_stride, sa_stride = _readable(aq, asf)
+    bq, bsf, pb, psb, b_stride, sb_stride = _readable(bq, bsf)
+    size, lo, last = 2 if dtype < 2 else 4, d.data_ptr(), m - 1
+    hi = lo + (last * d_stride + n_out) * size
+    if ((pa < hi and lo < pa + last * a_stride + size_a) or (pb < hi and lo < pb + (n - 1) * b_stride + size_b)
+            or (psa < hi and lo < psa + last * sa_stride + size_a // 16) or (psb < hi and lo < psb + (n - 1) * sb_stride + size_b // 16)):
         raise ValueError("d overlaps an operand")
     args = _lib.Mxfp4GemmArgs(pa, psa, pb, psb, 0, lo, m, n, k, a_stride, sa_stride, b_stride, sb_stride, 0, d_stride,
-                              _lib.SRC_DTYPES[d.dtype], swiglu, math.inf if activation_clamp is None else float(activation_clamp),
+                              dtype, swiglu, math.inf if activation_clamp is None else float(activation_clamp),
                               1 if fast_math else 0)
     if c is not None:
         if c.dim() == 1:
@@ -170,7 +189,7 @@ def mxfp4_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_
         else:
             c = _rows(c)
             c_stride = c.stride(0)
-            end = (m - 1) * c_stride + n_out
+            end = last * c_stride + n_out
         pc = c.data_ptr()
         if pc < hi and lo < pc + end * size and not (pc == lo and c.dim() == 2 and (m == 1 or c_stride == d_stride)):
             raise ValueError("c overlaps d other than as the same rows")
@@ -182,10 +201,6 @@ def mxfp4_gemm_nt(a, b, d, c=None, activation=None, activation_clamp=10.0, fast_
     _lib.check(_lib.load().dgm_mxfp4_gemm_nt(ctypes.byref(args), _lib.stream()))
     _lib.written(d)
     return d
-
-
-def _fits(m, n):
-    return ((m + 63) // 64) * ((n + 63) // 64) < 1 << 23
 
 
 def _check_linear(x, weight):
