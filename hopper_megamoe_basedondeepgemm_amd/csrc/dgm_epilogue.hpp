@@ -33,6 +33,11 @@ DGM_DEV float c_value(const void* p, int64_t i) {
   else return bf16_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
 }
 
+// 16 and 8 bytes of C or D, on 4 bytes at least
+typedef int g4i __attribute__((ext_vector_type(4), aligned(4)));
+typedef float g4f __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t g2u __attribute__((ext_vector_type(2), aligned(4)));
+
 // Orders a wave's LDS accesses before and after it, between its lanes.
 DGM_DEV void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -41,7 +46,7 @@ DGM_DEV void wave_sync() {
 }
 
 // A 16-byte piece of token m's row from channel n on (eight channels, fp32: four), from LDS: C added, rounded,
-// stored. vec: rows of D (and C) are 16-byte aligned; STREAM: 2 = and stored past the caches.
+// stored. vec: rows of D (and C) are 4-byte aligned; STREAM: 2 = and stored past the caches.
 template <int T, bool ADD, bool STREAM = false, class Args>
 DGM_DEV void put_piece(const Args& P, int64_t m, int64_t n, int64_t n_out, int vec, const float* from) {
   constexpr int E = T == DGM_SRC_F32 ? 4 : 8;
@@ -57,31 +62,31 @@ DGM_DEV void put_piece(const Args& P, int64_t m, int64_t n, int64_t n_out, int v
   if (vec && n + E <= n_out) {
     if constexpr (T == DGM_SRC_F32) {
       if constexpr (ADD) {
-        const v4f c = *reinterpret_cast<const v4f*>(reinterpret_cast<const float*>(P.c) + ct);
+        const v4f c = *reinterpret_cast<const g4f*>(reinterpret_cast<const float*>(P.c) + ct);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] += c[i];
       }
-      v4f* to = reinterpret_cast<v4f*>(reinterpret_cast<float*>(P.d) + at);
-      const v4f o = {v[0], v[1], v[2], v[3]};
+      g4f* to = reinterpret_cast<g4f*>(reinterpret_cast<float*>(P.d) + at);
+      const g4f o = {v[0], v[1], v[2], v[3]};
       if (STREAM && vec == 2) __builtin_nontemporal_store(o, to);
       else *to = o;
     } else {
       if constexpr (ADD) {
-        const v4i c = *reinterpret_cast<const v4i*>(reinterpret_cast<const uint16_t*>(P.c) + ct);
+        const v4i c = *reinterpret_cast<const g4i*>(reinterpret_cast<const uint16_t*>(P.c) + ct);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const uint16_t w[1] = {(uint16_t)((uint32_t)c[i >> 1] >> (16 * (i & 1)))};
           v[i] += c_value<T>(w, 0);
         }
       }
-      v4i o;
+      g4i o;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t lo = T == DGM_SRC_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[2 * i]) : __builtin_bit_cast(uint16_t, (__bf16)v[2 * i]);
         const uint32_t hi = T == DGM_SRC_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[2 * i + 1]) : __builtin_bit_cast(uint16_t, (__bf16)v[2 * i + 1]);
         o[i] = (int)(lo | hi << 16);
       }
-      v4i* to = reinterpret_cast<v4i*>(reinterpret_cast<uint16_t*>(P.d) + at);
+      g4i* to = reinterpret_cast<g4i*>(reinterpret_cast<uint16_t*>(P.d) + at);
       if (STREAM && vec == 2) __builtin_nontemporal_store(o, to);
       else *to = o;
     }
@@ -104,24 +109,25 @@ DGM_DEV void put4(const Args& P, int64_t m, int64_t n, int64_t n_out, float* v) 
   if constexpr (WHOLE) {
     if constexpr (ADD) {
       if constexpr (T == DGM_SRC_F32) {
-        const v4f c = *reinterpret_cast<const v4f*>(reinterpret_cast<const float*>(P.c) + ct);
+        const v4f c = *reinterpret_cast<const g4f*>(reinterpret_cast<const float*>(P.c) + ct);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] += c[i];
       } else {
-        const uint2 c = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(P.c) + ct);
-        const uint16_t w[4] = {(uint16_t)c.x, (uint16_t)(c.x >> 16), (uint16_t)c.y, (uint16_t)(c.y >> 16)};
+        const g2u c = *reinterpret_cast<const g2u*>(reinterpret_cast<const uint16_t*>(P.c) + ct);
+        const uint32_t lo = c[0], hi = c[1];
+        const uint16_t w[4] = {(uint16_t)lo, (uint16_t)(lo >> 16), (uint16_t)hi, (uint16_t)(hi >> 16)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] += c_value<T>(w, i);
       }
     }
     if constexpr (T == DGM_SRC_F32) {
-      *reinterpret_cast<v4f*>(reinterpret_cast<float*>(P.d) + at) = v4f{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<g4f*>(reinterpret_cast<float*>(P.d) + at) = g4f{v[0], v[1], v[2], v[3]};
     } else {
       uint32_t h[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         h[i] = T == DGM_SRC_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[i]) : __builtin_bit_cast(uint16_t, (__bf16)v[i]);
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(P.d) + at) = uint2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+      *reinterpret_cast<g2u*>(reinterpret_cast<uint16_t*>(P.d) + at) = g2u{h[0] | h[1] << 16, h[2] | h[3] << 16};
     }
   } else {
 #pragma unroll

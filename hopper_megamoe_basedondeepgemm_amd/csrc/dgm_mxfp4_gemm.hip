@@ -444,8 +444,9 @@ void launch_tiles(const DgmMxfp4GemmArgs& A, int vec, int splits, hipStream_t st
   const int per = (steps + splits - 1) / splits;
   splits = (steps + per - 1) / per;                // (every split has a step)
   const dim3 grid((unsigned)((tiles_m * tiles_n + 7) / 8 * 8), (unsigned)splits), block(64 * WM * WN);
-  if (A.swiglu) hipLaunchKernelGGL((k_mxfp4_gemm_tiles<BM, BN, WM, WN, STAGES, true>), grid, block, 0, stream, A, vec, tiles_m, tiles_n, per);
-  else hipLaunchKernelGGL((k_mxfp4_gemm_tiles<BM, BN, WM, WN, STAGES, false>), grid, block, 0, stream, A, vec, tiles_m, tiles_n, per);
+  if constexpr (BN / WN % 32 == 0)                 // (a wave's gate and up fragments)
+    if (A.swiglu) hipLaunchKernelGGL((k_mxfp4_gemm_tiles<BM, BN, WM, WN, STAGES, true>), grid, block, 0, stream, A, vec, tiles_m, tiles_n, per);
+  if (!A.swiglu) hipLaunchKernelGGL((k_mxfp4_gemm_tiles<BM, BN, WM, WN, STAGES, false>), grid, block, 0, stream, A, vec, tiles_m, tiles_n, per);
   if (splits == 1) return;
   const int64_t quads = ((A.swiglu ? A.n / 2 : A.n) + 3) / 4 * A.m;
   const dim3 join((unsigned)((quads + 255) / 256));
@@ -457,9 +458,11 @@ void launch_tiles(const DgmMxfp4GemmArgs& A, int vec, int splits, hipStream_t st
 // step of 256 of K, `alone` us while every workgroup has a CU to itself; when the CUs hold as many as fit, each round
 // of them takes `full` us a step and `out` us for its results. Splitting K costs a second launch and the sums' way
 // through memory. The times are fitted to 93 products of 1 to 8192 tokens with every form and split, three sets of
-// operands in turn: the estimates' choice takes 1.8 % longer than the best of twelve forms on average.
+// operands in turn: the estimates' choice takes 1.8 % longer than the best of twelve forms on average (64 x 64, by
+// eight waves, came later).
 // Where each form is the best (us; next best):
-//   64 x 128, 3 stages:   200 x 5120, K 2880: 9.5 (64 x 64 11.1);    384 x 4096, K 2048: 6.8 (64 x 64 7.6)
+//   64 x 64:              64 x 4096, K 7168: 10.7 (64 x 128, 4 splits 12.3); 256 x 4096, K 4096: 8.4 (64 x 128 9.6)
+//   64 x 128, 3 stages:   200 x 5120, K 2880: 9.5 (64 x 64 11.1);    777 x 1234, K 2880: 10.3 (64 x 64 12.1)
 //   128 x 128, 4 stages:  512 x 7168, K 7168: 22.1 (64 x 128 26.0);  777 x 2880, K 4096: 13.9 (15.8 with 2 stages)
 //   128 x 128, 2 stages:  777 x 2880, K 1248: 7.8 (8.1 with 4);      1234 x 2880, K 800: 7.7 (64 x 128 8.6)
 //   256 x 128:            2048 x 4096, K 4096: 25.2 (128 x 128 26.8); 777 x 8192, K 8192: 41.1 (42.6)
@@ -470,10 +473,11 @@ void launch_tiles(const DgmMxfp4GemmArgs& A, int vec, int splits, hipStream_t st
 // the rate at which that many tokens can be multiplied with them (SwiGLU with a fragment each for gate and up rows:
 // 1.75 times the former, 1.35 times the rate).
 struct Form { int kind, splits; };
-enum { ROWS = 0, T64_128, T128_DEEP, T128, T256_128, T192_128, T192_256, T256 };
+enum { ROWS = 0, T64, T64_128, T128_DEEP, T128, T256_128, T192_128, T192_256, T256 };
 Form choose(int64_t m, int64_t n, int64_t k, bool swiglu, int64_t workspace_bytes) {
   static const struct { int bm, bn, per_cu; double around, alone, full, out; } tiles[] = {
-      {0, 0, 0, 0, 0, 0, 0},                {64, 128, 2, 4.3, 0.32, 0.75, 1.4},  {128, 128, 1, 4.8, 0.46, 0.68, 1.8}, {128, 128, 2, 4.2, 0.6, 1.14, 2.0},
+      {0, 0, 0, 0, 0, 0, 0},                {64, 64, 2, 4.6, 0.24, 0.48, 1.0},
+      {64, 128, 2, 4.3, 0.32, 0.75, 1.4},  {128, 128, 1, 4.8, 0.46, 0.68, 1.8}, {128, 128, 2, 4.2, 0.6, 1.14, 2.0},
       {256, 128, 1, 5.4, 0.77, 1.18, 1.4}, {192, 128, 1, 5.0, 0.63, 0.87, 1.5}, {192, 256, 1, 5.8, 1.11, 1.47, 1.6}, {256, 256, 1, 6.4, 1.36, 2.24, 0}};
   const int64_t steps = (k + 255) / 256;
   Form best = {ROWS, 1};
@@ -487,7 +491,7 @@ Form choose(int64_t m, int64_t n, int64_t k, bool swiglu, int64_t workspace_byte
     const double weights_us = (double)n * (double)k * 17 / 32 * 1e-6 / rate;
     least = 2.4 + (steps_us > weights_us ? steps_us : weights_us);
   }
-  for (int t = T64_128; t <= T256; ++t)
+  for (int t = swiglu ? T64_128 : T64; t <= T256; ++t)           // (64 x 64: a wave has 16 channels, so no gate and up rows)
     for (int s = 1; s <= 8; s *= 2) {
       if (s > 1 && (steps < 2 * s || (int64_t)s * m * n * 4 > workspace_bytes)) break;
       const int64_t wgs = ((m + tiles[t].bm - 1) / tiles[t].bm) * ((n + tiles[t].bn - 1) / tiles[t].bn) * s;
@@ -534,13 +538,15 @@ int dgm_mxfp4_gemm_nt(const DgmMxfp4GemmArgs* args, hipStream_t stream) {
   // (a launch has fewer than 2^32 threads; the smallest tile has 64 x 64 results and 256 of them)
   DGM_CHECK_ARG(((A.m + 63) / 64) * ((A.n + 63) / 64) < (1 << 23), "m n / 4096 below 2^23");
   const int e = A.dtype == DGM_SRC_F32 ? 4 : 2;
-  // 16-byte stores (and loads of C): 1, and past the caches where the results would only push other data out of the
+  // 16-byte stores (and loads of C), which need 4-byte alignment (777 x 1234, K 2880 with single elements instead: 12.3
+  // us, so 11.1): 1, and past the caches where the results would only push other data out of the
   // last one (256 MB): 2. 8192 x 8192, K 4096 (134 MB) 188 -> 176 us; but 8192 x 4096 (67 MB) 81 -> 86.
-  int vec = (((uintptr_t)A.d | (uintptr_t)A.c | (uint64_t)(A.d_stride * e) | (uint64_t)(A.c_stride * e)) & 15) == 0;
+  int vec = (((uintptr_t)A.d | (uintptr_t)A.c | (uint64_t)(A.d_stride * e) | (uint64_t)(A.c_stride * e)) & 3) == 0;
   if (vec && A.m * (A.swiglu ? A.n / 2 : A.n) * e >= 100000000) vec = 2;
   const int64_t held = A.workspace && ((uintptr_t)A.workspace & 15) == 0 ? A.workspace_bytes : 0;
   const Form f = choose(A.m, A.n, A.k, A.swiglu != 0, held < MOST_WORKSPACE ? held : MOST_WORKSPACE);
-  if (f.kind == T64_128) launch_tiles<64, 128, 2, 4, 3>(A, vec, f.splits, stream);
+  if (f.kind == T64) launch_tiles<64, 64, 2, 4, 4>(A, vec, f.splits, stream);
+  else if (f.kind == T64_128) launch_tiles<64, 128, 2, 4, 3>(A, vec, f.splits, stream);
   else if (f.kind == T128_DEEP) launch_tiles<128, 128, 2, 4, 4>(A, vec, f.splits, stream);
   else if (f.kind == T128) launch_tiles<128, 128, 2, 4, 2>(A, vec, f.splits, stream);
   else if (f.kind == T256_128) launch_tiles<256, 128, 4, 2, 3>(A, vec, f.splits, stream);
