@@ -1,5 +1,5 @@
 // A linear layer on MXFP4 products, host side: the launches of a forward or a backward pass behind one call (a training
-// step of a small layer is the host's time: seven calls of its parts from Python took 190 us, two take TIMES).
+// step of a small layer is the host's time: seven calls of its parts from Python took 190 us, two take 125 us).
 #include "dgm_abi_internal.hpp"
 
 namespace {

@@ -178,7 +178,7 @@ def test_large_means_and_constant_rows():
         assert bool(torch.isnan(h[1]).any()) and torch.equal(h[[0, 2]], clean[[0, 2]])
 
 
-@pytest.mark.parametrize("T,H", [(1, 1), (3, 33), (5, 40), (64, 7168), (70, 96), (2, 8200), (300, 2880), (4, 5001), (1, 16384)])
+@pytest.mark.parametrize("T,H", [(1, 1), (3, 33), (5, 40), (64, 7168), (70, 96), (2, 8200), (300, 2880), (258, 7168), (4, 5001), (1, 16384)])
 def test_mxfp4_rows(T, H):
     """Bit for bit mxfp4_quantize of the rounded h, in one launch or two."""
     need_gpu()
