@@ -138,13 +138,19 @@ __global__ void __launch_bounds__(512) k_mxfp4_gemm_rows(const DgmMxfp4GemmArgs 
 // More tokens: a workgroup computes BM tokens x BN channels over steps of 256 of K (128 bytes a row, whole lines).
 // Both operands' codes go from HBM / L2 straight into LDS, STAGES - 1 steps ahead of the one that is multiplied, with
 // one barrier a step. A row's eight 16-byte pieces (block 2 g + j at place 4 j + g) lie permuted by the row's number, so
-// that the lanes of a read meet different banks (at place 2 g + j half of the LDS cycles were conflicts). Scales take the way through registers, a row's 16 bytes for two
-// steps by one thread, a pair of steps ahead: any alignment.
+// that the lanes of a read meet different banks (at place 2 g + j half of the LDS cycles were conflicts). Scales take the
+// way through registers, a row's 16 bytes for two steps by one thread, a pair of steps ahead: any alignment.
 // Behind K a row's last piece stands in for the missing ones (any finite codes), under scale bytes of 0 in both
 // operands: 2^-127 each, so that such products are below 2^-240 and add nothing to an fp32 sum.
 // SwiGLU: blocks of 16 channel rows alternate between gate and up rows, so that a wave holds both of a channel.
 // Few tiles: gridDim.y workgroups share a tile, each a range of K, and leave their sums in the workspace
 // [split][token][channel] for k_mxfp4_gemm_join.
+// Bound: up to some hundred tokens the latency of a step (0.24 to 0.6 us, the loads' way from L2 and one barrier); of
+// large products the matrix units' rate on such data (6.6 PFLOP/s from registers, where the card's power holds the clock)
+// together with the results' stores: 8192 x 8192, K 4096 156 us (3.5 PFLOP/s), 143 without stores, on zeros 103.
+// In the compiler's own order, everything read first and accumulators in scratch memory, it took 343. Not faster:
+// 256 workgroups that loop over tiles and request the next one's first step ahead (192 -> 197; 8192 x 4096 78 -> 87),
+// whole 16-bit rows through LDS, four waves of 128 x 128 or sixteen of 64 x 64, fragments read three ahead.
 template <int BM, int BN, int WM, int WN, int STAGES, bool SWIGLU>
 __global__ void __launch_bounds__(64 * WM * WN) k_mxfp4_gemm_tiles(const DgmMxfp4GemmArgs P, int vec, int tiles_m, int tiles_n,
                                                                    int steps_per_split) {
@@ -376,7 +382,9 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mxfp4_gemm_tiles(const DgmMxfp
   }
 }
 
-// The splits' sums added in their order, then as the tiles' epilogue: a thread takes four channels of a token.
+// The splits' sums added in their order, then as the tiles' epilogue: a thread takes four channels of a token. A second
+// launch (3 to 4 us): a counter that lets the last workgroup join would have to be zero between calls, and two captured
+// graphs would share it.
 template <bool SWIGLU>
 __global__ void __launch_bounds__(256) k_mxfp4_gemm_join(const DgmMxfp4GemmArgs P, int vec, int splits) {
   const int64_t n_out = SWIGLU ? P.n / 2 : P.n, quads = (n_out + 3) / 4;
@@ -538,9 +546,9 @@ int dgm_mxfp4_gemm_nt(const DgmMxfp4GemmArgs* args, hipStream_t stream) {
   // (a launch has fewer than 2^32 threads; the smallest tile has 64 x 64 results and 256 of them)
   DGM_CHECK_ARG(((A.m + 63) / 64) * ((A.n + 63) / 64) < (1 << 23), "m n / 4096 below 2^23");
   const int e = A.dtype == DGM_SRC_F32 ? 4 : 2;
-  // 16-byte stores (and loads of C), which need 4-byte alignment (777 x 1234, K 2880 with single elements instead: 12.3
-  // us, so 11.1): 1, and past the caches where the results would only push other data out of the
-  // last one (256 MB): 2. 8192 x 8192, K 4096 (134 MB) 188 -> 176 us; but 8192 x 4096 (67 MB) 81 -> 86.
+  // 1: 16-byte stores (and loads of C), which need 4-byte alignment (777 x 1234, K 2880: 11.1 us, single elements 12.3).
+  // 2: past the caches too, where the results would only push other data out of the last one (256 MB): 8192 x 8192,
+  // K 4096 (134 MB) 188 -> 176 us; but 8192 x 4096 (67 MB) 81 -> 86.
   int vec = (((uintptr_t)A.d | (uintptr_t)A.c | (uint64_t)(A.d_stride * e) | (uint64_t)(A.c_stride * e)) & 3) == 0;
   if (vec && A.m * (A.swiglu ? A.n / 2 : A.n) * e >= 100000000) vec = 2;
   const int64_t held = A.workspace && ((uintptr_t)A.workspace & 15) == 0 ? A.workspace_bytes : 0;

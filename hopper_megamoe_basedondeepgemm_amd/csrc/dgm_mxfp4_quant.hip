@@ -19,36 +19,20 @@ DGM_DEV void load_piece(const DgmMxfp4QuantArgs& P, int64_t row, int64_t c, floa
   for (int i = 0; i < 8; ++i) v[i] = row < P.rows && c + i < P.cols ? load1<T>(P.x, row * P.x_stride + c + i) : 0.f;
 }
 
-// The same as loaded, without a branch (a load in one is awaited at its end): at `p`, which is inside the matrix, and
-// zeros if !some.
+// The same as loaded, without a branch (a load in one is awaited at its end).
 template <int T>
-struct RawPiece {
-  u4 w[T == T_F32 ? 2 : 1];
-  DGM_DEV void load(const char* p) {
-    w[0] = reinterpret_cast<const u4*>(p)[0];
-    if constexpr (T == T_F32) w[1] = reinterpret_cast<const u4*>(p)[1];
-  }
+struct RawPiece : Piece<T> {
+  using Piece<T>::w;
   DGM_DEV void clear_unless(bool some) {
     const u4 none = {0u, 0u, 0u, 0u};
     w[0] = some ? w[0] : none;
     if constexpr (T == T_F32) w[1] = some ? w[1] : none;
   }
-  DGM_DEV void unpack(float* v) const {
-    if constexpr (T == T_F32) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t d = w[k / 4][k % 4];
-        v[k] = __uint_as_float(d);
-      }
-    } else {
-      unpack8<T>(w[0], v);
-    }
-  }
   // the largest magnitude's fp32 bits
   DGM_DEV uint32_t magnitude() const {
     if constexpr (T == T_F32) {
       float v[8];
-      unpack(v);
+      this->unpack(v);
       return magnitude8(v);
     } else {
       uint32_t m = 0;
@@ -58,11 +42,17 @@ struct RawPiece {
     }
   }
 };
-template <int T>
-constexpr int SIZE = T == T_F32 ? 4 : 2;
+// Where a row's eight elements from column c on are loaded: at c, or where they do not all exist (rows of eight
+// elements at least) at the row's last eight, which are then shifted by `by`.
+struct Place {
+  int64_t at;
+  int by;
+  DGM_DEV Place(int64_t c, int64_t cols) : at(c + 8 <= cols ? c : cols - 8), by((int)min(c - at, (int64_t)8)) {}
+};
 
-// Rows: a thread takes eight values, four neighbours a block. 2^log_row threads a row of the workgroup, `runs`
-// workgroups along a row.
+// Rows: a thread takes eight values, four neighbours a block, whose maximum goes by lane exchange; nothing is kept
+// between threads, so the loads of many waves are in flight (bf16 8192 x 4096: 15.2 us, 5.6 TB/s). 2^log_row threads a
+// row of the workgroup, `runs` workgroups along a row.
 template <int T, bool VEC>
 __global__ void __launch_bounds__(256) k_mxfp4_rows(const DgmMxfp4QuantArgs P, int log_row, int runs) {
   const int64_t group = blockIdx.x / (unsigned)runs;
@@ -73,10 +63,16 @@ __global__ void __launch_bounds__(256) k_mxfp4_rows(const DgmMxfp4QuantArgs P, i
   if (row >= P.rows || piece >= 4 * blocks) return;           // (whole blocks: four lanes share one)
   float v[8];
   uint32_t m;
-  if constexpr (VEC) {
+  const bool some = piece * 8 < P.cols;
+  if (VEC || P.cols >= 8) {
     RawPiece<T> raw;
-    const bool some = piece * 8 < P.cols;
-    raw.load(reinterpret_cast<const char*>(P.x) + (row * P.x_stride + (some ? piece * 8 : 0)) * SIZE<T>);
+    if constexpr (VEC) {
+      raw.load(P.x, row * P.x_stride + (some ? piece * 8 : 0));
+    } else {
+      const Place place(piece * 8, P.cols);
+      raw.load_loose(P.x, row * P.x_stride + place.at);
+      raw.shift(place.by);
+    }
     raw.clear_unless(some);
     raw.unpack(v);
     m = raw.magnitude();
@@ -91,7 +87,11 @@ __global__ void __launch_bounds__(256) k_mxfp4_rows(const DgmMxfp4QuantArgs P, i
 
 // Columns, and rows with them (BOTH): a tile of R rows x 128 columns is read once, its rows' codes are made on the
 // way into LDS, and a thread then takes 32 rows of a column (16 bits: of two, a dword a row). The columns' codes meet in
-// LDS again, so that what is stored for a column lies together (64 bytes; fp32 32).
+// LDS again, so that what is stored for a column lies together (64 bytes; fp32 32). All of a tile's loads are requested
+// before the first is used (with a branch around each, awaited at its end, columns took 20.2 us and both 33.8).
+// bf16 8192 x 4096: columns 15.1 us, 5.6 TB/s; both 26.9, 3.8 TB/s: each value is rounded twice, and the vector units are
+// as busy as memory. An order of tiles by XCD is no faster (27.8). Rows off 16 bytes are loaded on the elements'
+// alignment (777 x 1234: columns 4.0 us, both 5.9; by single elements 8.3 and 10.1).
 template <int T, bool VEC, bool BOTH>
 __global__ void __launch_bounds__(256) k_mxfp4_columns(const DgmMxfp4QuantArgs P, int tiles_c) {
   constexpr int R = T == T_F32 ? 64 : 128, C = 128, B = R / 32, PAIR = T == T_F32 ? 1 : 2;
@@ -108,11 +108,22 @@ __global__ void __launch_bounds__(256) k_mxfp4_columns(const DgmMxfp4QuantArgs P
   const int at = (threadIdx.x & 15) * 8, first = threadIdx.x >> 4;
   const int most = (int)min(P.rows - r0, (int64_t)R) - 1;              // last row of the tile
   const bool inside = c0 + at < P.cols;
-  RawPiece<T> raw[VEC ? R / 16 : 1];             // (all requested before the first is used)
-  if constexpr (VEC) {
-    const char* from = reinterpret_cast<const char*>(P.x) + (r0 * P.x_stride + (inside ? c0 + at : 0)) * SIZE<T>;
+  const bool pieces = VEC || P.cols >= 8;
+  RawPiece<T> raw[R / 16];                       // (all requested before the first is used)
+  int by = 0;
+  if (pieces) {
+    int64_t from = r0 * P.x_stride + (inside ? c0 + at : 0);
+    if constexpr (!VEC) {
+      const Place place(c0 + at, P.cols);
+      from = r0 * P.x_stride + place.at;
+      by = place.by;
+    }
 #pragma unroll
-    for (int i = 0; i < R / 16; ++i) raw[i].load(from + (int64_t)min(i * 16 + first, most) * P.x_stride * SIZE<T>);
+    for (int i = 0; i < R / 16; ++i) {
+      const int64_t place = from + (int64_t)min(i * 16 + first, most) * P.x_stride;
+      if constexpr (VEC) raw[i].load(P.x, place);
+      else raw[i].load_loose(P.x, place);
+    }
   }
   const int64_t piece = (c0 + at) / 8;
   uint32_t* const row_codes = reinterpret_cast<uint32_t*>(P.codes) + r0 * row_blocks * 4 + piece;
@@ -122,7 +133,8 @@ __global__ void __launch_bounds__(256) k_mxfp4_columns(const DgmMxfp4QuantArgs P
     const int r = i * 16 + first;
     float v[8];
     uint32_t m;
-    if constexpr (VEC) {
+    if (pieces) {
+      if constexpr (!VEC) raw[i].shift(by);
       raw[i].clear_unless(inside && r <= most);
       u4* to = reinterpret_cast<u4*>(&tile[r][at]);
       to[0] = raw[i].w[0];

@@ -59,6 +59,51 @@ struct Row {
   }
 };
 
+// The same elements as Row<NV, THREADS, true> holds, of rows of any length at any alignment: 16 bytes at a time on the
+// elements' alignment, a row's last piece from its last eight elements.
+template <int NV, int THREADS>
+struct LooseRow : Row<NV, THREADS, true> {
+  template <int T>
+  static DGM_DEV void load(const void* p, int64_t off, int H, float* v) {
+    if (H < 8) {                                   // (thread 0's alone)
+#pragma unroll
+      for (int k = 0; k < 8 * NV; ++k) v[k] = LooseRow::index(k) < H ? load1<T>(p, off + LooseRow::index(k)) : 0.f;
+      return;
+    }
+    Piece<T> piece[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) piece[j].load_loose(p, off + min(LooseRow::index(8 * j), H - 8));
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = LooseRow::index(8 * j);
+      piece[j].shift(min(max(i - (H - 8), 0), 7));
+      piece[j].unpack(v + 8 * j);
+      if (i >= H)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[8 * j + k] = 0.f;
+    }
+  }
+  template <int T>
+  static DGM_DEV void store(void* p, int64_t off, int H, const float* v) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = LooseRow::index(8 * j);
+      if (i + 8 <= H) {
+        store8_loose<T>(p, off + i, v + 8 * j);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (i + k < H) store1<T>(p, off + i + k, v[8 * j + k]);
+      }
+    }
+  }
+  template <int T>
+  static DGM_DEV void weight(const void* p, bool f32, int H, float* v) {
+    if (f32) load<T_F32>(p, 0, H, v);
+    else load<T>(p, 0, H, v);
+  }
+};
+
 // Workgroup reductions of up to two values, in a fixed order, one barrier each. Two LDS sets taken in
 // turn: a set is written again only after the barrier of the other one, which a wave reaches after it
 // has read the first. Behind the barrier every lane takes a wave's value and they meet by lane exchange (each

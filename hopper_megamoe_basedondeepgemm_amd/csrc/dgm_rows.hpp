@@ -72,6 +72,71 @@ DGM_DEV void store8(void* p, int64_t i, const float* v) {
   }
 }
 
+// Eight consecutive elements as they lie in memory.
+typedef uint32_t loose_u4 __attribute__((ext_vector_type(4), aligned(2)));
+template <int T>
+struct Piece {
+  u4 w[T == T_F32 ? 2 : 1];
+  static constexpr int SIZE = T == T_F32 ? 4 : 2;
+  // from element i on: on 16 bytes, or on an element's alignment
+  DGM_DEV void load(const void* p, int64_t i) {
+    const u4* q = reinterpret_cast<const u4*>(reinterpret_cast<const char*>(p) + i * SIZE);
+    w[0] = q[0];
+    if constexpr (T == T_F32) w[1] = q[1];
+  }
+  DGM_DEV void load_loose(const void* p, int64_t i) {
+    const loose_u4* q = reinterpret_cast<const loose_u4*>(reinterpret_cast<const char*>(p) + i * SIZE);
+    w[0] = q[0];
+    if constexpr (T == T_F32) w[1] = q[1];
+  }
+  // drops the first `by` elements (0 to 7), zeros behind the last
+  DGM_DEV void shift(int by) {
+    if (by == 0) return;
+    if constexpr (T == T_F32) {
+      auto drop = [&](bool some, int n) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t from = k + n < 8 ? w[(k + n) / 4 % 2][(k + n) % 4] : 0u;
+          if (some) w[k / 4][k % 4] = from;
+        }
+      };
+      drop(by & 4, 4);
+      drop(by & 2, 2);
+      drop(by & 1, 1);
+    } else {
+      if (by & 4) w[0] = u4{w[0][2], w[0][3], 0u, 0u};
+      if (by & 2) w[0] = u4{w[0][1], w[0][2], w[0][3], 0u};
+      if (by & 1)
+        w[0] = u4{w[0][0] >> 16 | w[0][1] << 16, w[0][1] >> 16 | w[0][2] << 16, w[0][2] >> 16 | w[0][3] << 16, w[0][3] >> 16};
+    }
+  }
+  DGM_DEV void unpack(float* v) const {
+    if constexpr (T == T_F32) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t d = w[k / 4][k % 4];
+        v[k] = __uint_as_float(d);
+      }
+    } else {
+      unpack8<T>(w[0], v);
+    }
+  }
+};
+// eight elements at an element's alignment, rounded to nearest even
+template <int T>
+DGM_DEV void store8_loose(void* p, int64_t i, const float* v) {
+  if constexpr (T == T_F32) {
+    loose_u4* q = reinterpret_cast<loose_u4*>(reinterpret_cast<float*>(p) + i);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      q[h] = u4{__float_as_uint(v[4 * h]), __float_as_uint(v[4 * h + 1]), __float_as_uint(v[4 * h + 2]), __float_as_uint(v[4 * h + 3])};
+  } else {
+    u4 w;
+    store8<T>(&w, 0, v);
+    *reinterpret_cast<loose_u4*>(reinterpret_cast<uint16_t*>(p) + i) = w;
+  }
+}
+
 // Sum and maximum over the 64 lanes (all active), in every lane, in a fixed order.
 DGM_DEV float wave_sum(float v) {
   v += dpp_f32<0xB1>(v);        // quad_perm [1,0,3,2]

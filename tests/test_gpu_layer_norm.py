@@ -231,6 +231,36 @@ def test_strides_and_outputs(dtype):
     assert torch.equal(dgm.layer_norm_residual(x, r, wide, b, 0.5)[1], want[1])
 
 
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("left", [1, 2, 8])
+def test_rows_of_any_length_between_others(dtype, left):
+    """Rows that start and end anywhere, beside NaN that no row may read and values that none may write over."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    for H in (1, 2, 5, 7, 8, 9, 10, 11, 12, 13, 14, 15, 16, 31, 511, 513, 1027, 8193, 9001):
+        x, r, w, b, dr, dh = make(3, H, dtype, dtype, seed=H)
+        f = Form(x, r, w, b, 0.5)
+
+        def within(t, fill):
+            big = torch.full((5, H + left + 9), fill, dtype=dtype, device="cuda")
+            view = big[1:4, left:left + H]
+            view.copy_(t)
+            return view, big
+        xs, rs, drs, dhs = (within(t, float("nan"))[0] for t in (x, r, dr, dh))
+        ws, bs = (torch.full((H + left + 9,), float("nan"), dtype=dtype, device="cuda")[left:left + H].copy_(t) for t in (w, b))
+        (o1, all1), (o2, all2) = within(torch.zeros_like(x), 5.0), within(torch.zeros_like(x), 5.0)
+        dgm.layer_norm_residual(xs, rs, ws, bs, 0.5, residual_out=o1, out=o2)
+        close(o1, f.t, f.t_mag, 128)
+        close(o2, f.h, f.h_mag, 128)
+        for o, big in ((o1, all1), (o2, all2)):
+            o.fill_(5.0)
+            assert bool((big == 5.0).all()), H
+        back = dgm.layer_norm_residual_backward(drs, dhs, xs, rs, *dgm.layer_norm_residual_forward(xs, rs, ws, bs, 0.5)[2:], ws, bs, 0.5)
+        want = f.grads(dr, dh)
+        for t, name in zip(back, ("x", "residual", "weight", "bias")):
+            close(t, *want[name], 384 + (3 if name in ("weight", "bias") else 0))
+
+
 def test_shared_leaves_no_rows_and_offsets():
     need_gpu()
     import hopper_megamoe_basedondeepgemm_amd as dgm

@@ -99,6 +99,24 @@ def test_quantize_strides(dtype):
 
 
 @pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("left", [1, 2, 8])
+def test_quantize_rows_of_any_length_between_others(dtype, left):
+    """Rows that start and end anywhere, beside NaN that no block may see."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    for n in (*range(1, 26), 31, 33, 97, 127, 129, 1021):
+        big = torch.full((140, n + left + 9), float("nan"), dtype=dtype, device="cuda")
+        x = big[3:136, left:left + n]
+        x.copy_(rows(133, n, dtype, seed=n))
+        want = quantized(x), quantized(x.t())
+        same(dgm.mxfp4_quantize(x), want[0])
+        got = dgm.mxfp4_quantize_both(x)
+        same(got[0], want[0])
+        same(got[1], want[1])
+        same(dgm.mxfp4_quantize(x, transpose=True), want[1])
+
+
+@pytest.mark.parametrize("dtype", DT)
 def test_quantize_every_value_beside_a_midpoint(dtype):
     """Midpoints and the numbers next to them in the type, under scales from the type's smallest to its largest."""
     need_gpu()
