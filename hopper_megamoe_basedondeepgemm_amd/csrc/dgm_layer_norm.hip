@@ -10,6 +10,8 @@
 #include "dgm_mxfp4.hpp"
 #include "dgm_row_tiles.hpp"
 
+#include <algorithm>
+
 using namespace dgm;
 
 namespace {
@@ -18,9 +20,10 @@ namespace {
 DGM_DEV float total(float r, float s, float x) { return fmaf(s, x, r); }
 
 // Forward: one read of x and residual, one write of r and h; two sums over the row one behind the other (the variance
-// waits for the mean, which costs the second exchange but no cancellation). bf16 8192 x 4096: 45.2 us, 5.9 TB/s; fp32
-// 4096 x 4096: 46; 2048 x 16384: 50. Rows off 16 bytes are loaded on the elements' alignment: 4096 x 5001 47.6 us, 3.5
-// TB/s (by single elements 70).
+// waits for the mean, which costs the second exchange but no cancellation). Over data that no cache holds: bf16
+// 8192 x 4096 48.2 us, 5.6 TB/s; fp32 8192 x 2880 73.5; rows off 16 bytes are loaded on the elements' alignment: 4096 x
+// 5001 47.6 us, 3.5 TB/s (by single elements 70). Requesting the residual and the weights with x is slower there (51.2).
+// Rows of one wave: four of them a workgroup are no faster (100 000 x 256 56 us, one 54; half its lanes have no elements).
 template <int T, int NV, int THREADS, bool VEC>
 __global__ void __launch_bounds__(THREADS) k_layer_norm_fwd(const DgmLayerNormArgs P) {
   using R = std::conditional_t<VEC, Row<NV, THREADS, true>, LooseRow<NV, THREADS>>;
@@ -32,36 +35,9 @@ __global__ void __launch_bounds__(THREADS) k_layer_norm_fwd(const DgmLayerNormAr
   const bool wf = P.weights_f32;
   const float inv_h = 1.0f / (float)H;
   float t[N], w[N];
-  // Rows of eight 16-bit elements a thread: everything is requested at the start, so that a row waits for memory once
-  // (100 000 bf16 rows of 256: 37 us instead of 48; 8192 rows of 4096: 45.2 instead of 46.3). fp32 rows would lose:
-  // 8192 of 2880 72 us instead of 69.
-  constexpr bool EARLY = VEC && NV == 1 && T != T_F32;
-  HeldRow hx, hr, hw, hb;
-  if constexpr (EARLY) {
-    hx.load<T>(P.x, row * P.x_stride, H);
-    if (P.residual) hr.load<T>(P.residual, row * P.residual_stride, H);
-    auto weights = [&](const void* p, HeldRow& held) {
-      if (wf) held.load<T_F32>(p, 0, H);
-      else held.load<T>(p, 0, H);
-    };
-    if (P.weight) weights(P.weight, hw);
-    if (P.bias) weights(P.bias, hb);
-  }
-  auto get = [&](const HeldRow& held, const void* p, int64_t off, float* v) {
-    if constexpr (EARLY) held.unpack<T>(v);
-    else R::template load<T>(p, off, H, v);
-  };
-  auto get_weight = [&](const HeldRow& held, const void* p) {
-    if constexpr (EARLY) {
-      if (wf) held.unpack<T_F32>(w);
-      else held.unpack<T>(w);
-    } else {
-      R::template weight<T>(p, wf, H, w);
-    }
-  };
-  get(hx, P.x, row * P.x_stride, t);
+  R::template load<T>(P.x, row * P.x_stride, H, t);
   if (P.residual) {
-    get(hr, P.residual, row * P.residual_stride, w);
+    R::template load<T>(P.residual, row * P.residual_stride, H, w);
 #pragma unroll
     for (int k = 0; k < N; ++k) t[k] = total(w[k], P.residual_scale, t[k]);
   } else {
@@ -86,12 +62,12 @@ __global__ void __launch_bounds__(THREADS) k_layer_norm_fwd(const DgmLayerNormAr
 #pragma unroll
   for (int k = 0; k < N; ++k) t[k] *= rstd;
   if (P.weight) {
-    get_weight(hw, P.weight);
+    R::template weight<T>(P.weight, wf, H, w);
 #pragma unroll
     for (int k = 0; k < N; ++k) t[k] *= w[k];
   }
   if (P.bias) {
-    get_weight(hb, P.bias);
+    R::template weight<T>(P.bias, wf, H, w);
 #pragma unroll
     for (int k = 0; k < N; ++k) t[k] += w[k];
   }
@@ -115,8 +91,8 @@ __global__ void __launch_bounds__(THREADS) k_layer_norm_fwd(const DgmLayerNormAr
 
 // Gradients: workgroup g takes rows g, g + G, ...; the columns' sums over its rows stay in registers and go to
 // partial[set][g][H] (set 0 weight, 1 bias), which k_layer_norm_columns adds up in a fixed order: atomics would give
-// another order every time. Both sums (du and du u) meet in one exchange. bf16 8192 x 4096, five tensors of rows: 85 us
-// with the column sums, 4.8 TB/s; fp32 4096 x 4096: 84; beyond hidden 8192 some registers go to scratch memory (2048 x
+// another order every time. Both sums (du and du u) meet in one exchange. bf16 8192 x 4096, five tensors of rows: 81 us
+// with the column sums, 5.0 TB/s; fp32 4096 x 4096: 84; beyond hidden 8192 some registers go to scratch memory (2048 x
 // 16384: 107 us, 3.8 TB/s); off 16 bytes 4096 x 5001: 84, 2.9 TB/s (by single elements 186).
 template <int T, int NV, int THREADS, bool VEC>
 __global__ void __launch_bounds__(THREADS) k_layer_norm_bwd(const DgmLayerNormGradArgs P) {
@@ -131,8 +107,8 @@ __global__ void __launch_bounds__(THREADS) k_layer_norm_bwd(const DgmLayerNormGr
 #pragma unroll
   for (int k = 0; k < N; ++k) dw[k] = db[k] = 0.f;
   // Rows of eight 16-bit elements a thread: the next row is requested before the current one is worked on, and the weight
-  // stays in registers (100 000 bf16 rows of 256: 67 us instead of 101; 4096 rows of 7168: 72 instead of 82; 8192 of 4096:
-  // 84.6 instead of 88.6). Sixteen elements, or fp32 ones, are too many for two rows (fp32 8192 rows of 2880: 112 us
+  // stays in registers (100 000 bf16 rows of 256: 70 us instead of 103; 4096 rows of 7168: 74 instead of 84; 8192 of 4096:
+  // 85 instead of 90). Sixteen elements, or fp32 ones, are too many for two rows (fp32 8192 rows of 2880: 112 us
   // without, 116 with).
   constexpr bool AHEAD = VEC && NV == 1 && T != T_F32;
   HeldRow hx, hr, hd, hg;
@@ -295,8 +271,8 @@ int dgm_layer_norm_residual(const DgmLayerNormArgs* args, hipStream_t stream) {
                          dim3(threads.value), 0, stream, A);
     };
     // Many 16-bit rows of 4096 < hidden <= 8192: 512 threads of sixteen elements. Two workgroups of 1024 fill a CU and wait
-    // together at their sums, four of 512 less so (4096 rows of 7168: 42.5 us instead of 45.0). Up to 4096 eight elements
-    // a thread are as fast or faster (8192 rows of 4096: 45.2, sixteen 46.7), and few rows want the shorter wait.
+    // together at their sums, four of 512 less so (4096 rows of 7168: 45.7 us instead of 47.0). Up to 4096 eight elements
+    // a thread are as fast (8192 rows of 4096: 48.2, sixteen 48.4), and few rows want the shorter wait.
     if constexpr (v.value && t.value != T_F32) {
       if (A.rows > 256 && A.hidden > 4096 && A.hidden <= 8192)
         return launch(std::integral_constant<int, 2>{}, std::integral_constant<int, 512>{});
@@ -308,8 +284,11 @@ int dgm_layer_norm_residual(const DgmLayerNormArgs* args, hipStream_t stream) {
 
 // As many workgroups as the CUs hold (16 waves each), a row each at least.
 int dgm_layer_norm_residual_groups(int64_t rows, int hidden) {
-  int64_t most = 4096;
+  // Two rows a workgroup at least: its column sums are as many bytes as two 16-bit rows, written and read again (300 x
+  // 4096 15.0 us with one, 11.9; 64 x 7168 10.2 and 10.4). And no more than the CUs hold at a time.
+  int64_t most = 0;
   dispatch_hidden(hidden, [&](auto, auto threads) { most = 4096 / (threads.value / 64); });
+  rows = (rows + 1) / 2;
   return (int)(rows < 1 ? 1 : rows < most ? rows : most);
 }
 
@@ -319,7 +298,7 @@ int dgm_layer_norm_residual_backward(const DgmLayerNormGradArgs* args, hipStream
   const DgmLayerNormArgs& F = A.forward;
   if (int st = check_forward(&F)) return st;
   const bool columns = A.d_weight || A.d_bias;
-  const int groups = dgm_layer_norm_residual_groups(F.rows, F.hidden);
+  int groups = dgm_layer_norm_residual_groups(F.rows, F.hidden);
   if (F.rows > 0) {
     DGM_CHECK_ARG(!A.d_h || (F.mean && F.rstd), "mean and rstd of the forward pass");
     DGM_CHECK_ARG(!A.d_residual || F.residual, "d_residual without a residual");
@@ -333,6 +312,11 @@ int dgm_layer_norm_residual_backward(const DgmLayerNormGradArgs* args, hipStream
   const bool vec = forward_aligned(&F) && aligned(A.d_residual_out, A.d_residual_out_stride, e) &&
                    aligned(A.d_h, A.d_h_stride, e) && aligned(A.d_x, A.d_x_stride, e) &&
                    aligned(A.d_residual, A.d_residual_stride, e);
+  // Rows requested ahead need half the waves, at least a workgroup a CU (bf16 8192 x 4096 80.5 us, twice as many groups
+  // 85, half as many 100; 4096 x 2048 23.4 and 26; 4096 x 7168 with 128 groups 90, 256 74.5); others all they can have
+  // (fp32 8192 x 2880 112 us, half 122).
+  if (vec && F.dtype != DGM_SRC_F32 && F.hidden <= 8192)
+    dispatch_hidden(F.hidden, [&](auto, auto threads) { groups = std::min(groups, std::max(2048 / (threads.value / 64), 256)); });
   // (no rows: the partial sums of the one group are written as zeros)
   dispatch_type(F.dtype, vec, [&](auto t, auto v) {
     dispatch_hidden(F.hidden, [&](auto nv, auto threads) {
