@@ -51,7 +51,8 @@ struct Place {
 };
 
 // Rows: a thread takes eight values, four neighbours a block, whose maximum goes by lane exchange; nothing is kept
-// between threads, so the loads of many waves are in flight (bf16 8192 x 4096: 15.2 us, 5.6 TB/s). 2^log_row threads a
+// between threads, so the loads of many waves are in flight (bf16 8192 x 4096, from the last cache: 15.2 us, 5.6 TB/s; 8192 x 7168 from HBM:
+// 28.3 us, 5.2 TB/s). 2^log_row threads a
 // row of the workgroup, `runs` workgroups along a row.
 template <int T, bool VEC>
 __global__ void __launch_bounds__(256) k_mxfp4_rows(const DgmMxfp4QuantArgs P, int log_row, int runs) {
