@@ -8,6 +8,8 @@
 #include "dgm_mxfp4.hpp"
 #include "dgm_row_tiles.hpp"
 
+#include <algorithm>
+
 using namespace dgm;
 
 namespace {
@@ -51,13 +53,13 @@ struct Place {
 };
 
 // Rows: a thread takes eight values, four neighbours a block, whose maximum goes by lane exchange; nothing is kept
-// between threads, so the loads of many waves are in flight (bf16 8192 x 4096, from the last cache: 15.2 us, 5.6 TB/s; 8192 x 7168 from HBM:
-// 28.3 us, 5.2 TB/s). 2^log_row threads a
-// row of the workgroup, `runs` workgroups along a row.
+// between threads, so the loads of many waves are in flight (bf16 8192 x 4096, from the last cache: 15.2 us, 5.6 TB/s;
+// 8192 x 7168 from HBM: 28.3 us, 5.2 TB/s). 2^log_row threads a row of the workgroup, `runs` workgroups along a row.
 template <int T, bool VEC>
 __global__ void __launch_bounds__(256) k_mxfp4_rows(const DgmMxfp4QuantArgs P, int log_row, int runs) {
-  const int64_t group = blockIdx.x / (unsigned)runs;
-  const int run = (int)(blockIdx.x - group * runs);
+  const uint32_t id = blockIdx.y * gridDim.x + blockIdx.x;       // (the last of gridDim.y may be behind the last row)
+  const int64_t group = id / (unsigned)runs;
+  const int run = (int)(id - group * runs);
   const int64_t row = (group << (8 - log_row)) + (threadIdx.x >> log_row);
   const int64_t piece = ((int64_t)run << log_row) + (threadIdx.x & ((1 << log_row) - 1));
   const int64_t blocks = (P.cols + 31) / 32;
@@ -234,14 +236,18 @@ int dgm_mxfp4_quantize(const DgmMxfp4QuantArgs* args, hipStream_t stream) {
   const int64_t groups = (A.rows + (256 >> log_row) - 1) >> (8 - log_row);
   const int tile_rows = A.dtype == DGM_SRC_F32 ? 64 : 128;
   const int64_t tiles_c = (A.cols + 127) / 128, tiles_r = (A.rows + tile_rows - 1) / tile_rows;
-  DGM_CHECK_ARG((A.t_codes ? tiles_c * tiles_r : groups * runs) < (1 << 24), "a launch has fewer than 2^32 threads");
+  DGM_CHECK_ARG(A.t_codes ? tiles_c * tiles_r < (1 << 24) : groups * runs < ((int64_t)1 << 32) - (1 << 23), "too many workgroups");
+  // (a launch has fewer than 2^32 threads along a grid's axis)
+  const unsigned grid_x = (unsigned)std::min(groups * runs, (int64_t)1 << 23);
   dispatch_type(A.dtype, vec, [&](auto t, auto v) {
+    const unsigned tiles = (unsigned)(tiles_c * tiles_r);
     if (!A.t_codes)
-      hipLaunchKernelGGL((k_mxfp4_rows<t.value, v.value>), dim3((unsigned)(groups * runs)), dim3(256), 0, stream, A, log_row, runs);
+      hipLaunchKernelGGL((k_mxfp4_rows<t.value, v.value>), dim3(grid_x, (unsigned)((groups * runs + grid_x - 1) / grid_x)), dim3(256), 0, stream,
+                         A, log_row, runs);
     else if (A.codes)
-      hipLaunchKernelGGL((k_mxfp4_columns<t.value, v.value, true>), dim3((unsigned)(tiles_c * tiles_r)), dim3(256), 0, stream, A, (int)tiles_c);
+      hipLaunchKernelGGL((k_mxfp4_columns<t.value, v.value, true>), dim3(tiles), dim3(256), 0, stream, A, (int)tiles_c);
     else
-      hipLaunchKernelGGL((k_mxfp4_columns<t.value, v.value, false>), dim3((unsigned)(tiles_c * tiles_r)), dim3(256), 0, stream, A, (int)tiles_c);
+      hipLaunchKernelGGL((k_mxfp4_columns<t.value, v.value, false>), dim3(tiles), dim3(256), 0, stream, A, (int)tiles_c);
   });
   return dgm_last_launch_status();
 }

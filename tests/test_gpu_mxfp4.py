@@ -536,3 +536,16 @@ def test_linear_no_tokens_and_refusals():
     with pytest.raises(RuntimeError, match="under graph capture"):
         with torch.cuda.graph(graph):
             dgm.mxfp4_linear(x, w)
+
+
+def test_quantize_more_workgroups_than_one_axis():
+    """2^23 and more workgroups: one row repeated, so that its codes are known."""
+    need_gpu()
+    import hopper_megamoe_basedondeepgemm_amd as dgm
+    x = rows(1, 2048, torch.bfloat16, seed=4)
+    want = quantized(x)
+    n = (1 << 23) + 3
+    codes, scales = dgm.mxfp4_quantize(x.expand(n, 2048))
+    for part in (codes[:2], codes[-5:], codes[(1 << 23) - 2:]):
+        assert bool((part == want[0]).all())
+    assert bool((codes.view(torch.int64) == want[0].view(torch.int64)).all()) and bool((scales == want[1]).all())
