@@ -236,7 +236,7 @@ int dgm_mxfp4_quantize(const DgmMxfp4QuantArgs* args, hipStream_t stream) {
   const int64_t groups = (A.rows + (256 >> log_row) - 1) >> (8 - log_row);
   const int tile_rows = A.dtype == DGM_SRC_F32 ? 64 : 128;
   const int64_t tiles_c = (A.cols + 127) / 128, tiles_r = (A.rows + tile_rows - 1) / tile_rows;
-  DGM_CHECK_ARG(A.t_codes ? tiles_c * tiles_r < (1 << 24) : groups * runs < ((int64_t)1 << 32) - (1 << 23), "too many workgroups");
+  DGM_CHECK_ARG(A.t_codes ? tiles_c * tiles_r < (1 << 24) : groups * runs < ((int64_t)1 << 32) - (1 << 23), "a launch has fewer than 2^32 threads (rows alone: workgroups)");
   // (a launch has fewer than 2^32 threads along a grid's axis)
   const unsigned grid_x = (unsigned)std::min(groups * runs, (int64_t)1 << 23);
   dispatch_type(A.dtype, vec, [&](auto t, auto v) {
