@@ -151,6 +151,8 @@ __global__ void __launch_bounds__(512) k_mxfp4_gemm_rows(const DgmMxfp4GemmArgs 
 // In the compiler's own order, everything read first and accumulators in scratch memory, it took 343. Not faster:
 // 256 workgroups that loop over tiles and request the next one's first step ahead (192 -> 197; 8192 x 4096 78 -> 87),
 // whole 16-bit rows through LDS, four waves of 128 x 128 or sixteen of 64 x 64, fragments read three ahead.
+// Eight waves a tile: with four, tiles of 128 x 128 wait longer for each step (8192 x 512, K 7168 23.6 -> 37; 777 x 5120,
+// K 7168 by 192 x 128 25.5 -> 46); sixteen are 1 to 5 % slower.
 template <int BM, int BN, int WM, int WN, int STAGES, bool SWIGLU>
 __global__ void __launch_bounds__(64 * WM * WN) k_mxfp4_gemm_tiles(const DgmMxfp4GemmArgs P, int vec, int tiles_m, int tiles_n,
                                                                    int steps_per_split) {
