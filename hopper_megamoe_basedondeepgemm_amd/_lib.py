@@ -39,7 +39,7 @@ EXPORTS = [
     "dgm_layer_norm_residual", "dgm_layer_norm_residual_groups", "dgm_layer_norm_residual_backward",
     "dgm_layer_norm_struct_sizes", "dgm_mxfp4_quantize", "dgm_mxfp4_quant_struct_size", "dgm_mxfp4_gemm_nt",
     "dgm_mxfp4_gemm_struct_size", "dgm_mxfp4_gemm_workspace_bytes", "dgm_mxfp4_linear", "dgm_mxfp4_linear_backward",
-    "dgm_mxfp4_linear_workspace_bytes", "dgm_mxfp4_linear_struct_size",
+    "dgm_mxfp4_linear_workspace_bytes", "dgm_mxfp4_linear_struct_size", "dgm_mxfp4_gemm_form",
 ]
 # source element types of the weight packers (DGM_SRC_*)
 SRC_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -227,6 +227,7 @@ def load():
     sig["dgm_mxfp4_quant_struct_size"] = ([ctypes.POINTER(ctypes.c_size_t)], i32)
     sig["dgm_mxfp4_gemm_nt"] = ([ctypes.POINTER(Mxfp4GemmArgs), vp], i32)
     sig["dgm_mxfp4_gemm_workspace_bytes"] = ([i64, i64, i64, i32], i64)
+    sig["dgm_mxfp4_gemm_form"] = ([i64, i64, i64, i32, i64, vp], i32)
     sig["dgm_mxfp4_gemm_struct_size"] = ([ctypes.POINTER(ctypes.c_size_t)], i32)
     sig["dgm_mxfp4_linear"] = ([ctypes.POINTER(Mxfp4LinearArgs), vp], i32)
     sig["dgm_mxfp4_linear_backward"] = ([ctypes.POINTER(Mxfp4LinearArgs), vp], i32)

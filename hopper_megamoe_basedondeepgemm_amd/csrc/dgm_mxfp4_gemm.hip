@@ -13,6 +13,8 @@
 #include "dgm_abi_internal.hpp"
 #include "dgm_epilogue.hpp"
 
+#include <algorithm>
+
 using namespace dgm;
 
 namespace {
@@ -427,33 +429,56 @@ Rows rows_form(int64_t m, int64_t n, int64_t k, bool swiglu) {
   return {parts, 16 / parts / (one ? 2 : 1), k % 512 == 0 || k >= 4096 ? 4 : 2};
 }
 
+// Threads of a tile's workgroup.
+constexpr int TILE_THREADS = 512;
+
+// A launch, or with `told` not the launch but what it would be (dgm_mxfp4_gemm_form).
+struct Launch {
+  int vec;
+  hipStream_t stream;
+  int64_t* told;
+};
+
 template <int MT, int KP, int CH, int J, bool SWIGLU>
-void launch_rows(const DgmMxfp4GemmArgs& A, int vec, hipStream_t stream) {
+void launch_rows(const DgmMxfp4GemmArgs& A, const Launch& L) {
   const int64_t n_out = SWIGLU ? A.n / 2 : A.n, tokens = 16 / KP * MT;
   const dim3 grid((unsigned)((n_out + CH - 1) / CH), (unsigned)((A.m + tokens - 1) / tokens));
-  hipLaunchKernelGGL((k_mxfp4_gemm_rows<MT, KP, CH, J, SWIGLU>), grid, dim3(512), 0, stream, A, vec);
+  if (L.told) {
+    const int64_t form[7] = {tokens, CH, 0, 1, KP, J, (int64_t)grid.x * 512};
+    std::copy(form, form + 7, L.told);
+    return;
+  }
+  hipLaunchKernelGGL((k_mxfp4_gemm_rows<MT, KP, CH, J, SWIGLU>), grid, dim3(512), 0, L.stream, A, L.vec);
 }
 template <int MT, int J>
-void launch_rows(const DgmMxfp4GemmArgs& A, const Rows& f, int vec, hipStream_t stream) {
+void launch_rows(const DgmMxfp4GemmArgs& A, const Rows& f, const Launch& L) {
   if constexpr (MT == 1)
-    if (f.parts == 2) return A.swiglu ? launch_rows<1, 2, 4, J, true>(A, vec, stream) : launch_rows<1, 2, 8, J, false>(A, vec, stream);
-  if (!A.swiglu) launch_rows<MT, 1, 16, J, false>(A, vec, stream);
-  else if (f.channels == 8) launch_rows<MT, 1, 8, J, true>(A, vec, stream);
-  else launch_rows<MT, 1, 16, J, true>(A, vec, stream);
+    if (f.parts == 2) return A.swiglu ? launch_rows<1, 2, 4, J, true>(A, L) : launch_rows<1, 2, 8, J, false>(A, L);
+  if (!A.swiglu) launch_rows<MT, 1, 16, J, false>(A, L);
+  else if (f.channels == 8) launch_rows<MT, 1, 8, J, true>(A, L);
+  else launch_rows<MT, 1, 16, J, true>(A, L);
 }
 template <int MT>
-void launch_rows(const DgmMxfp4GemmArgs& A, int vec, hipStream_t stream) {
+void launch_rows(const DgmMxfp4GemmArgs& A, const Launch& L) {
   const Rows f = rows_form(A.m, A.n, A.k, A.swiglu != 0);
-  if (f.blocks == 4) launch_rows<MT, 4>(A, f, vec, stream);
-  else launch_rows<MT, 2>(A, f, vec, stream);
+  if (f.blocks == 4) launch_rows<MT, 4>(A, f, L);
+  else launch_rows<MT, 2>(A, f, L);
 }
 
 template <int BM, int BN, int WM, int WN, int STAGES>
-void launch_tiles(const DgmMxfp4GemmArgs& A, int vec, int splits, hipStream_t stream) {
+void launch_tiles(const DgmMxfp4GemmArgs& A, int splits, const Launch& L) {
+  static_assert(64 * WM * WN == TILE_THREADS, "as choose counts them");
+  const int vec = L.vec;
+  const hipStream_t stream = L.stream;
   const int tiles_m = (int)((A.m + BM - 1) / BM), tiles_n = (int)((A.n + BN - 1) / BN), steps = (int)((A.k + 255) / 256);
   const int per = (steps + splits - 1) / splits;
   splits = (steps + per - 1) / per;                // (every split has a step)
   const dim3 grid((unsigned)((tiles_m * tiles_n + 7) / 8 * 8), (unsigned)splits), block(64 * WM * WN);
+  if (L.told) {
+    const int64_t form[7] = {BM, BN, STAGES, splits, 1, 1, (int64_t)grid.x * block.x};
+    std::copy(form, form + 7, L.told);
+    return;
+  }
   if constexpr (BN / WN % 32 == 0)                 // (a wave's gate and up fragments)
     if (A.swiglu) hipLaunchKernelGGL((k_mxfp4_gemm_tiles<BM, BN, WM, WN, STAGES, true>), grid, block, 0, stream, A, vec, tiles_m, tiles_n, per);
   if (!A.swiglu) hipLaunchKernelGGL((k_mxfp4_gemm_tiles<BM, BN, WM, WN, STAGES, false>), grid, block, 0, stream, A, vec, tiles_m, tiles_n, per);
@@ -504,7 +529,10 @@ Form choose(int64_t m, int64_t n, int64_t k, bool swiglu, int64_t workspace_byte
   for (int t = swiglu ? T64_128 : T64; t <= T256; ++t)           // (64 x 64: a wave has 16 channels, so no gate and up rows)
     for (int s = 1; s <= 8; s *= 2) {
       if (s > 1 && (steps < 2 * s || (int64_t)s * m * n * 4 > workspace_bytes)) break;
-      const int64_t wgs = ((m + tiles[t].bm - 1) / tiles[t].bm) * ((n + tiles[t].bn - 1) / tiles[t].bn) * s;
+      const int64_t grid = ((m + tiles[t].bm - 1) / tiles[t].bm) * ((n + tiles[t].bn - 1) / tiles[t].bn), wgs = grid * s;
+      // (a launch has fewer than 2^32 threads, and its tiles are rounded up to eights; only 64 x 64 tiles come that far
+      // within the call's limit: 128 channels a tile need at most two thirds as many, or one column of 2^18)
+      if ((grid + 7) / 8 * 8 * TILE_THREADS >= (int64_t)1 << 32) break;
       const int64_t rounds = (wgs + 256 * tiles[t].per_cu - 1) / (256 * tiles[t].per_cu), each = (steps + s - 1) / s;
       double us = tiles[t].around + (wgs <= 256 ? (double)each * tiles[t].alone : (double)rounds * ((double)each * tiles[t].full + tiles[t].out));
       if (s > 1) us += 3.4 + 0.1 * s + 1.06e-6 * (double)s * (double)m * (double)n;
@@ -514,6 +542,20 @@ Form choose(int64_t m, int64_t n, int64_t k, bool swiglu, int64_t workspace_byte
 }
 // Sums of a split call above this are not worth their way through memory.
 constexpr int64_t MOST_WORKSPACE = 64 << 20;
+
+void launch(const DgmMxfp4GemmArgs& A, const Form& f, const Launch& L) {
+  if (f.kind == T64) launch_tiles<64, 64, 2, 4, 4>(A, f.splits, L);
+  else if (f.kind == T64_128) launch_tiles<64, 128, 2, 4, 3>(A, f.splits, L);
+  else if (f.kind == T128_DEEP) launch_tiles<128, 128, 2, 4, 4>(A, f.splits, L);
+  else if (f.kind == T128) launch_tiles<128, 128, 2, 4, 2>(A, f.splits, L);
+  else if (f.kind == T256_128) launch_tiles<256, 128, 4, 2, 3>(A, f.splits, L);
+  else if (f.kind == T192_128) launch_tiles<192, 128, 2, 4, 3>(A, f.splits, L);
+  else if (f.kind == T192_256) launch_tiles<192, 256, 2, 4, 2>(A, f.splits, L);
+  else if (f.kind == T256) launch_tiles<256, 256, 2, 4, 2>(A, f.splits, L);
+  else if (A.m <= 16) launch_rows<1>(A, L);
+  else if (A.m <= 32) launch_rows<2>(A, L);
+  else launch_rows<4>(A, L);
+}
 
 }  // namespace
 
@@ -531,6 +573,17 @@ int64_t dgm_mxfp4_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int swig
   return f.splits == 1 ? 0 : (int64_t)f.splits * m * n * 4;
 }
 
+int dgm_mxfp4_gemm_form(int64_t m, int64_t n, int64_t k, int swiglu, int64_t workspace_bytes, int64_t* form) {
+  DGM_CHECK_ARG(form, "null pointer");
+  DGM_CHECK_ARG(m > 0 && m < (1 << 24) && n > 0 && n < (1 << 24) && k > 0 && k < (1 << 24) && k % 32 == 0 && (!swiglu || n % 2 == 0),
+                "sizes of a product");
+  DGM_CHECK_ARG(((m + 63) / 64) * ((n + 63) / 64) < (1 << 23), "m n / 4096 below 2^23");
+  DgmMxfp4GemmArgs A = {};
+  A.m = m, A.n = n, A.k = k, A.swiglu = swiglu;
+  launch(A, choose(m, n, k, swiglu != 0, std::min(workspace_bytes, MOST_WORKSPACE)), {0, nullptr, form});
+  return 0;
+}
+
 int dgm_mxfp4_gemm_nt(const DgmMxfp4GemmArgs* args, hipStream_t stream) {
   DGM_CHECK_ARG(args, "null arguments");
   const DgmMxfp4GemmArgs A = *args;
@@ -545,7 +598,7 @@ int dgm_mxfp4_gemm_nt(const DgmMxfp4GemmArgs* args, hipStream_t stream) {
   DGM_CHECK_ARG(A.a_stride < (1 << 23) && A.b_stride < (1 << 23), "code rows less than 2^23 bytes apart");
   if (A.m == 0 || A.n == 0) return 0;
   DGM_CHECK_ARG(A.a && A.b && A.sfa && A.sfb && A.d, "null pointer");
-  // (a launch has fewer than 2^32 threads; the smallest tile has 64 x 64 results and 256 of them)
+  // (choose leaves out tiles whose launch would have 2^32 threads)
   DGM_CHECK_ARG(((A.m + 63) / 64) * ((A.n + 63) / 64) < (1 << 23), "m n / 4096 below 2^23");
   const int e = A.dtype == DGM_SRC_F32 ? 4 : 2;
   // 1: 16-byte stores (and loads of C), which need 4-byte alignment (777 x 1234, K 2880: 11.1 us, single elements 12.3).
@@ -555,17 +608,7 @@ int dgm_mxfp4_gemm_nt(const DgmMxfp4GemmArgs* args, hipStream_t stream) {
   if (vec && A.m * (A.swiglu ? A.n / 2 : A.n) * e >= 100000000) vec = 2;
   const int64_t held = A.workspace && ((uintptr_t)A.workspace & 15) == 0 ? A.workspace_bytes : 0;
   const Form f = choose(A.m, A.n, A.k, A.swiglu != 0, held < MOST_WORKSPACE ? held : MOST_WORKSPACE);
-  if (f.kind == T64) launch_tiles<64, 64, 2, 4, 4>(A, vec, f.splits, stream);
-  else if (f.kind == T64_128) launch_tiles<64, 128, 2, 4, 3>(A, vec, f.splits, stream);
-  else if (f.kind == T128_DEEP) launch_tiles<128, 128, 2, 4, 4>(A, vec, f.splits, stream);
-  else if (f.kind == T128) launch_tiles<128, 128, 2, 4, 2>(A, vec, f.splits, stream);
-  else if (f.kind == T256_128) launch_tiles<256, 128, 4, 2, 3>(A, vec, f.splits, stream);
-  else if (f.kind == T192_128) launch_tiles<192, 128, 2, 4, 3>(A, vec, f.splits, stream);
-  else if (f.kind == T192_256) launch_tiles<192, 256, 2, 4, 2>(A, vec, f.splits, stream);
-  else if (f.kind == T256) launch_tiles<256, 256, 2, 4, 2>(A, vec, f.splits, stream);
-  else if (A.m <= 16) launch_rows<1>(A, vec, stream);
-  else if (A.m <= 32) launch_rows<2>(A, vec, stream);
-  else launch_rows<4>(A, vec, stream);
+  launch(A, f, {vec, stream, nullptr});
   return dgm_last_launch_status();
 }
 

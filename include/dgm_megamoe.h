@@ -558,6 +558,10 @@ typedef struct DgmMxfp4GemmArgs {
 int64_t dgm_mxfp4_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int swiglu);
 int dgm_mxfp4_gemm_nt(const DgmMxfp4GemmArgs* args, hipStream_t stream);
 int dgm_mxfp4_gemm_struct_size(size_t* args);
+/* Diagnostic: the kernel that a product of this size takes with so many bytes of workspace. form[7]: tokens and channels
+ * (swiglu, tiles: gate and up rows) of a workgroup, stages (0: weights straight into registers), ranges of K, parts of K in
+ * a fragment, blocks of a lane's step, threads along the grid's first axis. */
+int dgm_mxfp4_gemm_form(int64_t m, int64_t n, int64_t k, int swiglu, int64_t workspace_bytes, int64_t* form);
 
 /* A linear layer whose three products are MXFP4, each pass as one call over the two operators above. Forward:
  * y [m, n] (x_dtype) = q(x) q(w)^T for x [m, k] (x_dtype) and w [n, k] (w_dtype), rows at strides in elements; the
