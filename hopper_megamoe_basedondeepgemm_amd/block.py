@@ -74,9 +74,12 @@ def mega_moe_block(x, norm_weight, router_weight, l1, l2, sym_buffer, residual=N
         gate_up, down = operand("gate and up", shared_expert[0])[0], operand("down", shared_expert[1])[0]
         inner = unit * down.size(1)
         if tuple(gate_up.shape) != (2 * inner, x.size(1) // unit) or x.size(1) % unit or down.size(0) != x.size(1) or inner % least \
-                or not 0 < inner <= most or (mxfp4 and not _fits(x.size(0), 2 * inner)):
+                or not 0 < inner <= most:
             raise ValueError(f"shared_expert: gate and up rows [2 I, {x.size(1)}] for down [{x.size(1)}, I], I a multiple of {least} "
                              f"up to {most}; got {tuple(gate_up.shape)} and {tuple(down.shape)}" + (" (two codes a byte)" if mxfp4 else ""))
+        if mxfp4 and not (_fits(x.size(0), 2 * inner) and _fits(x.size(0), x.size(1))):
+            raise ValueError(f"shared_expert of {inner} channels for x {tuple(x.shape)}: ceil(tokens / 64) ceil(rows / 64) below 2^23 "
+                             "for both weights' rows")
         if activation_clamp is not None and not activation_clamp >= 0:
             raise ValueError(f"activation_clamp {activation_clamp}: at least 0, or None")
     _lib.require_one_device(*leaves)
