@@ -421,12 +421,14 @@ __global__ void __launch_bounds__(256) k_mxfp4_gemm_join(const DgmMxfp4GemmArgs 
 // SwiGLU with gate and up rows in one fragment: up to 8 tokens, or where it is needed to fill the CUs: 1 x 4096, K 7168
 // 7.9 -> 5.6; 16 x 4096, K 7168 9.8 -> 7.5; but 16 x 8192, K 4096 7.2 -> 8.0 (token rows are read twice as often).
 // Four blocks a lane, so that more loads are in flight: 4 x 4096, K 4096 4.3 -> 4.0; 16 x 1024, K 8192 7.4 -> 6.6; but
-// where they leave a wave without a step 64 x 2880, K 2880 5.5 -> 7.0.
+// where they leave a wave without a step 64 x 2880, K 2880 5.5 -> 7.0. More than 32 tokens under SwiGLU with two
+// fragments have no form of four: by the estimates below tiles are ahead of it at every size.
 struct Rows { int parts, channels, blocks; };
 Rows rows_form(int64_t m, int64_t n, int64_t k, bool swiglu) {
   const int parts = k >= 2048 && m <= 8 && (n <= 2048 || (m <= 2 && !swiglu)) ? 2 : 1;
   const bool one = swiglu && (parts == 2 || m <= 8 || n <= 4096);
-  return {parts, 16 / parts / (one ? 2 : 1), k % 512 == 0 || k >= 4096 ? 4 : 2};
+  const bool four = (k % 512 == 0 || k >= 4096) && !(m > 32 && swiglu && !one);
+  return {parts, 16 / parts / (one ? 2 : 1), four ? 4 : 2};
 }
 
 // Threads of a tile's workgroup.
@@ -456,7 +458,7 @@ void launch_rows(const DgmMxfp4GemmArgs& A, const Rows& f, const Launch& L) {
     if (f.parts == 2) return A.swiglu ? launch_rows<1, 2, 4, J, true>(A, L) : launch_rows<1, 2, 8, J, false>(A, L);
   if (!A.swiglu) launch_rows<MT, 1, 16, J, false>(A, L);
   else if (f.channels == 8) launch_rows<MT, 1, 8, J, true>(A, L);
-  else launch_rows<MT, 1, 16, J, true>(A, L);
+  else if constexpr (MT < 4 || J < 4) launch_rows<MT, 1, 16, J, true>(A, L);
 }
 template <int MT>
 void launch_rows(const DgmMxfp4GemmArgs& A, const Launch& L) {
