@@ -44,11 +44,14 @@ __global__ void __launch_bounds__(THREADS) k_layer_norm_fwd(const DgmLayerNormAr
 #pragma unroll
     for (int k = 0; k < N; ++k) t[k] *= P.residual_scale;
   }
-  if (P.residual_out) R::template store<T>(P.residual_out, row * P.residual_out_stride, H, t);
+  // (loose rows: a thread also reads elements of the one before it, which may be another wave's, and residual_out may be
+  // the row itself: stored behind the sum, which waits for every thread's elements)
+  if (VEC && P.residual_out) R::template store<T>(P.residual_out, row * P.residual_out_stride, H, t);
   float sum = 0.f;
 #pragma unroll
   for (int k = 0; k < N; ++k) sum += t[k];       // (zeros behind H)
   red.run(sum);
+  if (!VEC && P.residual_out) R::template store<T>(P.residual_out, row * P.residual_out_stride, H, t);
   const float mean = sum / (float)H;              // (by 1 / H, a row of equal elements would not have them for its mean)
   float ss = 0.f;
 #pragma unroll

@@ -60,7 +60,8 @@ struct Row {
 };
 
 // The same elements as Row<NV, THREADS, true> holds, of rows of any length at any alignment: 16 bytes at a time on the
-// elements' alignment, a row's last piece from its last eight elements.
+// elements' alignment, a row's last piece from its last eight elements (up to seven are the thread's before it, which may
+// be in another wave; they are dropped). Where a row's memory is written too, every thread has to have its elements first.
 template <int NV, int THREADS>
 struct LooseRow : Row<NV, THREADS, true> {
   template <int T>
