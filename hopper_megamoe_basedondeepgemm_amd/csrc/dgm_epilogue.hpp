@@ -46,8 +46,8 @@ DGM_DEV void wave_sync() {
 }
 
 // A 16-byte piece of token m's row from channel n on (eight channels, fp32: four), from LDS: C added, rounded,
-// stored. vec: rows of D (and C) are 4-byte aligned; STREAM: 2 = and stored past the caches.
-template <int T, bool ADD, bool STREAM = false, class Args>
+// stored. vec: rows of D (and C) are 4-byte aligned.
+template <int T, bool ADD, class Args>
 DGM_DEV void put_piece(const Args& P, int64_t m, int64_t n, int64_t n_out, int vec, const float* from) {
   constexpr int E = T == DGM_SRC_F32 ? 4 : 8;
   if (n >= n_out) return;
@@ -66,10 +66,7 @@ DGM_DEV void put_piece(const Args& P, int64_t m, int64_t n, int64_t n_out, int v
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] += c[i];
       }
-      g4f* to = reinterpret_cast<g4f*>(reinterpret_cast<float*>(P.d) + at);
-      const g4f o = {v[0], v[1], v[2], v[3]};
-      if (STREAM && vec == 2) __builtin_nontemporal_store(o, to);
-      else *to = o;
+      *reinterpret_cast<g4f*>(reinterpret_cast<float*>(P.d) + at) = g4f{v[0], v[1], v[2], v[3]};
     } else {
       if constexpr (ADD) {
         const v4i c = *reinterpret_cast<const g4i*>(reinterpret_cast<const uint16_t*>(P.c) + ct);
@@ -86,9 +83,7 @@ DGM_DEV void put_piece(const Args& P, int64_t m, int64_t n, int64_t n_out, int v
         const uint32_t hi = T == DGM_SRC_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[2 * i + 1]) : __builtin_bit_cast(uint16_t, (__bf16)v[2 * i + 1]);
         o[i] = (int)(lo | hi << 16);
       }
-      g4i* to = reinterpret_cast<g4i*>(reinterpret_cast<uint16_t*>(P.d) + at);
-      if (STREAM && vec == 2) __builtin_nontemporal_store(o, to);
-      else *to = o;
+      *reinterpret_cast<g4i*>(reinterpret_cast<uint16_t*>(P.d) + at) = o;
     }
   } else {
 #pragma unroll

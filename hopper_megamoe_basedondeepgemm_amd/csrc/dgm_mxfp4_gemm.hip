@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mxfp4_gemm_tiles(const DgmMxfp
       for (int j = 0; j < 32 * L / 64; ++j) {
         const int row = (64 * j + lane) / L, col = (64 * j + lane) % L * E;
         if (t0 + 32 * m + row < P.m)
-          put_piece<t.value, add.value, true>(P, t0 + 32 * m + row, c0 + col, n_out, vec, part + row * PITCH + col);
+          put_piece<t.value, add.value>(P, t0 + 32 * m + row, c0 + col, n_out, vec, part + row * PITCH + col);
       }
     });
     wave_sync();
@@ -603,11 +603,10 @@ int dgm_mxfp4_gemm_nt(const DgmMxfp4GemmArgs* args, hipStream_t stream) {
   // (choose leaves out tiles whose launch would have 2^32 threads)
   DGM_CHECK_ARG(((A.m + 63) / 64) * ((A.n + 63) / 64) < (1 << 23), "m n / 4096 below 2^23");
   const int e = A.dtype == DGM_SRC_F32 ? 4 : 2;
-  // 1: 16-byte stores (and loads of C), which need 4-byte alignment (777 x 1234, K 2880: 11.1 us, single elements 12.3).
-  // 2: past the caches too, where the results would only push other data out of the last one (256 MB): 8192 x 8192,
-  // K 4096 (134 MB) 188 -> 176 us; but 8192 x 4096 (67 MB) 81 -> 86.
-  int vec = (((uintptr_t)A.d | (uintptr_t)A.c | (uint64_t)(A.d_stride * e) | (uint64_t)(A.c_stride * e)) & 3) == 0;
-  if (vec && A.m * (A.swiglu ? A.n / 2 : A.n) * e >= 100000000) vec = 2;
+  // 16-byte stores (and loads of C), which need 4-byte alignment (777 x 1234, K 2880: 11.1 us, single elements 12.3). Past
+  // the caches, without regard to size, results are no faster: 8192 x 8192, K 4096 (134 MB) 160 -> 164 us, K 1024 64 -> 75;
+  // 8192 x 4096, K 4096 76 -> 79; 16384 x 8192, K 4096 317 -> 307.
+  const int vec = (((uintptr_t)A.d | (uintptr_t)A.c | (uint64_t)(A.d_stride * e) | (uint64_t)(A.c_stride * e)) & 3) == 0;
   const int64_t held = A.workspace && ((uintptr_t)A.workspace & 15) == 0 ? A.workspace_bytes : 0;
   const Form f = choose(A.m, A.n, A.k, A.swiglu != 0, held < MOST_WORKSPACE ? held : MOST_WORKSPACE);
   launch(A, f, {vec, stream, nullptr});

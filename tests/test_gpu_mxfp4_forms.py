@@ -1,5 +1,5 @@
 """mxfp4_gemm_nt against its definition in 64 bits, through every kernel that the host chooses from (tests/mxfp4_forms.py)
-and with results so large that they are stored past the caches. Tolerances as derived in tests/test_gpu_mxfp4.py."""
+and with results of many tiles a CU. Tolerances as derived in tests/test_gpu_mxfp4.py."""
 import pytest
 import torch
 
@@ -55,7 +55,7 @@ def test_every_form_with_swiglu(m, n, k):
     (5003, 5001, 288, torch.float32, 0), (5003, 5001, 288, torch.float32, 3), (7171, 7173, 96, torch.bfloat16, 1),
     (7171, 7173, 96, torch.float16, 0), (390001, 129, 64, torch.bfloat16, 1), (257, 200003, 64, torch.bfloat16, 5)])
 def test_results_of_100_megabytes(m, n, k, dtype, right):
-    """Stored past the caches, where rows lie on 4 bytes: whole pieces, edges in both directions, C added, over d itself."""
+    """Rows on 4 bytes and off them: whole pieces, edges in both directions, C added, over d itself."""
     need_gpu()
     import hopper_megamoe_basedondeepgemm_amd as dgm
     assert m * n * torch.empty(0, dtype=dtype).element_size() >= 100000000
