@@ -20,9 +20,11 @@ namespace {
 DGM_DEV float total(float r, float s, float x) { return fmaf(s, x, r); }
 
 // Forward: one read of x and residual, one write of r and h; two sums over the row one behind the other (the variance
-// waits for the mean, which costs the second exchange but no cancellation). Over data that no cache holds: bf16
-// 8192 x 4096 48.2 us, 5.6 TB/s; fp32 8192 x 2880 73.5; rows off 16 bytes are loaded on the elements' alignment: 4096 x
-// 5001 47.6 us, 3.5 TB/s (by single elements 70). Requesting the residual and the weights with x is slower there (51.2).
+// waits for the mean, which costs the second exchange but no cancellation). Over 800 MB of rows in turn, which no cache
+// holds: bf16 8192 x 4096 51.8 us, fp32 8192 x 2880 72.9, bf16 2048 x 16384 52.6, 5.1 to 5.2 TB/s each; rows off 16 bytes
+// are loaded on the elements' alignment, 4096 x 5001 54.4 us, 3.0 TB/s. Three sets of rows in turn, partly in the last
+// cache: 8192 x 4096 48.2 (51.2 with the residual and the weights requested with x), 4096 x 5001 47.6 (by single
+// elements 70).
 // Rows of one wave: four of them a workgroup are no faster (100 000 x 256 56 us, one 54; half its lanes have no elements).
 template <int T, int NV, int THREADS, bool VEC>
 __global__ void __launch_bounds__(THREADS) k_layer_norm_fwd(const DgmLayerNormArgs P) {
@@ -94,9 +96,10 @@ __global__ void __launch_bounds__(THREADS) k_layer_norm_fwd(const DgmLayerNormAr
 
 // Gradients: workgroup g takes rows g, g + G, ...; the columns' sums over its rows stay in registers and go to
 // partial[set][g][H] (set 0 weight, 1 bias), which k_layer_norm_columns adds up in a fixed order: atomics would give
-// another order every time. Both sums (du and du u) meet in one exchange. bf16 8192 x 4096, five tensors of rows: 81 us
-// with the column sums, 5.0 TB/s; fp32 4096 x 4096: 84; beyond hidden 8192 some registers go to scratch memory (2048 x
-// 16384: 107 us, 3.8 TB/s); off 16 bytes 4096 x 5001: 84, 2.9 TB/s (by single elements 186).
+// another order every time. Both sums (du and du u) meet in one exchange. bf16 8192 x 4096, six tensors of rows (403 MB):
+// 81 us with the column sums, 4.9 TB/s; fp32 4096 x 4096: 84, 4.8; off 16 bytes 4096 x 5001: 85, 2.9 TB/s (by single
+// elements 186). Beyond hidden 8192 registers go to scratch memory, 9 to 11 a lane of aligned rows (2048 x 16384 bf16 105
+// us, 3.8 TB/s; fp32 188, 4.3), 27 to 91 of others (2048 x 12345 bf16 135 us, 2.3 TB/s; fp16 233, 1.3).
 template <int T, int NV, int THREADS, bool VEC>
 __global__ void __launch_bounds__(THREADS) k_layer_norm_bwd(const DgmLayerNormGradArgs P) {
   using R = std::conditional_t<VEC, Row<NV, THREADS, true>, LooseRow<NV, THREADS>>;
@@ -285,7 +288,7 @@ int dgm_layer_norm_residual(const DgmLayerNormArgs* args, hipStream_t stream) {
   return dgm_last_launch_status();
 }
 
-// As many workgroups as the CUs hold (16 waves each), a row each at least.
+// As many workgroups as the CUs hold (16 waves each), two rows each at least (one, where there is no second).
 int dgm_layer_norm_residual_groups(int64_t rows, int hidden) {
   // Two rows a workgroup at least: its column sums are as many bytes as two 16-bit rows, written and read again (300 x
   // 4096 15.0 us with one, 11.9; 64 x 7168 10.2 and 10.4). And no more than the CUs hold at a time.

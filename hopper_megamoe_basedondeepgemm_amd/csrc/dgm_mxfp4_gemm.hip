@@ -147,12 +147,16 @@ __global__ void __launch_bounds__(512) k_mxfp4_gemm_rows(const DgmMxfp4GemmArgs 
 // SwiGLU: blocks of 16 channel rows alternate between gate and up rows, so that a wave holds both of a channel.
 // Few tiles: gridDim.y workgroups share a tile, each a range of K, and leave their sums in the workspace
 // [split][token][channel] for k_mxfp4_gemm_join.
-// Bound: up to some hundred tokens the latency of a step (0.24 to 0.6 us, the loads' way from L2 and one barrier); of
-// large products the matrix units' rate on such data (6.6 PFLOP/s from registers, where the card's power holds the clock)
-// together with the results' stores: 8192 x 8192, K 4096 156 us (3.5 PFLOP/s), 143 without stores, on zeros 103.
-// In the compiler's own order, everything read first and accumulators in scratch memory, it took 343. Not faster:
-// 256 workgroups that loop over tiles and request the next one's first step ahead (192 -> 197; 8192 x 4096 78 -> 87),
-// whole 16-bit rows through LDS, four waves of 128 x 128 or sixteen of 64 x 64, fragments read three ahead.
+// Bound: up to some hundred tokens the latency of a step (0.24 to 0.6 us, the loads' way from L2 and one barrier). Of
+// 8192 x 8192, K 4096, 159 us (3.5 PFLOP/s), the instructions take 81 on such data (6.8 PFLOP/s from registers, where the
+// card's power holds the clock; on zeros 61). Without results the kernel takes 120 (zeros 96): by count a step's 192 KB of
+// reads from LDS and 64 KB into it are as many cycles as its products. The results' 39 us are under nothing else: a CU
+// holds one workgroup and takes four tiles in turn.
+// In the compiler's own order, everything read first and accumulators in scratch memory, it took 343. Not faster at their
+// step: 256 workgroups that loop over tiles and request the next one's first step ahead (192 -> 197; 8192 x 4096 78 ->
+// 87), whole 16-bit rows through LDS, four waves of 128 x 128 (the statements that keep the order hold accumulators in the
+// 256 ordinary registers, which they fill; with them in the other 256 it is not tried) or sixteen of 64 x 64, fragments
+// read three ahead.
 // Eight waves a tile: with four, tiles of 128 x 128 wait longer for each step (8192 x 512, K 7168 23.6 -> 37; 777 x 5120,
 // K 7168 by 192 x 128 25.5 -> 46); sixteen are 1 to 5 % slower.
 template <int BM, int BN, int WM, int WN, int STAGES, bool SWIGLU>
@@ -494,18 +498,20 @@ void launch_tiles(const DgmMxfp4GemmArgs& A, int splits, const Launch& L) {
 // Which kernel takes a product, from estimates of its time in us (256 CUs). A tile form takes `around` us and, for each
 // step of 256 of K, `alone` us while every workgroup has a CU to itself; when the CUs hold as many as fit, each round
 // of them takes `full` us a step and `out` us for its results. Splitting K costs a second launch and the sums' way
-// through memory. The times are fitted to 93 products of 1 to 8192 tokens with every form and split, three sets of
-// operands in turn: the estimates' choice takes 1.8 % longer than the best of twelve forms on average (64 x 64, by
-// eight waves, came later).
-// Where each form is the best (us; next best):
-//   64 x 64:              64 x 4096, K 7168: 10.7 (64 x 128, 4 splits 12.3); 256 x 4096, K 4096: 8.4 (64 x 128 9.6)
-//   64 x 128, 3 stages:   200 x 5120, K 2880: 9.5 (64 x 64 11.1);    777 x 1234, K 2880: 10.3 (64 x 64 12.1)
-//   128 x 128, 4 stages:  512 x 7168, K 7168: 22.1 (64 x 128 26.0);  777 x 2880, K 4096: 13.9 (15.8 with 2 stages)
-//   128 x 128, 2 stages:  777 x 2880, K 1248: 7.8 (8.1 with 4);      1234 x 2880, K 800: 7.7 (64 x 128 8.6)
-//   256 x 128:            2048 x 4096, K 4096: 25.2 (128 x 128 26.8); 777 x 8192, K 8192: 41.1 (42.6)
-//   192 x 128:            777 x 5120, K 7168: 27.1 (256 x 128 30.9);  1536 x 4096, K 2880: 19.8 (19.8)
-//   192 x 256:            3000 x 2880, K 2880: 25.7 (256 x 256 28.7); 1536 x 7168, K 2048: 19.8 (22.2)
-//   256 x 256:            8192 x 8192, K 4096: 163 (256 x 128 189);   4096 x 4096, K 8192: 71 (256 x 128 84)
+// through memory. The times were fitted to 93 products of 1 to 8192 tokens before 64 x 64 took eight waves and launches
+// went into a graph: they rank the forms, and are off by up to a third themselves (1000 x 5120, K 2880: 12.6, takes 17.5).
+// Over 102 products the choice takes 1.3 % longer than the best form on average; 17 to 128 tokens 3.9 %, where rows, one
+// range of 64 x 64 and several are close: 48 x 512, K 2880 64 x 64, 6.5 (rows 4.8); 64 x 4096, K 7168 four ranges, 11.6
+// (one 10.6).
+// Where each form is taken and the best (us; next best):
+//   64 x 64:              64 x 8192, K 4096: 8.1 (64 x 128 9.6);     128 x 4096, K 2880: 7.2 (64 x 128 8.3)
+//   64 x 128, 3 stages:   200 x 5120, K 2880: 9.2 (128 x 128 11.5);  777 x 1234, K 2880: 10.0 (64 x 64 12.1)
+//   128 x 128, 4 stages:  512 x 7168, K 7168: 20.3 (64 x 128 24.7);  777 x 2880, K 4096: 12.8 (15.2 with 2 stages)
+//   128 x 128, 2 stages:  1234 x 2880, K 800: 7.6 (7.8 with 4);      2048 x 2048, K 1024, SwiGLU: 7.0 (7.3 with 4)
+//   256 x 128:            2048 x 4096, K 4096: 23.8 (128 x 128 26.2); 777 x 8192, K 8192: 39.4 (128 x 128 40.6)
+//   192 x 128:            777 x 5120, K 7168: 27.2 (256 x 128 29.3); 1536 x 4096, K 2880: 18.2 (256 x 128 19.0)
+//   192 x 256:            3000 x 2880, K 2880: 23.9 (256 x 256 26.5); 1536 x 7168, K 2048: 18.4 (256 x 256 20.8)
+//   256 x 256:            8192 x 8192, K 4096: 159 (192 x 256 172);  4096 x 4096, K 8192: 66 (256 x 128 79)
 // The rows form takes 2.4 us and the longer of a wave's steps (a time for each 4096 of a part of K) and the weights at
 // the rate at which that many tokens can be multiplied with them (SwiGLU with a fragment each for gate and up rows:
 // 1.75 times the former, 1.35 times the rate).
